@@ -246,7 +246,7 @@ def prepare(case, seed):
         starts = [0]
         for _, new in sizes:
             starts.append(starts[-1] + new)
-        s.update(book=book, layer=layer, rows=_i32(order), q_start=_i32(starts), max_new=max(new for _, new in sizes), max_tokens=max(n for n, _ in sizes),
+        s.update(book=book, n_packed=n_packed, layer=layer, rows=_i32(order), q_start=_i32(starts), max_new=max(new for _, new in sizes), max_tokens=max(n for n, _ in sizes),
                  q=torch.randn(starts[-1], case["heads"], D, generator=gen, device="cuda").half(), slopes=None, prefix=None, first=None)
         if case["alibi"]:
             s["slopes"] = torch.exp2(-8.0 * torch.arange(1, case["heads"] + 1, device="cuda") / case["heads"])
@@ -260,8 +260,9 @@ def prepare(case, seed):
     if case["kind"] == "admit":
         packed = _packed(length, case["residual"])
         # the prompts of the last pass are in the cache and leave
-        s["book"] = _book(seqs, pages, seqs * packed + 2, seqs * pages + 2)
-        s["layers"] = [_pool(seqs * packed + 2, seqs * pages + 2, heads, bits, group) for _ in range(layers)]
+        s["n_packed"] = seqs * packed + 2
+        s["book"] = _book(seqs, pages, s["n_packed"], seqs * pages + 2)
+        s["layers"] = [_pool(s["n_packed"], seqs * pages + 2, heads, bits, group) for _ in range(layers)]
         out = _outliers(heads, gen)
         s["k"] = [_kv((seqs * length, heads, D), gen, out) for _ in range(layers)]
         s["v"] = [_kv((seqs * length, heads, D), gen, None) for _ in range(layers)]
@@ -285,7 +286,7 @@ def prepare(case, seed):
         held = [(row, length, packed) for row in slots]
         s["turns"], s["turn"] = [_i32(slots[:seqs // 2]), _i32(slots[seqs // 2:])], [0]
         s["counts"] = _i32([length] * (seqs // 2))
-    s["book"], s["layers"] = book, [_pool(n_packed, n_fp16, heads, bits, group) for _ in range(layers)]
+    s["book"], s["n_packed"], s["layers"] = book, n_packed, [_pool(n_packed, n_fp16, heads, bits, group) for _ in range(layers)]
     for layer in s["layers"]:                                   # whatever the pages hold
         for i in (0, 4):
             layer[i].copy_(torch.randint(-2 ** 31, 2 ** 31 - 1, layer[i].shape, generator=gen, device="cuda", dtype=torch.int32))
@@ -535,7 +536,7 @@ def run(s):
     case = s["case"]
     if own:
         import kvmix_b200 as kv
-        pages = kv.PageBook(*s["book"])
+        pages = kv.PageBook(*s["book"], s["n_packed"])
         if case["kind"] == "attend":
             return kv.paged_attention(s["q"], s["q_start"], s["rows"], pages, kv.PageLayer(*s["layer"]), window=case["window"], prefix=s["prefix"],
                                       first=s["first"], softcap=case["softcap"], alibi_slopes=s["slopes"], max_new=s["max_new"], max_tokens=s["max_tokens"])
@@ -559,8 +560,7 @@ def run(s):
     else:
         if case["kind"] == "attend":
             return _attend_plain(s)
-        book, layers = s["book"], s["layers"]
-        n_packed = layers[0][0].shape[0]
+        book, layers, n_packed = s["book"], s["layers"], s["n_packed"]
         if case["kind"] == "admit":
             _free_plain(book, s["rows"], n_packed)
             _extend_plain(book, s["rows"], s["counts"], n_packed)
