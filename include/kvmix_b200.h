@@ -453,6 +453,128 @@ int kvq_decode_attn_plan(const kvq_attn_args *a, int32_t tensor_core, kvq_attn_p
 #define KVQ_STATIC_SCRATCH_BYTES (8u << 20)
 int kvq_decode_attn_static(const kvq_attn_args *a, kvq_stream_t stream);
 
+/*
+ * Paged cache.  (No counterpart in upstream KVmix, whose cache is one tuple of tensors per batch.)
+ *
+ * A page holds KVQ_PAGE_TOKENS = 128 tokens of one sequence, for every layer under the same number.  The oldest pages of a sequence
+ * are packed, the others fp16; both kinds have a pool of their own.  Page p of a layer:
+ *   kcode [n_packed, Hkv, 128 channels, words]   kscale, kmn [n_packed, Hkv, 128 channels, groups]     what kvq_quant_lastdim gives for
+ *   vcode [n_packed, Hkv, 128 tokens, words]     vscale, vmn [n_packed, Hkv, 128 tokens, groups]       the page's 128 tokens / channels
+ *   kfull, vfull [n_fp16, Hkv, 128 tokens, 128 channels] fp16
+ * all contiguous, words = 4 * bits (12 at 3 bits), groups = 128 / group (12 at 3 bits: groups of 11, the last of 7,
+ * the ragged_tail form of kvq_quant_lastdim); group 32, 64 or 128.  Heads have 128 channels.
+ *
+ * The bookkeeping lives on the device, is shared by all layers and changed by kernels only, so that no call waits for the host and
+ * every call can be captured:
+ *   table    [slots, max_pages]  page numbers of a sequence, oldest first: entry j is a packed page for j < packed[s], an fp16 page for
+ *                                j < ceil(length[s] / 128), -1 behind
+ *   length   [slots]             tokens;  packed [slots]: packed pages
+ *   refs     [n_packed + n_fp16] references of every page, fp16 pages behind the packed ones
+ *   free_ids [n_packed + n_fp16] the free pages' numbers, two stacks (packed from 0, fp16 from n_packed), the next one to be taken last
+ *   count    [4]                 free packed pages, free fp16 pages, status, 0
+ * A page that several sequences hold is full or packed and never written.
+ *
+ * count[2], the status, collects KVQ_PAGES_* bits.  A call that cannot be done in full does nothing but set one; while any is set, the
+ * calls that change the cache do nothing (lengths and pages stay consistent) until the caller has cleared it.
+ * `rows`: n slots, each at most once in a call.  Stacks are popped and pushed in the order of rows and pages (kvq_pages_extend, _fork,
+ * _settle) and of page numbers (pages that come free), so that equal calls give equal numbers.
+ */
+#define KVQ_PAGE_TOKENS 128
+#define KVQ_PAGES_NO_FP16 1     /* fewer free fp16 pages than asked for                                    */
+#define KVQ_PAGES_NO_PACKED 2   /* fewer free packed pages than asked for                                  */
+#define KVQ_PAGES_TOO_LONG 4    /* a sequence would need more than max_pages                               */
+#define KVQ_PAGES_BAD_ROWS 8    /* a row outside the table, named twice, or not as the call wants it       */
+#define KVQ_PAGES_STALLED 16    /* a kernel gave up waiting for its own copies                             */
+
+typedef struct {
+    int32_t *table, *length, *packed, *refs, *free_ids, *count;
+    int32_t slots, max_pages, n_packed, n_fp16;
+} kvq_page_book;
+
+typedef struct {
+    int32_t *kcode;
+    void *kscale, *kmn, *kfull;
+    int32_t *vcode;
+    void *vscale, *vmn, *vfull;
+    int32_t Hkv, k_bits, v_bits, group;
+    int32_t n_packed, n_fp16;
+} kvq_page_layer;
+
+/* length[rows[i]] += counts[i], with the fp16 pages that takes. */
+int kvq_pages_extend(const kvq_page_book *b, const int32_t *rows, const int32_t *counts, int32_t n, kvq_stream_t stream);
+
+/* The rows' sequences are dropped; pages that nobody holds any more are free. */
+int kvq_pages_free(const kvq_page_book *b, const int32_t *rows, int32_t n, kvq_stream_t stream);
+
+/*
+ * Every full page of the rows' sequences that ends `window` tokens or more before the sequence's end gets a packed page instead of its
+ * fp16 page (which comes free when nobody else holds it).  moves: int32 [4 + 2 * n_packed]; moves[0] becomes the number of (fp16 page,
+ * packed page) pairs that follow at moves[4], for kvq_page_pack to quantize, layer by layer, before anything else is written.
+ */
+int kvq_pages_settle(const kvq_page_book *b, const int32_t *rows, int32_t n, int32_t window, int32_t *moves, kvq_stream_t stream);
+/* Quantizes keys and values of the pages in `moves` (device memory), bit for bit as kvq_quant_lastdim (scale_by_division = 0). */
+int kvq_page_pack(const kvq_page_layer *l, const int32_t *moves, int32_t max_moves, kvq_stream_t stream);
+
+/*
+ * children[i] (an empty row) becomes a copy of parents[i]: full pages are shared, a last page that is not full gets a page of its own.
+ * moves: int32 [4 + 2 * n], the (old, new) pairs of those for kvq_page_copy on every layer's kfull and vfull.  A parent may have several
+ * children; no row is both.
+ */
+int kvq_pages_fork(const kvq_page_book *b, const int32_t *parents, const int32_t *children, int32_t n, int32_t *moves, kvq_stream_t stream);
+
+/*
+ * The pages in use move to the lowest numbers: those beyond the number of pages in use into the free ones below, in ascending order.
+ * moves: int32 [4 + 2 * n_packed], then int32 [4 + 2 * n_fp16] the same for fp16 pages, then n_packed + n_fp16 of scratch.
+ */
+int kvq_pages_compact(const kvq_page_book *b, int32_t *moves, kvq_stream_t stream);
+
+/* Copies whole pages (source, destination) of `moves` in n tensors; sources and destinations have no page in common. */
+typedef struct { void *base; int64_t page_bytes; } kvq_page_tensor;
+#define KVQ_MAX_PAGE_TENSORS 256
+int kvq_page_copy(const kvq_page_tensor *tensors, int32_t n, const int32_t *moves, int32_t max_moves, kvq_stream_t stream);
+
+/*
+ * Keys and values of new tokens into their fp16 pages: rows [q_start[i], q_start[i+1]) of k and v are the last tokens of sequence
+ * rows[i] (kvq_pages_extend has counted them already).  Element (token, head, channel) at k + token*k_sT + head*k_sH + channel.
+ */
+typedef struct {
+    const void *k, *v;
+    int64_t k_sT, k_sH, v_sT, v_sH;
+    const int32_t *q_start, *rows;
+    int32_t n, tokens;
+} kvq_page_write_args;
+
+int kvq_page_write(const kvq_page_book *b, const kvq_page_layer *l, const kvq_page_write_args *a, kvq_stream_t stream);
+
+/*
+ * Attention of new tokens over a paged cache.  Sequence rows[i]'s last q_start[i+1] - q_start[i] tokens ask (its keys and values, theirs
+ * among them, are in the pages): row u of q stands at position p = length - q_start[i+1] + u and sees the positions
+ *   max(first[u], p + 1 - window) <= j < max(p + 1, prefix[i]), at most length
+ * (first NULL: 0; window 0: no bound; prefix NULL: 0; causal = 0: all from the lower bound on), which covers causal and sliding-window
+ * attention, documents packed behind one another (first = the document's start) and prefixes whose tokens all see each other.
+ *   s = q.k * softmax_scale;  softcap > 0: s = softcap * tanh(s / softcap);  slopes: s += slopes[h] * (j - p);  out = softmax(s).v
+ * A row that sees nothing gives zeros.  Positions beyond `length`, pages without a number and rows of q behind q_start[n] are neither
+ * read nor written.  Keys and values that are not finite reach the queries that see them and may reach others of the same 128 tokens.
+ * GQA: query head h reads kv head h / (nh / Hkv).
+ *   q, out [tokens, nh, 128] fp16, strides *_sT, *_sH;  first [tokens], prefix [n] int32, slopes [nh] fp32
+ *   max_new: no sequence has more new tokens;  max_tokens: no sequence is longer (both only lay out the work)
+ * workspace: kvq_paged_attn_workspace_bytes(...) bytes, not shared by concurrent calls.
+ */
+typedef struct {
+    const void *q;
+    void *out;
+    int64_t q_sT, q_sH, o_sT, o_sH;
+    const int32_t *q_start, *rows, *first, *prefix;
+    const float *slopes;
+    int32_t n, tokens, nh, max_new, max_tokens, window, causal;
+    float softmax_scale, softcap;
+    void *workspace;
+    uint64_t workspace_bytes;
+} kvq_paged_attn_args;
+
+uint64_t kvq_paged_attn_workspace_bytes(int32_t n, int32_t tokens, int32_t nh, int32_t Hkv, int32_t max_new, int32_t max_tokens);
+int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, const kvq_paged_attn_args *a, kvq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

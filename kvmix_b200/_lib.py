@@ -88,6 +88,33 @@ class AttnPlan(C.Structure):
                 ("n_whole", i32), ("n_cut", i32), ("segments", i32), ("segment_units", i32), ("max_segment_tokens", i32)]
 
 
+class PageBookArgs(C.Structure):
+    _fields_ = [("table", vp), ("length", vp), ("packed", vp), ("refs", vp), ("free_ids", vp), ("count", vp),
+                ("slots", i32), ("max_pages", i32), ("n_packed", i32), ("n_fp16", i32)]
+
+
+class PageLayerArgs(C.Structure):
+    _fields_ = [("kcode", vp), ("kscale", vp), ("kmn", vp), ("kfull", vp), ("vcode", vp), ("vscale", vp), ("vmn", vp), ("vfull", vp),
+                ("Hkv", i32), ("k_bits", i32), ("v_bits", i32), ("group", i32), ("n_packed", i32), ("n_fp16", i32)]
+
+
+class PageTensor(C.Structure):
+    _fields_ = [("base", vp), ("page_bytes", i64)]
+
+
+class PageWriteArgs(C.Structure):
+    _fields_ = [("k", vp), ("v", vp), ("k_sT", i64), ("k_sH", i64), ("v_sT", i64), ("v_sH", i64), ("q_start", vp), ("rows", vp),
+                ("n", i32), ("tokens", i32)]
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = [("q", vp), ("out", vp), ("q_sT", i64), ("q_sH", i64), ("o_sT", i64), ("o_sH", i64),
+                ("q_start", vp), ("rows", vp), ("first", vp), ("prefix", vp), ("slopes", vp),
+                ("n", i32), ("tokens", i32), ("nh", i32), ("max_new", i32), ("max_tokens", i32), ("window", i32), ("causal", i32),
+                ("softmax_scale", C.c_float), ("softcap", C.c_float), ("workspace", vp), ("workspace_bytes", u64)]
+
+
+MAX_PAGE_TENSORS = 256
 ATTN_WORKSPACE_READY = 1
 
 
@@ -134,13 +161,23 @@ def lib():
         L.kvq_decode_attn_workspace_init.argtypes = [vp, u64, i32, i32, vp]
         L.kvq_decode_attn_workspace_bytes.restype = u64
         L.kvq_decode_attn_workspace_bytes.argtypes = [i32, i32, i32]
+        # the paged cache's calls take their argument blocks as bytes (paged.py packs them)
+        blk = C.c_char_p
+        for fn, types in ((L.kvq_pages_extend, [blk, vp, vp, i32, vp]), (L.kvq_pages_free, [blk, vp, i32, vp]),
+                          (L.kvq_pages_settle, [blk, vp, i32, i32, vp, vp]), (L.kvq_page_pack, [blk, vp, i32, vp]),
+                          (L.kvq_pages_fork, [blk, vp, vp, i32, vp, vp]), (L.kvq_pages_compact, [blk, vp, vp]),
+                          (L.kvq_page_copy, [blk, i32, vp, i32, vp]), (L.kvq_page_write, [blk, blk, blk, vp]), (L.kvq_paged_attn, [blk, blk, blk, vp])):
+            fn.restype, fn.argtypes = C.c_int, types
+        L.kvq_paged_attn_workspace_bytes.restype, L.kvq_paged_attn_workspace_bytes.argtypes = u64, [i32] * 6
         _lib = L
     return _lib
 
 
 EXPORTS = ["kvq_version", "kvq_error_string", "kvq_last_cuda_error", "kvq_features_per_int",
            "kvq_quant_lastdim", "kvq_append_kv", "kvq_gemv", "kvq_decode_attn", "kvq_decode_attn_workspace_bytes",
-           "kvq_decode_attn_static", "kvq_decode_attn_plan", "kvq_decode_attn_workspace_init", "kvq_prefill", "kvq_peer_wait", "kvq_peer_wait_next", "kvq_append_k", "kvq_append_v"]
+           "kvq_decode_attn_static", "kvq_decode_attn_plan", "kvq_decode_attn_workspace_init", "kvq_prefill", "kvq_peer_wait", "kvq_peer_wait_next", "kvq_append_k", "kvq_append_v",
+           "kvq_pages_extend", "kvq_pages_free", "kvq_pages_settle", "kvq_page_pack", "kvq_pages_fork", "kvq_pages_compact", "kvq_page_copy", "kvq_page_write",
+           "kvq_paged_attn", "kvq_paged_attn_workspace_bytes"]
 
 
 def check(rc):

@@ -1,0 +1,94 @@
+// kvq_paged_attn: checks, the plan of a call, its launches.
+#include "paged_attn.cuh"
+
+namespace kvq {
+
+int paged_few(const PagedArgs &p, cudaStream_t st);                              // paged_decode.cu
+int paged_merge(const PagedArgs &p, int few, cudaStream_t st);
+int paged_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st);             // paged_tiles.cu
+
+// How a call is cut.  Either kernel may cut the pages of a sequence into splits, whose partial sums meet in a second launch.
+struct PagedPlan {
+    bool few, tiles;                  // which kernels are launched
+    int few_rows;                     // sequences with more rows are the kernel of tiles'
+    int few_splits, tile_splits, max_tiles;
+};
+
+static PagedPlan paged_plan(int n, int tokens, int nh, int Hkv, int max_new, int max_tokens) {
+    PagedPlan r = {};
+    const int rep = nh / Hkv;
+    const int64_t most = (int64_t)max_new * rep;
+    r.tiles = most > kFewRows;
+    // every sequence has its max_new tokens, or it is the only one: nothing for the kernel of few rows in a call that needs the other
+    r.few = rep <= kFewRows && (!r.tiles || (n > 1 && tokens < (int64_t)n * max_new));
+    r.few_rows = r.few ? kFewRows : 0;
+    const int pages = (max_tokens + kPage - 1) / kPage;
+    const int64_t pairs = (int64_t)n * Hkv;
+    const int64_t want = (148 * 4 + pairs / 2) / pairs;           // four CTAs to an SM
+    r.few_splits = (int)(want < 1 ? 1 : want);
+    if (r.few_splits > (pages + 3) / 4) r.few_splits = (pages + 3) / 4;          // a page for each of a CTA's warps
+    if (r.few_splits < 1) r.few_splits = 1;
+    int64_t tiles = ((int64_t)tokens * rep) / 256 + n;
+    if (n == 1) tiles = ((int64_t)tokens * rep + 255) / 256;
+    r.max_tiles = (int)(tiles < INT32_MAX ? tiles : INT32_MAX);
+    const int64_t ctas = tiles * Hkv;
+    r.tile_splits = (int)(ctas < 1 ? 1 : 148 / ctas);
+    if (r.tile_splits > (pages + 3) / 4) r.tile_splits = (pages + 3) / 4;
+    if (r.tile_splits < 1) r.tile_splits = 1;
+    return r;
+}
+
+static uint64_t paged_bytes(const PagedPlan &r, int tokens, int nh) {
+    const int splits = (r.few && r.few_splits > 1) || (r.tiles && r.tile_splits > 1) ? (r.few && r.few_splits > r.tile_splits ? r.few_splits : r.tiles ? r.tile_splits : r.few_splits) : 0;
+    return (uint64_t)splits * tokens * nh * (kHeadDim + 2) * 4;
+}
+
+}  // namespace kvq
+
+extern "C" uint64_t kvq_paged_attn_workspace_bytes(int32_t n, int32_t tokens, int32_t nh, int32_t Hkv, int32_t max_new, int32_t max_tokens) {
+    using namespace kvq;
+    if (n <= 0 || tokens <= 0 || Hkv <= 0 || nh <= 0 || nh % Hkv || max_new <= 0 || max_tokens <= 0) return 0;
+    return paged_bytes(paged_plan(n, tokens, nh, Hkv, max_new, max_tokens), tokens, nh);
+}
+
+extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, const kvq_paged_attn_args *a, kvq_stream_t stream) {
+    using namespace kvq;
+    if (const int rc = check_book(b)) return rc;
+    if (const int rc = check_layer(l)) return rc;
+    if (!a) return KVQ_ERR_NULL;
+    if (a->n < 0 || a->tokens < 0 || a->nh <= 0 || a->window < 0) return KVQ_ERR_SHAPE;
+    if (a->nh % l->Hkv) return KVQ_ERR_HEADS;
+    if (a->n == 0 || a->tokens == 0) return KVQ_OK;
+    if (a->max_new <= 0 || a->max_tokens <= 0) return KVQ_ERR_SHAPE;
+    if (!a->q || !a->out || !a->q_start || !a->rows) return KVQ_ERR_NULL;
+    if (!(a->softcap >= 0.f) || !(a->softmax_scale == a->softmax_scale)) return KVQ_ERR_SHAPE;
+    const PagedPlan r = paged_plan(a->n, a->tokens, a->nh, l->Hkv, a->max_new, a->max_tokens);
+    const uint64_t need = paged_bytes(r, a->tokens, a->nh);
+    if (need && (!a->workspace || a->workspace_bytes < need)) return KVQ_ERR_WORKSPACE;
+    if (need && reinterpret_cast<uintptr_t>(a->workspace) % 16) return KVQ_ERR_ALIGN;
+    PagedArgs p = {};
+    p.b = *b;
+    p.l = *l;
+    p.a = *a;
+    p.rep = a->nh / l->Hkv;
+    p.k_groups = page_groups(l->k_bits, l->group);
+    p.v_groups = page_groups(l->v_bits, l->group);
+    p.few_rows = r.few_rows;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const int most = r.few && r.few_splits > r.tile_splits ? r.few_splits : r.tiles ? r.tile_splits : r.few_splits;
+    p.part_out = static_cast<float *>(a->workspace);
+    p.part_ml = need ? p.part_out + (uint64_t)most * a->tokens * a->nh * kHeadDim : nullptr;
+    if (r.few) {
+        p.splits = r.few_splits;
+        if (const int rc = paged_few(p, st)) return rc;
+        if (p.splits > 1)
+            if (const int rc = paged_merge(p, 1, st)) return rc;
+    }
+    if (r.tiles) {
+        p.splits = r.tile_splits;
+        if (const int rc = paged_tiles(p, r.max_tiles, st)) return rc;
+        if (p.splits > 1)
+            if (const int rc = paged_merge(p, 0, st)) return rc;
+    }
+    return KVQ_OK;
+}

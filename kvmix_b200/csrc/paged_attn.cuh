@@ -1,0 +1,120 @@
+// What the two attention kernels of the paged cache share: which positions a query sees, how a raw score becomes the exponent of
+// its weight, bounded waits for bulk copies, packed fields as fp16.
+#pragma once
+#include "attn_mma_common.cuh"
+#include "pages.cuh"
+
+namespace kvq {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Sequences with at most so many rows -- (query head of the kv head, new token) pairs -- go to the kernel of few rows, the others to the
+// kernel of tiles.
+constexpr int kFewRows = 8;
+
+struct PagedArgs {
+    kvq_page_book b;
+    kvq_page_layer l;
+    kvq_paged_attn_args a;
+    int rep, k_groups, v_groups;      // query heads of a kv head; groups of a page's row
+    int splits, few_rows;             // few_rows: sequences with at most so many rows are the other kernel's
+    float *part_out;                  // [splits][tokens * nh][128], unnormalised
+    float *part_ml;                   // [splits][tokens * nh][2]: the exponents' reference (log2), the weights' sum
+};
+
+// Sequence i as every thread sees it: its row of the table, length, packed pages, where its new tokens are.  Numbers that would lead
+// outside anything are made harmless.
+struct PagedSeq {
+    int row, length, packed, q0, n_new, prefix;
+    const int32_t *table;
+};
+__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs &p, int i) {
+    PagedSeq s;
+    s.row = p.a.rows[i];
+    const bool ok = s.row >= 0 && s.row < p.b.slots;
+    const int row = ok ? s.row : 0;
+    s.length = ok ? min(p.b.length[row], p.b.max_pages * kPage) : 0;
+    s.packed = ok ? p.b.packed[row] : 0;
+    s.table = p.b.table + (int64_t)row * p.b.max_pages;
+    s.q0 = max(p.a.q_start[i], 0);
+    s.n_new = min(p.a.q_start[i + 1], p.a.tokens) - s.q0;
+    s.prefix = p.a.prefix ? p.a.prefix[i] : 0;
+    return s;
+}
+// [lo, hi) of the positions that new token u (of n_new) sees
+__device__ __forceinline__ void paged_bounds(const PagedArgs &p, const PagedSeq &s, int u, int &pos, int &lo, int &hi) {
+    pos = s.length - s.n_new + u;
+    lo = p.a.first ? max(p.a.first[s.q0 + u], 0) : 0;
+    if (p.a.window > 0) lo = max(lo, pos + 1 - p.a.window);
+    hi = p.a.causal ? min(max(pos + 1, s.prefix), s.length) : s.length;
+    if (pos < 0) hi = lo;                                         // more new tokens than the sequence has
+}
+
+// 2^x for x <= some tens, one instruction; denormal results flush to zero.
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// softcap * tanh(s / softcap) as softcap * (1 - 2 / (exp(2 s / softcap) + 1)): absolute error 3e-7 * softcap (tanh.approx: 5e-4 * softcap).
+// `two`: 2 log2(e) / softcap * scale.
+__device__ __forceinline__ float cap_score(float raw, float two, float cap) { return cap - 2.f * cap * rcp_approx(exp2_approx(raw * two) + 1.f); }
+
+// ---------------------------------------------------------------------------------------------
+// mbarriers.  A wait gives up after two seconds, sets a bit of the status and lets the kernel end.
+__device__ __forceinline__ unsigned long long global_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, int count) { asm volatile("mbarrier.init.shared.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared.b64 _, [%0];\n" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok;
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int32_t *status) {
+    if (mbar_try(bar, parity)) return true;
+    const unsigned long long end = global_ns() + 2000000000ull;
+    do {
+        for (int i = 0; i < 64; ++i)
+            if (mbar_try(bar, parity)) return true;
+    } while (global_ns() < end);
+    atomicOr(status, KVQ_PAGES_STALLED);
+    return false;
+}
+// 16-byte aligned both ways, a multiple of 16 bytes
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// Factor of a partial sum with reference m (log2) and weights' sum l under the common reference: 0 for one that saw nothing; NaN stays.
+__device__ __forceinline__ float part_factor(float m, float l, float common) { return l == 0.f ? 0.f : m == -INFINITY ? 1.f : exp2_approx(m - common); }
+
+// ---------------------------------------------------------------------------------------------
+// A register holds two 16-bit halves, one of each of two words, with 16 / BITS fields of BITS bits.  A field left in place under an
+// exponent that gives its lowest bit the value 1 reads as 2^(10 - position) + code; less that power it is the code, exactly.  That
+// takes positions up to 10 - BITS; the fields above are shifted down first.
+template <int BITS>
+struct HalfFields {
+    static constexpr int N = 16 / BITS;                           // fields of a half
+    static constexpr int DIRECT = (10 - BITS) / BITS + 1;         // of them in reach without the shift
+    __device__ static __forceinline__ __half2 code(uint32_t x, int f) {
+        const int pos = f < DIRECT ? BITS * f : BITS * (f - DIRECT);
+        const uint32_t mask = ((1u << BITS) - 1u) << pos, expo = (uint32_t)(25 - pos) << 10;
+        uint32_t r;
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(f < DIRECT ? x : x >> (BITS * DIRECT)), "r"(mask * 0x10001u), "r"(expo * 0x10001u));   // (x & mask) | expo
+        return __hsub2(as_h2(r), as_h2(expo * 0x10001u));
+    }
+};
+
+}  // namespace kvq

@@ -1,0 +1,488 @@
+// Attention of many query rows of a kv head (chunks of prompts, the tokens of a speculative step) over a paged cache, on tcgen05.
+#include "paged_attn.cuh"
+
+namespace kvq {
+
+// A CTA takes 256 rows -- (token, query head of the group) pairs of one sequence and kv head, as two tiles of 128 -- and walks the pages
+// that any of them sees.  A page is one step of both products:
+//   S = Q K^T   128 x 128 x 128, Q and K in shared memory, S (fp32) in TMEM
+//   O += P V    P, the weights as fp16, over S in TMEM; V in shared memory; O (fp32) in TMEM
+// Sixteen warps: two warpgroups of softmax, one per tile, a row a thread; one that fills the operand buffers; one thread that issues the
+// MMAs.  While one tile's scores are worked on, the tensor core multiplies for the other.  TMEM: S0 S1 O0 O1, 128 columns each.
+//
+// Operand buffers hold 128 rows of 128 fp16 as two halves of 64 (128 bytes a row, 16-byte pieces swizzled by the row's number).  Rows are
+// tokens of fp16 pages and of packed values, channels of packed keys: what is contiguous in a row is the contraction axis of fp16 keys (K-major
+// operand) and the axis of output columns of everything else (MN-major operand), so that packed words are spread where
+// their fields lie side by side and nothing is transposed.
+// Packed rows become fp16 as code * scale + minimum with one rounding (2^-11 relative): the tensor core takes no wider operand without
+// half its rate.
+constexpr int kTileRows = 128, kTileThreads = 512;
+constexpr uint32_t kOperandBytes = 32768, kOperandHalf = 16384;
+constexpr int kRawBytes = 12288;                                  // the largest packed half of a page: 3 bits, or 4 bits and groups of 32
+// shared memory, from a 1024-byte boundary
+constexpr uint32_t kOffQ = 0, kOffK = 2 * kOperandBytes, kOffV = kOffK + 2 * kOperandBytes, kOffRaw = kOffV + 2 * kOperandBytes,
+                   kOffBar = kOffRaw + 2 * kRawBytes, kTileSmem = kOffBar + 256;
+// barriers
+constexpr int kBarQ = 0, kBarKFull = 1, kBarKFree = 3, kBarVFull = 5, kBarVFree = 7, kBarS = 9, kBarP = 11, kBarO = 13, kBarRaw = 14, kBarDrain = 16;
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
+}
+// Operand descriptor: swizzle of 128 bytes; `lbo`, `sbo` in bytes (see the layouts above).
+__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// fp16 x fp16 -> fp32, M = N = 128; bit 16: B is MN-major
+constexpr uint32_t kIdesc = 1u << 4 | (128u >> 3) << 17 | (128u >> 4) << 24, kIdescMn = kIdesc | 1u << 16;
+
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void tc_mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+
+#define KVQ_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
+#define KVQ_W8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
+// 32 columns of this thread's row
+__device__ __forceinline__ void tc_load32(uint32_t (&r)[32], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+                 : KVQ_R8(r, 0), KVQ_R8(r, 8), KVQ_R8(r, 16), KVQ_R8(r, 24) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tc_store32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(addr),
+                 KVQ_W8(r, 0), KVQ_W8(r, 8), KVQ_W8(r, 16), KVQ_W8(r, 24) : "memory");
+}
+
+// Piece c (16 bytes, 0..15) of row r of an operand buffer
+__device__ __forceinline__ uint32_t operand_at(uint32_t base, int r, int c) { return base + (c >> 3) * kOperandHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// One packed row -> 128 fp16 of an operand row.
+template <int BITS>
+__device__ __forceinline__ void unpack_row(uint32_t raw, uint32_t to, int r, int groups, int g_log2) {
+    constexpr int W = page_words(BITS);
+    const uint32_t codes = raw + r * W * 4, scale = raw + kPage * W * 4 + r * groups * 2, mn = scale + kPage * groups * 2;
+    if constexpr (BITS == 3) {
+        uint32_t out[4];
+        uint32_t w[12];
+#pragma unroll
+        for (int k = 0; k < 12; ++k) w[k] = lds32(codes + 4 * k);
+        auto code = [&](int i) { return i % 11 < 10 ? (w[i / 11] >> (3 * (i % 11))) & 7u : w[i / 11] >> 30; };
+        uint32_t sc[12], lo[12];
+#pragma unroll
+        for (int k = 0; k < 12; ++k) { sc[k] = lds16(scale + 2 * k); lo[k] = lds16(mn + 2 * k); }
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+            const int a = 2 * i / 11, b = (2 * i + 1) / 11;
+            const __half2 x = __hsub2(as_h2(code(2 * i) | code(2 * i + 1) << 16 | 0x64006400u), as_h2(0x64006400u));
+            out[i & 3] = as_u32(__hfma2(x, as_h2(sc[a] | sc[b] << 16), as_h2(lo[a] | lo[b] << 16)));
+            if ((i & 3) == 3) sts128(operand_at(to, r, i >> 2), out[0], out[1], out[2], out[3]);
+        }
+    } else {
+        using F = HalfFields<2 * BITS>;                           // every other field of a half: BITS bits at multiples of 2 BITS
+        constexpr int FPI = 32 / BITS;
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const int grp = (k * FPI) >> g_log2;
+            const __half2 sc = __half2half2(__ushort_as_half((unsigned short)lds16(scale + 2 * grp))), lo = __half2half2(__ushort_as_half((unsigned short)lds16(mn + 2 * grp)));
+            const uint32_t w = lds32(codes + 4 * k), odd = w >> BITS;
+            uint32_t out[FPI / 2];                                // pairs of neighbours
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t x = prmt(w, odd, h ? 0x7632 : 0x5410);
+#pragma unroll
+                for (int i = 0; i < F::N; ++i) {
+                    constexpr int DIRECT = (10 - BITS) / (2 * BITS) + 1;
+                    const int pos = i < DIRECT ? 2 * BITS * i : 2 * BITS * (i - DIRECT);
+                    const uint32_t mask = ((1u << BITS) - 1u) << pos, expo = (uint32_t)(25 - pos) << 10;
+                    uint32_t v;
+                    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(i < DIRECT ? x : x >> (2 * BITS * DIRECT)), "r"(mask * 0x10001u), "r"(expo * 0x10001u));
+                    out[h * F::N + i] = as_u32(__hfma2(__hsub2(as_h2(v), as_h2(expo * 0x10001u)), sc, lo));
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < FPI / 8; ++c) sts128(operand_at(to, r, k * (FPI / 8) + c), out[4 * c], out[4 * c + 1], out[4 * c + 2], out[4 * c + 3]);
+        }
+    }
+}
+
+template <int KB, int VB>
+__global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __grid_constant__ PagedArgs p, int max_tiles) {
+    extern __shared__ __align__(1024) char smem[];
+    __shared__ uint32_t s_tmem;
+    // where this CTA's rows are: tiles of later tokens first, they see more
+    const int split = blockIdx.x % p.splits, hs = blockIdx.x / p.splits, head = hs % p.l.Hkv;
+    int tile = max_tiles - 1 - hs / p.l.Hkv, seq = 0;
+    for (; seq < p.a.n; ++seq) {
+        const int rows = max(0, min(p.a.q_start[seq + 1], p.a.tokens) - max(p.a.q_start[seq], 0)) * p.rep;
+        const int tiles = rows > p.few_rows ? (rows + 2 * kTileRows - 1) / (2 * kTileRows) : 0;
+        if (tile < tiles) break;
+        tile -= tiles;
+    }
+    if (seq == p.a.n) return;
+    const PagedSeq s = paged_seq(p, seq);
+    const int row0 = tile * 2 * kTileRows, rows = min(s.n_new * p.rep - row0, 2 * kTileRows), two_tiles = rows > kTileRows;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31, wg = warp >> 2;
+
+    const uint32_t base = smem_u32(smem), bars = base + kOffBar;
+    auto bar = [&](int k) { return bars + 8 * k; };
+    if (threadIdx.x == 0) {
+        mbar_init(bar(kBarQ), two_tiles ? 256 : 128);
+        for (int k = 0; k < 2; ++k) {
+            mbar_init(bar(kBarKFull + k), 1);
+            mbar_init(bar(kBarKFree + k), 1);
+            mbar_init(bar(kBarVFull + k), 1);
+            mbar_init(bar(kBarVFree + k), 1);
+            mbar_init(bar(kBarS + k), 1);
+            mbar_init(bar(kBarP + k), 128);
+            mbar_init(bar(kBarRaw + k), 1);
+        }
+        mbar_init(bar(kBarO), 1);
+        mbar_init(bar(kBarDrain), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+    }
+    // the pages that any row sees: bounds of the first and last tokens hold for those between, unless they are given token by token
+    int first = INT32_MAX, last = 0;
+    {
+        const int u0 = row0 / p.rep, u1 = (row0 + rows - 1) / p.rep;
+        for (int u = u0 + threadIdx.x; u <= u1; u += kTileThreads) {
+            int pos, lo, hi;
+            paged_bounds(p, s, u, pos, lo, hi);
+            if (lo < hi) { first = min(first, lo); last = max(last, hi); }
+        }
+        first = (int)__reduce_min_sync(0xffffffffu, (unsigned)first);
+        last = (int)__reduce_max_sync(0xffffffffu, (unsigned)last);
+        __shared__ int s_first[kTileThreads / 32], s_last[kTileThreads / 32];
+        if (lane == 0) { s_first[warp] = first; s_last[warp] = last; }
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+#pragma unroll
+        for (int w = 0; w < kTileThreads / 32; ++w) { first = min(first, s_first[w]); last = max(last, s_last[w]); }
+    }
+    const uint32_t tmem = s_tmem;
+    const int p_lo = first < last ? first / kPage : 0, p_hi = first < last ? pages_of(last) : 0, per = (p_hi - p_lo + p.splits - 1) / p.splits;
+    const int p0 = p_lo + split * per, np = max(0, min(p_hi, p0 + per) - p0);
+    int32_t *const status = &p.b.count[2];
+    auto page_id = [&](int page) {
+        const int id = s.table[page];
+        return id >= 0 && id < (page < s.packed ? p.l.n_packed : p.l.n_fp16) ? id : -1;
+    };
+
+    if (wg < 2) {
+        // ------------------------------------------------------------------ softmax, one row a thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;\n");
+        const int r = threadIdx.x & 127, idx = row0 + wg * kTileRows + r, u = idx / p.rep, h = head * p.rep + (idx - u * p.rep);
+        const bool mine = wg * kTileRows + r < rows;
+        if (wg == 0 || two_tiles) {
+            int pos = 0, lo = 0, hi = 0;
+            {
+                const __half *q = static_cast<const __half *>(p.a.q) + (int64_t)(s.q0 + u) * p.a.q_sT + (int64_t)h * p.a.q_sH;
+                const bool vec = (reinterpret_cast<uintptr_t>(p.a.q) % 16 | p.a.q_sT % 8 | p.a.q_sH % 8) == 0;
+                const uint32_t to = base + kOffQ + wg * kOperandBytes;
+#pragma unroll 4
+                for (int c = 0; c < 16; ++c) {
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (mine) {
+                        if (vec) x = *reinterpret_cast<const uint4 *>(q + 8 * c);
+                        else {
+                            alignas(16) __half y[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) y[j] = q[8 * c + j];
+                            x = *reinterpret_cast<const uint4 *>(y);
+                        }
+                    }
+                    sts128(operand_at(to, r, c), x.x, x.y, x.z, x.w);
+                }
+                fence_async();
+                mbar_arrive(bar(kBarQ));
+                if (mine) paged_bounds(p, s, u, pos, lo, hi);
+            }
+            const bool cap = p.a.softcap > 0.f, bias = p.a.slopes != nullptr, plain = !cap && !bias && p.a.softmax_scale > 0.f;
+            const float scale2 = p.a.softmax_scale * kLog2e, two = cap ? 2.f * scale2 / p.a.softcap : 0.f, cap2 = p.a.softcap * kLog2e;
+            const float slope = bias && mine ? p.a.slopes[h] * kLog2e : 0.f, mul = plain ? scale2 : 1.f;
+            const uint32_t lanes = (uint32_t)(warp & 3) << 21, t_s = tmem + wg * 128 + lanes, t_o = tmem + 256 + wg * 128 + lanes;
+            float m = -INFINITY, l = 0.f;
+            bool ok = true;
+            for (int it = 0; it < np; ++it) {
+                const int page = p0 + it, b0 = page * kPage;
+                const bool there = page_id(page) >= 0;
+                ok = mbar_wait(bar(kBarS + wg), it & 1, status);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                tc_fence_after();
+                uint32_t x[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tc_load32(x[c], t_s + 32 * c);
+                tc_wait_ld();
+                auto at = [&](int j) -> uint32_t & { return x[j >> 5][j & 31]; };
+                if (!plain) {
+#pragma unroll
+                    for (int j = 0; j < 128; ++j) {
+                        float v = __uint_as_float(at(j));
+                        v = cap ? cap_score(v, two, cap2) : v * scale2;
+                        at(j) = __float_as_uint(fmaf(slope, (float)(b0 + j - pos), v));
+                    }
+                }
+                if (!__all_sync(0xffffffffu, lo <= b0 && hi >= b0 + kPage && there)) {
+                    const int from = there ? lo - b0 : kPage, to = there ? hi - b0 : 0;
+#pragma unroll
+                    for (int j = 0; j < 128; ++j)
+                        if (j < from || j >= to) at(j) = 0xff800000u;
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < 128; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(at(j)));
+                const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mul;
+                // The reference follows the maximum only when it grows by more than 2^8: weights up to 256 are as exact in fp16, and O is
+                // rescaled a few times a row in place of at every page.
+                const bool grow = best > m + 8.f;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float f = grow ? exp2_approx(m - best) : 1.f;
+                    if (grow) m = best;
+                    l *= f;
+                    if (it > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t o[32];
+                            tc_load32(o, t_o + 32 * c);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            tc_store32(t_o + 32 * c, o);
+                        }
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.f : m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const float a = exp2_approx(fmaf(__uint_as_float(at(64 * c + 2 * j)), mul, -ref)), b = exp2_approx(fmaf(__uint_as_float(at(64 * c + 2 * j + 1)), mul, -ref));
+                        sum[2 * (j & 1)] += a;
+                        sum[2 * (j & 1) + 1] += b;
+                        w[j] = as_u32(__floats2half2_rn(a, b));
+                    }
+                    tc_store32(t_s + 32 * c, w);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(bar(kBarP + wg));
+            }
+            if (ok && np > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarO), 0, status));
+            tc_fence_after();
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            __half *out = static_cast<__half *>(p.a.out) + (int64_t)(s.q0 + u) * p.a.o_sT + (int64_t)h * p.a.o_sH;
+            const int64_t part = (int64_t)split * p.a.tokens * p.a.nh + (int64_t)(s.q0 + u) * p.a.nh + h;
+            const bool vec = (reinterpret_cast<uintptr_t>(p.a.out) % 16 | p.a.o_sT % 8 | p.a.o_sH % 8) == 0;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                uint32_t o[32];
+                __syncwarp();
+                if (np > 0) {
+                    tc_load32(o, t_o + 32 * c);
+                    tc_wait_ld();
+                }
+                if (!mine) continue;
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (np == 0 || l == 0.f) o[j] = 0;
+                if (p.splits > 1) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) reinterpret_cast<uint4 *>(p.part_out + part * 128 + 32 * c)[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                } else {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) w[j] = as_u32(__floats2half2_rn(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv));
+                    if (vec) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) reinterpret_cast<uint4 *>(out + 32 * c)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) out[32 * c + j] = __ushort_as_half((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
+                    }
+                }
+            }
+            if (mine && p.splits > 1) {
+                p.part_ml[2 * part] = m;
+                p.part_ml[2 * part + 1] = l;
+            }
+            tc_fence_before();
+        }
+    } else if (wg == 2) {
+        // ------------------------------------------------------------------ operands: job 2i is page i's keys, 2i + 1 its values
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
+        const int r = threadIdx.x & 127;
+        const int kg_log2 = KB == 3 ? 0 : 31 - __clz(p.l.group);
+        const int n_old = max(0, min(np, s.packed - p0)), jobs = 2 * np, packed_jobs = 2 * n_old;   // packed pages come first
+        auto raw_load = [&](int j) {                              // one thread
+            const bool values = j & 1;
+            const int id = page_id(p0 + (j >> 1));
+            if (id < 0) { mbar_arrive(bar(kBarRaw + (j & 1))); return; }
+            const int64_t row = ((int64_t)id * p.l.Hkv + head) * kPage;
+            const int words = values ? page_words(VB) : page_words(KB), groups = values ? p.v_groups : p.k_groups;
+            const uint32_t cb = kPage * words * 4, sz = kPage * groups * 2, dst = base + kOffRaw + (j & 1) * kRawBytes;
+            mbar_expect(bar(kBarRaw + (j & 1)), cb + 2 * sz);
+            bulk_load(dst, (values ? p.l.vcode : p.l.kcode) + row * words, cb, bar(kBarRaw + (j & 1)));
+            bulk_load(dst + cb, static_cast<const __half *>(values ? p.l.vscale : p.l.kscale) + row * groups, sz, bar(kBarRaw + (j & 1)));
+            bulk_load(dst + cb + sz, static_cast<const __half *>(values ? p.l.vmn : p.l.kmn) + row * groups, sz, bar(kBarRaw + (j & 1)));
+        };
+        auto full_bar = [&](int j) { return bar((j & 1 ? kBarVFull : kBarKFull) + (j >> 1 & 1)); };
+        auto together = [&]() { asm volatile("bar.sync 1, 128;\n" ::: "memory"); };
+        if (r == 0) {
+            if (packed_jobs > 0) raw_load(0);
+            if (packed_jobs > 1) raw_load(1);
+        }
+        bool ok = true;
+        int j = 0, raw_done = 0;
+        for (; j < packed_jobs; ++j) {
+            const uint32_t to = base + (j & 1 ? kOffV : kOffK) + (j >> 1 & 1) * kOperandBytes, raw = base + kOffRaw + (j & 1) * kRawBytes;
+            ok = ok && mbar_wait(bar((j & 1 ? kBarVFree : kBarKFree) + (j >> 1 & 1)), (j >> 2 & 1) ^ 1, status);
+            ok = ok && mbar_wait(bar(kBarRaw + (j & 1)), j >> 1 & 1, status);
+            ok = __all_sync(0xffffffffu, ok);                     // after a wait that gave up: through the barriers to the end, without work
+            if (ok) raw_done = j + 1;
+            if (!ok) {
+            } else if (page_id(p0 + (j >> 1)) < 0) {                     // nobody sees it; its operand must not be NaN
+#pragma unroll
+                for (int c = 0; c < 16; ++c) sts128(operand_at(to, r, c), 0, 0, 0, 0);
+            } else if (j & 1) {
+                unpack_row<VB>(raw, to, r, p.v_groups, kg_log2 ? kg_log2 : 31 - __clz(p.l.group));
+            } else {
+                unpack_row<KB>(raw, to, r, p.k_groups, kg_log2);
+            }
+            fence_async();
+            together();
+            if (r == 0 && ok) {
+                mbar_arrive(full_bar(j));
+                if (j + 2 < packed_jobs) raw_load(j + 2);
+            }
+        }
+        if (!ok && r == 0)                                        // raw copies in flight land before the CTA ends
+            for (int q = raw_done; q < min(packed_jobs, raw_done + 2); ++q) mbar_wait(bar(kBarRaw + (q & 1)), q >> 1 & 1, status);
+        // fp16 pages: two jobs' copies run ahead of the one that is handed over
+        constexpr int LAG = 2;
+        for (int issue = j; j < jobs; ++issue) {
+            if (issue < jobs) {
+                const int page = p0 + (issue >> 1), id = page_id(page), there = min(kPage, s.length - page * kPage);
+                const uint32_t to = base + (issue & 1 ? kOffV : kOffK) + (issue >> 1 & 1) * kOperandBytes;
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(bar((issue & 1 ? kBarVFree : kBarKFree) + (issue >> 1 & 1)), (issue >> 2 & 1) ^ 1, status));
+                const __half *src = static_cast<const __half *>(issue & 1 ? p.l.vfull : p.l.kfull) + ((int64_t)max(id, 0) * p.l.Hkv + head) * kPageHalf;
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {                    // eight rows of 16 pieces a turn; rows behind the last token become zero
+                    const int row = c * 8 + (r >> 4), piece = r & 15;
+                    if (!ok) break;
+                    if (id >= 0 && row < there) cp_async<16>(operand_at(to, row, piece), src + row * kHeadDim + piece * 8);
+                    else sts128(operand_at(to, row, piece), 0, 0, 0, 0);
+                }
+            }
+            cp_async_commit();
+            if (issue - j < LAG) continue;
+            cp_async_wait<LAG>();
+            fence_async();
+            together();
+            if (r == 0 && ok) mbar_arrive(full_bar(j));
+            ++j;
+        }
+        cp_async_wait<0>();
+    } else {
+        // ------------------------------------------------------------------ MMAs
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
+        if (warp == 12 && lane == 0) {
+            const int n_old = s.packed - p0;
+            bool ok = np == 0 || mbar_wait(bar(kBarQ), 0, status);
+            auto scores = [&](int it, int w) {                    // S[w] = Q[w] K^T of page `it`
+                const uint32_t q = base + kOffQ + w * kOperandBytes, k = base + kOffK + (it & 1) * kOperandBytes;
+                const bool packed = it < n_old;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint64_t a = tc_desc(q + (e >> 2) * kOperandHalf + (e & 3) * 32, 16, 1024);
+                    const uint64_t b = packed ? tc_desc(k + e * 2048, kOperandHalf, 1024) : tc_desc(k + (e >> 2) * kOperandHalf + (e & 3) * 32, 16, 1024);
+                    tc_mma(tmem + w * 128, a, b, packed ? kIdescMn : kIdesc, e > 0);
+                }
+                tc_commit(bar(kBarS + w));
+            };
+            auto values = [&](int it, int w) {                    // O[w] += P[w] V
+                const uint32_t v = base + kOffV + (it & 1) * kOperandBytes;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    tc_mma_tmem(tmem + 256 + w * 128, tmem + w * 128 + e * 8, tc_desc(v + e * 2048, kOperandHalf, 1024), kIdescMn, it > 0 || e > 0);
+            };
+            const int tiles = two_tiles ? 2 : 1;
+            if (ok && np > 0) {
+                ok = mbar_wait(bar(kBarKFull), 0, status);
+                if (ok) {
+                    tc_fence_after();
+                    for (int w = 0; w < tiles; ++w) scores(0, w);
+                    tc_commit(bar(kBarKFree));
+                }
+            }
+            for (int it = 0; ok && it < np; ++it) {
+                ok = mbar_wait(bar(kBarVFull + (it & 1)), it >> 1 & 1, status);
+                if (ok && it + 1 < np) ok = mbar_wait(bar(kBarKFull + (it + 1 & 1)), (it + 1) >> 1 & 1, status);
+                for (int w = 0; ok && w < tiles; ++w) {
+                    ok = mbar_wait(bar(kBarP + w), it & 1, status);
+                    if (!ok) break;
+                    tc_fence_after();
+                    values(it, w);
+                    if (it + 1 < np) scores(it + 1, w);
+                }
+                if (!ok) break;
+                tc_commit(bar(kBarVFree + (it & 1)));
+                if (it + 1 < np) tc_commit(bar(kBarKFree + (it + 1 & 1)));
+            }
+            if (ok && np > 0) tc_commit(bar(kBarO));
+            tc_commit(bar(kBarDrain));                            // whatever was begun is done before the memory is given up
+            mbar_wait(bar(kBarDrain), 0, status);
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
+    }
+}
+
+template <int KB, int VB>
+static int launch_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
+    const cudaError_t e = cudaFuncSetAttribute(paged_tile_kernel<KB, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem);
+    if (e != cudaSuccess) return record_cuda_error(e);
+    const int64_t grid = (int64_t)max_tiles * p.l.Hkv * p.splits;
+    if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
+    if (grid == 0) return KVQ_OK;
+    paged_tile_kernel<KB, VB><<<(unsigned)grid, kTileThreads, kTileSmem, st>>>(p, max_tiles);
+    return check_launch();
+}
+
+int paged_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
+#define KVQ_V(KB)                                                                                                             \
+    switch (p.l.v_bits) {                                                                                                     \
+        case 1: return launch_tiles<KB, 1>(p, max_tiles, st);                                                                 \
+        case 2: return launch_tiles<KB, 2>(p, max_tiles, st);                                                                 \
+        case 3: return launch_tiles<KB, 3>(p, max_tiles, st);                                                                 \
+        default: return launch_tiles<KB, 4>(p, max_tiles, st);                                                                \
+    }
+    switch (p.l.k_bits) {
+        case 1: KVQ_V(1)
+        case 2: KVQ_V(2)
+        case 3: KVQ_V(3)
+        default: KVQ_V(4)
+    }
+#undef KVQ_V
+}
+
+}  // namespace kvq
