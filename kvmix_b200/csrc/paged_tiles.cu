@@ -1,5 +1,8 @@
 // Attention of many query rows of a kv head (chunks of prompts, the tokens of a speculative step) over a paged cache, on tcgen05.
 #include "paged_attn.cuh"
+#include "quant_core.cuh"
+
+#include <cuda.h>
 
 namespace kvq {
 
@@ -16,22 +19,38 @@ namespace kvq {
 // their fields lie side by side and nothing is transposed.
 // Packed rows become fp16 as code * scale + minimum with one rounding (2^-11 relative): the tensor core takes no wider operand without
 // half its rate.
+#ifndef POLY
+#define POLY 8
+#endif
+constexpr int kPolyOf = POLY;
 constexpr int kTileRows = 128, kTileThreads = 512;
 constexpr uint32_t kOperandBytes = 32768, kOperandHalf = 16384;
 constexpr int kRawBytes = 12288;                                  // the largest packed half of a page: 3 bits, or 4 bits and groups of 32
 // shared memory, from a 1024-byte boundary
 constexpr uint32_t kOffQ = 0, kOffK = 2 * kOperandBytes, kOffV = kOffK + 2 * kOperandBytes, kOffRaw = kOffV + 2 * kOperandBytes,
                    kOffBar = kOffRaw + 2 * kRawBytes, kTileSmem = kOffBar + 256;
-// barriers
-constexpr int kBarQ = 0, kBarKFull = 1, kBarKFree = 3, kBarVFull = 5, kBarVFree = 7, kBarS = 9, kBarP = 11, kBarO = 13, kBarRaw = 14, kBarDrain = 16;
+// barriers; kBarP: tile and half of the page's tokens
+constexpr int kBarQ = 0, kBarKFull = 1, kBarKFree = 3, kBarVFull = 5, kBarVFree = 7, kBarS = 9, kBarP = 11, kBarO = 15, kBarRaw = 16, kBarRawFree = 18, kBarDrain = 20, kBarTail = 21;
+
+// fp16 pages as rows of 128 channels, for copies of 64 channels x 128 rows that swizzle on the way
+struct PagedMaps {
+    CUtensorMap k, v;
+    int there;                        // whether they are (pools of 2^31 rows and more have none)
+};
+__device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
+// One thread (`lead`) issues an MMA or a commit, but its whole warp walks there with values that are the same in all lanes: operands then
+// stand in uniform registers, where these instructions want them.  In a branch of that thread alone each descriptor was moved there
+// word by word: a page took 4400 cycles and %s so.
+__device__ __forceinline__ void tc_commit(uint32_t bar, uint32_t lead) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %1, 0;\n@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar), "r"(lead) : "memory");
 }
 // Operand descriptor: swizzle of 128 bytes; `lbo`, `sbo` in bytes (see the layouts above).
 __device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
@@ -40,11 +59,11 @@ __device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lbo, uint32_
 // fp16 x fp16 -> fp32, M = N = 128; bit 16: B is MN-major
 constexpr uint32_t kIdesc = 1u << 4 | (128u >> 3) << 17 | (128u >> 4) << 24, kIdescMn = kIdesc | 1u << 16;
 
-__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add, uint32_t lead) {
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %4, 0;\nsetp.ne.u32 q, %5, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void tc_mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+__device__ __forceinline__ void tc_mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add, uint32_t lead) {
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %4, 0;\nsetp.ne.u32 q, %5, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(lead) : "memory");
 }
 
 #define KVQ_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
@@ -66,56 +85,77 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
 }
 
 // One packed row -> 128 fp16 of an operand row.
-template <int BITS>
-__device__ __forceinline__ void unpack_row(uint32_t raw, uint32_t to, int r, int groups, int g_log2) {
+template <int BITS, int NG>
+__device__ __forceinline__ void unpack_row(uint32_t raw, uint32_t to, int r) {
     constexpr int W = page_words(BITS);
-    const uint32_t codes = raw + r * W * 4, scale = raw + kPage * W * 4 + r * groups * 2, mn = scale + kPage * groups * 2;
+    const uint32_t codes = raw + r * W * 4, scale = raw + kPage * W * 4 + r * NG * 2, mn = scale + kPage * NG * 2;
+    uint32_t w[W];
+#pragma unroll
+    for (int k = 0; k < W; k += 4) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(w[k]), "=r"(w[k + 1]), "=r"(w[k + 2]), "=r"(w[k + 3]) : "r"(codes + 4 * k));
+    uint32_t sc[NG], lo[NG];                                      // both halves alike
+#pragma unroll
+    for (int k = 0; k < NG; ++k) { sc[k] = lds16(scale + 2 * k) * 0x10001u; lo[k] = lds16(mn + 2 * k) * 0x10001u; }
+    uint32_t out[4];
     if constexpr (BITS == 3) {
-        uint32_t out[4];
-        uint32_t w[12];
-#pragma unroll
-        for (int k = 0; k < 12; ++k) w[k] = lds32(codes + 4 * k);
         auto code = [&](int i) { return i % 11 < 10 ? (w[i / 11] >> (3 * (i % 11))) & 7u : w[i / 11] >> 30; };
-        uint32_t sc[12], lo[12];
-#pragma unroll
-        for (int k = 0; k < 12; ++k) { sc[k] = lds16(scale + 2 * k); lo[k] = lds16(mn + 2 * k); }
 #pragma unroll
         for (int i = 0; i < 64; ++i) {
             const int a = 2 * i / 11, b = (2 * i + 1) / 11;
             const __half2 x = __hsub2(as_h2(code(2 * i) | code(2 * i + 1) << 16 | 0x64006400u), as_h2(0x64006400u));
-            out[i & 3] = as_u32(__hfma2(x, as_h2(sc[a] | sc[b] << 16), as_h2(lo[a] | lo[b] << 16)));
+            const uint32_t s2 = a == b ? sc[a] : prmt(sc[a], sc[b], 0x5410), l2 = a == b ? lo[a] : prmt(lo[a], lo[b], 0x5410);
+            out[i & 3] = as_u32(__hfma2(x, as_h2(s2), as_h2(l2)));
             if ((i & 3) == 3) sts128(operand_at(to, r, i >> 2), out[0], out[1], out[2], out[3]);
         }
     } else {
-        using F = HalfFields<2 * BITS>;                           // every other field of a half: BITS bits at multiples of 2 BITS
-        constexpr int FPI = 32 / BITS;
+        constexpr int PAIRS = 8 / BITS, DIRECT = (10 - BITS) / (2 * BITS) + 1;      // pairs of neighbours in a half word; in reach without a shift
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-            const int grp = (k * FPI) >> g_log2;
-            const __half2 sc = __half2half2(__ushort_as_half((unsigned short)lds16(scale + 2 * grp))), lo = __half2half2(__ushort_as_half((unsigned short)lds16(mn + 2 * grp)));
-            const uint32_t w = lds32(codes + 4 * k), odd = w >> BITS;
-            uint32_t out[FPI / 2];                                // pairs of neighbours
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t x = prmt(w, odd, h ? 0x7632 : 0x5410);
-#pragma unroll
-                for (int i = 0; i < F::N; ++i) {
-                    constexpr int DIRECT = (10 - BITS) / (2 * BITS) + 1;
-                    const int pos = i < DIRECT ? 2 * BITS * i : 2 * BITS * (i - DIRECT);
-                    const uint32_t mask = ((1u << BITS) - 1u) << pos, expo = (uint32_t)(25 - pos) << 10;
-                    uint32_t v;
-                    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(i < DIRECT ? x : x >> (2 * BITS * DIRECT)), "r"(mask * 0x10001u), "r"(expo * 0x10001u));
-                    out[h * F::N + i] = as_u32(__hfma2(__hsub2(as_h2(v), as_h2(expo * 0x10001u)), sc, lo));
-                }
-            }
-#pragma unroll
-            for (int c = 0; c < FPI / 8; ++c) sts128(operand_at(to, r, k * (FPI / 8) + c), out[4 * c], out[4 * c + 1], out[4 * c + 2], out[4 * c + 3]);
+        for (int i = 0; i < 64; ++i) {                            // elements 2i, 2i + 1
+            const int half = i / PAIRS, f = i % PAIRS, k = half / 2, g = 2 * i / (kPage / NG);
+            const uint32_t x = prmt(w[k], w[k] >> BITS, half & 1 ? 0x7632 : 0x5410);
+            const int pos = f < DIRECT ? 2 * BITS * f : 2 * BITS * (f - DIRECT);
+            const uint32_t mask = ((1u << BITS) - 1u) << pos, expo = (uint32_t)(25 - pos) << 10;
+            uint32_t v;
+            asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(f < DIRECT ? x : x >> (2 * BITS * DIRECT)), "r"(mask * 0x10001u), "r"(expo * 0x10001u));
+            out[i & 3] = as_u32(__hfma2(__hsub2(as_h2(v), as_h2(expo * 0x10001u)), as_h2(sc[g]), as_h2(lo[g])));
+            if ((i & 3) == 3) sts128(operand_at(to, r, i >> 2), out[0], out[1], out[2], out[3]);
         }
     }
 }
+template <int BITS>
+__device__ __forceinline__ void unpack_row(uint32_t raw, uint32_t to, int r, int groups) {
+    if constexpr (BITS == 3) {
+        unpack_row<3, 12>(raw, to, r);
+    } else {
+        if (groups == 1) unpack_row<BITS, 1>(raw, to, r);
+        else if (groups == 2) unpack_row<BITS, 2>(raw, to, r);
+        else unpack_row<BITS, 4>(raw, to, r);
+    }
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of two x <= some tens without the special function unit: x = n + f, n the nearest integer (by adding 1.5 * 2^23), |f| <= 0.5; 2^f by
+// the polynomial below, n into the exponent.  Below -126: 2^-126, which fp16 weights and fp32 sums do not feel.  NaN comes out as a number.
+__device__ __forceinline__ float2 exp2_poly(unsigned long long x) {
+    float2 c = f32x2_split(x);
+    c.x = fmaxf(c.x, -126.f);
+    c.y = fmaxf(c.y, -126.f);
+    x = f32x2(c.x, c.y);
+    const unsigned long long magic = f32x2(12582912.f, 12582912.f), n = add_f32x2(x, magic);
+    const unsigned long long f = add_f32x2(x, mul_f32x2(add_f32x2(n, f32x2(-12582912.f, -12582912.f)), f32x2(-1.f, -1.f)));
+    constexpr float C[5] = {0.999999261f, 0.693121815f, 0.240247448f, 0.0559178603f, 0.00957010191f};      // minimax in relative error, 2.6e-6 (the weights keep 2^-11), by a Remez exchange
+    unsigned long long p = f32x2(C[4], C[4]);
+#pragma unroll
+    for (int i = 3; i >= 0; --i) p = fma_f32x2(p, f, f32x2(C[i], C[i]));
+    const float2 q = f32x2_split(p), m = f32x2_split(n);
+    return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(m.x) << 23)), __int_as_float(__float_as_int(q.y) + (__float_as_int(m.y) << 23)));
+}
 
 template <int KB, int VB>
-__global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __grid_constant__ PagedArgs p, int max_tiles) {
+__global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ PagedMaps maps, int max_tiles) {
     extern __shared__ __align__(1024) char smem[];
     __shared__ uint32_t s_tmem;
     // where this CTA's rows are: tiles of later tokens first, they see more
@@ -142,9 +182,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             mbar_init(bar(kBarVFull + k), 1);
             mbar_init(bar(kBarVFree + k), 1);
             mbar_init(bar(kBarS + k), 1);
-            mbar_init(bar(kBarP + k), 128);
+            mbar_init(bar(kBarP + 2 * k), 128);
+            mbar_init(bar(kBarP + 2 * k + 1), 128);
             mbar_init(bar(kBarRaw + k), 1);
+            mbar_init(bar(kBarRawFree + k), 1);
         }
+        for (int k = 0; k < 4; ++k) mbar_init(bar(kBarTail + k), 1);
         mbar_init(bar(kBarO), 1);
         mbar_init(bar(kBarDrain), 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -180,6 +223,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         const int id = s.table[page];
         return id >= 0 && id < (page < s.packed ? p.l.n_packed : p.l.n_fp16) ? id : -1;
     };
+
+    // Whether a full fp16 page comes by the loader's copies.  The others are filled by the warpgroup that unpacks, at the loader's word: a
+    // barrier's parity tells a phase from the one before only, so whoever waits by it has to see every phase, and for the buffers of fp16
+    // pages that is the loader.
+    auto by_loader = [&](int page, int id) { return maps.there && (page + 1) * kPage <= s.length && id >= 0; };
 
     if (wg < 2) {
         // ------------------------------------------------------------------ softmax, one row a thread
@@ -243,8 +291,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int j = 0; j < 128; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(at(j)));
-                const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mul;
+                for (int j = 0; j < 128; j += 2) top[j >> 1 & 3] = max3(top[j >> 1 & 3], __uint_as_float(at(j)), __uint_as_float(at(j + 1)));
+                const float best = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * mul;
+                if (best != best) l = best;                       // a score is not a number: neither is the row
                 // The reference follows the maximum only when it grows by more than 2^8: weights up to 256 are as exact in fp16, and O is
                 // rescaled a few times a row in place of at every page.
                 const bool grow = best > m + 8.f;
@@ -265,23 +314,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                unsigned long long sum[2] = {0ull, 0ull};
+                const unsigned long long mul2 = f32x2(mul, mul), ref2 = f32x2(-ref, -ref);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     uint32_t w[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
-                        const float a = exp2_approx(fmaf(__uint_as_float(at(64 * c + 2 * j)), mul, -ref)), b = exp2_approx(fmaf(__uint_as_float(at(64 * c + 2 * j + 1)), mul, -ref));
-                        sum[2 * (j & 1)] += a;
-                        sum[2 * (j & 1) + 1] += b;
-                        w[j] = as_u32(__floats2half2_rn(a, b));
+                        const unsigned long long e = fma_f32x2(f32x2(__uint_as_float(at(64 * c + 2 * j)), __uint_as_float(at(64 * c + 2 * j + 1))), mul2, ref2);
+                        float2 v;
+                        if (j % kPolyOf == kPolyOf - 1) {         // some of the exponentials on the FMA pipe
+                            v = exp2_poly(e);
+                        } else {
+                            v = f32x2_split(e);
+                            v.x = exp2_approx(v.x);
+                            v.y = exp2_approx(v.y);
+                        }
+                        sum[j & 1] = add_f32x2(sum[j & 1], f32x2(v.x, v.y));
+                        w[j] = as_u32(__floats2half2_rn(v.x, v.y));
                     }
                     tc_store32(t_s + 32 * c, w);
+                    tc_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(bar(kBarP + 2 * wg + c));
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tc_wait_st();
-                tc_fence_before();
-                mbar_arrive(bar(kBarP + wg));
+                const float2 both = f32x2_split(add_f32x2(sum[0], sum[1]));
+                l += both.x + both.y;
             }
             if (ok && np > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarO), 0, status));
             tc_fence_after();
@@ -324,129 +382,143 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             tc_fence_before();
         }
     } else if (wg == 2) {
-        // ------------------------------------------------------------------ operands: job 2i is page i's keys, 2i + 1 its values
+        // ------------------------------------------------------------------ operands: job 2i is page i's keys, 2i + 1 its values.  Packed
+        // ones are unpacked here, and the fp16 page that holds the sequence's end is copied here, with zeros behind the end.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
         const int r = threadIdx.x & 127;
-        const int kg_log2 = KB == 3 ? 0 : 31 - __clz(p.l.group);
-        const int n_old = max(0, min(np, s.packed - p0)), jobs = 2 * np, packed_jobs = 2 * n_old;   // packed pages come first
-        auto raw_load = [&](int j) {                              // one thread
-            const bool values = j & 1;
-            const int id = page_id(p0 + (j >> 1));
-            if (id < 0) { mbar_arrive(bar(kBarRaw + (j & 1))); return; }
-            const int64_t row = ((int64_t)id * p.l.Hkv + head) * kPage;
-            const int words = values ? page_words(VB) : page_words(KB), groups = values ? p.v_groups : p.k_groups;
-            const uint32_t cb = kPage * words * 4, sz = kPage * groups * 2, dst = base + kOffRaw + (j & 1) * kRawBytes;
-            mbar_expect(bar(kBarRaw + (j & 1)), cb + 2 * sz);
-            bulk_load(dst, (values ? p.l.vcode : p.l.kcode) + row * words, cb, bar(kBarRaw + (j & 1)));
-            bulk_load(dst + cb, static_cast<const __half *>(values ? p.l.vscale : p.l.kscale) + row * groups, sz, bar(kBarRaw + (j & 1)));
-            bulk_load(dst + cb + sz, static_cast<const __half *>(values ? p.l.vmn : p.l.kmn) + row * groups, sz, bar(kBarRaw + (j & 1)));
-        };
-        auto full_bar = [&](int j) { return bar((j & 1 ? kBarVFull : kBarKFull) + (j >> 1 & 1)); };
-        auto together = [&]() { asm volatile("bar.sync 1, 128;\n" ::: "memory"); };
-        if (r == 0) {
-            if (packed_jobs > 0) raw_load(0);
-            if (packed_jobs > 1) raw_load(1);
-        }
         bool ok = true;
-        int j = 0, raw_done = 0;
-        for (; j < packed_jobs; ++j) {
+        uint32_t tails = 0;
+        for (int j = 0; j < 2 * np; ++j) {
+            const int page = p0 + (j >> 1);
+            const bool packed = page < s.packed;
+            const int id = page_id(page);
+            if (!packed && by_loader(page, id)) continue;
             const uint32_t to = base + (j & 1 ? kOffV : kOffK) + (j >> 1 & 1) * kOperandBytes, raw = base + kOffRaw + (j & 1) * kRawBytes;
-            ok = ok && mbar_wait(bar((j & 1 ? kBarVFree : kBarKFree) + (j >> 1 & 1)), (j >> 2 & 1) ^ 1, status);
-            ok = ok && mbar_wait(bar(kBarRaw + (j & 1)), j >> 1 & 1, status);
-            ok = __all_sync(0xffffffffu, ok);                     // after a wait that gave up: through the barriers to the end, without work
-            if (ok) raw_done = j + 1;
-            if (!ok) {
-            } else if (page_id(p0 + (j >> 1)) < 0) {                     // nobody sees it; its operand must not be NaN
-#pragma unroll
-                for (int c = 0; c < 16; ++c) sts128(operand_at(to, r, c), 0, 0, 0, 0);
-            } else if (j & 1) {
-                unpack_row<VB>(raw, to, r, p.v_groups, kg_log2 ? kg_log2 : 31 - __clz(p.l.group));
+            if (packed) {
+                ok = ok && mbar_wait(bar((j & 1 ? kBarVFree : kBarKFree) + (j >> 1 & 1)), (j >> 2 & 1) ^ 1, status);
+                ok = ok && mbar_wait(bar(kBarRaw + (j & 1)), j >> 1 & 1, status);
             } else {
-                unpack_row<KB>(raw, to, r, p.k_groups, kg_log2);
+                ok = ok && mbar_wait(bar(kBarTail + (j & 3)), tails >> (j & 3) & 1, status);
+                tails ^= 1u << (j & 3);
             }
-            fence_async();
-            together();
-            if (r == 0 && ok) {
-                mbar_arrive(full_bar(j));
-                if (j + 2 < packed_jobs) raw_load(j + 2);
-            }
-        }
-        if (!ok && r == 0)                                        // raw copies in flight land before the CTA ends
-            for (int q = raw_done; q < min(packed_jobs, raw_done + 2); ++q) mbar_wait(bar(kBarRaw + (q & 1)), q >> 1 & 1, status);
-        // fp16 pages: two jobs' copies run ahead of the one that is handed over
-        constexpr int LAG = 2;
-        for (int issue = j; j < jobs; ++issue) {
-            if (issue < jobs) {
-                const int page = p0 + (issue >> 1), id = page_id(page), there = min(kPage, s.length - page * kPage);
-                const uint32_t to = base + (issue & 1 ? kOffV : kOffK) + (issue >> 1 & 1) * kOperandBytes;
-                ok = __all_sync(0xffffffffu, ok && mbar_wait(bar((issue & 1 ? kBarVFree : kBarKFree) + (issue >> 1 & 1)), (issue >> 2 & 1) ^ 1, status));
-                const __half *src = static_cast<const __half *>(issue & 1 ? p.l.vfull : p.l.kfull) + ((int64_t)max(id, 0) * p.l.Hkv + head) * kPageHalf;
-#pragma unroll
-                for (int c = 0; c < 16; ++c) {                    // eight rows of 16 pieces a turn; rows behind the last token become zero
+            ok = __all_sync(0xffffffffu, ok);                     // after a wait that gave up: through the barriers to the end, without work
+            if (!ok) {
+            } else if (packed && id >= 0) {
+                if (j & 1) unpack_row<VB>(raw, to, r, p.v_groups);
+                else unpack_row<KB>(raw, to, r, p.k_groups);
+            } else {
+                const __half *src = static_cast<const __half *>(j & 1 ? p.l.vfull : p.l.kfull) + ((int64_t)max(id, 0) * p.l.Hkv + head) * kPageHalf;
+                const int there = id >= 0 ? min(kPage, s.length - page * kPage) : 0;      // a page without a number: zeros
+#pragma unroll 4
+                for (int c = 0; c < 16; ++c) {                    // eight rows of 16 pieces a turn
                     const int row = c * 8 + (r >> 4), piece = r & 15;
-                    if (!ok) break;
-                    if (id >= 0 && row < there) cp_async<16>(operand_at(to, row, piece), src + row * kHeadDim + piece * 8);
-                    else sts128(operand_at(to, row, piece), 0, 0, 0, 0);
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (row < there) x = *reinterpret_cast<const uint4 *>(src + row * kHeadDim + piece * 8);
+                    sts128(operand_at(to, row, piece), x.x, x.y, x.z, x.w);
                 }
             }
-            cp_async_commit();
-            if (issue - j < LAG) continue;
-            cp_async_wait<LAG>();
             fence_async();
-            together();
-            if (r == 0 && ok) mbar_arrive(full_bar(j));
-            ++j;
+            asm volatile("bar.sync 1, 128;\n" ::: "memory");
+            if (r == 0 && ok) {
+                mbar_arrive(bar((j & 1 ? kBarVFull : kBarKFull) + (j >> 1 & 1)));
+                if (packed) mbar_arrive(bar(kBarRawFree + (j & 1)));
+            }
         }
-        cp_async_wait<0>();
     } else {
         // ------------------------------------------------------------------ MMAs
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
-        if (warp == 12 && lane == 0) {
-            const int n_old = s.packed - p0;
-            bool ok = np == 0 || mbar_wait(bar(kBarQ), 0, status);
+        if (warp == 12) {
+            uint32_t lead;
+            asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
+            auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+            const int n_old = same(s.packed - p0), pages = same(np), tiles = same(two_tiles) ? 2 : 1;            // n_old: pages of packed keys
+            const uint32_t tm = (uint32_t)same((int)tmem);
+            const uint64_t q_desc = tc_desc(base + kOffQ, 16, 1024), k_desc = tc_desc(base + kOffK, 16, 1024), k_mn = tc_desc(base + kOffK, kOperandHalf, 1024),
+                           v_desc = tc_desc(base + kOffV, kOperandHalf, 1024);
+            auto wait = [&](int b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar(b), parity, status)); };
+            bool ok = pages == 0 || wait(kBarQ, 0);
+            // the address fields of descriptors count 16 bytes, and no operand's end carries out of them
             auto scores = [&](int it, int w) {                    // S[w] = Q[w] K^T of page `it`
-                const uint32_t q = base + kOffQ + w * kOperandBytes, k = base + kOffK + (it & 1) * kOperandBytes;
-                const bool packed = it < n_old;
+                const uint64_t q = q_desc + w * (kOperandBytes / 16);
+                const uint32_t stage = (it & 1) * (kOperandBytes / 16);
+                if (it < n_old) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint64_t a = tc_desc(q + (e >> 2) * kOperandHalf + (e & 3) * 32, 16, 1024);
-                    const uint64_t b = packed ? tc_desc(k + e * 2048, kOperandHalf, 1024) : tc_desc(k + (e >> 2) * kOperandHalf + (e & 3) * 32, 16, 1024);
-                    tc_mma(tmem + w * 128, a, b, packed ? kIdescMn : kIdesc, e > 0);
+                    for (int e = 0; e < 8; ++e) tc_mma(tm + w * 128, q + (e >> 2) * (kOperandHalf / 16) + (e & 3) * 2, k_mn + stage + e * 128, kIdescMn, e > 0, lead);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        tc_mma(tm + w * 128, q + (e >> 2) * (kOperandHalf / 16) + (e & 3) * 2, k_desc + stage + (e >> 2) * (kOperandHalf / 16) + (e & 3) * 2, kIdesc, e > 0, lead);
                 }
-                tc_commit(bar(kBarS + w));
+                tc_commit(bar(kBarS + w), lead);
             };
-            auto values = [&](int it, int w) {                    // O[w] += P[w] V
-                const uint32_t v = base + kOffV + (it & 1) * kOperandBytes;
+            auto values = [&](int it, int w, int half) {          // O[w] += P[w] V, half of the tokens
+                const uint64_t v = v_desc + (it & 1) * (kOperandBytes / 16) + half * 512;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    tc_mma_tmem(tmem + 256 + w * 128, tmem + w * 128 + e * 8, tc_desc(v + e * 2048, kOperandHalf, 1024), kIdescMn, it > 0 || e > 0);
+                for (int e = 0; e < 4; ++e) tc_mma_tmem(tm + 256 + w * 128, tm + w * 128 + half * 32 + e * 8, v + e * 128, kIdescMn, it > 0 || half > 0 || e > 0, lead);
             };
-            const int tiles = two_tiles ? 2 : 1;
-            if (ok && np > 0) {
-                ok = mbar_wait(bar(kBarKFull), 0, status);
+            if (ok && pages > 0) {
+                ok = wait(kBarKFull, 0);
                 if (ok) {
                     tc_fence_after();
                     for (int w = 0; w < tiles; ++w) scores(0, w);
-                    tc_commit(bar(kBarKFree));
+                    tc_commit(bar(kBarKFree), lead);
                 }
             }
-            for (int it = 0; ok && it < np; ++it) {
-                ok = mbar_wait(bar(kBarVFull + (it & 1)), it >> 1 & 1, status);
-                if (ok && it + 1 < np) ok = mbar_wait(bar(kBarKFull + (it + 1 & 1)), (it + 1) >> 1 & 1, status);
+            for (int it = 0; ok && it < pages; ++it) {
+                ok = wait(kBarVFull + (it & 1), it >> 1 & 1);
                 for (int w = 0; ok && w < tiles; ++w) {
-                    ok = mbar_wait(bar(kBarP + w), it & 1, status);
-                    if (!ok) break;
-                    tc_fence_after();
-                    values(it, w);
-                    if (it + 1 < np) scores(it + 1, w);
+                    for (int half = 0; ok && half < 2; ++half) {
+                        ok = wait(kBarP + 2 * w + half, it & 1);
+                        tc_fence_after();
+                        if (ok) values(it, w, half);
+                    }
+                    if (ok && w == tiles - 1) tc_commit(bar(kBarVFree + (it & 1)), lead);
+                    if (ok && it + 1 < pages && w == 0) ok = wait(kBarKFull + (it + 1 & 1), (it + 1) >> 1 & 1);
+                    if (ok && it + 1 < pages) scores(it + 1, w);
                 }
                 if (!ok) break;
-                tc_commit(bar(kBarVFree + (it & 1)));
-                if (it + 1 < np) tc_commit(bar(kBarKFree + (it + 1 & 1)));
+                if (it + 1 < pages) tc_commit(bar(kBarKFree + (it + 1 & 1)), lead);
             }
-            if (ok && np > 0) tc_commit(bar(kBarO));
-            tc_commit(bar(kBarDrain));                            // whatever was begun is done before the memory is given up
-            mbar_wait(bar(kBarDrain), 0, status);
+            if (ok && pages > 0) tc_commit(bar(kBarO), lead);
+            tc_commit(bar(kBarDrain), lead);                      // whatever was begun is done before the memory is given up
+            wait(kBarDrain, 0);
+        } else if (warp == 13 && lane == 0) {
+            // -------------------------------------------------------------- copies: packed pages as they are, fp16 pages into their operands
+            bool ok = true;
+            int j = 0, next = np > 0 ? page_id(p0) : -1, id = -1;
+            auto landed = [&](int q) { return p0 + (q >> 1) < s.packed ? bar(kBarRaw + (q & 1)) : bar((q & 1 ? kBarVFull : kBarKFull) + (q >> 1 & 1)); };
+            for (; ok && j < 2 * np; ++j) {
+                const int page = p0 + (j >> 1);
+                const bool values = j & 1;
+                if (!values) {
+                    id = next;
+                    if (page + 1 < p0 + np) next = page_id(page + 1);
+                }
+                const uint32_t full = landed(j);
+                if (page < s.packed) {
+                    ok = mbar_wait(bar(kBarRawFree + (j & 1)), (j >> 1 & 1) ^ 1, status);
+                    if (!ok) break;
+                    if (id < 0) { mbar_arrive(full); continue; }
+                    const int64_t row = ((int64_t)id * p.l.Hkv + head) * kPage;
+                    const int words = values ? page_words(VB) : page_words(KB), groups = values ? p.v_groups : p.k_groups;
+                    const uint32_t cb = kPage * words * 4, sz = kPage * groups * 2, dst = base + kOffRaw + (j & 1) * kRawBytes;
+                    mbar_expect(full, cb + 2 * sz);
+                    bulk_load(dst, (values ? p.l.vcode : p.l.kcode) + row * words, cb, full);
+                    bulk_load(dst + cb, static_cast<const __half *>(values ? p.l.vscale : p.l.kscale) + row * groups, sz, full);
+                    bulk_load(dst + cb + sz, static_cast<const __half *>(values ? p.l.vmn : p.l.kmn) + row * groups, sz, full);
+                } else {
+                    ok = mbar_wait(bar((values ? kBarVFree : kBarKFree) + (j >> 1 & 1)), (j >> 2 & 1) ^ 1, status);
+                    if (!ok) break;
+                    if (!by_loader(page, id)) { mbar_arrive(bar(kBarTail + (j & 3))); continue; }
+                    const uint32_t dst = base + (values ? kOffV : kOffK) + (j >> 1 & 1) * kOperandBytes;
+                    const int y = (id * p.l.Hkv + head) * kPage;
+                    mbar_expect(full, kOperandBytes);
+                    tile_load(dst, values ? &maps.v : &maps.k, 0, y, full);
+                    tile_load(dst + kOperandHalf, values ? &maps.v : &maps.k, 64, y, full);
+                }
+            }
+            if (!ok)                                              // copies in flight land before the CTA ends
+                for (int q = max(0, j - 4); q < j; ++q) mbar_wait(landed(q), p0 + (q >> 1) < s.packed ? q >> 1 & 1 : q >> 2 & 1, status);
         }
         __syncwarp();
     }
@@ -457,6 +529,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     }
 }
 
+// The rows of a pool of fp16 pages as a tensor map.  The encoder is the driver's; the library links the runtime only.
+static bool page_map(CUtensorMap *map, void *base, int64_t rows) {
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
+                                CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<Encode>(f);
+    }();
+    if (!encode || rows <= 0 || rows >= 1LL << 31) return false;
+    const cuuint64_t sizes[2] = {kHeadDim, (cuuint64_t)rows}, strides[1] = {kHeadDim * 2};
+    const cuuint32_t box[2] = {64, kPage}, step[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, sizes, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int KB, int VB>
 static int launch_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
     const cudaError_t e = cudaFuncSetAttribute(paged_tile_kernel<KB, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem);
@@ -464,7 +553,10 @@ static int launch_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
     const int64_t grid = (int64_t)max_tiles * p.l.Hkv * p.splits;
     if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
     if (grid == 0) return KVQ_OK;
-    paged_tile_kernel<KB, VB><<<(unsigned)grid, kTileThreads, kTileSmem, st>>>(p, max_tiles);
+    PagedMaps maps = {};
+    const int64_t rows = (int64_t)p.l.n_fp16 * p.l.Hkv * kPage;
+    maps.there = page_map(&maps.k, p.l.kfull, rows) && page_map(&maps.v, p.l.vfull, rows);
+    paged_tile_kernel<KB, VB><<<(unsigned)grid, kTileThreads, kTileSmem, st>>>(p, maps, max_tiles);
     return check_launch();
 }
 

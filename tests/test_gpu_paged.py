@@ -228,6 +228,14 @@ def test_chunk_options(cuda, opt):
     check(c, q, counts, attend(c, q, counts, **dict(opt)), **opt)
 
 
+@pytest.mark.parametrize("length,new,packed", [(2500, 130, 3), (2500, 130, 0), (3000, 300, 11), (2560, 2560, 0), (5000, 40, 20)])
+def test_chunk_many_fp16_pages(cuda, length, new, packed):
+    """Every buffer of the pipeline in use several times, and a last page that is not full."""
+    c = Cache([length], [packed], 1, 4, 4, 32, seed=length)
+    q = queries(new, 1)
+    check(c, q, [new], attend(c, q, [new], window=2000), window=2000)
+
+
 def test_mixed_step(cuda):
     counts = [1, 130, 1, 0, 7, 1]
     c = Cache([900, 500, 129, 77, 300, 1], [6, 2, 1, 0, 2, 0], 2, 3, 2, 128, seed=9)
