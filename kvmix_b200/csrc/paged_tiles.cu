@@ -19,10 +19,6 @@ namespace kvq {
 // their fields lie side by side and nothing is transposed.
 // Packed rows become fp16 as code * scale + minimum with one rounding (2^-11 relative): the tensor core takes no wider operand without
 // half its rate.
-#ifndef POLY
-#define POLY 8
-#endif
-constexpr int kPolyOf = POLY;
 constexpr int kTileRows = 128, kTileThreads = 512;
 constexpr uint32_t kOperandBytes = 32768, kOperandHalf = 16384;
 constexpr int kRawBytes = 12288;                                  // the largest packed half of a page: 3 bits, or 4 bits and groups of 32
@@ -137,24 +133,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x of two x <= some tens without the special function unit: x = n + f, n the nearest integer (by adding 1.5 * 2^23), |f| <= 0.5; 2^f by
-// the polynomial below, n into the exponent.  Below -126: 2^-126, which fp16 weights and fp32 sums do not feel.  NaN comes out as a number.
-__device__ __forceinline__ float2 exp2_poly(unsigned long long x) {
-    float2 c = f32x2_split(x);
-    c.x = fmaxf(c.x, -126.f);
-    c.y = fmaxf(c.y, -126.f);
-    x = f32x2(c.x, c.y);
-    const unsigned long long magic = f32x2(12582912.f, 12582912.f), n = add_f32x2(x, magic);
-    const unsigned long long f = add_f32x2(x, mul_f32x2(add_f32x2(n, f32x2(-12582912.f, -12582912.f)), f32x2(-1.f, -1.f)));
-    constexpr float C[5] = {0.999999261f, 0.693121815f, 0.240247448f, 0.0559178603f, 0.00957010191f};      // minimax in relative error, 2.6e-6 (the weights keep 2^-11), by a Remez exchange
-    unsigned long long p = f32x2(C[4], C[4]);
+// x * tanh(x) / x of two |x| <= 0.75: tanh(x) / x as a polynomial in x * x, minimax in relative error (2.9e-8, by a Remez exchange), times `by`.
+// No special function and both at once: 10 instructions where cap_score() takes 12 and four turns of the special function unit.
+__device__ __forceinline__ unsigned long long cap_small(unsigned long long x, unsigned long long by) {
+    constexpr float C[6] = {0.999999971f, -0.333329589f, 0.13325406f, -0.0533444301f, 0.0195829082f, -0.00471625725f};
+    const unsigned long long t = mul_f32x2(x, x);
+    unsigned long long r = f32x2(C[5], C[5]);
 #pragma unroll
-    for (int i = 3; i >= 0; --i) p = fma_f32x2(p, f, f32x2(C[i], C[i]));
-    const float2 q = f32x2_split(p), m = f32x2_split(n);
-    return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(m.x) << 23)), __int_as_float(__float_as_int(q.y) + (__float_as_int(m.y) << 23)));
+    for (int i = 4; i >= 0; --i) r = fma_f32x2(r, t, f32x2(C[i], C[i]));
+    return mul_f32x2(mul_f32x2(x, by), r);
 }
 
-template <int KB, int VB>
+// MODS: scores are capped, biased or scaled by a negative number.  Calls without have an instance of their own: with the code beside it the
+// 128 scores of a thread no longer fit its registers (2048 tokens over 32k: 1261 us in place of %s).
+template <int KB, int VB, bool MODS>
 __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ PagedMaps maps, int max_tiles) {
     extern __shared__ __align__(1024) char smem[];
     __shared__ uint32_t s_tmem;
@@ -258,9 +250,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                 mbar_arrive(bar(kBarQ));
                 if (mine) paged_bounds(p, s, u, pos, lo, hi);
             }
-            const bool cap = p.a.softcap > 0.f, bias = p.a.slopes != nullptr, plain = !cap && !bias && p.a.softmax_scale > 0.f;
-            const float scale2 = p.a.softmax_scale * kLog2e, two = cap ? 2.f * scale2 / p.a.softcap : 0.f, cap2 = p.a.softcap * kLog2e;
-            const float slope = bias && mine ? p.a.slopes[h] * kLog2e : 0.f, mul = plain ? scale2 : 1.f;
+            const bool cap = MODS && p.a.softcap > 0.f, bias = MODS && p.a.slopes != nullptr, flip = MODS && !cap && !bias;
+            const float scale2 = p.a.softmax_scale * kLog2e, two = cap ? 2.f * scale2 / p.a.softcap : 0.f, cap2 = p.a.softcap * kLog2e,
+                        small = cap ? p.a.softmax_scale / p.a.softcap : 0.f;
+            const float slope = bias && mine ? p.a.slopes[h] * kLog2e : 0.f, mul = cap || bias || flip ? 1.f : scale2;
             const uint32_t lanes = (uint32_t)(warp & 3) << 21, t_s = tmem + wg * 128 + lanes, t_o = tmem + 256 + wg * 128 + lanes;
             float m = -INFINITY, l = 0.f;
             bool ok = true;
@@ -275,13 +268,38 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                 for (int c = 0; c < 4; ++c) tc_load32(x[c], t_s + 32 * c);
                 tc_wait_ld();
                 auto at = [&](int j) -> uint32_t & { return x[j >> 5][j & 31]; };
-                if (!plain) {
+                auto pair = [&](int j) { return f32x2(__uint_as_float(at(j)), __uint_as_float(at(j + 1))); };
+                auto put = [&](int j, unsigned long long v) {
+                    const float2 w = f32x2_split(v);
+                    at(j) = __float_as_uint(w.x);
+                    at(j + 1) = __float_as_uint(w.y);
+                };
+                if (cap) {
+                    float most = 0.f;
 #pragma unroll
-                    for (int j = 0; j < 128; ++j) {
-                        float v = __uint_as_float(at(j));
-                        v = cap ? cap_score(v, two, cap2) : v * scale2;
-                        at(j) = __float_as_uint(fmaf(slope, (float)(b0 + j - pos), v));
+                    for (int j = 0; j < 128; j += 2) most = max_abs(most, __uint_as_float(at(j)), __uint_as_float(at(j + 1)));
+                    if (__all_sync(0xffffffffu, most * fabsf(small) <= 0.75f)) {
+                        const unsigned long long in = f32x2(small, small), by = f32x2(cap2, cap2);
+#pragma unroll
+                        for (int j = 0; j < 128; j += 2) put(j, cap_small(mul_f32x2(pair(j), in), by));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 128; ++j) at(j) = __float_as_uint(cap_score(__uint_as_float(at(j)), two, cap2));
                     }
+                }
+                if (bias) {
+                    unsigned long long b = f32x2(slope * (float)(b0 - pos), slope * (float)(b0 + 1 - pos));
+                    const unsigned long long by = f32x2(cap ? 1.f : scale2, cap ? 1.f : scale2), step = f32x2(2.f * slope, 2.f * slope);
+#pragma unroll
+                    for (int j = 0; j < 128; j += 2) {
+                        // eight running sums of one page drift by less than the rounding of a bias this large; started anew every 16 positions
+                        if (j && j % 16 == 0) b = f32x2(slope * (float)(b0 + j - pos), slope * (float)(b0 + j + 1 - pos));
+                        put(j, fma_f32x2(pair(j), by, b));
+                        b = add_f32x2(b, step);
+                    }
+                } else if (flip) {
+#pragma unroll
+                    for (int j = 0; j < 128; j += 2) put(j, mul_f32x2(pair(j), f32x2(scale2, scale2)));
                 }
                 if (!__all_sync(0xffffffffu, lo <= b0 && hi >= b0 + kPage && there)) {
                     const int from = there ? lo - b0 : kPage, to = there ? hi - b0 : 0;
@@ -322,14 +340,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
                         const unsigned long long e = fma_f32x2(f32x2(__uint_as_float(at(64 * c + 2 * j)), __uint_as_float(at(64 * c + 2 * j + 1))), mul2, ref2);
-                        float2 v;
-                        if (j % kPolyOf == kPolyOf - 1) {         // some of the exponentials on the FMA pipe
-                            v = exp2_poly(e);
-                        } else {
-                            v = f32x2_split(e);
-                            v.x = exp2_approx(v.x);
-                            v.y = exp2_approx(v.y);
-                        }
+                        float2 v = f32x2_split(e);
+                        v.x = exp2_approx(v.x);
+                        v.y = exp2_approx(v.y);
                         sum[j & 1] = add_f32x2(sum[j & 1], f32x2(v.x, v.y));
                         w[j] = as_u32(__floats2half2_rn(v.x, v.y));
                     }
@@ -546,9 +559,9 @@ static bool page_map(CUtensorMap *map, void *base, int64_t rows) {
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int KB, int VB>
+template <int KB, int VB, bool MODS>
 static int launch_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_tile_kernel<KB, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem);
+    const cudaError_t e = cudaFuncSetAttribute(paged_tile_kernel<KB, VB, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem);
     if (e != cudaSuccess) return record_cuda_error(e);
     const int64_t grid = (int64_t)max_tiles * p.l.Hkv * p.splits;
     if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
@@ -556,25 +569,28 @@ static int launch_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
     PagedMaps maps = {};
     const int64_t rows = (int64_t)p.l.n_fp16 * p.l.Hkv * kPage;
     maps.there = page_map(&maps.k, p.l.kfull, rows) && page_map(&maps.v, p.l.vfull, rows);
-    paged_tile_kernel<KB, VB><<<(unsigned)grid, kTileThreads, kTileSmem, st>>>(p, maps, max_tiles);
+    paged_tile_kernel<KB, VB, MODS><<<(unsigned)grid, kTileThreads, kTileSmem, st>>>(p, maps, max_tiles);
     return check_launch();
 }
 
+template <int KB>
+static int launch_tiles(const PagedArgs &p, int max_tiles, bool mods, cudaStream_t st) {
+    switch (p.l.v_bits) {
+        case 1: return mods ? launch_tiles<KB, 1, true>(p, max_tiles, st) : launch_tiles<KB, 1, false>(p, max_tiles, st);
+        case 2: return mods ? launch_tiles<KB, 2, true>(p, max_tiles, st) : launch_tiles<KB, 2, false>(p, max_tiles, st);
+        case 3: return mods ? launch_tiles<KB, 3, true>(p, max_tiles, st) : launch_tiles<KB, 3, false>(p, max_tiles, st);
+        default: return mods ? launch_tiles<KB, 4, true>(p, max_tiles, st) : launch_tiles<KB, 4, false>(p, max_tiles, st);
+    }
+}
+
 int paged_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
-#define KVQ_V(KB)                                                                                                             \
-    switch (p.l.v_bits) {                                                                                                     \
-        case 1: return launch_tiles<KB, 1>(p, max_tiles, st);                                                                 \
-        case 2: return launch_tiles<KB, 2>(p, max_tiles, st);                                                                 \
-        case 3: return launch_tiles<KB, 3>(p, max_tiles, st);                                                                 \
-        default: return launch_tiles<KB, 4>(p, max_tiles, st);                                                                \
-    }
+    const bool mods = p.a.softcap > 0.f || p.a.slopes || !(p.a.softmax_scale > 0.f);
     switch (p.l.k_bits) {
-        case 1: KVQ_V(1)
-        case 2: KVQ_V(2)
-        case 3: KVQ_V(3)
-        default: KVQ_V(4)
+        case 1: return launch_tiles<1>(p, max_tiles, mods, st);
+        case 2: return launch_tiles<2>(p, max_tiles, mods, st);
+        case 3: return launch_tiles<3>(p, max_tiles, mods, st);
+        default: return launch_tiles<4>(p, max_tiles, mods, st);
     }
-#undef KVQ_V
 }
 
 }  // namespace kvq
