@@ -100,21 +100,4 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
 // Factor of a partial sum with reference m (log2) and weights' sum l under the common reference: 0 for one that saw nothing; NaN stays.
 __device__ __forceinline__ float part_factor(float m, float l, float common) { return l == 0.f ? 0.f : m == -INFINITY ? 1.f : exp2_approx(m - common); }
 
-// ---------------------------------------------------------------------------------------------
-// A register holds two 16-bit halves, one of each of two words, with 16 / BITS fields of BITS bits.  A field left in place under an
-// exponent that gives its lowest bit the value 1 reads as 2^(10 - position) + code; less that power it is the code, exactly.  That
-// takes positions up to 10 - BITS; the fields above are shifted down first.
-template <int BITS>
-struct HalfFields {
-    static constexpr int N = 16 / BITS;                           // fields of a half
-    static constexpr int DIRECT = (10 - BITS) / BITS + 1;         // of them in reach without the shift
-    __device__ static __forceinline__ __half2 code(uint32_t x, int f) {
-        const int pos = f < DIRECT ? BITS * f : BITS * (f - DIRECT);
-        const uint32_t mask = ((1u << BITS) - 1u) << pos, expo = (uint32_t)(25 - pos) << 10;
-        uint32_t r;
-        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(f < DIRECT ? x : x >> (BITS * DIRECT)), "r"(mask * 0x10001u), "r"(expo * 0x10001u));   // (x & mask) | expo
-        return __hsub2(as_h2(r), as_h2(expo * 0x10001u));
-    }
-};
-
 }  // namespace kvq

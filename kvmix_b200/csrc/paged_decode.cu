@@ -3,23 +3,26 @@
 
 namespace kvq {
 
-// A CTA of four warps takes one (sequence, kv head, split of its pages); a warp takes every fourth page by itself -- scores, online
-// softmax, values -- so nothing in the loop waits for another warp.
-//   scores   S[token][row] = K[token][channel] q[row][channel]: mma m16n8k16 with 16 tokens as rows and up to eight query rows as
-//            columns
-//   values   O[channel][row] = V^T[channel][token] p[row][token]: the same with 16 channels as rows
+// A CTA of four warps takes one (sequence, kv head, block of query rows, split of the pages); a warp takes every fourth page by itself --
+// scores, online softmax, values -- so nothing in the loop waits for another warp.
+//   scores   S[token][column] = K[token][channel] B[channel][column]: mma m16n8k16 with 16 tokens as rows
+//   values   O[channel][column] = V^T[channel][token] B[token][column]: the same with 16 channels as rows
 // In both the packed axis runs along the MMA's rows and the contraction across words, so that the two elements of an operand register
-// come from the same place of two words.  Words arrive by bulk copies, 32 contraction rows (codes, scales, minima) a stage, in the warp's own ring; fp16
-// pages go straight to registers.
+// come from the same place of two words, and a field of 1, 2 or 4 bits is an operand as it stands: masked in place it is the fp16 subnormal
+// code * 2^(position - 24), and the power of two, the same for a whole accumulator, comes off at the end.  Scales go to the other
+// operand, whose columns are (group of the packed axis, query row) pairs:
+//   keys     B = q * scale of a channel's token group, as an exact pair hi + lo of two columns (rounded once it would cost 2^-11 of every term)
+//   values   B = p * scale of a token's channel group, rounded to fp16 as weights are everywhere
+// An accumulator row needs the column of its own group only; what the others hold is not read.  Minima times q or p come from one more MMA
+// a k-step, whose rows are the groups.  3-bit words are groups of their own, so their fields become fp16 values (code * scale + minimum,
+// rounded once) and the columns are query rows.
+// Words arrive by bulk copies, 32 contraction rows (codes, scales, minima) a stage, in the warp's own ring; fp16 pages go straight to
+// registers, first, and their sums are put aside in shared memory.
 constexpr int kFewWarps = 4;
 constexpr int kStageRows = 32;
 constexpr int kMaxStages = 8;
-constexpr int kPStride = 136;                                     // halves between rows of weights: 2-way conflicts at most
-
-template <int BITS> struct FewGeom {
-    static constexpr int W = page_words(BITS);
-    static constexpr int TILES = BITS == 3 ? 11 : 8;              // accumulator tiles of 128 packed elements
-};
+constexpr int kPStride = 136;                                     // halves between rows of weights
+constexpr float kWeightBits = 7.f;                                // weights are 2^7 p: p * scale keeps away from fp16's smallest numbers
 
 // Which of a page's 128 elements accumulator (tile m, half e) of lane group g stands for: element 16g + f(2m + e) where a lane group owns 16
 // neighbours, in the order that puts the four a lane needs for a k-step side by side; 3 bits: field m of word g + 8e (none beyond the end).
@@ -32,51 +35,27 @@ template <int BITS> __device__ __forceinline__ int few_element(int g, int m, int
         return 16 * g + (s & 3) * 4 + (s >> 2);
     }
 }
+// Where element el of a page stands among weights and scores: those of a lane's k-step side by side.
+__device__ __forceinline__ int few_slot(int el) { return (el & ~15) + 4 * (el & 3) + ((el & 15) >> 2); }
 
-// acc[tile] += A(16 contraction rows starting at `row` of the stage) * B.  Contraction rows of lane t: row + t + 4j.
+// Field f of two half words, moved to bit 2 and above (see VHalf: lower ones lose product bits in the tensor core).
+template <int BITS> __device__ __forceinline__ uint32_t few_field(uint32_t x, int f) {
+    if constexpr (BITS == 4) return (f < 2 ? x << 2 : x >> 6) & (0x003c003cu << (f & 1 ? 4 : 0));
+    else if constexpr (BITS == 2) return f < 2 ? (x << 6) & (0x00030003u << (6 + 2 * f)) : f < 5 ? x & (0x00030003u << (2 * f)) : (x >> 6) & (0x00030003u << (2 * f - 6));
+    else return f < 4 ? (x << 6) & (0x00010001u << (f + 6)) : f < 10 ? x & (0x00010001u << f) : (x >> 6) & (0x00010001u << (f - 6));
+}
+// 2^(24 - position) of accumulator (m, e)
+template <int BITS> __device__ __forceinline__ float few_power(int m, int e) {
+    const int s = 2 * m + e, i = (s & 3) * 4 + (s >> 2);
+    return (float)(1 << (24 - VHalf<BITS>::pos(i % (16 / BITS))));
+}
+
+// The A registers of a k-step: a(m, r) for tile m, register r.  Contraction rows of lane t: row + t + 4j.
 template <int BITS>
-__device__ __forceinline__ void few_packed_step(float (&acc)[FewGeom<BITS>::TILES][4], uint32_t codes, uint32_t scale, uint32_t mn, int groups, int g_log2,
-                                                int row, int g, int t, uint32_t b0, uint32_t b1) {
-    constexpr int W = FewGeom<BITS>::W;
-    if constexpr (BITS == 3) {
-        uint32_t w[2][4];
-        __half2 sc[2][2], lo[2][2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int word = min(g + 8 * e, 11);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[e][j] = lds32(codes + ((row + t + 4 * j) * W + word) * 4);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int r0 = ((row + t + 8 * j) * 12 + word) * 2, r1 = r0 + 4 * 12 * 2;
-                sc[e][j] = as_h2(lds16(scale + r0) | lds16(scale + r1) << 16);
-                lo[e][j] = as_h2(lds16(mn + r0) | lds16(mn + r1) << 16);
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < 11; ++m) {
-            uint32_t a[4];
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint32_t x = (m < 10 ? (w[e][2 * j] >> (3 * m)) & 7u : w[e][2 * j] >> 30) | ((m < 10 ? (w[e][2 * j + 1] >> (3 * m)) & 7u : w[e][2 * j + 1] >> 30) << 16);
-                    a[e + 2 * j] = as_u32(__hfma2(__hsub2(as_h2(x | 0x64006400u), as_h2(0x64006400u)), sc[e][j], lo[e][j]));
-                }
-            mma16816(acc[m], a[0], a[1], a[2], a[3], b0, b1);
-        }
-    } else {
-        using F = HalfFields<BITS>;
-        const int grp = (16 * g) >> g_log2;
-        __half2 sc[2], lo[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int r0 = ((row + t + 8 * j) * groups + grp) * 2, r1 = r0 + 4 * groups * 2;
-            sc[j] = as_h2(lds16(scale + r0) | lds16(scale + r1) << 16);
-            lo[j] = as_h2(lds16(mn + r0) | lds16(mn + r1) << 16);
-        }
-        // the 16 elements of the lane group are BITS halves of words, x[h][j]: half h of rows t + 8j and t + 8j + 4
-        uint32_t x[BITS][2];
+struct FewWords {
+    uint32_t x[BITS][2];                                          // half h of rows t + 8j and t + 8j + 4
+    __device__ __forceinline__ FewWords(uint32_t codes, int row, int g, int t) {
+        constexpr int W = page_words(BITS);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const uint32_t at = codes + (row + t + 8 * j) * W * 4;
@@ -91,102 +70,179 @@ __device__ __forceinline__ void few_packed_step(float (&acc)[FewGeom<BITS>::TILE
                 }
             }
         }
+    }
+    __device__ __forceinline__ uint32_t a(int m, int r) const {
+        const int s = 2 * m + (r & 1), i = (s & 3) * 4 + (s >> 2), n = 16 / BITS;
+        return few_field<BITS>(x[i / n][r >> 1], i % n);
+    }
+};
+
+// Scales or minima of a lane's four contraction rows, group `grp`, as two pairs.
+__device__ __forceinline__ void few_pairs(uint32_t at, int row, int t, int groups, int grp, uint32_t (&v)[2]) {
 #pragma unroll
-        for (int m = 0; m < 8; ++m) {
-            uint32_t a[4];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int s = 2 * m + e, i = (s & 3) * 4 + (s >> 2);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) a[e + 2 * j] = as_u32(__hfma2(F::code(x[i / F::N][j], i % F::N), sc[j], lo[j]));
-            }
-            mma16816(acc[m], a[0], a[1], a[2], a[3], b0, b1);
-        }
+    for (int j = 0; j < 2; ++j) {
+        const uint32_t r0 = at + ((row + t + 8 * j) * groups + grp) * 2;
+        v[j] = lds16(r0) | lds16(r0 + 8 * groups) << 16;
     }
 }
 
-struct FewState {
-    float m[2], l[2];                                             // of columns 2t, 2t + 1: reference (log2 units) and this lane's part of the sum
+// 3 bits: acc[tile] += A * B with A the dequantised values.
+__device__ __forceinline__ void few_step3(float (&acc)[11][4], uint32_t codes, uint32_t scale, uint32_t mn, int row, int g, int t, uint32_t b0, uint32_t b1) {
+    uint32_t w[2][4];
+    uint32_t sc[2][2], lo[2][2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int word = min(g + 8 * e, 11);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[e][j] = lds32(codes + ((row + t + 4 * j) * 12 + word) * 4);
+        few_pairs(scale, row, t, 12, word, sc[e]);
+        few_pairs(mn, row, t, 12, word, lo[e]);
+    }
+#pragma unroll
+    for (int m = 0; m < 11; ++m) {
+        uint32_t a[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                // the field at the same place of two half words, or shifted there
+                const uint32_t u = w[e][2 * j], v = w[e][2 * j + 1];
+                const uint32_t x = m < 5 ? prmt(u, v, 0x5410) >> (m < 3 ? 0 : 9) : m < 10 ? prmt(u >> 15, v >> 15, 0x5410) >> (m < 8 ? 0 : 9) : prmt(u, v, 0x7632) >> 14;
+                const int pos = m < 3 ? 3 * m : m < 5 ? 3 * m - 9 : m < 8 ? 3 * m - 15 : m < 10 ? 3 * m - 24 : 0;
+                const uint32_t mask = (m < 10 ? 7u : 3u) << pos, expo = (uint32_t)(25 - pos) << 10;
+                uint32_t f;
+                asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(f) : "r"(x), "r"(mask * 0x10001u), "r"(expo * 0x10001u));        // (x & mask) | expo
+                a[e + 2 * j] = as_u32(__hfma2(__hsub2(as_h2(f), as_h2(expo * 0x10001u)), as_h2(sc[e][j]), as_h2(lo[e][j])));
+            }
+        mma16816(acc[m], a[0], a[1], a[2], a[3], b0, b1);
+    }
+}
+
+__device__ __forceinline__ float warp_max_f32(float x) {
+    float r;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;\n" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ void sts_f4(uint32_t at, float x, float y, float z, float w) {
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(at), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+}
+
+// Shared memory of a CTA for blocks of R query rows: q as it is and with a lane's four channels of a k-step side by side, the rows' bounds, and for
+// every warp weights, scores, sums put aside, sums of weights, barriers, the ring.
+struct FewShared {
+    int q, bounds, factor, warps, weights, scores, aside, sums, bars, ring, warp_bytes, total;
+    __host__ __device__ FewShared(int R, int stages, int stage_bytes) {
+        q = 0;
+        bounds = 2 * R * 256;
+        factor = bounds + R * 16;
+        warps = factor + (R + 1) / 2 * 16;
+        weights = 0;
+        scores = R * kPStride * 2;
+        aside = scores + R * 512;
+        sums = aside + R * 512;
+        bars = sums + R * 128;
+        ring = bars + kMaxStages * 8;
+        warp_bytes = ring + stages * stage_bytes;
+        total = warps + kFewWarps * warp_bytes;
+    }
 };
 
-template <int KB, int VB>
-__global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 ? 3 : 4) paged_few_kernel(const __grid_constant__ PagedArgs p, int stages, int stage_bytes) {
+template <int KB, int VB, int CK>
+__global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 ? 3 : 4)
+    paged_few_kernel(const __grid_constant__ PagedArgs p, int R, int row_blocks, int stages, int stage_bytes) {
     extern __shared__ __align__(128) char smem[];
+    const FewShared sh(R, stages, stage_bytes);
     const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x % p.splits, hs = blockIdx.x / p.splits, head = hs % p.l.Hkv, i = hs / p.l.Hkv;
+    int hs = blockIdx.x;
+    const int split = hs % p.splits;
+    hs /= p.splits;
+    const int block = hs % row_blocks;
+    hs /= row_blocks;
+    const int head = hs % p.l.Hkv, i = hs / p.l.Hkv;
     const PagedSeq s = paged_seq(p, i);
-    const int rows = s.n_new * p.rep;
-    if (rows <= 0 || rows > kFewRows) return;
+    if (s.n_new * p.rep > kFewRows) return;
+    const int row0 = block * R, rows = min(R, s.n_new * p.rep - row0);
+    if (rows <= 0) return;
 
-    // shared memory of the CTA: q rows, then per warp: weights, barriers, ring; the outputs meet in [warp][8][128] floats over the rings
-    __half *s_q = reinterpret_cast<__half *>(smem);               // [8][128], rows beyond the last zero
-    char *mine = smem + 2048 + warp * (kFewRows * kPStride * 2 + kMaxStages * 8 + stages * stage_bytes);
-    const uint32_t s_p = smem_u32(mine), s_bar = s_p + kFewRows * kPStride * 2, s_ring = s_bar + kMaxStages * 8;
-    for (int k = threadIdx.x; k < kFewRows * 16; k += kFewWarps * 32) {
-        const int r = k >> 4, c = (k & 15) * 8;
-        alignas(16) __half x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __ushort_as_half(0);
+    const uint32_t base = smem_u32(smem), mine = base + sh.warps + warp * sh.warp_bytes;
+    const uint32_t s_p = mine + sh.weights, s_s = mine + sh.scores, s_sum = mine + sh.sums, s_bar = mine + sh.bars, s_ring = mine + sh.ring;
+    float *s_out = reinterpret_cast<float *>(smem + sh.warps + warp * sh.warp_bytes + sh.aside);                // [R][128]
+    __half *s_q = reinterpret_cast<__half *>(smem), *s_qs = s_q + R * 128;
+    // q by a power of two below 1, so that no product with a scale leaves fp16
+    float2 *s_factor = reinterpret_cast<float2 *>(smem + sh.factor);              // raw scores to log2 units; to cap_score's argument
+    for (int r = warp; r < R; r += kFewWarps) {
+        const int row = row0 + r;
+        float x[4] = {0.f, 0.f, 0.f, 0.f}, top = 0.f;
         if (r < rows) {
-            const __half *q = static_cast<const __half *>(p.a.q) + (int64_t)(s.q0 + r / p.rep) * p.a.q_sT + (int64_t)(head * p.rep + r % p.rep) * p.a.q_sH + c;
+            const __half *q = static_cast<const __half *>(p.a.q) + (int64_t)(s.q0 + row / p.rep) * p.a.q_sT + (int64_t)(head * p.rep + row % p.rep) * p.a.q_sH;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = q[j];
+            for (int c = 0; c < 4; ++c) { x[c] = __half2float(q[lane + 32 * c]); top = fmaxf(top, fabsf(x[c])); }
         }
-        *reinterpret_cast<uint4 *>(s_q + r * 128 + c) = *reinterpret_cast<const uint4 *>(x);
+        top = warp_max_f32(top);
+        const int e = top > 0.f && top < INFINITY ? (__float_as_int(top) >> 23 & 255) - 126 : 0;
+        const float down = __int_as_float((127 - e) << 23), up = __int_as_float((127 + e) << 23), scale2 = p.a.softmax_scale * kLog2e;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s_q[r * 128 + lane + 32 * c] = s_qs[r * 128 + few_slot(lane + 32 * c)] = __float2half_rn(x[c] * down);
+        if (lane == 0) s_factor[r] = make_float2(scale2 * up, p.a.softcap > 0.f ? 2.f * scale2 / p.a.softcap * up : 0.f);
+    }
+    int4 *s_bounds = reinterpret_cast<int4 *>(smem + sh.bounds);  // lowest position, end, position, slope of a row
+    if (threadIdx.x < R) {
+        int lo = 0, hi = 0, pos = 0;
+        float slope = 0.f;
+        const int row = row0 + threadIdx.x;
+        if ((int)threadIdx.x < rows) {
+            paged_bounds(p, s, row / p.rep, pos, lo, hi);
+            if (p.a.slopes) slope = p.a.slopes[head * p.rep + row % p.rep] * kLog2e;
+        }
+        s_bounds[threadIdx.x] = make_int4(lo, hi, pos, __float_as_int(slope));
     }
     if (lane < stages) mbar_init(s_bar + 8 * lane, 1);
+    for (int k = lane; k < R * 32; k += 32) asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(s_sum + 4 * k), "r"(0) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     __syncthreads();
 
-    // bounds and bias of this lane's two columns; the pages that any row sees
-    int lo[2], hi[2], pos[2], first = INT32_MAX, last = 0;
-    float slope[2];
-    for (int u = 0; u < s.n_new; ++u) {
-        int a, b, c;
-        paged_bounds(p, s, u, c, a, b);
-        if (a < b) { first = min(first, a); last = max(last, b); }
-    }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        const int r = 2 * t + c;
-        lo[c] = hi[c] = pos[c] = 0;
-        slope[c] = 0.f;
-        if (r < rows) {
-            paged_bounds(p, s, r / p.rep, pos[c], lo[c], hi[c]);
-            if (p.a.slopes) slope[c] = p.a.slopes[head * p.rep + r % p.rep] * kLog2e;
-        }
+    // the pages that any row sees
+    int first = INT32_MAX, last = 0;
+    for (int r = 0; r < rows; ++r) {
+        const int4 b = s_bounds[r];
+        if (b.x < b.y) { first = min(first, b.x); last = max(last, b.y); }
     }
     const int p_lo = first < last ? first / kPage : 0, p_hi = first < last ? pages_of(last) : 0, per = (p_hi - p_lo + p.splits - 1) / p.splits;
     const int p0 = p_lo + split * per, p1 = min(p_hi, p0 + per), n_mine = max(0, (p1 - p0 - warp + kFewWarps - 1) / kFewWarps);
-    // pages newest first: where values are packed in 3 bits the fp16 pages' sums are kept apart, and they come at the beginning
-    auto page_at = [&](int k) { return p1 - 1 - (k * kFewWarps + warp); };
+    auto page_at = [&](int k) { return p1 - 1 - (k * kFewWarps + warp); };        // newest first: fp16 pages come at the beginning
 
-    constexpr int KW = FewGeom<KB>::W, VW = FewGeom<VB>::W, KT = FewGeom<KB>::TILES, VT = FewGeom<VB>::TILES;
-    const int kg_log2 = KB == 3 ? 0 : 31 - __clz(p.l.group), vg_log2 = VB == 3 ? 0 : 31 - __clz(p.l.group);
+    constexpr int KW = page_words(KB), VW = page_words(VB), VT = VB == 3 ? 11 : 8;
     const uint32_t k_sz = kStageRows * p.k_groups * 2, v_sz = kStageRows * p.v_groups * 2;
     constexpr int SPH = kPage / kStageRows;                       // stages of a page's keys, and of its values
+    const int ng_log2 = p.l.group == 128 ? 0 : p.l.group == 64 ? 1 : 2;            // of both sides, where they are not 3 bits
+    const int own_group = g >> (3 - ng_log2);                     // of the 16 packed elements that this lane's accumulator rows stand for
 
     // page numbers, 32 of the warp's pages at a time, one a lane; -1: not there
     int ids = -1, ids_base = 0;
-    auto fetch_ids = [&](int base) {
-        ids_base = base;
+    auto fetch_ids = [&](int at) {
+        ids_base = at;
         ids = -1;
-        if (base + lane < n_mine) {
-            const int page = page_at(base + lane), id = s.table[page];
+        if (at + lane < n_mine) {
+            const int page = page_at(at + lane), id = s.table[page];
             if (id >= 0 && id < (page < s.packed ? p.l.n_packed : p.l.n_fp16)) ids = id;
         }
     };
     auto id_of = [&](int k) { return __shfl_sync(0xffffffffu, ids, k - ids_base); };
 
     // the producer's place: page number `pk` of the warp's, its next stage; ids are those of the consumer's window, so it stops at its end
-    int pk = 0, pstage = 0, filled = 0, used = 0;
+    int pk = 0, pstage = 0, fill_slot = 0, in_flight = 0, use_slot = 0;
+    uint32_t parity = 0;
     auto produce = [&]() {
-        while (pk < n_mine && pk < ids_base + 32 && filled - used < stages) {
+        while (pk < n_mine && pk < ids_base + 32 && in_flight < stages) {
             const int id = id_of(pk);
             if (page_at(pk) >= s.packed || id < 0) { ++pk; continue; }
             if (lane == 0) {
-                const int slot = filled % stages;
-                const uint32_t bar = s_bar + 8 * slot, dst = s_ring + slot * stage_bytes;
+                const uint32_t bar = s_bar + 8 * fill_slot, dst = s_ring + fill_slot * stage_bytes;
                 const bool values = pstage >= SPH;
                 const int64_t row = ((int64_t)id * p.l.Hkv + head) * kPage + (pstage % SPH) * kStageRows;
                 const uint32_t cb = kStageRows * 4 * (values ? VW : KW), sz = values ? v_sz : k_sz;
@@ -196,271 +252,370 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 ? 3 : 4) pa
                 bulk_load(dst + cb, static_cast<const __half *>(values ? p.l.vscale : p.l.kscale) + row * groups, sz, bar);
                 bulk_load(dst + cb + sz, static_cast<const __half *>(values ? p.l.vmn : p.l.kmn) + row * groups, sz, bar);
             }
-            ++filled;
+            if (++fill_slot == stages) fill_slot = 0;
+            ++in_flight;
             if (++pstage == 2 * SPH) { pstage = 0; ++pk; }
         }
     };
-
-    float out[VT][4];
-#pragma unroll
-    for (int m = 0; m < VT; ++m)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[m][e] = 0.f;
-    FewState st = {{-INFINITY, -INFINITY}, {0.f, 0.f}};
-    float aside_m[2] = {-INFINITY, -INFINITY};                    // 3-bit values: reference of the sums put aside, see below
-    bool aside = false, ok = true;
-    float *s_out = reinterpret_cast<float *>(smem + 2048 + kFewWarps * (kFewRows * kPStride * 2 + kMaxStages * 8 + stages * stage_bytes)) + warp * kFewRows * 128;
-
-    const float two = p.a.softcap > 0.f ? 2.f * kLog2e * p.a.softmax_scale / p.a.softcap : 0.f, cap2 = p.a.softcap * kLog2e, scale2 = p.a.softmax_scale * kLog2e;
-
-    // scores of a page -> weights in s_p, sums and references in st; returns the factors for what is summed already
-    auto softmax_page = [&](auto &sc, auto element, int base, float (&alpha)[2]) {
-        constexpr int T = sizeof(sc) / sizeof(sc[0]);
-        const bool whole = base >= 0 && __all_sync(0xffffffffu, (2 * t >= rows || (lo[0] <= base && hi[0] >= base + kPage)) &&
-                                                                    (2 * t + 1 >= rows || (lo[1] <= base && hi[1] >= base + kPage)));
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int m = 0; m < T; ++m)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int el = element(m, e), j = base + el;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float x = sc[m][2 * e + c];
-                    x = p.a.softcap > 0.f ? cap_score(x, two, cap2) : x * scale2;
-                    if (p.a.slopes) x = fmaf(slope[c], (float)(j - pos[c]), x);
-                    if (el < 0 || (!whole && (j < lo[c] || j >= hi[c]))) x = -INFINITY;
-                    sc[m][2 * e + c] = x;
-                    top[c] = fmaxf(top[c], x);
-                }
-            }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
-            const float ref = fmaxf(st.m[c], top[c]);
-            alpha[c] = ref == -INFINITY ? 1.f : exp2_approx(st.m[c] - ref);
-            st.m[c] = ref;
-            st.l[c] *= alpha[c];
-        }
-        __syncwarp();                                             // the weights of the page before are read
-#pragma unroll
-        for (int m = 0; m < T; ++m)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const float ref = st.m[c] == -INFINITY ? 0.f : st.m[c];
-                const float x = exp2_approx(sc[m][c] - ref), y = exp2_approx(sc[m][2 + c] - ref);
-                st.l[c] += x + y;
-                const uint32_t h = as_u32(__floats2half2_rn(x, y));
-                const int e0 = element(m, 0), e1 = element(m, 1);
-                const uint32_t at = s_p + (2 * t + c) * kPStride * 2;
-                auto slot = [](int el) { return (el & ~15) + 4 * (el & 3) + ((el & 15) >> 2); };
-                if constexpr (T == 8) {
-                    asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(at + slot(e0) * 2), "r"(h) : "memory");
-                } else {
-                    if (e0 >= 0) asm volatile("st.shared.u16 [%0], %1;\n" ::"r"(at + slot(e0) * 2), "h"((unsigned short)(h & 0xffff)) : "memory");
-                    if (e1 >= 0) asm volatile("st.shared.u16 [%0], %1;\n" ::"r"(at + slot(e1) * 2), "h"((unsigned short)(h >> 16)) : "memory");
-                }
-            }
+    bool ok = true;
+    auto stage_ready = [&]() {
+        ok = __all_sync(0xffffffffu, mbar_wait(s_bar + 8 * use_slot, parity, &p.b.count[2]));
+        return s_ring + use_slot * stage_bytes;
+    };
+    auto stage_done = [&]() {
+        if (++use_slot == stages) { use_slot = 0; parity ^= 1; }
+        --in_flight;
         __syncwarp();
-    };
-    auto rescale = [&](auto &o, const float (&alpha)[2]) {
-        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-            constexpr int T = sizeof(o) / sizeof(o[0]);
-#pragma unroll
-            for (int m = 0; m < T; ++m)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[m][e] *= alpha[e & 1];
-        }
-    };
-    auto weights = [&](int step, uint32_t &b0, uint32_t &b1) {    // B operand of contraction rows 16 step + t + 4j for query row g
-        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(b0), "=r"(b1) : "r"(s_p + (g * kPStride + 16 * step + 4 * t) * 2));
+        produce();
     };
 
-    auto fp16_page = [&](int id, int page, auto &o) {
-        const int base = page * kPage, there = min(kPage, s.length - base);
-        const __half *k = static_cast<const __half *>(p.l.kfull) + ((int64_t)id * p.l.Hkv + head) * kPageHalf;
-        const __half *v = static_cast<const __half *>(p.l.vfull) + ((int64_t)id * p.l.Hkv + head) * kPageHalf;
-        float sc[8][4];
-#pragma unroll
-        for (int m = 0; m < 8; ++m) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[m][e] = 0.f;
-#pragma unroll
-            for (int blk = 0; blk < 4; ++blk) {                   // 32 channels, eight neighbours a lane
-                const int r0 = min(few_element<1>(g, m, 0), there - 1), r1 = min(few_element<1>(g, m, 1), there - 1);
-                const uint4 x = *reinterpret_cast<const uint4 *>(k + r0 * kHeadDim + 32 * blk + 8 * t);
-                const uint4 y = *reinterpret_cast<const uint4 *>(k + r1 * kHeadDim + 32 * blk + 8 * t);
-                const uint4 q = *reinterpret_cast<const uint4 *>(s_q + g * 128 + 32 * blk + 8 * t);
-                mma16816(sc[m], x.x, y.x, x.y, y.y, q.x, q.y);
-                mma16816(sc[m], x.z, y.z, x.w, y.w, q.z, q.w);
-            }
-        }
-        float alpha[2];
-        softmax_page(sc, [&](int m, int e) { return few_element<1>(g, m, e); }, base, alpha);
-        rescale(o, alpha);
+    const float cap2 = p.a.softcap * kLog2e;
+    float ref = -INFINITY, alpha = 1.f;                           // of row `lane`: reference (log2 units), factor of what is summed already
+
+    // Scores of a page, [row][slot] in s_s -> weights in s_p, sums in s_sum, ref and alpha.  A lane takes four tokens of each row.
+    auto softmax_page = [&](int page_base) {
+        __syncwarp();
+        const int j0 = page_base + 16 * (lane >> 2) + (lane & 3);
+        float change = 1.f;
 #pragma unroll 1
-        for (int step = 0; step < 8; ++step) {
-            if (16 * step >= there) break;
-            uint32_t x[4][8], b0, b1;
+        for (int r = 0; r < rows; ++r) {
+            const float4 raw = lds_f4(s_s + r * 512 + lane * 16);
+            const int4 b = s_bounds[r];
+            const float2 by_row = s_factor[r];
+            const float slope = __int_as_float(b.w);
+            float x[4] = {raw.x, raw.y, raw.z, raw.w}, top = -INFINITY;
+            const bool whole = b.x <= page_base && b.y >= page_base + kPage;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {                         // tokens t + 4j, channels 16g .. 16g + 15; nothing behind the last token
-                const int r = 16 * step + t + 4 * j;
-                uint4 a = make_uint4(0, 0, 0, 0), b = a;
-                if (r < there) {
-                    a = *reinterpret_cast<const uint4 *>(v + r * kHeadDim + 16 * g);
-                    b = *reinterpret_cast<const uint4 *>(v + r * kHeadDim + 16 * g + 8);
-                }
-                x[j][0] = a.x; x[j][1] = a.y; x[j][2] = a.z; x[j][3] = a.w;
-                x[j][4] = b.x; x[j][5] = b.y; x[j][6] = b.z; x[j][7] = b.w;
+            for (int c = 0; c < 4; ++c) {
+                x[c] = p.a.softcap > 0.f ? cap_score(x[c], by_row.y, cap2) : x[c] * by_row.x;
+                x[c] = fmaf(slope, (float)(j0 + 4 * c - b.z), x[c]);
+                if (!whole && (j0 + 4 * c < b.x || j0 + 4 * c >= b.y)) x[c] = -INFINITY;
             }
-            weights(step, b0, b1);
+            asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(top) : "f"(x[0]), "f"(x[1]), "f"(x[2]));
+            asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(x[3]));
+            top = warp_max_f32(top);
+            const float old = __shfl_sync(0xffffffffu, ref, r), now = fmaxf(old, top), by = now == -INFINITY ? 1.f : exp2_approx(old - now);
+            if (lane == r) { ref = now; alpha = by; }
+            change = fminf(change, by);
+            const float to = (now == -INFINITY ? 0.f : now) - kWeightBits;
+            float sum = 0.f;
 #pragma unroll
-            for (int m = 0; m < 8; ++m) {
-                uint32_t a[4];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int q = 2 * m + e, c = (q & 3) * 4 + (q >> 2);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) a[e + 2 * j] = prmt(x[2 * j][c >> 1], x[2 * j + 1][c >> 1], c & 1 ? 0x7632 : 0x5410);
-                }
-                mma16816(o[m], a[0], a[1], a[2], a[3], b0, b1);
-            }
+            for (int c = 0; c < 4; ++c) { x[c] = exp2_approx(x[c] - to); sum += x[c]; }
+            const uint32_t w0 = as_u32(__floats2half2_rn(x[0], x[1])), w1 = as_u32(__floats2half2_rn(x[2], x[3]));
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(s_p + r * kPStride * 2 + lane * 8), "r"(w0), "r"(w1) : "memory");
+            const uint32_t at = s_sum + r * 128 + lane * 4;
+            sum = fmaf(__uint_as_float(lds32(at)), by, sum);
+            asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(at), "f"(sum) : "memory");
         }
+        __syncwarp();
+        return change != 1.f;                                     // the same in all lanes
     };
-    // `o` of the layout of fp16 pages and of 1, 2 and 4 bits, or of 3 bits, as [row][channel]
-    auto each_out = [&](auto &o, auto element, auto f) {
-        constexpr int T = sizeof(o) / sizeof(o[0]);
+    auto weights = [&](int row, int step, uint32_t &b0, uint32_t &b1) {           // contraction rows 16 step + t + 4j
+        b0 = b1 = 0;
+        if (row < rows) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(b0), "=r"(b1) : "r"(s_p + (row * kPStride + 16 * step + 4 * t) * 2));
+    };
+    // Columns that are query rows: scores of accumulators into s_s, factors of columns 2t, 2t + 1
+    auto dense_scores = [&](auto &sc, auto element) {
+        constexpr int T = sizeof(sc) / sizeof(sc[0]);
 #pragma unroll
         for (int m = 0; m < T; ++m)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int c = element(m, e);
-                if (c >= 0) {
-                    f(2 * t, c, o[m][2 * e]);
-                    f(2 * t + 1, c, o[m][2 * e + 1]);
-                }
+                const int el = element(m, e);
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    if (el >= 0 && 2 * t + c < rows) asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(s_s + (2 * t + c) * 512 + few_slot(el) * 4), "f"(sc[m][2 * e + c]) : "memory");
             }
     };
+    auto rescale = [&](auto &o, int r0, int r1) {                 // columns 2t, 2t + 1 belong to rows r0, r1
+        constexpr int T = sizeof(o) / sizeof(o[0]);
+        const float a0 = __shfl_sync(0xffffffffu, alpha, r0), a1 = __shfl_sync(0xffffffffu, alpha, r1);
+#pragma unroll
+        for (int m = 0; m < T; ++m) { o[m][0] *= a0; o[m][1] *= a1; o[m][2] *= a0; o[m][3] *= a1; }
+    };
 
+    // ---- fp16 pages
     int k = 0;
     if (n_mine > 0) fetch_ids(0);
-    if constexpr (VB == 3) {
-        // fp16 pages sum in the layout of eight tiles; the sums go to shared memory before the packed pages begin
+    produce();
+    {
         float o[8][4];
 #pragma unroll
         for (int m = 0; m < 8; ++m)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[m][e] = 0.f;
-        produce();
+#pragma unroll 1
         for (; k < n_mine && page_at(k) >= s.packed; ++k) {
             if (k == ids_base + 32) { fetch_ids(k); pk = max(pk, k); produce(); }
-            const int id = id_of(k);
-            if (id >= 0) { fp16_page(id, page_at(k), o); aside = true; }
-        }
-        each_out(o, [&](int m, int e) { return few_element<1>(g, m, e); }, [&](int r, int c, float v) { s_out[r * 128 + c] = v; });
-        aside_m[0] = st.m[0];
-        aside_m[1] = st.m[1];
-    } else {
-        produce();
-    }
-    for (; k < n_mine; ++k) {
-        if (k == ids_base + 32) { fetch_ids(k); produce(); }
-        const int id = id_of(k), page = page_at(k);
-        if (id < 0) continue;
-        if (page >= s.packed) {
-            if constexpr (VB != 3) fp16_page(id, page, out);
-            continue;
-        }
-        float sc[KT][4], alpha[2];
+            const int id = id_of(k), page = page_at(k);
+            if (id < 0) continue;
+            const int page_base = page * kPage, there = min(kPage, s.length - page_base);
+            const __half *kp = static_cast<const __half *>(p.l.kfull) + ((int64_t)id * p.l.Hkv + head) * kPageHalf;
+            const __half *vp = static_cast<const __half *>(p.l.vfull) + ((int64_t)id * p.l.Hkv + head) * kPageHalf;
+            float sc[8][4];
 #pragma unroll
-        for (int m = 0; m < KT; ++m)
+            for (int m = 0; m < 8; ++m) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[m][e] = 0.f;
-#pragma unroll 1
-        for (int q = 0; q < SPH; ++q) {
-            const int slot = used % stages;
-            ok = __all_sync(0xffffffffu, mbar_wait(s_bar + 8 * slot, used / stages & 1, &p.b.count[2]));
-            if (!ok) break;
-            const uint32_t c = s_ring + slot * stage_bytes;
+                for (int e = 0; e < 4; ++e) sc[m][e] = 0.f;
 #pragma unroll
-            for (int step = 0; step < kStageRows / 16; ++step) {
-                const __half *qr = s_q + g * 128 + q * kStageRows + step * 16 + t;
-                const uint32_t b0 = as_u32(__halves2half2(qr[0], qr[4])), b1 = as_u32(__halves2half2(qr[8], qr[12]));
-                few_packed_step<KB>(sc, c, c + kStageRows * 4 * KW, c + kStageRows * 4 * KW + k_sz, p.k_groups, kg_log2, step * 16, g, t, b0, b1);
+                for (int blk = 0; blk < 4; ++blk) {               // 32 channels, eight neighbours a lane
+                    const int r0 = min(few_element<1>(g, m, 0), there - 1), r1 = min(few_element<1>(g, m, 1), there - 1);
+                    const uint4 x = *reinterpret_cast<const uint4 *>(kp + r0 * kHeadDim + 32 * blk + 8 * t);
+                    const uint4 y = *reinterpret_cast<const uint4 *>(kp + r1 * kHeadDim + 32 * blk + 8 * t);
+                    const uint4 q = *reinterpret_cast<const uint4 *>(s_q + min(g, R - 1) * 128 + 32 * blk + 8 * t);           // columns beyond R are not read
+                    mma16816(sc[m], x.x, y.x, x.y, y.y, q.x, q.y);
+                    mma16816(sc[m], x.z, y.z, x.w, y.w, q.z, q.w);
+                }
             }
-            ++used;
-            __syncwarp();
-            produce();
-        }
-        if (!ok) break;
-        softmax_page(sc, [&](int m, int e) { return few_element<KB>(g, m, e); }, page * kPage, alpha);
-        rescale(out, alpha);
+            dense_scores(sc, [&](int m, int e) { return few_element<1>(g, m, e); });
+            if (softmax_page(page_base)) rescale(o, 2 * t, 2 * t + 1);
 #pragma unroll 1
-        for (int q = 0; q < SPH; ++q) {
-            const int slot = used % stages;
-            ok = __all_sync(0xffffffffu, mbar_wait(s_bar + 8 * slot, used / stages & 1, &p.b.count[2]));
-            if (!ok) break;
-            const uint32_t c = s_ring + slot * stage_bytes;
+            for (int step = 0; step < 8; ++step) {
+                if (16 * step >= there) break;
+                uint32_t x[4][8], b0, b1;
 #pragma unroll
-            for (int step = 0; step < kStageRows / 16; ++step) {
-                uint32_t b0, b1;
-                weights(q * (kStageRows / 16) + step, b0, b1);
-                few_packed_step<VB>(out, c, c + kStageRows * 4 * VW, c + kStageRows * 4 * VW + v_sz, p.v_groups, vg_log2, step * 16, g, t, b0, b1);
+                for (int j = 0; j < 4; ++j) {                     // tokens t + 4j, channels 16g .. 16g + 15; nothing behind the last token
+                    const int r = 16 * step + t + 4 * j;
+                    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+                    if (r < there) {
+                        a = *reinterpret_cast<const uint4 *>(vp + r * kHeadDim + 16 * g);
+                        b = *reinterpret_cast<const uint4 *>(vp + r * kHeadDim + 16 * g + 8);
+                    }
+                    x[j][0] = a.x; x[j][1] = a.y; x[j][2] = a.z; x[j][3] = a.w;
+                    x[j][4] = b.x; x[j][5] = b.y; x[j][6] = b.z; x[j][7] = b.w;
+                }
+                weights(g, step, b0, b1);
+#pragma unroll
+                for (int m = 0; m < 8; ++m) {
+                    uint32_t a[4];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int q = 2 * m + e, c = (q & 3) * 4 + (q >> 2);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) a[e + 2 * j] = prmt(x[2 * j][c >> 1], x[2 * j + 1][c >> 1], c & 1 ? 0x7632 : 0x5410);
+                    }
+                    mma16816(o[m], a[0], a[1], a[2], a[3], b0, b1);
+                }
             }
-            ++used;
-            __syncwarp();
-            produce();
         }
-        if (!ok) break;
+#pragma unroll
+        for (int m = 0; m < 8; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (2 * t + (e & 1) < rows) s_out[(2 * t + (e & 1)) * 128 + few_element<1>(g, m, e >> 1)] = o[m][e];
     }
-    if (!ok) {                                                    // give the copies in flight time to land before the memory is given up
-        for (; used < filled; ++used) mbar_wait(s_bar + 8 * (used % stages), used / stages & 1, &p.b.count[2]);
-    }
+    const float aside_ref = ref;
 
-    // the warps' parts meet
+    // ---- packed pages
+    float out[VT][4], out_mn[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int m = 0; m < VT; ++m)
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) st.l[c] += __shfl_xor_sync(0xffffffffu, st.l[c], o);
-    float *s_ml = reinterpret_cast<float *>(mine);                // [8][2], over the warp's weights
+        for (int e = 0; e < 4; ++e) out[m][e] = 0.f;
+    // values' columns: group and row of B's column g, and of the accumulators' columns 2t, 2t + 1
+    const int vr_log2 = VB == 3 ? 3 : 3 - ng_log2, v_grp = g >> vr_log2, v_row = g & ((1 << vr_log2) - 1), o_row = 2 * t & ((1 << vr_log2) - 1), o_grp = 2 * t >> vr_log2;
+    // p * scale * 2^expo: the power of two starts from the first scales (the largest of them becomes 4 to 8) and goes down where one would exceed 256
+    int expo = 32;
+#pragma unroll 1
+    for (; k < n_mine; ++k) {
+        if (k == ids_base + 32) { fetch_ids(k); pk = max(pk, k); produce(); }
+        const int id = id_of(k), page = page_at(k);
+        if (id < 0 || page >= s.packed) continue;
+        if constexpr (KB == 3) {
+            float sc[11][4];
+#pragma unroll
+            for (int m = 0; m < 11; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[m][e] = 0.f;
+#pragma unroll 1
+            for (int q = 0; q < SPH; ++q) {
+                const uint32_t c = stage_ready();
+                if (!ok) break;
+#pragma unroll 1
+                for (int step = 0; step < kStageRows / 16; ++step) {
+                    uint2 b = make_uint2(0, 0);
+                    if (g < rows) b = *reinterpret_cast<const uint2 *>(s_qs + g * 128 + q * kStageRows + step * 16 + 4 * t);
+                    few_step3(sc, c, c + kStageRows * 4 * KW, c + kStageRows * 4 * KW + k_sz, step * 16, g, t, b.x, b.y);
+                }
+                stage_done();
+            }
+            if (!ok) break;
+            dense_scores(sc, [&](int m, int e) { return few_element<3>(g, m, e); });
+        } else {
+            float sc[CK][8][4], z[CK][4];
+            int row[CK], grp[CK];                                 // of B's column g of each set: pairs (hi, lo) of (group, row)
+            const int kr_log2 = 1 + CK - ng_log2;                 // log2 of the rows that 4 CK pairs hold
+#pragma unroll
+            for (int n = 0; n < CK; ++n) {
+                const int pair = 4 * n + (g >> 1);
+                row[n] = pair & ((1 << kr_log2) - 1);
+                grp[n] = pair >> kr_log2;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    z[n][e] = 0.f;
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) sc[n][m][e] = 0.f;
+                }
+            }
+            const uint32_t lo_mask = g & 1 ? 0xffffffffu : 0u;
+#pragma unroll 1
+            for (int q = 0; q < SPH; ++q) {
+                const uint32_t c = stage_ready(), c_sc = c + kStageRows * 4 * KW, c_mn = c_sc + k_sz;
+                if (!ok) break;
+#pragma unroll 1
+                for (int step = 0; step < kStageRows / 16; ++step) {
+                    const FewWords<KB> a(c, step * 16, g, t);
+                    uint32_t mn[2] = {0, 0}, b[CK][2];
+                    if (g < p.k_groups) few_pairs(c_mn, step * 16, t, p.k_groups, g, mn);
+#pragma unroll
+                    for (int n = 0; n < CK; ++n) {
+                        uint2 qv = make_uint2(0, 0);
+                        uint32_t sv[2];
+                        if (row[n] < rows) qv = *reinterpret_cast<const uint2 *>(s_qs + row[n] * 128 + q * kStageRows + step * 16 + 4 * t);
+                        few_pairs(c_sc, step * 16, t, p.k_groups, grp[n], sv);
+                        b[n][0] = hilo(as_h2(qv.x), as_h2(sv[0]), lo_mask);
+                        b[n][1] = hilo(as_h2(qv.y), as_h2(sv[1]), lo_mask);
+                        mma16816(z[n], mn[0], 0u, mn[1], 0u, qv.x & ~lo_mask, qv.y & ~lo_mask);
+                    }
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) {
+                        const uint32_t a0 = a.a(m, 0), a1 = a.a(m, 1), a2 = a.a(m, 2), a3 = a.a(m, 3);
+#pragma unroll
+                        for (int n = 0; n < CK; ++n) mma16816(sc[n][m], a0, a1, a2, a3, b[n][0], b[n][1]);
+                    }
+                }
+                stage_done();
+            }
+            if (!ok) break;
+#pragma unroll
+            for (int n = 0; n < CK; ++n) {
+                const int pair = 4 * n + t, r = pair & ((1 << kr_log2) - 1);
+                const float zero = __shfl_sync(0xffffffffu, z[n][0], 4 * own_group + t);
+                if (pair >> kr_log2 == own_group && r < rows) {
+#pragma unroll
+                    for (int m = 0; m < 8; m += 2) {
+                        float v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = fmaf(sc[n][m + (e >> 1)][2 * (e & 1)] + sc[n][m + (e >> 1)][2 * (e & 1) + 1], few_power<KB>(m + (e >> 1), e & 1), zero);
+                        sts_f4(s_s + r * 512 + (16 * g + 2 * m) * 4, v[0], v[1], v[2], v[3]);
+                    }
+                }
+            }
+        }
+        if (softmax_page(page * kPage)) {
+            rescale(out, o_row, o_row + 1);
+            if constexpr (VB != 3) {
+                const float a0 = __shfl_sync(0xffffffffu, alpha, o_row), a1 = __shfl_sync(0xffffffffu, alpha, o_row + 1);
+                out_mn[0] *= a0;
+                out_mn[1] *= a1;
+            }
+        }
+#pragma unroll 1
+        for (int q = 0; q < SPH; ++q) {
+            const uint32_t c = stage_ready(), c_sc = c + kStageRows * 4 * VW, c_mn = c_sc + v_sz;
+            if (!ok) break;
+            if constexpr (VB == 3) {
+#pragma unroll 1
+                for (int step = 0; step < kStageRows / 16; ++step) {
+                    uint32_t b0, b1;
+                    weights(g, q * (kStageRows / 16) + step, b0, b1);
+                    few_step3(out, c, c_sc, c_mn, step * 16, g, t, b0, b1);
+                }
+            } else {
+                uint32_t sv[2][2];
+#pragma unroll
+                for (int step = 0; step < 2; ++step) few_pairs(c_sc, step * 16, t, p.v_groups, v_grp, sv[step]);
+                const uint32_t m2 = as_u32(__hmax2(__hmax2(as_h2(sv[0][0]), as_h2(sv[0][1])), __hmax2(as_h2(sv[1][0]), as_h2(sv[1][1]))));
+                const int top = (int)(__reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16)) >> 10 & 31);       // exponent of the stage's largest scale
+                if (top + expo > 15 + 7) {                        // rare: the first stage, and where scales grow 2^5 fold
+                    const int want = min(max(17 - top, -13), 15);
+                    if (want < expo) {
+                        const float f = expo == 32 ? 0.f : exp2f((float)(want - expo));
+#pragma unroll
+                        for (int m = 0; m < 8; ++m)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) out[m][e] *= f;
+                        expo = want;
+                    }
+                }
+                const __half2 by = as_h2((uint32_t)(expo + 15) << 10 | (uint32_t)(expo + 15) << 26);
+#pragma unroll
+                for (int step = 0; step < 2; ++step) {
+                    const FewWords<VB> a(c, step * 16, g, t);
+                    uint32_t b0, b1, mn[2] = {0, 0};
+                    weights(v_row, q * 2 + step, b0, b1);
+                    if (g < p.v_groups) few_pairs(c_mn, step * 16, t, p.v_groups, g, mn);
+                    mma16816(out_mn, mn[0], 0u, mn[1], 0u, b0, b1);
+                    b0 = as_u32(__hmul2(as_h2(b0), __hmul2(as_h2(sv[step][0]), by)));
+                    b1 = as_u32(__hmul2(as_h2(b1), __hmul2(as_h2(sv[step][1]), by)));
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) mma16816(out[m], a.a(m, 0), a.a(m, 1), a.a(m, 2), a.a(m, 3), b0, b1);
+                }
+            }
+            stage_done();
+        }
+        if (!ok) break;
+    }
+    if (!ok)                                                      // copies in flight land before the memory is given up
+        for (; in_flight > 0; --in_flight) {
+            mbar_wait(s_bar + 8 * use_slot, parity, &p.b.count[2]);
+            if (++use_slot == stages) { use_slot = 0; parity ^= 1; }
+        }
+
+    // ---- the warps' parts meet: sums put aside and sums of packed pages under the last reference
+    const float aside_by = ref == -INFINITY ? 0.f : exp2_approx(aside_ref - ref);         // of row `lane`
     __syncwarp();
-    if (g == 0) {
+    auto add = [&](int r, int c, float v, float by) { s_out[r * 128 + c] = fmaf(s_out[r * 128 + c], by, v); };
+    if constexpr (VB == 3) {
+        const float f0 = __shfl_sync(0xffffffffu, aside_by, 2 * t), f1 = __shfl_sync(0xffffffffu, aside_by, 2 * t + 1);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            s_ml[2 * (2 * t + c)] = st.m[c];
-            s_ml[2 * (2 * t + c) + 1] = st.l[c];
+        for (int m = 0; m < 11; ++m)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = few_element<3>(g, m, e);
+                if (c >= 0 && 2 * t < rows) add(2 * t, c, out[m][2 * e], f0);
+                if (c >= 0 && 2 * t + 1 < rows) add(2 * t + 1, c, out[m][2 * e + 1], f1);
+            }
+    } else {
+        const float f0 = __shfl_sync(0xffffffffu, aside_by, o_row), f1 = __shfl_sync(0xffffffffu, aside_by, o_row + 1);
+        const float z0 = __shfl_sync(0xffffffffu, out_mn[0], 4 * own_group + t), z1 = __shfl_sync(0xffffffffu, out_mn[1], 4 * own_group + t);
+        const float undo = expo == 32 ? 0.f : exp2f((float)-expo);
+        if (o_grp == own_group) {
+#pragma unroll
+            for (int m = 0; m < 8; ++m)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int c = few_element<1>(g, m, e);
+                    const float f = few_power<VB>(m, e) * undo;
+                    if (o_row < rows) add(o_row, c, fmaf(out[m][2 * e], f, z0), f0);
+                    if (o_row + 1 < rows) add(o_row + 1, c, fmaf(out[m][2 * e + 1], f, z1), f1);
+                }
         }
     }
-    if constexpr (VB == 3) {
-        float f[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) f[c] = aside && aside_m[c] != -INFINITY ? exp2_approx(aside_m[c] - st.m[c]) : 0.f;
-        __syncwarp();
-        each_out(out, [&](int m, int e) { return few_element<3>(g, m, e); }, [&](int r, int c, float v) { s_out[r * 128 + c] = s_out[r * 128 + c] * f[r & 1] + v; });
-    } else {
-        each_out(out, [&](int m, int e) { return few_element<1>(g, m, e); }, [&](int r, int c, float v) { s_out[r * 128 + c] = v; });
-    }
+    __syncwarp();
+    // reference and sum of weights of row `lane`, over the first scores
+    float l = 0.f;
+    if (lane < rows)
+        for (int j = 0; j < 32; ++j) l += __uint_as_float(lds32(s_sum + lane * 128 + 4 * j));
+    if (lane < rows) asm volatile("st.shared.v2.f32 [%0], {%1, %2};\n" ::"r"(s_s + lane * 8), "f"(ref), "f"(l) : "memory");
     __syncthreads();
-    const int warp_bytes = kFewRows * kPStride * 2 + kMaxStages * 8 + stages * stage_bytes;
-    const float *all_out = reinterpret_cast<const float *>(smem + 2048 + kFewWarps * warp_bytes);
     for (int r = 0; r < rows; ++r) {
-        float m = -INFINITY, l = 0.f, v = 0.f;
+        float m = -INFINITY, v = 0.f;
+        l = 0.f;
+        auto part = [&](int w) { return reinterpret_cast<const float *>(smem + sh.warps + w * sh.warp_bytes + sh.scores) + 2 * r; };
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) m = fmaxf(m, reinterpret_cast<const float *>(smem + 2048 + w * warp_bytes)[2 * r]);
+        for (int w = 0; w < kFewWarps; ++w) m = fmaxf(m, part(w)[0]);
 #pragma unroll
         for (int w = 0; w < kFewWarps; ++w) {
-            const float *ml = reinterpret_cast<const float *>(smem + 2048 + w * warp_bytes) + 2 * r;
-            const float f = part_factor(ml[0], ml[1], m);
-            l += f * ml[1];
-            if (f != 0.f) v += f * all_out[(w * kFewRows + r) * 128 + threadIdx.x];
+            const float f = part_factor(part(w)[0], part(w)[1], m);
+            l += f * part(w)[1];
+            if (f != 0.f) v += f * reinterpret_cast<const float *>(smem + sh.warps + w * sh.warp_bytes + sh.aside)[r * 128 + threadIdx.x];
         }
-        const int64_t row = (int64_t)(s.q0 + r / p.rep) * p.a.nh + head * p.rep + r % p.rep;
+        const int u = s.q0 + (row0 + r) / p.rep, h = head * p.rep + (row0 + r) % p.rep;
         if (p.splits == 1) {
-            static_cast<__half *>(p.a.out)[(int64_t)(s.q0 + r / p.rep) * p.a.o_sT + (int64_t)(head * p.rep + r % p.rep) * p.a.o_sH + threadIdx.x] =
-                __float2half_rn(l == 0.f ? 0.f : v / l);
+            static_cast<__half *>(p.a.out)[(int64_t)u * p.a.o_sT + (int64_t)h * p.a.o_sH + threadIdx.x] = __float2half_rn(l == 0.f ? 0.f : v / l);
         } else {
-            const int64_t at = (int64_t)split * p.a.tokens * p.a.nh + row;
+            const int64_t at = (int64_t)split * p.a.tokens * p.a.nh + (int64_t)u * p.a.nh + h;
             p.part_out[at * 128 + threadIdx.x] = v;
             if (threadIdx.x == 0) { p.part_ml[2 * at] = m; p.part_ml[2 * at + 1] = l; }
         }
@@ -487,22 +642,39 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant_
     static_cast<__half *>(p.a.out)[(int64_t)u * p.a.o_sT + (int64_t)h * p.a.o_sH + threadIdx.x] = __float2half_rn(l == 0.f ? 0.f : v / l);
 }
 
-template <int KB, int VB>
-static int launch_few(const PagedArgs &p, cudaStream_t st) {
+template <int KB, int VB, int CK>
+static int launch_few(const PagedArgs &p, int R, int row_blocks, cudaStream_t st) {
     const int k_bytes = kStageRows * (4 * page_words(KB) + 4 * p.k_groups), v_bytes = kStageRows * (4 * page_words(VB) + 4 * p.v_groups);
-    const int stage_bytes = (k_bytes > v_bytes ? k_bytes : v_bytes), ctas = KB == 3 || VB == 3 ? 3 : 4;
+    const int stage_bytes = k_bytes > v_bytes ? k_bytes : v_bytes, ctas = KB == 3 || VB == 3 || CK == 2 ? 3 : 4;
     // what 227 KB leave each of the CTAs of an SM (1 KB of each is the system's)
-    const int fixed = 2048 + kFewWarps * (kFewRows * kPStride * 2 + kMaxStages * 8) + kFewWarps * kFewRows * 128 * 4;
-    const int room = (227 * 1024 / ctas - 1024 - fixed) / kFewWarps;
+    const int room = (227 * 1024 / ctas - 1024 - FewShared(R, 0, 0).total) / kFewWarps;
     int stages = room / stage_bytes;
     stages = stages < 2 ? 2 : stages > kMaxStages ? kMaxStages : stages;
-    const size_t smem = fixed + (size_t)kFewWarps * stages * stage_bytes;
-    const cudaError_t e = cudaFuncSetAttribute(paged_few_kernel<KB, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const size_t smem = FewShared(R, stages, stage_bytes).total;
+    const cudaError_t e = cudaFuncSetAttribute(paged_few_kernel<KB, VB, CK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return record_cuda_error(e);
-    const int64_t grid = (int64_t)p.a.n * p.l.Hkv * p.splits;
+    const int64_t grid = (int64_t)p.a.n * p.l.Hkv * row_blocks * p.splits;
     if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
-    paged_few_kernel<KB, VB><<<(unsigned)grid, kFewWarps * 32, smem, st>>>(p, stages, stage_bytes);
+    paged_few_kernel<KB, VB, CK><<<(unsigned)grid, kFewWarps * 32, smem, st>>>(p, R, row_blocks, stages, stage_bytes);
     return check_launch();
+}
+
+// Query rows of a CTA: as many as the columns of an MMA hold with all groups (keys twice, as hi and lo, in one or two sets of columns).
+template <int KB, int VB>
+static int launch_few(const PagedArgs &p, cudaStream_t st) {
+    const int64_t most = (int64_t)p.a.max_new * p.rep;
+    const int rows = most < kFewRows ? (int)most : kFewRows, ng = kHeadDim / p.l.group;
+    int R = kFewRows;
+    if (VB != 3) R = 8 / ng;
+    if constexpr (KB != 3) {
+        if (rows <= 4 / ng) R = 4 / ng;
+        else if (R > 8 / ng) R = 8 / ng;
+        if (R == 4 / ng) return launch_few<KB, VB, 1>(p, R, (rows + R - 1) / R, st);
+        return launch_few<KB, VB, 2>(p, R, (rows + R - 1) / R, st);
+    } else {
+        if (R > rows) R = rows;
+        return launch_few<KB, VB, 1>(p, R, (rows + R - 1) / R, st);
+    }
 }
 
 int paged_few(const PagedArgs &p, cudaStream_t st) {
