@@ -572,7 +572,7 @@ typedef struct {
     uint64_t workspace_bytes;
 } kvq_paged_attn_args;
 
-uint64_t kvq_paged_attn_workspace_bytes(int32_t n, int32_t tokens, int32_t nh, int32_t Hkv, int32_t max_new, int32_t max_tokens);
+uint64_t kvq_paged_attn_workspace_bytes(const kvq_page_layer *l, int32_t n, int32_t tokens, int32_t nh, int32_t max_new, int32_t max_tokens);
 int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, const kvq_paged_attn_args *a, kvq_stream_t stream);
 
 #ifdef __cplusplus

@@ -168,7 +168,7 @@ def lib():
                           (L.kvq_pages_fork, [blk, vp, vp, i32, vp, vp]), (L.kvq_pages_compact, [blk, vp, vp]),
                           (L.kvq_page_copy, [blk, i32, vp, i32, vp]), (L.kvq_page_write, [blk, blk, blk, vp]), (L.kvq_paged_attn, [blk, blk, blk, vp])):
             fn.restype, fn.argtypes = C.c_int, types
-        L.kvq_paged_attn_workspace_bytes.restype, L.kvq_paged_attn_workspace_bytes.argtypes = u64, [i32] * 6
+        L.kvq_paged_attn_workspace_bytes.restype, L.kvq_paged_attn_workspace_bytes.argtypes = u64, [blk] + [i32] * 5
         _lib = L
     return _lib
 

@@ -14,24 +14,31 @@ struct PagedPlan {
     int few_splits, tile_splits, max_tiles;
 };
 
-static PagedPlan paged_plan(int n, int tokens, int nh, int Hkv, int max_new, int max_tokens) {
+static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, int max_new, int max_tokens) {
     PagedPlan r = {};
-    const int rep = nh / Hkv;
+    const int rep = nh / l.Hkv;
     const int64_t most = (int64_t)max_new * rep;
     r.tiles = most > kFewRows;
     // every sequence has its max_new tokens, or it is the only one: nothing for the kernel of few rows in a call that needs the other
     r.few = rep <= kFewRows && (!r.tiles || (n > 1 && tokens < (int64_t)n * max_new));
     r.few_rows = r.few ? kFewRows : 0;
     const int pages = (max_tokens + kPage - 1) / kPage;
-    const int64_t pairs = (int64_t)n * Hkv;
-    const int64_t want = (148 * 4 + pairs / 2) / pairs;           // four CTAs to an SM
-    r.few_splits = (int)(want < 1 ? 1 : want);
-    if (r.few_splits > (pages + 3) / 4) r.few_splits = (pages + 3) / 4;          // a page for each of a CTA's warps
-    if (r.few_splits < 1) r.few_splits = 1;
+    // Kernel of few rows: the splits that take the fewest rounds of pages (four warps a CTA), over all waves of CTAs; a CTA's beginning and
+    // end count two rounds, the launch that joins the splits another two.
+    const FewShape f = few_shape(l, rep, max_new);
+    const int64_t pairs = (int64_t)n * l.Hkv * f.row_blocks, slots = 148 * f.ctas;
+    double best = 1e30;
+    r.few_splits = 1;
+    for (int s = 1; s <= 128 && (s == 1 || s <= pages / 2); ++s) {
+        const double w = (double)(pairs * s) / slots, waves = w <= 1 ? 1 : w < 4 ? (double)((pairs * s + slots - 1) / slots) : w + 0.5;
+        const int rounds = ((pages + s - 1) / s + 3) / 4;
+        const double cost = waves * (rounds + 2) + (s > 1 ? 2 : 0);
+        if (cost < best) { best = cost; r.few_splits = s; }
+    }
     int64_t tiles = ((int64_t)tokens * rep) / 256 + n;
     if (n == 1) tiles = ((int64_t)tokens * rep + 255) / 256;
     r.max_tiles = (int)(tiles < INT32_MAX ? tiles : INT32_MAX);
-    const int64_t ctas = tiles * Hkv;
+    const int64_t ctas = tiles * l.Hkv;
     r.tile_splits = (int)(ctas < 1 ? 1 : 148 / ctas);
     if (r.tile_splits > (pages + 3) / 4) r.tile_splits = (pages + 3) / 4;
     if (r.tile_splits < 1) r.tile_splits = 1;
@@ -45,10 +52,10 @@ static uint64_t paged_bytes(const PagedPlan &r, int tokens, int nh) {
 
 }  // namespace kvq
 
-extern "C" uint64_t kvq_paged_attn_workspace_bytes(int32_t n, int32_t tokens, int32_t nh, int32_t Hkv, int32_t max_new, int32_t max_tokens) {
+extern "C" uint64_t kvq_paged_attn_workspace_bytes(const kvq_page_layer *l, int32_t n, int32_t tokens, int32_t nh, int32_t max_new, int32_t max_tokens) {
     using namespace kvq;
-    if (n <= 0 || tokens <= 0 || Hkv <= 0 || nh <= 0 || nh % Hkv || max_new <= 0 || max_tokens <= 0) return 0;
-    return paged_bytes(paged_plan(n, tokens, nh, Hkv, max_new, max_tokens), tokens, nh);
+    if (check_layer(l) || n <= 0 || tokens <= 0 || nh <= 0 || nh % l->Hkv || max_new <= 0 || max_tokens <= 0) return 0;
+    return paged_bytes(paged_plan(*l, n, tokens, nh, max_new, max_tokens), tokens, nh);
 }
 
 extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, const kvq_paged_attn_args *a, kvq_stream_t stream) {
@@ -62,7 +69,7 @@ extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, c
     if (a->max_new <= 0 || a->max_tokens <= 0) return KVQ_ERR_SHAPE;
     if (!a->q || !a->out || !a->q_start || !a->rows) return KVQ_ERR_NULL;
     if (!(a->softcap >= 0.f) || !(a->softmax_scale == a->softmax_scale)) return KVQ_ERR_SHAPE;
-    const PagedPlan r = paged_plan(a->n, a->tokens, a->nh, l->Hkv, a->max_new, a->max_tokens);
+    const PagedPlan r = paged_plan(*l, a->n, a->tokens, a->nh, a->max_new, a->max_tokens);
     const uint64_t need = paged_bytes(r, a->tokens, a->nh);
     if (need && (!a->workspace || a->workspace_bytes < need)) return KVQ_ERR_WORKSPACE;
     if (need && reinterpret_cast<uintptr_t>(a->workspace) % 16) return KVQ_ERR_ALIGN;

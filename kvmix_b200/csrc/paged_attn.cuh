@@ -50,6 +50,24 @@ __device__ __forceinline__ void paged_bounds(const PagedArgs &p, const PagedSeq 
     if (pos < 0) hi = lo;                                         // more new tokens than the sequence has
 }
 
+// A CTA of the kernel of few rows: as many query rows as the columns of an MMA hold with all groups (keys twice, as hi and lo, in one or two
+// sets of columns); CTAs of an SM.
+struct FewShape { int rows, row_blocks, key_sets, ctas; };
+inline FewShape few_shape(const kvq_page_layer &l, int rep, int max_new) {
+    const int64_t most = (int64_t)max_new * rep;
+    const int rows = most < kFewRows ? (int)most : kFewRows, ng = kHeadDim / l.group;
+    FewShape f = {kFewRows, 1, 1, l.k_bits == 3 || l.v_bits == 3 ? 3 : 4};
+    if (l.v_bits != 3) f.rows = 8 / ng;
+    if (l.k_bits != 3) {
+        if (rows <= 4 / ng) f.rows = 4 / ng;
+        else { f.rows = 8 / ng; f.key_sets = 2; f.ctas = 3; }
+    } else if (f.rows > rows) {
+        f.rows = rows < 1 ? 1 : rows;
+    }
+    f.row_blocks = (rows + f.rows - 1) / f.rows;
+    return f;
+}
+
 // 2^x for x <= some tens, one instruction; denormal results flush to zero.
 __device__ __forceinline__ float exp2_approx(float x) {
     float r;

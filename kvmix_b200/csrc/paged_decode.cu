@@ -16,10 +16,9 @@ namespace kvq {
 // An accumulator row needs the column of its own group only; what the others hold is not read.  Minima times q or p come from one more MMA
 // a k-step, whose rows are the groups.  3-bit words are groups of their own, so their fields become fp16 values (code * scale + minimum,
 // rounded once) and the columns are query rows.
-// Words arrive by bulk copies, 32 contraction rows (codes, scales, minima) a stage, in the warp's own ring; fp16 pages go straight to
+// Words arrive by bulk copies, 32 to 128 contraction rows (codes, scales, minima) a stage, in the warp's own ring; fp16 pages go straight to
 // registers, first, and their sums are put aside in shared memory.
 constexpr int kFewWarps = 4;
-constexpr int kStageRows = 32;
 constexpr int kMaxStages = 8;
 constexpr int kPStride = 136;                                     // halves between rows of weights
 constexpr float kWeightBits = 7.f;                                // weights are 2^7 p: p * scale keeps away from fp16's smallest numbers
@@ -82,7 +81,7 @@ __device__ __forceinline__ void few_pairs(uint32_t at, int row, int t, int group
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const uint32_t r0 = at + ((row + t + 8 * j) * groups + grp) * 2;
-        v[j] = lds16(r0) | lds16(r0 + 8 * groups) << 16;
+        v[j] = prmt(lds16(r0), lds16(r0 + 8 * groups), 0x5410);
     }
 }
 
@@ -154,7 +153,7 @@ struct FewShared {
 
 template <int KB, int VB, int CK>
 __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 ? 3 : 4)
-    paged_few_kernel(const __grid_constant__ PagedArgs p, int R, int row_blocks, int stages, int stage_bytes) {
+    paged_few_kernel(const __grid_constant__ PagedArgs p, int R, int row_blocks, int stages, int stage_rows, int stage_bytes) {
     extern __shared__ __align__(128) char smem[];
     const FewShared sh(R, stages, stage_bytes);
     const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -217,8 +216,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
     auto page_at = [&](int k) { return p1 - 1 - (k * kFewWarps + warp); };        // newest first: fp16 pages come at the beginning
 
     constexpr int KW = page_words(KB), VW = page_words(VB), VT = VB == 3 ? 11 : 8;
-    const uint32_t k_sz = kStageRows * p.k_groups * 2, v_sz = kStageRows * p.v_groups * 2;
-    constexpr int SPH = kPage / kStageRows;                       // stages of a page's keys, and of its values
+    const uint32_t k_cb = stage_rows * 4 * KW, v_cb = stage_rows * 4 * VW, k_sz = stage_rows * p.k_groups * 2, v_sz = stage_rows * p.v_groups * 2;
+    const int half_stages = kPage / stage_rows;                   // stages of a page's keys, and of its values
     const int ng_log2 = p.l.group == 128 ? 0 : p.l.group == 64 ? 1 : 2;            // of both sides, where they are not 3 bits
     const int own_group = g >> (3 - ng_log2);                     // of the 16 packed elements that this lane's accumulator rows stand for
 
@@ -243,18 +242,24 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
             if (page_at(pk) >= s.packed || id < 0) { ++pk; continue; }
             if (lane == 0) {
                 const uint32_t bar = s_bar + 8 * fill_slot, dst = s_ring + fill_slot * stage_bytes;
-                const bool values = pstage >= SPH;
-                const int64_t row = ((int64_t)id * p.l.Hkv + head) * kPage + (pstage % SPH) * kStageRows;
-                const uint32_t cb = kStageRows * 4 * (values ? VW : KW), sz = values ? v_sz : k_sz;
-                const int groups = values ? p.v_groups : p.k_groups;
-                mbar_expect(bar, cb + 2 * sz);
-                bulk_load(dst, (values ? p.l.vcode + row * VW : p.l.kcode + row * KW), cb, bar);
-                bulk_load(dst + cb, static_cast<const __half *>(values ? p.l.vscale : p.l.kscale) + row * groups, sz, bar);
-                bulk_load(dst + cb + sz, static_cast<const __half *>(values ? p.l.vmn : p.l.kmn) + row * groups, sz, bar);
+                const int64_t at = (int64_t)id * p.l.Hkv + head;
+                if (pstage < half_stages) {
+                    const int off = pstage * stage_rows * p.k_groups;
+                    mbar_expect(bar, k_cb + 2 * k_sz);
+                    bulk_load(dst, p.l.kcode + at * (kPage * KW) + pstage * stage_rows * KW, k_cb, bar);
+                    bulk_load(dst + k_cb, static_cast<const __half *>(p.l.kscale) + at * (kPage * p.k_groups) + off, k_sz, bar);
+                    bulk_load(dst + k_cb + k_sz, static_cast<const __half *>(p.l.kmn) + at * (kPage * p.k_groups) + off, k_sz, bar);
+                } else {
+                    const int st = pstage - half_stages, off = st * stage_rows * p.v_groups;
+                    mbar_expect(bar, v_cb + 2 * v_sz);
+                    bulk_load(dst, p.l.vcode + at * (kPage * VW) + st * stage_rows * VW, v_cb, bar);
+                    bulk_load(dst + v_cb, static_cast<const __half *>(p.l.vscale) + at * (kPage * p.v_groups) + off, v_sz, bar);
+                    bulk_load(dst + v_cb + v_sz, static_cast<const __half *>(p.l.vmn) + at * (kPage * p.v_groups) + off, v_sz, bar);
+                }
             }
             if (++fill_slot == stages) fill_slot = 0;
             ++in_flight;
-            if (++pstage == 2 * SPH) { pstage = 0; ++pk; }
+            if (++pstage == 2 * half_stages) { pstage = 0; ++pk; }
         }
     };
     bool ok = true;
@@ -310,9 +315,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
         __syncwarp();
         return change != 1.f;                                     // the same in all lanes
     };
-    auto weights = [&](int row, int step, uint32_t &b0, uint32_t &b1) {           // contraction rows 16 step + t + 4j
-        b0 = b1 = 0;
-        if (row < rows) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(b0), "=r"(b1) : "r"(s_p + (row * kPStride + 16 * step + 4 * t) * 2));
+    auto weights = [&](int row, int step, uint32_t &b0, uint32_t &b1) {           // contraction rows 16 step + t + 4j; columns beyond R are not read
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(b0), "=r"(b1) : "r"(s_p + (row * kPStride + 16 * step + 4 * t) * 2));
     };
     // Columns that are query rows: scores of accumulators into s_s, factors of columns 2t, 2t + 1
     auto dense_scores = [&](auto &sc, auto element) {
@@ -384,7 +388,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
                     x[j][0] = a.x; x[j][1] = a.y; x[j][2] = a.z; x[j][3] = a.w;
                     x[j][4] = b.x; x[j][5] = b.y; x[j][6] = b.z; x[j][7] = b.w;
                 }
-                weights(g, step, b0, b1);
+                weights(min(g, R - 1), step, b0, b1);
 #pragma unroll
                 for (int m = 0; m < 8; ++m) {
                     uint32_t a[4];
@@ -413,7 +417,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[m][e] = 0.f;
     // values' columns: group and row of B's column g, and of the accumulators' columns 2t, 2t + 1
-    const int vr_log2 = VB == 3 ? 3 : 3 - ng_log2, v_grp = g >> vr_log2, v_row = g & ((1 << vr_log2) - 1), o_row = 2 * t & ((1 << vr_log2) - 1), o_grp = 2 * t >> vr_log2;
+    const int vr_log2 = VB == 3 ? 3 : 3 - ng_log2, v_grp = g >> vr_log2, v_row = min(g & ((1 << vr_log2) - 1), R - 1), o_row = 2 * t & ((1 << vr_log2) - 1), o_grp = 2 * t >> vr_log2;
     // p * scale * 2^expo: the power of two starts from the first scales (the largest of them becomes 4 to 8) and goes down where one would exceed 256
     int expo = 32;
 #pragma unroll 1
@@ -428,14 +432,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[m][e] = 0.f;
 #pragma unroll 1
-            for (int q = 0; q < SPH; ++q) {
+            for (int q = 0; q < half_stages; ++q) {
                 const uint32_t c = stage_ready();
                 if (!ok) break;
+                const __half *qv = s_qs + min(g, R - 1) * 128 + q * stage_rows + 4 * t;
 #pragma unroll 1
-                for (int step = 0; step < kStageRows / 16; ++step) {
-                    uint2 b = make_uint2(0, 0);
-                    if (g < rows) b = *reinterpret_cast<const uint2 *>(s_qs + g * 128 + q * kStageRows + step * 16 + 4 * t);
-                    few_step3(sc, c, c + kStageRows * 4 * KW, c + kStageRows * 4 * KW + k_sz, step * 16, g, t, b.x, b.y);
+                for (int row = 0; row < stage_rows; row += 16) {
+                    const uint2 b = *reinterpret_cast<const uint2 *>(qv + row);
+                    few_step3(sc, c, c + k_cb, c + k_cb + k_sz, row, g, t, b.x, b.y);
                 }
                 stage_done();
             }
@@ -459,20 +463,20 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
             }
             const uint32_t lo_mask = g & 1 ? 0xffffffffu : 0u;
 #pragma unroll 1
-            for (int q = 0; q < SPH; ++q) {
-                const uint32_t c = stage_ready(), c_sc = c + kStageRows * 4 * KW, c_mn = c_sc + k_sz;
+            for (int q = 0; q < half_stages; ++q) {
+                const uint32_t c = stage_ready(), c_sc = c + k_cb, c_mn = c_sc + k_sz;
                 if (!ok) break;
+                const __half *q_at = s_qs + q * stage_rows + 4 * t;
 #pragma unroll 1
-                for (int step = 0; step < kStageRows / 16; ++step) {
-                    const FewWords<KB> a(c, step * 16, g, t);
-                    uint32_t mn[2] = {0, 0}, b[CK][2];
-                    if (g < p.k_groups) few_pairs(c_mn, step * 16, t, p.k_groups, g, mn);
+                for (int at = 0; at < stage_rows; at += 16) {
+                    const FewWords<KB> a(c, at, g, t);
+                    uint32_t mn[2], b[CK][2];
+                    few_pairs(c_mn, at, t, p.k_groups, g & (p.k_groups - 1), mn);              // rows beyond the groups are not read
 #pragma unroll
                     for (int n = 0; n < CK; ++n) {
-                        uint2 qv = make_uint2(0, 0);
+                        const uint2 qv = *reinterpret_cast<const uint2 *>(q_at + row[n] * 128 + at);
                         uint32_t sv[2];
-                        if (row[n] < rows) qv = *reinterpret_cast<const uint2 *>(s_qs + row[n] * 128 + q * kStageRows + step * 16 + 4 * t);
-                        few_pairs(c_sc, step * 16, t, p.k_groups, grp[n], sv);
+                        few_pairs(c_sc, at, t, p.k_groups, grp[n], sv);
                         b[n][0] = hilo(as_h2(qv.x), as_h2(sv[0]), lo_mask);
                         b[n][1] = hilo(as_h2(qv.y), as_h2(sv[1]), lo_mask);
                         mma16816(z[n], mn[0], 0u, mn[1], 0u, qv.x & ~lo_mask, qv.y & ~lo_mask);
@@ -511,22 +515,22 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
             }
         }
 #pragma unroll 1
-        for (int q = 0; q < SPH; ++q) {
-            const uint32_t c = stage_ready(), c_sc = c + kStageRows * 4 * VW, c_mn = c_sc + v_sz;
+        for (int q = 0; q < half_stages; ++q) {
+            const uint32_t c = stage_ready(), c_sc = c + v_cb, c_mn = c_sc + v_sz;
             if (!ok) break;
+            const int step0 = q * (stage_rows / 16);
             if constexpr (VB == 3) {
 #pragma unroll 1
-                for (int step = 0; step < kStageRows / 16; ++step) {
+                for (int at = 0; at < stage_rows; at += 16) {
                     uint32_t b0, b1;
-                    weights(g, q * (kStageRows / 16) + step, b0, b1);
-                    few_step3(out, c, c_sc, c_mn, step * 16, g, t, b0, b1);
+                    weights(min(g, R - 1), step0 + at / 16, b0, b1);
+                    few_step3(out, c, c_sc, c_mn, at, g, t, b0, b1);
                 }
             } else {
-                uint32_t sv[2][2];
-#pragma unroll
-                for (int step = 0; step < 2; ++step) few_pairs(c_sc, step * 16, t, p.v_groups, v_grp, sv[step]);
-                const uint32_t m2 = as_u32(__hmax2(__hmax2(as_h2(sv[0][0]), as_h2(sv[0][1])), __hmax2(as_h2(sv[1][0]), as_h2(sv[1][1]))));
-                const int top = (int)(__reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16)) >> 10 & 31);       // exponent of the stage's largest scale
+                // the exponent of the stage's largest scale: its scales are stage_rows * groups / 32 a lane, two at a time
+                uint32_t m2 = 0;
+                for (int w = lane; w < stage_rows * p.v_groups / 2; w += 32) m2 = as_u32(__hmax2(as_h2(m2), as_h2(lds32(c_sc + 4 * w))));
+                const int top = (int)(__reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16)) >> 10 & 31);
                 if (top + expo > 15 + 7) {                        // rare: the first stage, and where scales grow 2^5 fold
                     const int want = min(max(17 - top, -13), 15);
                     if (want < expo) {
@@ -538,16 +542,17 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
                         expo = want;
                     }
                 }
-                const __half2 by = as_h2((uint32_t)(expo + 15) << 10 | (uint32_t)(expo + 15) << 26);
-#pragma unroll
-                for (int step = 0; step < 2; ++step) {
-                    const FewWords<VB> a(c, step * 16, g, t);
-                    uint32_t b0, b1, mn[2] = {0, 0};
-                    weights(v_row, q * 2 + step, b0, b1);
-                    if (g < p.v_groups) few_pairs(c_mn, step * 16, t, p.v_groups, g, mn);
+                const __half2 by = as_h2((uint32_t)(expo + 15) * 0x04000400u);
+#pragma unroll 1
+                for (int at = 0; at < stage_rows; at += 16) {
+                    const FewWords<VB> a(c, at, g, t);
+                    uint32_t b0, b1, mn[2], sv[2];
+                    weights(v_row, step0 + at / 16, b0, b1);
+                    few_pairs(c_mn, at, t, p.v_groups, g & (p.v_groups - 1), mn);
+                    few_pairs(c_sc, at, t, p.v_groups, v_grp, sv);
                     mma16816(out_mn, mn[0], 0u, mn[1], 0u, b0, b1);
-                    b0 = as_u32(__hmul2(as_h2(b0), __hmul2(as_h2(sv[step][0]), by)));
-                    b1 = as_u32(__hmul2(as_h2(b1), __hmul2(as_h2(sv[step][1]), by)));
+                    b0 = as_u32(__hmul2(as_h2(b0), __hmul2(as_h2(sv[0]), by)));
+                    b1 = as_u32(__hmul2(as_h2(b1), __hmul2(as_h2(sv[1]), by)));
 #pragma unroll
                     for (int m = 0; m < 8; ++m) mma16816(out[m], a.a(m, 0), a.a(m, 1), a.a(m, 2), a.a(m, 3), b0, b1);
                 }
@@ -644,10 +649,14 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant_
 
 template <int KB, int VB, int CK>
 static int launch_few(const PagedArgs &p, int R, int row_blocks, cudaStream_t st) {
-    const int k_bytes = kStageRows * (4 * page_words(KB) + 4 * p.k_groups), v_bytes = kStageRows * (4 * page_words(VB) + 4 * p.v_groups);
-    const int stage_bytes = k_bytes > v_bytes ? k_bytes : v_bytes, ctas = KB == 3 || VB == 3 || CK == 2 ? 3 : 4;
-    // what 227 KB leave each of the CTAs of an SM (1 KB of each is the system's)
+    const int k_row = 4 * page_words(KB) + 4 * p.k_groups, v_row = 4 * page_words(VB) + 4 * p.v_groups, row = k_row > v_row ? k_row : v_row;
+    const int ctas = KB == 3 || VB == 3 || CK == 2 ? 3 : 4;
+    // what 227 KB leave each of the CTAs of an SM (1 KB of each is the system's): two stages at least, of as many rows as that allows (a stage costs some
+    // 100 instructions besides its rows)
     const int room = (227 * 1024 / ctas - 1024 - FewShared(R, 0, 0).total) / kFewWarps;
+    int stage_rows = kPage;
+    while (stage_rows > 32 && 2 * stage_rows * row > room) stage_rows /= 2;
+    const int stage_bytes = stage_rows * row;
     int stages = room / stage_bytes;
     stages = stages < 2 ? 2 : stages > kMaxStages ? kMaxStages : stages;
     const size_t smem = FewShared(R, stages, stage_bytes).total;
@@ -655,26 +664,16 @@ static int launch_few(const PagedArgs &p, int R, int row_blocks, cudaStream_t st
     if (e != cudaSuccess) return record_cuda_error(e);
     const int64_t grid = (int64_t)p.a.n * p.l.Hkv * row_blocks * p.splits;
     if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
-    paged_few_kernel<KB, VB, CK><<<(unsigned)grid, kFewWarps * 32, smem, st>>>(p, R, row_blocks, stages, stage_bytes);
+    paged_few_kernel<KB, VB, CK><<<(unsigned)grid, kFewWarps * 32, smem, st>>>(p, R, row_blocks, stages, stage_rows, stage_bytes);
     return check_launch();
 }
 
-// Query rows of a CTA: as many as the columns of an MMA hold with all groups (keys twice, as hi and lo, in one or two sets of columns).
 template <int KB, int VB>
 static int launch_few(const PagedArgs &p, cudaStream_t st) {
-    const int64_t most = (int64_t)p.a.max_new * p.rep;
-    const int rows = most < kFewRows ? (int)most : kFewRows, ng = kHeadDim / p.l.group;
-    int R = kFewRows;
-    if (VB != 3) R = 8 / ng;
-    if constexpr (KB != 3) {
-        if (rows <= 4 / ng) R = 4 / ng;
-        else if (R > 8 / ng) R = 8 / ng;
-        if (R == 4 / ng) return launch_few<KB, VB, 1>(p, R, (rows + R - 1) / R, st);
-        return launch_few<KB, VB, 2>(p, R, (rows + R - 1) / R, st);
-    } else {
-        if (R > rows) R = rows;
-        return launch_few<KB, VB, 1>(p, R, (rows + R - 1) / R, st);
-    }
+    const FewShape f = few_shape(p.l, p.rep, p.a.max_new);
+    if constexpr (KB != 3)
+        if (f.key_sets == 2) return launch_few<KB, VB, 2>(p, f.rows, f.row_blocks, st);
+    return launch_few<KB, VB, 1>(p, f.rows, f.row_blocks, st);
 }
 
 int paged_few(const PagedArgs &p, cudaStream_t st) {

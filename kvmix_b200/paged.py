@@ -279,7 +279,7 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     if tokens and n and (max_new <= 0 or max_tokens <= 0):
         raise RuntimeError("max_new and max_tokens must be positive")
     L = _library()
-    need = L.kvq_paged_attn_workspace_bytes(n, tokens, nh, Hkv, max_new, max_tokens)
+    need = L.kvq_paged_attn_workspace_bytes(block, n, tokens, nh, max_new, max_tokens)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     a = _pack_attn(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), _ints(dev, "q_start", q_start, n + 1),
                    _rows(dev, "rows", rows), 0 if first is None else _ints(dev, "first", first, tokens), 0 if prefix is None else _ints(dev, "prefix", prefix, n),

@@ -81,11 +81,11 @@ def test_workspace_holds_every_split():
         for tokens in (1, 7, 300, 4096):
             for nh, Hkv in ((1, 1), (32, 8), (64, 8), (40, 8)):
                 for length in (1, 128, 5000, 131072):
-                    b = L.kvq_paged_attn_workspace_bytes(n, tokens, nh, Hkv, tokens, length)
+                    b = L.kvq_paged_attn_workspace_bytes(layer(Hkv=Hkv), n, tokens, nh, tokens, length)
                     assert b % (tokens * nh * 520) == 0
                     splits = b // (tokens * nh * 520)
                     assert splits != 1 and splits <= -(-length // 128)
-    assert L.kvq_paged_attn_workspace_bytes(1, 1, 3, 2, 1, 100) == 0
+    assert L.kvq_paged_attn_workspace_bytes(layer(), 1, 1, 3, 1, 100) == 0
 
 
 def test_no_cpu_path():
