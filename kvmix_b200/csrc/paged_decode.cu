@@ -3,8 +3,8 @@
 
 namespace kvq {
 
-// A CTA of four warps takes one (sequence, kv head, block of query rows, split of the pages); a warp takes every fourth page by itself --
-// scores, online softmax, values -- so nothing in the loop waits for another warp.
+// A CTA of four warps takes one (sequence, kv head, block of query rows, split of the pages); a warp takes every fourth packed page, and 32
+// tokens of every fp16 page, by itself -- scores, online softmax, values -- so nothing in the loop waits for another warp.
 //   scores   S[token][column] = K[token][channel] B[channel][column]: mma m16n8k16 with 16 tokens as rows
 //   values   O[channel][column] = V^T[channel][token] B[token][column]: the same with 16 channels as rows
 // In both the packed axis runs along the MMA's rows and the contraction across words, so that the two elements of an operand register
@@ -212,8 +212,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
         if (b.x < b.y) { first = min(first, b.x); last = max(last, b.y); }
     }
     const int p_lo = first < last ? first / kPage : 0, p_hi = first < last ? pages_of(last) : 0, per = (p_hi - p_lo + p.splits - 1) / p.splits;
-    const int p0 = p_lo + split * per, p1 = min(p_hi, p0 + per), n_mine = max(0, (p1 - p0 - warp + kFewWarps - 1) / kFewWarps);
-    auto page_at = [&](int k) { return p1 - 1 - (k * kFewWarps + warp); };        // newest first: fp16 pages come at the beginning
+    const int p0 = p_lo + split * per, p1 = min(p_hi, p0 + per), p_old = max(p0, min(p1, s.packed));            // [p0, p_old) packed
+    const int n_mine = max(0, (p_old - p0 - warp + kFewWarps - 1) / kFewWarps);
+    auto page_at = [&](int k) { return p0 + k * kFewWarps + warp; };
 
     constexpr int KW = page_words(KB), VW = page_words(VB), VT = VB == 3 ? 11 : 8;
     const uint32_t k_cb = stage_rows * 4 * KW, v_cb = stage_rows * 4 * VW, k_sz = stage_rows * p.k_groups * 2, v_sz = stage_rows * p.v_groups * 2;
@@ -227,8 +228,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
         ids_base = at;
         ids = -1;
         if (at + lane < n_mine) {
-            const int page = page_at(at + lane), id = s.table[page];
-            if (id >= 0 && id < (page < s.packed ? p.l.n_packed : p.l.n_fp16)) ids = id;
+            const int id = s.table[page_at(at + lane)];
+            if (id >= 0 && id < p.l.n_packed) ids = id;
         }
     };
     auto id_of = [&](int k) { return __shfl_sync(0xffffffffu, ids, k - ids_base); };
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
     auto produce = [&]() {
         while (pk < n_mine && pk < ids_base + 32 && in_flight < stages) {
             const int id = id_of(pk);
-            if (page_at(pk) >= s.packed || id < 0) { ++pk; continue; }
+            if (id < 0) { ++pk; continue; }
             if (lane == 0) {
                 const uint32_t bar = s_bar + 8 * fill_slot, dst = s_ring + fill_slot * stage_bytes;
                 const int64_t at = (int64_t)id * p.l.Hkv + head;
@@ -277,8 +278,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
     const float cap2 = p.a.softcap * kLog2e;
     float ref = -INFINITY, alpha = 1.f;                           // of row `lane`: reference (log2 units), factor of what is summed already
 
-    // Scores of a page, [row][slot] in s_s -> weights in s_p, sums in s_sum, ref and alpha.  A lane takes four tokens of each row.
-    auto softmax_page = [&](int page_base) {
+    // Scores of `count` tokens, [row][slot] in s_s -> weights in s_p, sums in s_sum, ref and alpha.  A lane takes four tokens of each row.
+    auto softmax_page = [&](int page_base, int count) {
         __syncwarp();
         const int j0 = page_base + 16 * (lane >> 2) + (lane & 3);
         float change = 1.f;
@@ -289,12 +290,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
             const float2 by_row = s_factor[r];
             const float slope = __int_as_float(b.w);
             float x[4] = {raw.x, raw.y, raw.z, raw.w}, top = -INFINITY;
-            const bool whole = b.x <= page_base && b.y >= page_base + kPage;
+            const bool whole = b.x <= page_base && b.y >= page_base + kPage && count == kPage;
+            const int end = min(b.y, page_base + count);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 x[c] = p.a.softcap > 0.f ? cap_score(x[c], by_row.y, cap2) : x[c] * by_row.x;
                 x[c] = fmaf(slope, (float)(j0 + 4 * c - b.z), x[c]);
-                if (!whole && (j0 + 4 * c < b.x || j0 + 4 * c >= b.y)) x[c] = -INFINITY;
+                if (!whole && (j0 + 4 * c < b.x || j0 + 4 * c >= end)) x[c] = -INFINITY;
             }
             asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(top) : "f"(x[0]), "f"(x[1]), "f"(x[2]));
             asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(x[3]));
@@ -338,8 +340,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
         for (int m = 0; m < T; ++m) { o[m][0] *= a0; o[m][1] *= a1; o[m][2] *= a0; o[m][3] *= a1; }
     };
 
-    // ---- fp16 pages
-    int k = 0;
+    // ---- fp16 pages: tokens 32 warp .. 32 warp + 31 of each
     if (n_mine > 0) fetch_ids(0);
     produce();
     {
@@ -349,46 +350,44 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[m][e] = 0.f;
 #pragma unroll 1
-        for (; k < n_mine && page_at(k) >= s.packed; ++k) {
-            if (k == ids_base + 32) { fetch_ids(k); pk = max(pk, k); produce(); }
-            const int id = id_of(k), page = page_at(k);
-            if (id < 0) continue;
-            const int page_base = page * kPage, there = min(kPage, s.length - page_base);
-            const __half *kp = static_cast<const __half *>(p.l.kfull) + ((int64_t)id * p.l.Hkv + head) * kPageHalf;
-            const __half *vp = static_cast<const __half *>(p.l.vfull) + ((int64_t)id * p.l.Hkv + head) * kPageHalf;
-            float sc[8][4];
+        for (int page = p_old; page < p1; ++page) {
+            const int id = s.table[page], token0 = page * kPage + 32 * warp, there = min(32, s.length - token0);
+            if (id < 0 || id >= p.l.n_fp16 || there <= 0) continue;
+            const int64_t at = ((int64_t)id * p.l.Hkv + head) * kPageHalf + 32 * warp * kHeadDim;
+            const __half *kp = static_cast<const __half *>(p.l.kfull) + at, *vp = static_cast<const __half *>(p.l.vfull) + at;
+            float sc[2][4];
 #pragma unroll
-            for (int m = 0; m < 8; ++m) {
+            for (int m = 0; m < 2; ++m) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[m][e] = 0.f;
 #pragma unroll
-                for (int blk = 0; blk < 4; ++blk) {               // 32 channels, eight neighbours a lane
-                    const int r0 = min(few_element<1>(g, m, 0), there - 1), r1 = min(few_element<1>(g, m, 1), there - 1);
-                    const uint4 x = *reinterpret_cast<const uint4 *>(kp + r0 * kHeadDim + 32 * blk + 8 * t);
-                    const uint4 y = *reinterpret_cast<const uint4 *>(kp + r1 * kHeadDim + 32 * blk + 8 * t);
+                for (int blk = 0; blk < 4; ++blk) {               // 32 channels, eight neighbours a lane; tokens 16m + g, 16m + g + 8
+                    const uint4 x = *reinterpret_cast<const uint4 *>(kp + min(16 * m + g, there - 1) * kHeadDim + 32 * blk + 8 * t);
+                    const uint4 y = *reinterpret_cast<const uint4 *>(kp + min(16 * m + g + 8, there - 1) * kHeadDim + 32 * blk + 8 * t);
                     const uint4 q = *reinterpret_cast<const uint4 *>(s_q + min(g, R - 1) * 128 + 32 * blk + 8 * t);           // columns beyond R are not read
                     mma16816(sc[m], x.x, y.x, x.y, y.y, q.x, q.y);
                     mma16816(sc[m], x.z, y.z, x.w, y.w, q.z, q.w);
                 }
             }
-            dense_scores(sc, [&](int m, int e) { return few_element<1>(g, m, e); });
-            if (softmax_page(page_base)) rescale(o, 2 * t, 2 * t + 1);
-#pragma unroll 1
-            for (int step = 0; step < 8; ++step) {
-                if (16 * step >= there) break;
-                uint32_t x[4][8], b0, b1;
+            uint4 x[2][4][2];                                     // tokens 16 step + t + 4j, channels 16g .. 16g + 15; nothing behind the last token
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {                     // tokens t + 4j, channels 16g .. 16g + 15; nothing behind the last token
+            for (int step = 0; step < 2; ++step)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
                     const int r = 16 * step + t + 4 * j;
-                    uint4 a = make_uint4(0, 0, 0, 0), b = a;
-                    if (r < there) {
-                        a = *reinterpret_cast<const uint4 *>(vp + r * kHeadDim + 16 * g);
-                        b = *reinterpret_cast<const uint4 *>(vp + r * kHeadDim + 16 * g + 8);
-                    }
-                    x[j][0] = a.x; x[j][1] = a.y; x[j][2] = a.z; x[j][3] = a.w;
-                    x[j][4] = b.x; x[j][5] = b.y; x[j][6] = b.z; x[j][7] = b.w;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) x[step][j][h] = r < there ? *reinterpret_cast<const uint4 *>(vp + r * kHeadDim + 16 * g + 8 * h) : make_uint4(0, 0, 0, 0);
                 }
+            dense_scores(sc, [&](int m, int e) { return 16 * m + g + 8 * e; });
+            if (softmax_page(token0, 32)) rescale(o, 2 * t, 2 * t + 1);
+#pragma unroll
+            for (int step = 0; step < 2; ++step) {
+                uint32_t b0, b1;
                 weights(min(g, R - 1), step, b0, b1);
+                auto word = [&](int j, int c) {                   // channels 2c, 2c + 1 of token t + 4j
+                    const uint4 &v = x[step][j][c >> 2];
+                    return (c & 3) == 0 ? v.x : (c & 3) == 1 ? v.y : (c & 3) == 2 ? v.z : v.w;
+                };
 #pragma unroll
                 for (int m = 0; m < 8; ++m) {
                     uint32_t a[4];
@@ -396,7 +395,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
                     for (int e = 0; e < 2; ++e) {
                         const int q = 2 * m + e, c = (q & 3) * 4 + (q >> 2);
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) a[e + 2 * j] = prmt(x[2 * j][c >> 1], x[2 * j + 1][c >> 1], c & 1 ? 0x7632 : 0x5410);
+                        for (int j = 0; j < 2; ++j) a[e + 2 * j] = prmt(word(2 * j, c >> 1), word(2 * j + 1, c >> 1), c & 1 ? 0x7632 : 0x5410);
                     }
                     mma16816(o[m], a[0], a[1], a[2], a[3], b0, b1);
                 }
@@ -421,10 +420,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
     // p * scale * 2^expo: the power of two starts from the first scales (the largest of them becomes 4 to 8) and goes down where one would exceed 256
     int expo = 32;
 #pragma unroll 1
-    for (; k < n_mine; ++k) {
-        if (k == ids_base + 32) { fetch_ids(k); pk = max(pk, k); produce(); }
-        const int id = id_of(k), page = page_at(k);
-        if (id < 0 || page >= s.packed) continue;
+    for (int k = 0; k < n_mine; ++k) {
+        if (k == ids_base + 32) { fetch_ids(k); produce(); }
+        if (id_of(k) < 0) continue;
         if constexpr (KB == 3) {
             float sc[11][4];
 #pragma unroll
@@ -506,7 +504,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
                 }
             }
         }
-        if (softmax_page(page * kPage)) {
+        if (softmax_page(page_at(k) * kPage, kPage)) {
             rescale(out, o_row, o_row + 1);
             if constexpr (VB != 3) {
                 const float a0 = __shfl_sync(0xffffffffu, alpha, o_row), a1 = __shfl_sync(0xffffffffu, alpha, o_row + 1);
@@ -627,24 +625,48 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
     }
 }
 
-// Partial sums of the splits -> outputs, in the splits' order.  A CTA takes one row of q and head; `few`: rows of the kernel above, else of
-// the kernel of tiles.
-__global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedArgs p, int few) {
-    const int u = blockIdx.x / p.a.nh, h = blockIdx.x - u * p.a.nh;
-    if (u < p.a.q_start[0] || u >= p.a.q_start[p.a.n]) return;
-    const PagedSeq s = paged_seq(p, sequence_of(p.a.q_start, p.a.n, u));
-    const int rows = s.n_new * p.rep;
-    if (few ? rows > kFewRows : rows <= p.few_rows) return;
-    const int64_t step = (int64_t)p.a.tokens * p.a.nh, row = (int64_t)u * p.a.nh + h;
-    float m = -INFINITY, l = 0.f, v = 0.f;
-    for (int i = 0; i < p.splits; ++i) m = fmaxf(m, p.part_ml[2 * (i * step + row)]);
-    for (int i = 0; i < p.splits; ++i) {
-        const float mi = p.part_ml[2 * (i * step + row)], li = p.part_ml[2 * (i * step + row) + 1], x = p.part_out[(i * step + row) * 128 + threadIdx.x];
-        const float f = part_factor(mi, li, m);
-        l += f * li;
-        if (f != 0.f) v += f * x;
+// Partial sums of the splits -> outputs, in the splits' order: a row a warp.  `few`: rows of the kernel above, kFewRows places for every (sequence,
+// kv head); else rows of q, of which those that the kernel of tiles had are joined.
+__global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant__ PagedArgs p, int few) {
+    const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    int u, h;
+    if (few) {
+        const int r = (int)(at % kFewRows), head = (int)(at / kFewRows % p.l.Hkv);
+        const int64_t i = at / kFewRows / p.l.Hkv;
+        if (i >= p.a.n) return;
+        const PagedSeq s = paged_seq(p, (int)i);
+        if (s.n_new * p.rep > kFewRows || r >= s.n_new * p.rep) return;
+        u = s.q0 + r / p.rep;
+        h = head * p.rep + r % p.rep;
+    } else {
+        const int64_t q = at / p.a.nh;
+        if (q >= p.a.tokens || q < p.a.q_start[0] || q >= p.a.q_start[p.a.n]) return;
+        u = (int)q;
+        h = (int)(at - q * p.a.nh);
+        if (p.few_rows) {
+            const PagedSeq s = paged_seq(p, sequence_of(p.a.q_start, p.a.n, u));
+            if (s.n_new * p.rep <= p.few_rows) return;
+        }
     }
-    static_cast<__half *>(p.a.out)[(int64_t)u * p.a.o_sT + (int64_t)h * p.a.o_sH + threadIdx.x] = __float2half_rn(l == 0.f ? 0.f : v / l);
+    const int64_t step = (int64_t)p.a.tokens * p.a.nh, row = (int64_t)u * p.a.nh + h;
+    float m = -INFINITY, l = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = lane; i < p.splits; i += 32) m = fmaxf(m, p.part_ml[2 * (i * step + row)]);
+    m = warp_max(m);
+    for (int i = 0; i < p.splits; ++i) {
+        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * (i * step + row));
+        const float4 x = *reinterpret_cast<const float4 *>(p.part_out + (i * step + row) * 128 + 4 * lane);
+        const float f = part_factor(ml.x, ml.y, m);
+        l += f * ml.y;
+        if (f != 0.f) { v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w; }
+    }
+    __half *out = static_cast<__half *>(p.a.out) + (int64_t)u * p.a.o_sT + (int64_t)h * p.a.o_sH + 4 * lane;
+    auto put = [&](int c, float x) { out[c] = __float2half_rn(l == 0.f ? 0.f : x / l); };
+    put(0, v.x);
+    put(1, v.y);
+    put(2, v.z);
+    put(3, v.w);
 }
 
 template <int KB, int VB, int CK>
@@ -694,9 +716,9 @@ int paged_few(const PagedArgs &p, cudaStream_t st) {
 }
 
 int paged_merge(const PagedArgs &p, int few, cudaStream_t st) {
-    const int64_t grid = (int64_t)p.a.tokens * p.a.nh;
+    const int64_t rows = few ? (int64_t)p.a.n * p.l.Hkv * kFewRows : (int64_t)p.a.tokens * p.a.nh, grid = (rows + 7) / 8;
     if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
-    paged_merge_kernel<<<(unsigned)grid, 128, 0, st>>>(p, few);
+    paged_merge_kernel<<<(unsigned)grid, 256, 0, st>>>(p, few);
     return check_launch();
 }
 
