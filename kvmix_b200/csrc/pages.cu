@@ -415,16 +415,22 @@ __global__ void __launch_bounds__(256) page_copy_kernel(const __grid_constant__ 
 // elements.  Keys: a thread owns two neighbouring channels and 32 of the tokens, so that a row is read by 64 threads in one go; the
 // parts of a group meet in shared memory.  Values: a thread owns 32 channels of two tokens, the parts of a group meet by
 // shuffles.  3 bits: a word (a group of 11, the last of 7) a thread and turn.
+// Words, scales and minima of keys go through shared memory, from where they leave in one run.
+template <int BITS>
 struct PackShared {
+    static constexpr int W = page_words(BITS), PAD = W + (BITS == 3 ? 1 : 4);     // rows stay 16-byte aligned where they are read that way
+    uint32_t code[128 * PAD];
+    __half scale[128 * 12], mn[128 * 12];
     __half2 lo[4][64], hi[4][64];
 };
 
 template <int BITS>
-__device__ __forceinline__ void pack_keys(const __half *x, int32_t *code, __half *scale, __half *mn, int group, PackShared &s) {
-    constexpr int QMAX = (1 << BITS) - 1;
+__device__ __forceinline__ void pack_keys(const __half *x, int32_t *code, __half *scale, __half *mn, int group, PackShared<BITS> &s) {
+    constexpr int QMAX = (1 << BITS) - 1, W = page_words(BITS), PAD = PackShared<BITS>::PAD;
     const __half2 *px = reinterpret_cast<const __half2 *>(x);
-    const int pair = threadIdx.x & 63;
+    const int pair = threadIdx.x & 63, groups = page_groups(BITS, group);
     if constexpr (BITS == 3) {
+#pragma unroll 1
         for (int w = threadIdx.x >> 6; w < 12; w += 4) {
             const int n = min(11, kPage - 11 * w);
             __half2 raw[11], lo2, hi2;
@@ -436,15 +442,15 @@ __device__ __forceinline__ void pack_keys(const __half *x, int32_t *code, __half
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float lo = e ? __high2float(lo2) : __low2float(lo2), range = (e ? __high2float(hi2) : __low2float(hi2)) - lo, sc = range / 7.0f;
-                const int o = (2 * pair + e) * 12 + w;
-                code[o] = (int32_t)quant_word<3>([&](int i) { return i < n ? (e ? __high2float(raw[i]) : __low2float(raw[i])) : lo; }, lo, sc, __frcp_rn(sc));
-                scale[o] = __float2half_rn(stored_scale<7>(range, sc, 0));
-                mn[o] = __float2half_rn(lo);
+                const int c = 2 * pair + e;
+                s.code[c * PAD + w] = quant_word<3>([&](int i) { return i < n ? (e ? __high2float(raw[i]) : __low2float(raw[i])) : lo; }, lo, sc, __frcp_rn(sc));
+                s.scale[c * 12 + w] = __float2half_rn(stored_scale<7>(range, sc, 0));
+                s.mn[c * 12 + w] = __float2half_rn(lo);
             }
         }
     } else {
-        constexpr int W = 4 * BITS, FPI = 32 / BITS;
-        const int part = threadIdx.x >> 6, span = group / 32, groups = 4 / span, p0 = part / span * span;
+        constexpr int FPI = 32 / BITS;
+        const int part = threadIdx.x >> 6, span = group / 32, p0 = part / span * span;
         __half2 raw[32], lo2, hi2;
 #pragma unroll
         for (int i = 0; i < 32; ++i) raw[i] = px[(part * 32 + i) * 64 + pair];
@@ -456,22 +462,33 @@ __device__ __forceinline__ void pack_keys(const __half *x, int32_t *code, __half
             s.hi[part][pair] = hi2;
             __syncthreads();
             for (int p = p0; p < p0 + span; ++p) { lo2 = __hmin2(lo2, s.lo[p][pair]); hi2 = __hmax2(hi2, s.hi[p][pair]); }
-            __syncthreads();
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const float lo = e ? __high2float(lo2) : __low2float(lo2), range = (e ? __high2float(hi2) : __low2float(hi2)) - lo, sc = range / (float)QMAX;
-            uint32_t word[BITS];
-            quant_words<BITS, BITS>([&](int k, int i) { return e ? __high2float(raw[k * FPI + i]) : __low2float(raw[k * FPI + i]); }, lo, sc, __frcp_rn(sc), word);
+            const float lo = e ? __high2float(lo2) : __low2float(lo2), range = (e ? __high2float(hi2) : __low2float(hi2)) - lo, sc = range / (float)QMAX, rinv = __frcp_rn(sc);
             const int c = 2 * pair + e;
 #pragma unroll
-            for (int k = 0; k < BITS; ++k) code[c * W + part * BITS + k] = (int32_t)word[k];
+            for (int k = 0; k < BITS; ++k)                        // a word at a time: the words of a thread at once take 120 registers
+                s.code[c * PAD + part * BITS + k] = quant_word<BITS>([&](int i) { return e ? __high2float(raw[k * FPI + i]) : __low2float(raw[k * FPI + i]); }, lo, sc, rinv);
             if (part == p0) {
-                scale[c * groups + part / span] = __float2half_rn(stored_scale<QMAX>(range, sc, 0));
-                mn[c * groups + part / span] = __float2half_rn(lo);
+                s.scale[c * groups + part / span] = __float2half_rn(stored_scale<QMAX>(range, sc, 0));
+                s.mn[c * groups + part / span] = __float2half_rn(lo);
             }
         }
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 128 * W / 4; i += 256) {
+        const int c = 4 * i / W, w = 4 * i % W;                   // W is a multiple of 4
+        uint4 v;
+        if constexpr (BITS == 3) v = make_uint4(s.code[c * PAD + w], s.code[c * PAD + w + 1], s.code[c * PAD + w + 2], s.code[c * PAD + w + 3]);
+        else v = *reinterpret_cast<const uint4 *>(&s.code[c * PAD + w]);
+        reinterpret_cast<uint4 *>(code)[i] = v;
+    }
+    for (int i = threadIdx.x; i < 128 * groups / 8; i += 256) {
+        reinterpret_cast<uint4 *>(scale)[i] = reinterpret_cast<const uint4 *>(s.scale)[i];
+        reinterpret_cast<uint4 *>(mn)[i] = reinterpret_cast<const uint4 *>(s.mn)[i];
+    }
+    __syncthreads();
 }
 
 template <int BITS>
@@ -488,8 +505,8 @@ __device__ __forceinline__ void pack_values(const __half *x, int32_t *code, __ha
 }
 
 template <int KB, int VB>
-__global__ void __launch_bounds__(256) page_pack_kernel(const kvq_page_layer l, const int32_t *moves, int max_moves) {
-    __shared__ PackShared s;
+__global__ void __launch_bounds__(256, 3) page_pack_kernel(const kvq_page_layer l, const int32_t *moves, int max_moves) {
+    __shared__ __align__(16) PackShared<KB> s;
     const int64_t units = 2LL * min(moves[0], max_moves) * l.Hkv;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
         const bool values = u & 1;
@@ -585,7 +602,7 @@ extern "C" int kvq_page_pack(const kvq_page_layer *l, const int32_t *moves, int3
     if (!moves) return KVQ_ERR_NULL;
     if (max_moves <= 0 || !l->n_fp16 || !l->n_packed) return KVQ_OK;
     const int64_t units = 2LL * max_moves * l->Hkv;
-    const unsigned grid = (unsigned)(units < 148 * 4 ? units : 148 * 4);
+    const unsigned grid = (unsigned)(units < 148 * 6 ? units : 148 * 6);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     switch (l->k_bits) {
         case 1: launch_pack<1>(*l, moves, max_moves, grid, st); break;

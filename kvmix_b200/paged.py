@@ -83,25 +83,43 @@ def _library():
     return _lib.lib()
 
 
-def _ints(device, name, t, *shape):
-    if t.dtype is not torch.int32 or not t.is_contiguous() or t.device != device or t.shape != shape:
-        raise RuntimeError(f"{name} must be a contiguous int32 tensor {shape} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+_i32, _f16 = torch.int32, torch.float16
+
+
+def _ints(dev, name, t, n):
+    """Address of an int32 [n] on device number `dev`."""
+    if t.dtype is _i32 and t.get_device() == dev and t.dim() == 1 and t.numel() == n and t.is_contiguous():
+        return t.data_ptr()
+    raise RuntimeError(f"{name} must be a contiguous int32 tensor [{n}] on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def _book(pages):
-    """(device, argument block) of a PageBook."""
-    table, n_packed = pages.table, pages.n_packed
-    if not table.is_cuda:
+    """(device number, argument block) of a PageBook."""
+    table, length, packed, refs, free_ids, count, n_packed = pages
+    dev = table.get_device()
+    if dev < 0:
         raise RuntimeError("kvmix_b200 operators need CUDA tensors (there is no CPU path)")
-    if table.dim() != 2:
-        raise RuntimeError("the page table is [slots, max_pages]")
-    dev, (slots, max_pages), total = table.device, table.shape, pages.refs.numel()
+    if table.dtype is not _i32 or table.dim() != 2 or not table.is_contiguous():
+        raise RuntimeError("the page table is a contiguous int32 tensor [slots, max_pages]")
+    (slots, max_pages), total = table.shape, refs.numel()
     if not 0 <= n_packed <= total:
         raise RuntimeError("n_packed is the number of packed pages among refs")
-    return dev, _pack_book(_ints(dev, "table", table, slots, max_pages), _ints(dev, "length", pages.length, slots), _ints(dev, "packed", pages.packed, slots),
-                           _ints(dev, "refs", pages.refs, total), _ints(dev, "free_ids", pages.free_ids, total), _ints(dev, "count", pages.count, 4),
-                           slots, max_pages, n_packed, total - n_packed)
+    return dev, _pack_book(table.data_ptr(), _ints(dev, "length", length, slots), _ints(dev, "packed", packed, slots), _ints(dev, "refs", refs, total),
+                           _ints(dev, "free_ids", free_ids, total), _ints(dev, "count", count, 4), slots, max_pages, n_packed, total - n_packed)
+
+
+def _page_tensor(dev, t, dtype, shape):
+    # the address is asked for in the same breath: a layer has eight such tensors, a call of many layers hundreds
+    if t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
+    raise RuntimeError(f"page tensor {tuple(t.shape)} {t.dtype} on {t.device}: contiguous {dtype} {shape} on cuda:{dev} expected")
+
+
+def _fp16_pages(pages, dev, layer):
+    """Addresses of a layer's fp16 pages."""
+    kfull, vfull = layer.kfull, layer.vfull
+    shape = (pages.refs.numel() - pages.n_packed, kfull.shape[1], PAGE_TOKENS, 128)
+    return _page_tensor(dev, kfull, _f16, shape), _page_tensor(dev, vfull, _f16, shape)
 
 
 def _layer(pages, dev, layer):
@@ -111,37 +129,32 @@ def _layer(pages, dev, layer):
         check(-1)
     if group not in (32, 64, 128):
         raise RuntimeError("pages are quantized in groups of 32, 64 or 128")
-    n, n16, heads = pages.n_packed, pages.refs.numel() - pages.n_packed, kfull.shape[1]
-    kg, vg = page_groups(kb, group), page_groups(vb, group)
-    i32, f16 = torch.int32, torch.float16
-    for t, dtype, shape in ((kcode, i32, (n, heads, PAGE_TOKENS, page_words(kb))), (kscale, f16, (n, heads, PAGE_TOKENS, kg)), (kmn, f16, (n, heads, PAGE_TOKENS, kg)),
-                            (kfull, f16, (n16, heads, PAGE_TOKENS, 128)), (vcode, i32, (n, heads, PAGE_TOKENS, page_words(vb))),
-                            (vscale, f16, (n, heads, PAGE_TOKENS, vg)), (vmn, f16, (n, heads, PAGE_TOKENS, vg)), (vfull, f16, (n16, heads, PAGE_TOKENS, 128))):
-        if t.dtype is not dtype or t.shape != shape or t.device != dev or not t.is_contiguous():
-            raise RuntimeError(f"page tensor {tuple(t.shape)} {t.dtype} on {t.device}: contiguous {dtype} {shape} on {dev} expected")
-    return _pack_layer(kcode.data_ptr(), kscale.data_ptr(), kmn.data_ptr(), kfull.data_ptr(), vcode.data_ptr(), vscale.data_ptr(), vmn.data_ptr(),
-                       vfull.data_ptr(), heads, kb, vb, group, n, n16)
+    n, heads = pages.n_packed, kfull.shape[1]
+    n16 = pages.refs.numel() - n
+    kw, vw, kg, vg = (n, heads, PAGE_TOKENS, page_words(kb)), (n, heads, PAGE_TOKENS, page_words(vb)), (n, heads, PAGE_TOKENS, page_groups(kb, group)), \
+        (n, heads, PAGE_TOKENS, page_groups(vb, group))
+    full = (n16, heads, PAGE_TOKENS, 128)
+    return _pack_layer(_page_tensor(dev, kcode, _i32, kw), _page_tensor(dev, kscale, _f16, kg), _page_tensor(dev, kmn, _f16, kg), _page_tensor(dev, kfull, _f16, full),
+                       _page_tensor(dev, vcode, _i32, vw), _page_tensor(dev, vscale, _f16, vg), _page_tensor(dev, vmn, _f16, vg), _page_tensor(dev, vfull, _f16, full),
+                       heads, kb, vb, group, n, n16)
 
 
 def _rows(dev, name, rows):
-    if rows.dim() != 1:
-        raise RuntimeError(f"{name} must be one-dimensional")
     return _ints(dev, name, rows, rows.numel())
 
 
-def _on_its_device(f):
-    """Kernels are launched on the current stream of the tensors' device, whichever is current."""
-    @functools.wraps(f)
-    def call(*args, **kwargs):
-        for a in args:
-            if isinstance(a, PageBook):
-                dev = a.table.device
-                if dev.type == "cuda" and dev.index != _current_device():
-                    with torch.cuda.device(dev):
-                        return f(*args, **kwargs)
-                break
-        return f(*args, **kwargs)
-    return call
+def _on_its_device(where):
+    """Kernels are launched on the current stream of the tensors' device, whichever is current.  `where`: place of `pages` among the arguments."""
+    def wrap(f):
+        @functools.wraps(f)
+        def call(*args, **kwargs):
+            dev = (args[where] if len(args) > where else kwargs["pages"]).table.get_device()
+            if dev < 0 or dev == _current_device():
+                return f(*args, **kwargs)
+            with torch.cuda.device(dev):
+                return f(*args, **kwargs)
+        return call
+    return wrap
 
 
 def _launched(rc, n=1):
@@ -150,30 +163,28 @@ def _launched(rc, n=1):
     ops.LAUNCHES[0] += n
 
 
-def _copy(dev, tensors, moves, max_moves):
-    """Whole pages of every tensor [pages, ..], from and to the numbers in `moves`."""
-    tensors = [t for t in tensors if t.numel()]
-    for at in range(0, len(tensors), _lib.MAX_PAGE_TENSORS):
-        some = tensors[at:at + _lib.MAX_PAGE_TENSORS]
-        flat = [v for t in some for v in (t.data_ptr(), t.stride(0) * t.element_size())]
-        _launched(_library().kvq_page_copy(struct.pack("@" + "Pq" * len(some), *flat), len(some), moves, max_moves, ops.raw_stream()))
+def _copy(tensors, moves, max_moves):
+    """Whole pages of tensors given as (address, bytes of a page), from and to the numbers in `moves`."""
+    for at in range(0, len(tensors), 2 * _lib.MAX_PAGE_TENSORS):
+        some = tensors[at:at + 2 * _lib.MAX_PAGE_TENSORS]
+        _launched(_library().kvq_page_copy(struct.pack("@" + "Pq" * (len(some) // 2), *some), len(some) // 2, moves, max_moves, ops.raw_stream()))
 
 
-@_on_its_device
+@_on_its_device(2)
 def pages_extend(rows, counts, pages):
     """``length[rows[i]] += counts[i]``, with the fp16 pages that takes.  rows, counts: int32 [n] on the device, no row twice."""
     dev, book = _book(pages)
     _launched(_library().kvq_pages_extend(book, _rows(dev, "rows", rows), _ints(dev, "counts", counts, rows.numel()), rows.numel(), ops.raw_stream()))
 
 
-@_on_its_device
+@_on_its_device(1)
 def pages_free(rows, pages):
     """The rows' sequences go; pages that nobody holds any more are free."""
     dev, book = _book(pages)
     _launched(_library().kvq_pages_free(book, _rows(dev, "rows", rows), rows.numel(), ops.raw_stream()))
 
 
-@_on_its_device
+@_on_its_device(4)
 def page_write(k, v, q_start, rows, pages, layer):
     """Keys (rotated) and values of new tokens into one layer's fp16 pages.  k, v [tokens, Hkv, 128] fp16, any strides; tokens
     [q_start[i], q_start[i+1]) are the last ones of sequence rows[i], which ``pages_extend`` has counted already."""
@@ -181,8 +192,8 @@ def page_write(k, v, q_start, rows, pages, layer):
     heads = layer.kfull.shape[1]
     if k.dim() != 3 or k.shape[1:] != (heads, 128) or v.shape != k.shape or k.dtype is not torch.float16 or v.dtype is not torch.float16:
         raise RuntimeError(f"page_write takes fp16 keys and values [tokens, {heads}, 128]")
-    if k.device != dev or v.device != dev:
-        raise RuntimeError(f"keys and values must be on {dev}")
+    if k.get_device() != dev or v.get_device() != dev:
+        raise RuntimeError(f"keys and values must be on cuda:{dev}")
     if k.stride(2) != 1:
         k = k.contiguous()
     if v.stride(2) != 1:
@@ -193,14 +204,14 @@ def page_write(k, v, q_start, rows, pages, layer):
     _launched(_library().kvq_page_write(book, _layer(pages, dev, layer), a, ops.raw_stream()))
 
 
-@_on_its_device
+@_on_its_device(2)
 def pages_settle(rows, window, pages, layers):
     """Full pages that end ``window`` tokens or more before their sequence's end are quantized in every layer and their fp16 pages given
     back.  Sequences that share an fp16 page settle it each for itself."""
     dev, book = _book(pages)
     if window < 0:
         raise RuntimeError("window must not be negative")
-    moves = torch.empty(4 + 2 * pages.n_packed, dtype=torch.int32, device=dev)
+    moves = pages.count.new_empty(4 + 2 * pages.n_packed)
     blocks, n = [_layer(pages, dev, layer) for layer in layers], rows.numel()
     L, st, at = _library(), ops.raw_stream(), moves.data_ptr()
     _launched(L.kvq_pages_settle(book, _rows(dev, "rows", rows), n, int(window), at, st))
@@ -208,34 +219,40 @@ def pages_settle(rows, window, pages, layers):
         _launched(L.kvq_page_pack(block, at, min(pages.n_packed, n * pages.table.shape[1]), st))
 
 
-@_on_its_device
+@_on_its_device(2)
 def pages_fork(parents, children, pages, layers):
     """Row children[i] (empty) becomes a copy of row parents[i]: full pages are shared, a last page that is not full is copied in every
     layer.  A parent may have several children; no row is both."""
     dev, book = _book(pages)
-    n = parents.numel()
+    n, tensors = parents.numel(), []
     for layer in layers:
-        _layer(pages, dev, layer)
-    moves = torch.empty(4 + 2 * n, dtype=torch.int32, device=dev)
+        size = layer.kfull.shape[1] * PAGE_TOKENS * 256
+        for at in _fp16_pages(pages, dev, layer):
+            tensors += (at, size)
+    moves = pages.count.new_empty(4 + 2 * n)
     _launched(_library().kvq_pages_fork(book, _rows(dev, "parents", parents), _ints(dev, "children", children, n), n, moves.data_ptr(), ops.raw_stream()))
-    _copy(dev, [t for layer in layers for t in (layer.kfull, layer.vfull)], moves.data_ptr(), n)
+    _copy(tensors, moves.data_ptr(), n)
 
 
-@_on_its_device
+@_on_its_device(0)
 def pages_compact(pages, layers):
     """The pages in use move to the lowest numbers of their pools."""
     dev, book = _book(pages)
+    total, n, packed, fp16 = pages.refs.numel(), pages.n_packed, [], []
     for layer in layers:
         _layer(pages, dev, layer)
-    total, n = pages.refs.numel(), pages.n_packed
-    moves = torch.empty(8 + 3 * total, dtype=torch.int32, device=dev)
+        for tensors, some in ((packed, (layer.kcode, layer.kscale, layer.kmn, layer.vcode, layer.vscale, layer.vmn)), (fp16, (layer.kfull, layer.vfull))):
+            for t in some:
+                tensors += (t.data_ptr(), t.stride(0) * t.element_size())
+    moves = pages.count.new_empty(8 + 3 * total)
     _launched(_library().kvq_pages_compact(book, moves.data_ptr(), ops.raw_stream()))
-    at16 = moves.data_ptr() + 4 * (4 + 2 * n)
-    _copy(dev, [t for layer in layers for t in (layer.kcode, layer.kscale, layer.kmn, layer.vcode, layer.vscale, layer.vmn)], moves.data_ptr(), n)
-    _copy(dev, [t for layer in layers for t in (layer.kfull, layer.vfull)], at16, total - n)
+    if n:
+        _copy(packed, moves.data_ptr(), n)
+    if total > n:
+        _copy(fp16, moves.data_ptr() + 4 * (4 + 2 * n), total - n)
 
 
-@_on_its_device
+@_on_its_device(3)
 def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, prefix=None, first=None, softcap=None, alibi_slopes=None,
                     softmax_scale=None, max_new=None, max_tokens=None, out=None):
     """Attention of the last tokens of every sequence over its pages.
@@ -251,8 +268,8 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     (host integers that lay out the work; None: whatever fits the tensors).  Tokens that see nothing get zeros.
     Returns [tokens, nh, 128] fp16; rows behind q_start[n] are left as they are."""
     dev, book = _book(pages)
-    if q.dim() != 3 or q.shape[2] != 128 or q.dtype is not torch.float16 or q.device != dev:
-        raise RuntimeError(f"paged_attention takes fp16 queries [tokens, heads, 128] on {dev}")
+    if q.dim() != 3 or q.dtype is not _f16 or q.get_device() != dev or q.shape[2] != 128:
+        raise RuntimeError(f"paged_attention takes fp16 queries [tokens, heads, 128] on cuda:{dev}")
     tokens, nh, _ = q.shape
     n = rows.numel()
     block = _layer(pages, dev, layer)
@@ -262,16 +279,16 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     if q.stride(2) != 1:
         q = q.contiguous()
     if out is None:
-        out = torch.empty((tokens, nh, 128), dtype=torch.float16, device=dev)
-    elif out.shape != q.shape or out.dtype is not torch.float16 or out.device != dev or out.stride(2) != 1:
+        out = q.new_empty((tokens, nh, 128))
+    elif out.shape != q.shape or out.dtype is not _f16 or out.get_device() != dev or out.stride(2) != 1:
         raise RuntimeError("out must be fp16 like q, contiguous along the channels")
     window, softcap = window or 0, softcap or 0.0
     if window < 0 or not softcap >= 0.0:
         raise RuntimeError("window and softcap must not be negative")
     at_slopes = 0
     if alibi_slopes is not None:
-        if alibi_slopes.dtype is not torch.float32 or alibi_slopes.shape != (nh,) or alibi_slopes.device != dev or not alibi_slopes.is_contiguous():
-            raise RuntimeError(f"alibi_slopes must be float32 [{nh}] on {dev}")
+        if alibi_slopes.dtype is not torch.float32 or alibi_slopes.shape != (nh,) or alibi_slopes.get_device() != dev or not alibi_slopes.is_contiguous():
+            raise RuntimeError(f"alibi_slopes must be float32 [{nh}] on cuda:{dev}")
         at_slopes = alibi_slopes.data_ptr()
     max_new = tokens if max_new is None else min(int(max_new), tokens)
     most = pages.table.shape[1] * PAGE_TOKENS
@@ -280,7 +297,7 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
         raise RuntimeError("max_new and max_tokens must be positive")
     L = _library()
     need = L.kvq_paged_attn_workspace_bytes(block, n, tokens, nh, max_new, max_tokens)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = pages.count.new_empty((need + 3) // 4) if need else None
     a = _pack_attn(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), _ints(dev, "q_start", q_start, n + 1),
                    _rows(dev, "rows", rows), 0 if first is None else _ints(dev, "first", first, tokens), 0 if prefix is None else _ints(dev, "prefix", prefix, n),
                    at_slopes, n, tokens, nh, max_new, max_tokens, int(window), int(bool(causal)),
