@@ -26,7 +26,7 @@ constexpr int kRawBytes = 12288;                                  // the largest
 constexpr uint32_t kOffQ = 0, kOffK = 2 * kOperandBytes, kOffV = kOffK + 2 * kOperandBytes, kOffRaw = kOffV + 2 * kOperandBytes,
                    kOffBar = kOffRaw + 2 * kRawBytes, kTileSmem = kOffBar + 256;
 // barriers; kBarP: tile and half of the page's tokens
-constexpr int kBarQ = 0, kBarKFull = 1, kBarKFree = 3, kBarVFull = 5, kBarVFree = 7, kBarS = 9, kBarP = 11, kBarO = 15, kBarRaw = 16, kBarRawFree = 18, kBarDrain = 20, kBarTail = 21;
+constexpr int kBarKFull = 1, kBarKFree = 3, kBarVFull = 5, kBarVFree = 7, kBarS = 9, kBarP = 11, kBarO = 15, kBarRaw = 16, kBarRawFree = 18, kBarDrain = 20, kBarTail = 21;
 
 // fp16 pages as rows of 128 channels, for copies of 64 channels x 128 rows that swizzle on the way
 struct PagedMaps {
@@ -44,7 +44,7 @@ __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sy
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 // One thread (`lead`) issues an MMA or a commit, but its whole warp walks there with values that are the same in all lanes: operands then
 // stand in uniform registers, where these instructions want them.  In a branch of that thread alone each descriptor was moved there
-// word by word: a page took 4400 cycles and %s so.
+// word by word: a page took 4400 cycles, and 3200 so.
 __device__ __forceinline__ void tc_commit(uint32_t bar, uint32_t lead) {
     asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %1, 0;\n@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar), "r"(lead) : "memory");
 }
@@ -145,7 +145,7 @@ __device__ __forceinline__ unsigned long long cap_small(unsigned long long x, un
 }
 
 // MODS: scores are capped, biased or scaled by a negative number.  Calls without have an instance of their own: with the code beside it the
-// 128 scores of a thread no longer fit its registers (2048 tokens over 32k: 1261 us in place of %s).
+// 128 scores of a thread no longer fit its registers (2048 tokens over 32k: 1261 us in place of 1132).
 template <int KB, int VB, bool MODS>
 __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ PagedMaps maps, int max_tiles) {
     extern __shared__ __align__(1024) char smem[];
@@ -165,9 +165,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     const int warp = uniform_warp(), lane = threadIdx.x & 31, wg = warp >> 2;
 
     const uint32_t base = smem_u32(smem), bars = base + kOffBar;
+    // Q, 16 threads a row, asked for before anything that does not have to come first: a row a thread, after the barrier, the same loads took 6 us
+    // of a CTA that has some 30 us of pages
+    uint4 qv[8];
+    {
+        const bool vec = (reinterpret_cast<uintptr_t>(p.a.q) % 16 | p.a.q_sT % 8 | p.a.q_sH % 8) == 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = (threadIdx.x >> 4) + 32 * i, idx = row0 + row, u = idx / p.rep, h = head * p.rep + (idx - u * p.rep);
+            const __half *q = static_cast<const __half *>(p.a.q) + (int64_t)(s.q0 + u) * p.a.q_sT + (int64_t)h * p.a.q_sH + 8 * (threadIdx.x & 15);
+            qv[i] = make_uint4(0, 0, 0, 0);
+            if (row >= rows) continue;
+            if (vec) qv[i] = *reinterpret_cast<const uint4 *>(q);
+            else {
+                alignas(16) __half y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = q[j];
+                qv[i] = *reinterpret_cast<const uint4 *>(y);
+            }
+        }
+    }
     auto bar = [&](int k) { return bars + 8 * k; };
     if (threadIdx.x == 0) {
-        mbar_init(bar(kBarQ), two_tiles ? 256 : 128);
         for (int k = 0; k < 2; ++k) {
             mbar_init(bar(kBarKFull + k), 1);
             mbar_init(bar(kBarKFree + k), 1);
@@ -201,6 +220,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         last = (int)__reduce_max_sync(0xffffffffu, (unsigned)last);
         __shared__ int s_first[kTileThreads / 32], s_last[kTileThreads / 32];
         if (lane == 0) { s_first[warp] = first; s_last[warp] = last; }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = (threadIdx.x >> 4) + 32 * i;
+            sts128(operand_at(base + kOffQ + (row >> 7) * kOperandBytes, row & 127, threadIdx.x & 15), qv[i].x, qv[i].y, qv[i].z, qv[i].w);
+        }
+        fence_async();
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
@@ -228,28 +253,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         const bool mine = wg * kTileRows + r < rows;
         if (wg == 0 || two_tiles) {
             int pos = 0, lo = 0, hi = 0;
-            {
-                const __half *q = static_cast<const __half *>(p.a.q) + (int64_t)(s.q0 + u) * p.a.q_sT + (int64_t)h * p.a.q_sH;
-                const bool vec = (reinterpret_cast<uintptr_t>(p.a.q) % 16 | p.a.q_sT % 8 | p.a.q_sH % 8) == 0;
-                const uint32_t to = base + kOffQ + wg * kOperandBytes;
-#pragma unroll 4
-                for (int c = 0; c < 16; ++c) {
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (mine) {
-                        if (vec) x = *reinterpret_cast<const uint4 *>(q + 8 * c);
-                        else {
-                            alignas(16) __half y[8];
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) y[j] = q[8 * c + j];
-                            x = *reinterpret_cast<const uint4 *>(y);
-                        }
-                    }
-                    sts128(operand_at(to, r, c), x.x, x.y, x.z, x.w);
-                }
-                fence_async();
-                mbar_arrive(bar(kBarQ));
-                if (mine) paged_bounds(p, s, u, pos, lo, hi);
-            }
+            if (mine) paged_bounds(p, s, u, pos, lo, hi);
             const bool cap = MODS && p.a.softcap > 0.f, bias = MODS && p.a.slopes != nullptr, flip = MODS && !cap && !bias;
             const float scale2 = p.a.softmax_scale * kLog2e, two = cap ? 2.f * scale2 / p.a.softcap : 0.f, cap2 = p.a.softcap * kLog2e,
                         small = cap ? p.a.softmax_scale / p.a.softcap : 0.f;
@@ -449,7 +453,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             const uint64_t q_desc = tc_desc(base + kOffQ, 16, 1024), k_desc = tc_desc(base + kOffK, 16, 1024), k_mn = tc_desc(base + kOffK, kOperandHalf, 1024),
                            v_desc = tc_desc(base + kOffV, kOperandHalf, 1024);
             auto wait = [&](int b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar(b), parity, status)); };
-            bool ok = pages == 0 || wait(kBarQ, 0);
+            bool ok = true;
             // the address fields of descriptors count 16 bytes, and no operand's end carries out of them
             auto scores = [&](int it, int w) {                    // S[w] = Q[w] K^T of page `it`
                 const uint64_t q = q_desc + w * (kOperandBytes / 16);
