@@ -10,8 +10,12 @@ namespace kvq {
 // that any of them sees.  A page is one step of both products:
 //   S = Q K^T   128 x 128 x 128, Q and K in shared memory, S (fp32) in TMEM
 //   O += P V    P, the weights as fp16, over S in TMEM; V in shared memory; O (fp32) in TMEM
-// Sixteen warps: two warpgroups of softmax, one per tile, a row a thread; one that fills the operand buffers; one thread that issues the
-// MMAs.  While one tile's scores are worked on, the tensor core multiplies for the other.  TMEM: S0 S1 O0 O1, 128 columns each.
+// Twenty-four warps: four warpgroups of softmax, two per tile, half a row a thread (a row a thread: the same time for plain scores, 221 in place of
+// 190 us for four capped chunks of 501 tokens); one that fills the operand buffers; a warp that issues the MMAs and a thread that issues
+// copies.  While one tile's scores are worked on, the tensor core multiplies for the other.  TMEM: S0 S1 O0 O1, 128 columns each.
+// Bound: a page is 2048 cycles of MMA and as many of the special function unit (one exponential a score) and takes some 3200; under it the
+// card runs at its power limit (1.5 to 1.6 GHz).  2048 tokens x 32 heads over 34816: 1055 TFLOP/s, 0.65 of the rate measured in bursts and 0.77 of
+// the sustained one.  Tried without gain: a part of the exponentials as polynomials (2 to 20 % slower), weights handed over in quarters.
 //
 // Operand buffers hold 128 rows of 128 fp16 as two halves of 64 (128 bytes a row, 16-byte pieces swizzled by the row's number).  Rows are
 // tokens of fp16 pages and of packed values, channels of packed keys: what is contiguous in a row is the contraction axis of fp16 keys (K-major
@@ -19,14 +23,14 @@ namespace kvq {
 // their fields lie side by side and nothing is transposed.
 // Packed rows become fp16 as code * scale + minimum with one rounding (2^-11 relative): the tensor core takes no wider operand without
 // half its rate.
-constexpr int kTileRows = 128, kTileThreads = 512;
+constexpr int kTileRows = 128, kTileThreads = 768;
 constexpr uint32_t kOperandBytes = 32768, kOperandHalf = 16384;
 constexpr int kRawBytes = 12288;                                  // the largest packed half of a page: 3 bits, or 4 bits and groups of 32
 // shared memory, from a 1024-byte boundary
 constexpr uint32_t kOffQ = 0, kOffK = 2 * kOperandBytes, kOffV = kOffK + 2 * kOperandBytes, kOffRaw = kOffV + 2 * kOperandBytes,
-                   kOffBar = kOffRaw + 2 * kRawBytes, kTileSmem = kOffBar + 256;
-// barriers; kBarP: tile and half of the page's tokens
-constexpr int kBarKFull = 1, kBarKFree = 3, kBarVFull = 5, kBarVFree = 7, kBarS = 9, kBarP = 11, kBarO = 15, kBarRaw = 16, kBarRawFree = 18, kBarDrain = 20, kBarTail = 21;
+                   kOffBar = kOffRaw + 2 * kRawBytes, kOffTop = kOffBar + 256, kTileSmem = kOffTop + 2 * 2 * 2 * kTileRows * 4;      // tops: page, tile, half
+// barriers
+constexpr int kBarKFull = 1, kBarKFree = 3, kBarVFull = 5, kBarVFree = 7, kBarS = 9, kBarP = 11, kBarO = 13, kBarRaw = 14, kBarRawFree = 16, kBarDrain = 18, kBarTail = 19;
 
 // fp16 pages as rows of 128 channels, for copies of 64 channels x 128 rows that swizzle on the way
 struct PagedMaps {
@@ -64,14 +68,16 @@ __device__ __forceinline__ void tc_mma_tmem(uint32_t d, uint32_t a, uint64_t b, 
 
 #define KVQ_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
 #define KVQ_W8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
-// 32 columns of this thread's row
+// 32 or 16 columns of this thread's row
 __device__ __forceinline__ void tc_load32(uint32_t (&r)[32], uint32_t addr) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
                  : KVQ_R8(r, 0), KVQ_R8(r, 8), KVQ_R8(r, 16), KVQ_R8(r, 24) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void tc_store32(uint32_t addr, const uint32_t (&r)[32]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(addr),
-                 KVQ_W8(r, 0), KVQ_W8(r, 8), KVQ_W8(r, 16), KVQ_W8(r, 24) : "memory");
+__device__ __forceinline__ void tc_load16(uint32_t (&r)[16], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n" : KVQ_R8(r, 0), KVQ_R8(r, 8) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tc_store16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr), KVQ_W8(r, 0), KVQ_W8(r, 8) : "memory");
 }
 
 // Piece c (16 bytes, 0..15) of row r of an operand buffer
@@ -167,12 +173,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     const uint32_t base = smem_u32(smem), bars = base + kOffBar;
     // Q, 16 threads a row, asked for before anything that does not have to come first: a row a thread, after the barrier, the same loads took 6 us
     // of a CTA that has some 30 us of pages
-    uint4 qv[8];
+    uint4 qv[6];
     {
         const bool vec = (reinterpret_cast<uintptr_t>(p.a.q) % 16 | p.a.q_sT % 8 | p.a.q_sH % 8) == 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int row = (threadIdx.x >> 4) + 32 * i, idx = row0 + row, u = idx / p.rep, h = head * p.rep + (idx - u * p.rep);
+        for (int i = 0; i < 6; ++i) {
+            const int row = (threadIdx.x >> 4) + 48 * i, idx = row0 + row, u = idx / p.rep, h = head * p.rep + (idx - u * p.rep);
             const __half *q = static_cast<const __half *>(p.a.q) + (int64_t)(s.q0 + u) * p.a.q_sT + (int64_t)h * p.a.q_sH + 8 * (threadIdx.x & 15);
             qv[i] = make_uint4(0, 0, 0, 0);
             if (row >= rows) continue;
@@ -193,8 +199,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             mbar_init(bar(kBarVFull + k), 1);
             mbar_init(bar(kBarVFree + k), 1);
             mbar_init(bar(kBarS + k), 1);
-            mbar_init(bar(kBarP + 2 * k), 128);
-            mbar_init(bar(kBarP + 2 * k + 1), 128);
+            mbar_init(bar(kBarP + k), 256);
             mbar_init(bar(kBarRaw + k), 1);
             mbar_init(bar(kBarRawFree + k), 1);
         }
@@ -203,7 +208,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         mbar_init(bar(kBarDrain), 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 20) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
     }
@@ -221,9 +226,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         __shared__ int s_first[kTileThreads / 32], s_last[kTileThreads / 32];
         if (lane == 0) { s_first[warp] = first; s_last[warp] = last; }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int row = (threadIdx.x >> 4) + 32 * i;
-            sts128(operand_at(base + kOffQ + (row >> 7) * kOperandBytes, row & 127, threadIdx.x & 15), qv[i].x, qv[i].y, qv[i].z, qv[i].w);
+        for (int i = 0; i < 6; ++i) {
+            const int row = (threadIdx.x >> 4) + 48 * i;
+            if (row < 2 * kTileRows) sts128(operand_at(base + kOffQ + (row >> 7) * kOperandBytes, row & 127, threadIdx.x & 15), qv[i].x, qv[i].y, qv[i].z, qv[i].w);
         }
         fence_async();
         tc_fence_before();
@@ -246,30 +251,31 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     // pages that is the loader.
     auto by_loader = [&](int page, int id) { return maps.there && (page + 1) * kPage <= s.length && id >= 0; };
 
-    if (wg < 2) {
-        // ------------------------------------------------------------------ softmax, one row a thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;\n");
-        const int r = threadIdx.x & 127, idx = row0 + wg * kTileRows + r, u = idx / p.rep, h = head * p.rep + (idx - u * p.rep);
-        const bool mine = wg * kTileRows + r < rows;
-        if (wg == 0 || two_tiles) {
+    if (wg < 4) {
+        // ------------------------------------------------------------------ softmax, 64 columns of one row a thread
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 88;\n");
+        constexpr int N = 64;
+        const int tile_of = wg >> 1, half = wg & 1, r = threadIdx.x & 127, idx = row0 + tile_of * kTileRows + r, u = idx / p.rep, h = head * p.rep + (idx - u * p.rep);
+        const bool mine = tile_of * kTileRows + r < rows;
+        if (tile_of == 0 || two_tiles) {
             int pos = 0, lo = 0, hi = 0;
             if (mine) paged_bounds(p, s, u, pos, lo, hi);
             const bool cap = MODS && p.a.softcap > 0.f, bias = MODS && p.a.slopes != nullptr, flip = MODS && !cap && !bias;
-            const float scale2 = p.a.softmax_scale * kLog2e, two = cap ? 2.f * scale2 / p.a.softcap : 0.f, cap2 = p.a.softcap * kLog2e,
-                        small = cap ? p.a.softmax_scale / p.a.softcap : 0.f;
+            const float scale2 = p.a.softmax_scale * kLog2e, cap2 = p.a.softcap * kLog2e;
             const float slope = bias && mine ? p.a.slopes[h] * kLog2e : 0.f, mul = cap || bias || flip ? 1.f : scale2;
-            const uint32_t lanes = (uint32_t)(warp & 3) << 21, t_s = tmem + wg * 128 + lanes, t_o = tmem + 256 + wg * 128 + lanes;
+            const uint32_t lanes = (uint32_t)(warp & 3) << 21, t_s = tmem + tile_of * 128 + lanes, t_o = tmem + 256 + tile_of * 128 + half * N + lanes;
+            const uint32_t my_top = base + kOffTop + ((tile_of * 2 + half) * kTileRows + r) * 4, other_top = half ? my_top - kTileRows * 4 : my_top + kTileRows * 4;
+            auto pair_meets = [&]() { asm volatile("bar.sync %0, 256;\n" ::"r"(2 + tile_of) : "memory"); };
             float m = -INFINITY, l = 0.f;
             bool ok = true;
             for (int it = 0; it < np; ++it) {
-                const int page = p0 + it, b0 = page * kPage;
+                const int page = p0 + it, b0 = page * kPage + half * N;
                 const bool there = page_id(page) >= 0;
-                ok = mbar_wait(bar(kBarS + wg), it & 1, status);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(bar(kBarS + tile_of), it & 1, status));            // given up: through the barriers to the end
                 tc_fence_after();
-                uint32_t x[4][32];
+                uint32_t x[2][32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tc_load32(x[c], t_s + 32 * c);
+                for (int c = 0; c < 2; ++c) tc_load32(x[c], t_s + half * N + 32 * c);
                 tc_wait_ld();
                 auto at = [&](int j) -> uint32_t & { return x[j >> 5][j & 31]; };
                 auto pair = [&](int j) { return f32x2(__uint_as_float(at(j)), __uint_as_float(at(j + 1))); };
@@ -279,42 +285,52 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                     at(j + 1) = __float_as_uint(w.y);
                 };
                 if (cap) {
+                    const float small = p.a.softmax_scale / p.a.softcap;
                     float most = 0.f;
 #pragma unroll
-                    for (int j = 0; j < 128; j += 2) most = max_abs(most, __uint_as_float(at(j)), __uint_as_float(at(j + 1)));
+                    for (int j = 0; j < N; j += 2) most = max_abs(most, __uint_as_float(at(j)), __uint_as_float(at(j + 1)));
                     if (__all_sync(0xffffffffu, most * fabsf(small) <= 0.75f)) {
                         const unsigned long long in = f32x2(small, small), by = f32x2(cap2, cap2);
 #pragma unroll
-                        for (int j = 0; j < 128; j += 2) put(j, cap_small(mul_f32x2(pair(j), in), by));
+                        for (int j = 0; j < N; j += 2) put(j, cap_small(mul_f32x2(pair(j), in), by));
                     } else {
+                        const float two = 2.f * scale2 / p.a.softcap;
 #pragma unroll
-                        for (int j = 0; j < 128; ++j) at(j) = __float_as_uint(cap_score(__uint_as_float(at(j)), two, cap2));
+                        for (int j = 0; j < N; ++j) at(j) = __float_as_uint(cap_score(__uint_as_float(at(j)), two, cap2));
                     }
                 }
                 if (bias) {
                     unsigned long long b = f32x2(slope * (float)(b0 - pos), slope * (float)(b0 + 1 - pos));
                     const unsigned long long by = f32x2(cap ? 1.f : scale2, cap ? 1.f : scale2), step = f32x2(2.f * slope, 2.f * slope);
 #pragma unroll
-                    for (int j = 0; j < 128; j += 2) {
-                        // eight running sums of one page drift by less than the rounding of a bias this large; started anew every 16 positions
+                    for (int j = 0; j < N; j += 2) {
+                        // eight running sums drift by less than the rounding of a bias this large; started anew every 16 positions
                         if (j && j % 16 == 0) b = f32x2(slope * (float)(b0 + j - pos), slope * (float)(b0 + j + 1 - pos));
                         put(j, fma_f32x2(pair(j), by, b));
                         b = add_f32x2(b, step);
                     }
                 } else if (flip) {
 #pragma unroll
-                    for (int j = 0; j < 128; j += 2) put(j, mul_f32x2(pair(j), f32x2(scale2, scale2)));
+                    for (int j = 0; j < N; j += 2) put(j, mul_f32x2(pair(j), f32x2(scale2, scale2)));
                 }
-                if (!__all_sync(0xffffffffu, lo <= b0 && hi >= b0 + kPage && there)) {
-                    const int from = there ? lo - b0 : kPage, to = there ? hi - b0 : 0;
+                if (!__all_sync(0xffffffffu, lo <= b0 && hi >= b0 + N && there)) {
+                    const int from = there ? lo - b0 : N, to = there ? hi - b0 : 0;
 #pragma unroll
-                    for (int j = 0; j < 128; ++j)
+                    for (int j = 0; j < N; ++j)
                         if (j < from || j >= to) at(j) = 0xff800000u;
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int j = 0; j < 128; j += 2) top[j >> 1 & 3] = max3(top[j >> 1 & 3], __uint_as_float(at(j)), __uint_as_float(at(j + 1)));
-                const float best = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * mul;
+                for (int j = 0; j < N; j += 2) top[j >> 1 & 3] = max3(top[j >> 1 & 3], __uint_as_float(at(j)), __uint_as_float(at(j + 1)));
+                // the other half of the row; two places by turns, so that one meeting a page is enough.  It also stands between the other half's reading
+                // of S and the weights that are written over it.
+                const float half_best = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * mul;
+                const uint32_t turn = (it & 1) * (4 * kTileRows * 4);
+                asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(my_top + turn), "f"(half_best) : "memory");
+                tc_fence_before();
+                pair_meets();
+                tc_fence_after();
+                const float best = max3(half_best, __uint_as_float(lds32(other_top + turn)), half_best);
                 if (best != best) l = best;                       // a score is not a number: neither is the row
                 // The reference follows the maximum only when it grows by more than 2^8: weights up to 256 are as exact in fp16, and O is
                 // rescaled a few times a row in place of at every page.
@@ -326,12 +342,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                     if (it > 0) {
 #pragma unroll 1
                         for (int c = 0; c < 4; ++c) {
-                            uint32_t o[32];
-                            tc_load32(o, t_o + 32 * c);
+                            uint32_t o[16];
+                            tc_load16(o, t_o + 16 * c);
                             tc_wait_ld();
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                            tc_store32(t_o + 32 * c, o);
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            tc_store16(t_o + 16 * c, o);
                         }
                     }
                 }
@@ -340,68 +356,69 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                 const unsigned long long mul2 = f32x2(mul, mul), ref2 = f32x2(-ref, -ref);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    uint32_t w[32];
+                    uint32_t w[16];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const unsigned long long e = fma_f32x2(f32x2(__uint_as_float(at(64 * c + 2 * j)), __uint_as_float(at(64 * c + 2 * j + 1))), mul2, ref2);
-                        float2 v = f32x2_split(e);
+                    for (int j = 0; j < 16; ++j) {
+                        float2 v = f32x2_split(fma_f32x2(pair(32 * c + 2 * j), mul2, ref2));
                         v.x = exp2_approx(v.x);
                         v.y = exp2_approx(v.y);
                         sum[j & 1] = add_f32x2(sum[j & 1], f32x2(v.x, v.y));
                         w[j] = as_u32(__floats2half2_rn(v.x, v.y));
                     }
-                    tc_store32(t_s + 32 * c, w);
-                    tc_wait_st();
-                    tc_fence_before();
-                    mbar_arrive(bar(kBarP + 2 * wg + c));
+                    tc_store16(t_s + half * 32 + 16 * c, w);
                 }
+                tc_wait_st();
+                tc_fence_before();
+                if (ok) mbar_arrive(bar(kBarP + tile_of));
                 const float2 both = f32x2_split(add_f32x2(sum[0], sum[1]));
                 l += both.x + both.y;
             }
-            if (ok && np > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarO), 0, status));
+            if (np > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(bar(kBarO), 0, status));
             tc_fence_after();
+            asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(my_top), "f"(l) : "memory");
+            pair_meets();
+            l = half ? __uint_as_float(lds32(other_top)) + l : l + __uint_as_float(lds32(other_top));
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            __half *out = static_cast<__half *>(p.a.out) + (int64_t)(s.q0 + u) * p.a.o_sT + (int64_t)h * p.a.o_sH;
+            __half *out = static_cast<__half *>(p.a.out) + (int64_t)(s.q0 + u) * p.a.o_sT + (int64_t)h * p.a.o_sH + half * N;
             const int64_t part = (int64_t)split * p.a.tokens * p.a.nh + (int64_t)(s.q0 + u) * p.a.nh + h;
             const bool vec = (reinterpret_cast<uintptr_t>(p.a.out) % 16 | p.a.o_sT % 8 | p.a.o_sH % 8) == 0;
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
-                uint32_t o[32];
+                uint32_t o[16];
                 __syncwarp();
                 if (np > 0) {
-                    tc_load32(o, t_o + 32 * c);
+                    tc_load16(o, t_o + 16 * c);
                     tc_wait_ld();
                 }
                 if (!mine) continue;
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
+                for (int j = 0; j < 16; ++j)
                     if (np == 0 || l == 0.f) o[j] = 0;
                 if (p.splits > 1) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) reinterpret_cast<uint4 *>(p.part_out + part * 128 + 32 * c)[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                    for (int j = 0; j < 4; ++j) reinterpret_cast<uint4 *>(p.part_out + part * 128 + half * N + 16 * c)[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                 } else {
-                    uint32_t w[16];
+                    uint32_t w[8];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) w[j] = as_u32(__floats2half2_rn(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv));
+                    for (int j = 0; j < 8; ++j) w[j] = as_u32(__floats2half2_rn(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv));
                     if (vec) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) reinterpret_cast<uint4 *>(out + 32 * c)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                        for (int j = 0; j < 2; ++j) reinterpret_cast<uint4 *>(out + 16 * c)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) out[32 * c + j] = __ushort_as_half((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
+                        for (int j = 0; j < 16; ++j) out[16 * c + j] = __ushort_as_half((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
                     }
                 }
             }
-            if (mine && p.splits > 1) {
+            if (mine && half == 0 && p.splits > 1) {
                 p.part_ml[2 * part] = m;
                 p.part_ml[2 * part + 1] = l;
             }
             tc_fence_before();
         }
-    } else if (wg == 2) {
+    } else if (wg == 4) {
         // ------------------------------------------------------------------ operands: job 2i is page i's keys, 2i + 1 its values.  Packed
         // ones are unpacked here, and the fp16 page that holds the sequence's end is copied here, with zeros behind the end.
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
         const int r = threadIdx.x & 127;
         bool ok = true;
         uint32_t tails = 0;
@@ -444,7 +461,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     } else {
         // ------------------------------------------------------------------ MMAs
         asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
-        if (warp == 12) {
+        if (warp == 20) {
             uint32_t lead;
             asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
             auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
@@ -468,10 +485,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                 }
                 tc_commit(bar(kBarS + w), lead);
             };
-            auto values = [&](int it, int w, int half) {          // O[w] += P[w] V, half of the tokens
-                const uint64_t v = v_desc + (it & 1) * (kOperandBytes / 16) + half * 512;
+            auto values = [&](int it, int w) {                    // O[w] += P[w] V
+                const uint64_t v = v_desc + (it & 1) * (kOperandBytes / 16);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) tc_mma_tmem(tm + 256 + w * 128, tm + w * 128 + half * 32 + e * 8, v + e * 128, kIdescMn, it > 0 || half > 0 || e > 0, lead);
+                for (int e = 0; e < 8; ++e) tc_mma_tmem(tm + 256 + w * 128, tm + w * 128 + e * 8, v + e * 128, kIdescMn, it > 0 || e > 0, lead);
             };
             if (ok && pages > 0) {
                 ok = wait(kBarKFull, 0);
@@ -484,11 +501,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             for (int it = 0; ok && it < pages; ++it) {
                 ok = wait(kBarVFull + (it & 1), it >> 1 & 1);
                 for (int w = 0; ok && w < tiles; ++w) {
-                    for (int half = 0; ok && half < 2; ++half) {
-                        ok = wait(kBarP + 2 * w + half, it & 1);
-                        tc_fence_after();
-                        if (ok) values(it, w, half);
-                    }
+                    ok = wait(kBarP + w, it & 1);
+                    tc_fence_after();
+                    if (ok) values(it, w);
                     if (ok && w == tiles - 1) tc_commit(bar(kBarVFree + (it & 1)), lead);
                     if (ok && it + 1 < pages && w == 0) ok = wait(kBarKFull + (it + 1 & 1), (it + 1) >> 1 & 1);
                     if (ok && it + 1 < pages) scores(it + 1, w);
@@ -499,7 +514,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             if (ok && pages > 0) tc_commit(bar(kBarO), lead);
             tc_commit(bar(kBarDrain), lead);                      // whatever was begun is done before the memory is given up
             wait(kBarDrain, 0);
-        } else if (warp == 13 && lane == 0) {
+        } else if (warp == 21 && lane == 0) {
             // -------------------------------------------------------------- copies: packed pages as they are, fp16 pages into their operands
             bool ok = true;
             int j = 0, next = np > 0 ? page_id(p0) : -1, id = -1;
@@ -540,7 +555,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         __syncwarp();
     }
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 20) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
     }
