@@ -12,7 +12,8 @@ namespace kvq {
 // code * 2^(position - 24), and the power of two, the same for a whole accumulator, comes off at the end.  Scales go to the other
 // operand, whose columns are (group of the packed axis, query row) pairs:
 //   keys     B = q * scale of a channel's token group, as an exact pair hi + lo of two columns (rounded once it would cost 2^-11 of every term)
-//   values   B = p * scale of a token's channel group, rounded to fp16 as weights are everywhere
+//   values   B = p * scale of a token's channel group, rounded to fp16 as weights are everywhere; a pair as well where columns are left (one
+//            sequence of 1, 2 or 4 rows at groups of 32, 64 or 128: 2.5e-4 of an output's size in place of 3.2e-4, at 2 bits)
 // An accumulator row needs the column of its own group only; what the others hold is not read.  Minima times q or p come from one more MMA
 // a k-step, whose rows are the groups.  3-bit words are groups of their own, so their fields become fp16 values (code * scale + minimum,
 // rounded once) and the columns are query rows.
@@ -415,8 +416,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
     for (int m = 0; m < VT; ++m)
 #pragma unroll
         for (int e = 0; e < 4; ++e) out[m][e] = 0.f;
-    // values' columns: group and row of B's column g, and of the accumulators' columns 2t, 2t + 1
-    const int vr_log2 = VB == 3 ? 3 : 3 - ng_log2, v_grp = g >> vr_log2, v_row = min(g & ((1 << vr_log2) - 1), R - 1), o_row = 2 * t & ((1 << vr_log2) - 1), o_grp = 2 * t >> vr_log2;
+    // values' columns: group and row of B's column g, and of the accumulators' columns 2t, 2t + 1 (VPAIR: hi and lo of one row)
+    constexpr bool VPAIR = KB != 3 && VB != 3 && CK == 1;
+    const int vr_log2 = VB == 3 ? 3 : (VPAIR ? 2 : 3) - ng_log2, v_col = VPAIR ? g >> 1 : g, o_col = VPAIR ? t : 2 * t;
+    const int v_grp = v_col >> vr_log2, v_row = min(v_col & ((1 << vr_log2) - 1), R - 1), o_row = o_col & ((1 << vr_log2) - 1), o_grp = o_col >> vr_log2;
+    const int o_row1 = VPAIR ? o_row : o_row + 1;
+    const uint32_t v_lo = VPAIR && (g & 1) ? 0xffffffffu : 0u;
     // p * scale * 2^expo: the power of two starts from the first scales (the largest of them becomes 4 to 8) and goes down where one would exceed 256
     int expo = 32;
 #pragma unroll 1
@@ -505,9 +510,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
             }
         }
         if (softmax_page(page_at(k) * kPage, kPage)) {
-            rescale(out, o_row, o_row + 1);
+            rescale(out, o_row, o_row1);
             if constexpr (VB != 3) {
-                const float a0 = __shfl_sync(0xffffffffu, alpha, o_row), a1 = __shfl_sync(0xffffffffu, alpha, o_row + 1);
+                const float a0 = __shfl_sync(0xffffffffu, alpha, o_row), a1 = __shfl_sync(0xffffffffu, alpha, o_row1);
                 out_mn[0] *= a0;
                 out_mn[1] *= a1;
             }
@@ -548,9 +553,16 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
                     weights(v_row, step0 + at / 16, b0, b1);
                     few_pairs(c_mn, at, t, p.v_groups, g & (p.v_groups - 1), mn);
                     few_pairs(c_sc, at, t, p.v_groups, v_grp, sv);
-                    mma16816(out_mn, mn[0], 0u, mn[1], 0u, b0, b1);
-                    b0 = as_u32(__hmul2(as_h2(b0), __hmul2(as_h2(sv[0]), by)));
-                    b1 = as_u32(__hmul2(as_h2(b1), __hmul2(as_h2(sv[1]), by)));
+                    const __half2 s0 = __hmul2(as_h2(sv[0]), by), s1 = __hmul2(as_h2(sv[1]), by);
+                    if constexpr (VPAIR) {
+                        mma16816(out_mn, mn[0], 0u, mn[1], 0u, b0 & ~v_lo, b1 & ~v_lo);
+                        b0 = hilo(as_h2(b0), s0, v_lo);
+                        b1 = hilo(as_h2(b1), s1, v_lo);
+                    } else {
+                        mma16816(out_mn, mn[0], 0u, mn[1], 0u, b0, b1);
+                        b0 = as_u32(__hmul2(as_h2(b0), s0));
+                        b1 = as_u32(__hmul2(as_h2(b1), s1));
+                    }
 #pragma unroll
                     for (int m = 0; m < 8; ++m) mma16816(out[m], a.a(m, 0), a.a(m, 1), a.a(m, 2), a.a(m, 3), b0, b1);
                 }
@@ -580,7 +592,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
                 if (c >= 0 && 2 * t + 1 < rows) add(2 * t + 1, c, out[m][2 * e + 1], f1);
             }
     } else {
-        const float f0 = __shfl_sync(0xffffffffu, aside_by, o_row), f1 = __shfl_sync(0xffffffffu, aside_by, o_row + 1);
+        const float f0 = __shfl_sync(0xffffffffu, aside_by, o_row), f1 = __shfl_sync(0xffffffffu, aside_by, o_row1);
         const float z0 = __shfl_sync(0xffffffffu, out_mn[0], 4 * own_group + t), z1 = __shfl_sync(0xffffffffu, out_mn[1], 4 * own_group + t);
         const float undo = expo == 32 ? 0.f : exp2f((float)-expo);
         if (o_grp == own_group) {
@@ -590,8 +602,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
                 for (int e = 0; e < 2; ++e) {
                     const int c = few_element<1>(g, m, e);
                     const float f = few_power<VB>(m, e) * undo;
-                    if (o_row < rows) add(o_row, c, fmaf(out[m][2 * e], f, z0), f0);
-                    if (o_row + 1 < rows) add(o_row + 1, c, fmaf(out[m][2 * e + 1], f, z1), f1);
+                    if (o_row < rows) add(o_row, c, fmaf(VPAIR ? out[m][2 * e] + out[m][2 * e + 1] : out[m][2 * e], f, z0), f0);
+                    if (!VPAIR && o_row1 < rows) add(o_row1, c, fmaf(out[m][2 * e + 1], f, z1), f1);
                 }
         }
     }
