@@ -554,7 +554,9 @@ int kvq_page_write(const kvq_page_book *b, const kvq_page_layer *l, const kvq_pa
  * attention, documents packed behind one another (first = the document's start) and prefixes whose tokens all see each other.
  *   s = q.k * softmax_scale;  softcap > 0: s = softcap * tanh(s / softcap);  slopes: s += slopes[h] * (j - p);  out = softmax(s).v
  * A row that sees nothing gives zeros.  Positions beyond `length`, pages without a number and rows of q behind q_start[n] are neither
- * read nor written.  Keys and values that are not finite reach the queries that see them and may reach others of the same 128 tokens.
+ * read nor written.  Keys that are not finite reach the queries that see them.  Values have to be finite: one that is not reaches the
+ * queries that see it, and may reach (a weight of zero times infinity) every query that is worked on with one of those -- new tokens of the same
+ * sequence less than 256 positions before -- and every one that sees a token of its page.
  * GQA: query head h reads kv head h / (nh / Hkv).
  *   q, out [tokens, nh, 128] fp16, strides *_sT, *_sH;  first [tokens], prefix [n] int32, slopes [nh] fp32
  *   max_new: no sequence has more new tokens;  max_tokens: no sequence is longer (both only lay out the work)

@@ -1,4 +1,5 @@
 // Attention of few query rows of a kv head (a new token of a group of query heads) over a paged cache.
+#pragma once
 #include "paged_attn.cuh"
 
 namespace kvq {
@@ -637,50 +638,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
     }
 }
 
-// Partial sums of the splits -> outputs, in the splits' order: a row a warp.  `few`: rows of the kernel above, kFewRows places for every (sequence,
-// kv head); else rows of q, of which those that the kernel of tiles had are joined.
-__global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant__ PagedArgs p, int few) {
-    const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    int u, h;
-    if (few) {
-        const int r = (int)(at % kFewRows), head = (int)(at / kFewRows % p.l.Hkv);
-        const int64_t i = at / kFewRows / p.l.Hkv;
-        if (i >= p.a.n) return;
-        const PagedSeq s = paged_seq(p, (int)i);
-        if (s.n_new * p.rep > kFewRows || r >= s.n_new * p.rep) return;
-        u = s.q0 + r / p.rep;
-        h = head * p.rep + r % p.rep;
-    } else {
-        const int64_t q = at / p.a.nh;
-        if (q >= p.a.tokens || q < p.a.q_start[0] || q >= p.a.q_start[p.a.n]) return;
-        u = (int)q;
-        h = (int)(at - q * p.a.nh);
-        if (p.few_rows) {
-            const PagedSeq s = paged_seq(p, sequence_of(p.a.q_start, p.a.n, u));
-            if (s.n_new * p.rep <= p.few_rows) return;
-        }
-    }
-    const int64_t step = (int64_t)p.a.tokens * p.a.nh, row = (int64_t)u * p.a.nh + h;
-    float m = -INFINITY, l = 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = lane; i < p.splits; i += 32) m = fmaxf(m, p.part_ml[2 * (i * step + row)]);
-    m = warp_max(m);
-    for (int i = 0; i < p.splits; ++i) {
-        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * (i * step + row));
-        const float4 x = *reinterpret_cast<const float4 *>(p.part_out + (i * step + row) * 128 + 4 * lane);
-        const float f = part_factor(ml.x, ml.y, m);
-        l += f * ml.y;
-        if (f != 0.f) { v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w; }
-    }
-    __half *out = static_cast<__half *>(p.a.out) + (int64_t)u * p.a.o_sT + (int64_t)h * p.a.o_sH + 4 * lane;
-    auto put = [&](int c, float x) { out[c] = __float2half_rn(l == 0.f ? 0.f : x / l); };
-    put(0, v.x);
-    put(1, v.y);
-    put(2, v.z);
-    put(3, v.w);
-}
-
 template <int KB, int VB, int CK>
 static int launch_few(const PagedArgs &p, int R, int row_blocks, cudaStream_t st) {
     const int k_row = 4 * page_words(KB) + 4 * p.k_groups, v_row = 4 * page_words(VB) + 4 * p.v_groups, row = k_row > v_row ? k_row : v_row;
@@ -710,28 +667,14 @@ static int launch_few(const PagedArgs &p, cudaStream_t st) {
     return launch_few<KB, VB, 1>(p, f.rows, f.row_blocks, st);
 }
 
-int paged_few(const PagedArgs &p, cudaStream_t st) {
-#define KVQ_V(KB)                                                                                                             \
-    switch (p.l.v_bits) {                                                                                                     \
-        case 1: return launch_few<KB, 1>(p, st);                                                                              \
-        case 2: return launch_few<KB, 2>(p, st);                                                                              \
-        case 3: return launch_few<KB, 3>(p, st);                                                                              \
-        default: return launch_few<KB, 4>(p, st);                                                                             \
+template <int KB>
+static int launch_few(const PagedArgs &p, cudaStream_t st) {
+    switch (p.l.v_bits) {
+        case 1: return launch_few<KB, 1>(p, st);
+        case 2: return launch_few<KB, 2>(p, st);
+        case 3: return launch_few<KB, 3>(p, st);
+        default: return launch_few<KB, 4>(p, st);
     }
-    switch (p.l.k_bits) {
-        case 1: KVQ_V(1)
-        case 2: KVQ_V(2)
-        case 3: KVQ_V(3)
-        default: KVQ_V(4)
-    }
-#undef KVQ_V
-}
-
-int paged_merge(const PagedArgs &p, int few, cudaStream_t st) {
-    const int64_t rows = few ? (int64_t)p.a.n * p.l.Hkv * kFewRows : (int64_t)p.a.tokens * p.a.nh, grid = (rows + 7) / 8;
-    if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
-    paged_merge_kernel<<<(unsigned)grid, 256, 0, st>>>(p, few);
-    return check_launch();
 }
 
 }  // namespace kvq

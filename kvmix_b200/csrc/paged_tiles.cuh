@@ -1,4 +1,6 @@
-// Attention of many query rows of a kv head (chunks of prompts, the tokens of a speculative step) over a paged cache, on tcgen05.
+// Attention of many query rows of a kv head (chunks of prompts, the tokens of a speculative step) over a paged cache, on tcgen05.  A source
+// file for each width of the keys (paged_tiles_1.cu ..): their instances build side by side.
+#pragma once
 #include "paged_attn.cuh"
 #include "quant_core.cuh"
 
@@ -599,16 +601,6 @@ static int launch_tiles(const PagedArgs &p, int max_tiles, bool mods, cudaStream
         case 2: return mods ? launch_tiles<KB, 2, true>(p, max_tiles, st) : launch_tiles<KB, 2, false>(p, max_tiles, st);
         case 3: return mods ? launch_tiles<KB, 3, true>(p, max_tiles, st) : launch_tiles<KB, 3, false>(p, max_tiles, st);
         default: return mods ? launch_tiles<KB, 4, true>(p, max_tiles, st) : launch_tiles<KB, 4, false>(p, max_tiles, st);
-    }
-}
-
-int paged_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
-    const bool mods = p.a.softcap > 0.f || p.a.slopes || !(p.a.softmax_scale > 0.f);
-    switch (p.l.k_bits) {
-        case 1: return launch_tiles<1>(p, max_tiles, mods, st);
-        case 2: return launch_tiles<2>(p, max_tiles, mods, st);
-        case 3: return launch_tiles<3>(p, max_tiles, mods, st);
-        default: return launch_tiles<4>(p, max_tiles, mods, st);
     }
 }
 

@@ -265,7 +265,8 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     window: sliding window, None or 0 for none.  prefix int32 [n]: the first prefix[i] tokens see each other.  first int32 [tokens]: where the
     token's document begins, for documents packed behind one another.  softcap: scores become softcap * tanh(score / softcap).
     alibi_slopes fp32 [nh]: slopes[h] * (j - p) is added.  max_new, max_tokens: no sequence has more new tokens, or is longer
-    (host integers that lay out the work; None: whatever fits the tensors).  Tokens that see nothing get zeros.
+    (host integers that lay out the work; None: whatever fits the tensors).  Tokens that see nothing get zeros.  Cached values have
+    to be finite: one that is not may reach queries that do not see it (include/kvmix_b200.h).
     Returns [tokens, nh, 128] fp16; rows behind q_start[n] are left as they are."""
     dev, book = _book(pages)
     if q.dim() != 3 or q.dtype is not _f16 or q.get_device() != dev or q.shape[2] != 128:

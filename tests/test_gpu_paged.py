@@ -241,3 +241,150 @@ def test_mixed_step(cuda):
     c = Cache([900, 500, 129, 77, 300, 1], [6, 2, 1, 0, 2, 0], 2, 3, 2, 128, seed=9)
     q = queries(sum(counts), 8)
     check(c, q, counts, attend(c, q, counts, max_new=130))
+
+
+# ---- values and sizes at the edges ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("new,rep", [(1, 4), (1, 8), (60, 2)])
+@pytest.mark.parametrize("kb,vb,group", [(2, 2, 32), (4, 1, 64), (3, 3, 128), (1, 4, 128)])
+@pytest.mark.parametrize("k_size,v_size", [(1.0, 2e-4), (1e-3, 1.0), (1.0, 3e3), (600.0, 1.0), (1.0, 0.0)])
+def test_large_and_small_values(cuda, new, rep, kb, vb, group, k_size, v_size):
+    """Keys and values far from 1, constant ones (scales of zero) among them: scales and minima are multiplied, fp16 pages too.  Values below 1e-3
+    are subnormal fp16: half a step there is 2^-25, which the bound carries."""
+    c = Cache([500], [2], 1, kb, vb, group, seed=5, outliers=False)
+    for side, full, size in ((c.host["k"], c.host["kf"], k_size), (c.host["v"], c.host["vf"], v_size)):
+        for t in (*side[1:], full):
+            t.mul_(size)
+    c.layer = kv.PageLayer(*(t.cuda() for t in c.host["k"]), c.host["kf"].cuda(), *(t.cuda() for t in c.host["v"]), c.host["vf"].cuda(), kb, vb, group)
+    q = queries(new, rep) / (k_size if k_size > 1 else 1.0)
+    got, (want, slack) = attend(c, q, [new]), plain(c, q, [new])
+    err = np.abs(got.double().cpu().numpy() - want)
+    # of packed keys and values an element is code * scale + minimum rounded to fp16, or products rounded there: half a step of the smallest fp16
+    # numbers, 2^-25, a term, and weights are scaled by 2^7 at most
+    assert (err <= slack + 16 * 2.0 ** -24 * max(1.0, v_size)).all(), (err / slack).max()
+
+
+def test_scales_that_grow_along_the_sequence(cuda):
+    """p * scale is kept in fp16's range by a power of two that follows the largest scale: pages whose scales grow 2^24 fold, and fall again."""
+    c = Cache([128 * 13], [13], 1, 2, 2, 64, seed=8, outliers=False)
+    ids = c.host["table"][c.host["rows"][0]].tolist()
+    for j, i in enumerate(ids):
+        for t in c.host["v"][1:]:
+            t[i] *= 2.0 ** (-12 + 2 * min(j, 24 - 2 * j if j > 8 else j))
+    c.layer = c.layer._replace(vscale=c.host["v"][1].cuda(), vmn=c.host["v"][2].cuda())
+    for nh in (1, 2, 4, 8):
+        q = queries(1, nh)
+        check(c, q, [1], attend(c, q, [1]))
+
+
+@pytest.mark.parametrize("what", ["nan key", "inf value", "nan query"])
+@pytest.mark.parametrize("new", [1, 200])
+def test_not_finite(cuda, what, new):
+    """A key or query that is not finite is seen by every query that sees it, and by none that sees no token of its page.  A value that is not
+    may besides reach queries of the same tile: 64 tokens of 4 heads, so that of the chunk 500 .. 699 the tokens from 628 on share theirs with 670."""
+    c = Cache([700], [0], 1, 4, 4, 64, seed=2)
+    ids = c.host["table"][c.host["rows"][0]].tolist()
+    q = queries(new, 4)
+    if what == "nan key":
+        c.layer.kfull[ids[5], 0, 30, 7] = float("nan")              # position 670
+    elif what == "inf value":
+        c.layer.vfull[ids[5], 0, 30, 7] = float("inf")
+    else:
+        q[0, 1, 3] = float("nan")
+    out = attend(c, q, [new])
+    if what == "nan query":
+        assert out[0, 1].isnan().all() and out[:, [0, 2, 3]].isfinite().all() and out[1:].isfinite().all()
+        return
+    pos = torch.arange(700 - new, 700, device="cuda")
+    bad = ~out.isfinite()
+    assert bad[pos >= 670].any(-1).all()
+    assert not bad[pos < (628 if what == "inf value" else 640)].any()
+    far = attend(c, q, [new], first=[640 if p < 640 else 0 for p in pos.tolist()]) if new > 1 else out
+    assert not far[pos < 628].any()                                  # they see nothing
+
+
+def test_masked_keys_of_any_value_do_not_matter(cuda):
+    """Keys behind a mask may be anything: NaN, infinities, the lowest number."""
+    c = Cache([700], [3], 1, 2, 2, 64, seed=12)
+    q1, q = queries(1, 4), queries(100, 4)
+    want1, want = attend(c, q1, [1], window=200), attend(c, q, [100], window=200)
+    ids = c.host["table"][c.host["rows"][0]].tolist()
+    for j, bad in ((0, float("nan")), (1, float("inf")), (2, -65504.0)):
+        c.layer.kmn[ids[j]] = bad                                    # positions below 384 are seen by nobody (700 - 100 - 200 = 400)
+    c.layer.kfull[ids[3], :, :16] = float("nan")
+    got1, got = attend(c, q1, [1], window=200), attend(c, q, [100], window=200)
+    assert torch.equal(got1, want1) and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rep,new", [(1, 1), (4, 1), (3, 40)])
+def test_odd_layouts_of_queries_and_outputs(cuda, rep, new):
+    c = Cache([300], [2], 2, 4, 2, 64, seed=21)
+    nh = 2 * rep
+    want = attend(c, queries(new, nh), [new])
+    flat = torch.zeros(new * nh * 131 + 3, dtype=torch.half, device="cuda")
+    q = flat[3:].view(new, nh, 131)[..., 1:129]                      # rows that begin at any fp16
+    q.copy_(queries(new, nh))
+    out = torch.full((new, nh + 1, 137), 5.0, dtype=torch.half, device="cuda")
+    got = attend(c, q, [new], out=out[:, :nh, 3:131])
+    assert torch.equal(got, want)
+    assert (out[:, nh] == 5).all() and (out[:, :, :3] == 5).all() and (out[:, :, 131:] == 5).all()
+    wide = torch.zeros(new, nh, 256, dtype=torch.half, device="cuda")
+    wide[..., ::2] = queries(new, nh)                                # channels two apart
+    assert torch.equal(attend(c, wide[..., ::2], [new]), want)
+
+
+def test_no_work(cuda):
+    c = Cache([300, 5], [2, 0], 1, 4, 2, 64)
+    assert attend(c, queries(0, 4), [0, 0]).shape == (0, 4, 128)
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    out = torch.full((3, 4, 128), 9.0, dtype=torch.half, device="cuda")
+    kv.paged_attention(queries(3, 4), torch.zeros(1, dtype=torch.int32, device="cuda"), none, c.book, c.layer, out=out)
+    assert (out == 9).all()
+    out = attend(c, queries(2, 4), [0, 0], out=torch.full((2, 4, 128), 9.0, dtype=torch.half, device="cuda"))
+    assert (out == 9).all()
+
+
+@pytest.mark.parametrize("splits", [dict(max_tokens=640), dict(max_tokens=1), dict(), dict(max_new=1)])
+def test_hints_lay_out_the_work_only(cuda, splits):
+    """max_tokens below a sequence's length, or none given: other splits, the same sums."""
+    c = Cache([5000, 640], [30, 4], 1, 2, 4, 64, seed=31, max_pages=60)
+    q = queries(2, 4)
+    check(c, q, [1, 1], attend(c, q, [1, 1], **splits))
+    if "max_new" not in splits:
+        q = queries(50, 4)
+        check(c, q, [30, 20], attend(c, q, [30, 20], **splits))
+
+
+def test_many_sequences(cuda):
+    """More sequences than a CTA has threads, most of them one token long."""
+    g = torch.Generator().manual_seed(3)
+    lengths = [int(n) for n in torch.randint(1, 4, (2500,), generator=g)]
+    lengths[1700], lengths[2499] = 300, 129
+    c = Cache(lengths, [2 if n == 300 else 1 if n == 129 else 0 for n in lengths], 1, 4, 2, 64, seed=33)
+    q = queries(2500, 2)
+    check(c, q, [1] * 2500, attend(c, q, [1] * 2500, max_new=1))
+
+
+def test_pages_beyond_32_bits(cuda):
+    """Numbers of pages whose elements lie beyond 2^32: the first and the last of a pool of 8.6 GB."""
+    n16, heads = 16500, 16                                           # 16500 * 16 * 16384 elements a tensor
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    g = torch.Generator().manual_seed(4)
+    small = Cache([200], [0], heads, 2, 2, 128, seed=40)
+    ids = small.host["table"][small.host["rows"][0]].tolist()
+    kf, vf = (torch.empty(n16, heads, P, 128, dtype=torch.half, device="cuda") for _ in range(2))
+    to = [n16 - 1, 0]
+    for i, j in zip(ids, to):
+        kf[j], vf[j] = small.layer.kfull[i], small.layer.vfull[i]
+    layer = small.layer._replace(kfull=kf, vfull=vf)
+    book = kv.PageBook(small.book.table.clone(), small.book.length, small.book.packed, torch.ones(small.book.n_packed + n16, dtype=torch.int32, device="cuda"),
+                       torch.zeros(small.book.n_packed + n16, dtype=torch.int32, device="cuda"), small.book.count, small.book.n_packed)
+    book.table[small.host["rows"][0], :2] = torch.tensor(to, dtype=torch.int32, device="cuda")
+    for new in (1, 150):
+        q = torch.randn(new, 2 * heads, 128, generator=g).half().cuda()
+        got = kv.paged_attention(q, starts([new]), small.rows, book, layer)
+        assert torch.equal(got, kv.paged_attention(q, starts([new]), small.rows, small.book, small.layer))
+    x, y = (torch.randn(150, heads, 128, generator=g).half().cuda() for _ in range(2))
+    kv.page_write(x, y, starts([150]), small.rows, book, layer)      # positions 50 .. 199
+    assert torch.equal(kf[n16 - 1, :, 50:], x[:78].transpose(0, 1)) and torch.equal(vf[0, :, :72], y[78:].transpose(0, 1))

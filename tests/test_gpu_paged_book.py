@@ -447,3 +447,89 @@ def test_a_sequence_in_chunks_is_the_sequence_at_once(cuda):
     got, want = cache.attend(0, q[at:at + 1], s), exact(0, q[at:at + 1], at)
     assert ((got.double() - want).norm(dim=-1) <= 4e-3 * want.norm(dim=-1)).all()
     cache.check()
+
+
+def test_more_rows_than_a_cta_has_threads(cuda):
+    """Prefix sums that go on over several turns of 1024 rows, stacks and tables against the simulation; the pools are odd sizes."""
+    rng = random.Random(1)
+    n = 2600
+    cache = kv.KVmixPagedCache([(2, 2)], 1, 128, n, 512, 5001, 6003, 128, 0)
+    sim = Sim(n, 4, 5001, 6003)
+    rows = list(range(n))
+    rng.shuffle(rows)
+    counts = [rng.choice([0, 1, 128, 200, 256]) for _ in rows]
+    cache.extend(rows, counts)
+    sim.extend(rows, counts)
+    for l in cache.layers:
+        l.kfull.zero_()
+        l.vfull.zero_()
+    cache.settle(rows[:2000])
+    sim.settle(rows[:2000], 0)
+    sim.same(cache.book)
+    gone = rows[::2]
+    cache.free(gone)
+    sim.free_rows(gone)
+    sim.same(cache.book)
+    parents = [r for r in rows[1::2] if sim.seq[r][1]]
+    cache.fork(parents, gone[:len(parents)])
+    sim.fork(parents, gone[:len(parents)])
+    sim.same(cache.book)
+    cache.free(parents[:700])
+    sim.free_rows(parents[:700])
+    cache.compact()
+    sim.compact()
+    sim.same(cache.book)
+    cache.check()
+
+
+def test_calls_without_rows(cuda):
+    cache = small()
+    before = snapshot(cache)
+    none = ints()
+    kv.pages_extend(none, none, cache.book)
+    kv.pages_free(none, cache.book)
+    kv.pages_settle(none, 0, cache.book, cache.layers)
+    kv.pages_fork(none, none, cache.book, cache.layers)
+    x = torch.zeros(0, 1, 128, device="cuda").half()
+    kv.page_write(x, x, ints(0), none, cache.book, cache.layers[0])
+    unchanged(cache, before)
+    cache.check()
+    bare = kv.KVmixPagedCache([(2, 2)], 1, 128, 2, 300, 0, 3, 64, 1000)          # no packed page at all
+    s = bare.extend([0], [200])
+    x = torch.randn(200, 1, 128, device="cuda").half()
+    bare.write(0, x, x, s)
+    assert bare.attend(0, x, s).isfinite().all()
+    bare.settle()
+    bare.fork([0], [1])
+    bare.compact()
+    bare.check()
+
+
+def test_layers_beyond_one_launch_of_copies(cuda):
+    """More tensors than one launch copies: every layer's page follows."""
+    cache = kv.KVmixPagedCache([(2, 2)] * 140, 1, 128, 2, 256, 1, 3, 128, 256)
+    s = cache.extend([0], [5])
+    for l in range(140):
+        x = torch.full((5, 1, 128), float(l), device="cuda").half()
+        cache.write(l, x, -x, s)
+    cache.fork([0], [1])
+    page = int(cache.book.table[1, 0])
+    assert page != int(cache.book.table[0, 0])
+    for l in range(140):
+        assert (cache.layers[l].kfull[page, 0, :5] == l).all() and (cache.layers[l].vfull[page, 0, :5] == -l).all()
+    cache.check()
+
+
+def test_two_streams_read_one_cache(cuda):
+    """Attention changes nothing and shares nothing: calls over one cache may run at once."""
+    cache = small()
+    q = torch.randn(64, 1, 4, 128, device="cuda").half()
+    at, row = ints(0, 1), ints(0)
+    want = [kv.paged_attention(q[i], at, row, cache.book, cache.layers[0], max_tokens=1024) for i in range(64)]
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [None] * 64
+    torch.cuda.synchronize()
+    for i in range(64):
+        with torch.cuda.stream(streams[i % 2]):
+            got[i] = kv.paged_attention(q[i], at, row, cache.book, cache.layers[0], max_tokens=1024)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
