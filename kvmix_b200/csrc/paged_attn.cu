@@ -58,12 +58,20 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i = lane; i < p.splits; i += 32) m = fmaxf(m, p.part_ml[2 * (i * step + row)]);
     m = warp_max(m);
-    for (int i = 0; i < p.splits; ++i) {
-        const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + 2 * (i * step + row));
-        const float4 x = *reinterpret_cast<const float4 *>(p.part_out + (i * step + row) * 128 + 4 * lane);
-        const float f = part_factor(ml.x, ml.y, m);
-        l += f * ml.y;
-        if (f != 0.f) { v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w; }
+    for (int base = 0; base < p.splits; base += 8) {              // eight splits' loads under way at once: one by one each waits for L2
+        float2 ml[8];
+        float4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t at_i = (int64_t)min(base + k, p.splits - 1) * step + row;
+            ml[k] = *reinterpret_cast<const float2 *>(p.part_ml + 2 * at_i);
+            x[k] = *reinterpret_cast<const float4 *>(p.part_out + at_i * 128 + 4 * lane);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float f = base + k < p.splits ? part_factor(ml[k].x, ml[k].y, m) : 0.f;
+            if (f != 0.f) { l += f * ml[k].y; v.x += f * x[k].x; v.y += f * x[k].y; v.z += f * x[k].z; v.w += f * x[k].w; }
+        }
     }
     __half *out = static_cast<__half *>(p.a.out) + (int64_t)u * p.a.o_sT + (int64_t)h * p.a.o_sH + 4 * lane;
     auto put = [&](int c, float x) { out[c] = __float2half_rn(l == 0.f ? 0.f : x / l); };

@@ -141,16 +141,25 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// x * tanh(x) / x of two |x| <= 0.75: tanh(x) / x as a polynomial in x * x, minimax in relative error (2.9e-8, by a Remez exchange), times `by`.
-// No special function and both at once: 10 instructions where cap_score() takes 12 and four turns of the special function unit.
-__device__ __forceinline__ unsigned long long cap_small(unsigned long long x, unsigned long long by) {
-    constexpr float C[6] = {0.999999971f, -0.333329589f, 0.13325406f, -0.0533444301f, 0.0195829082f, -0.00471625725f};
-    const unsigned long long t = mul_f32x2(x, x);
-    unsigned long long r = f32x2(C[5], C[5]);
+// softcap * tanh(score / softcap) in log2 units of two raw scores, |score / softcap| <= 0.75: tanh(x) / x as a polynomial in x * x, minimax in relative
+// error (5.7e-7, by a Remez exchange: 2e-5 of an exponent of 30), with the factors of score and softcap in its coefficients.  Six instructions
+// for both where cap_score() takes twelve and four turns of the special function unit.
+struct CapSmall {
+    float c[5];
+    __device__ __forceinline__ CapSmall(float in, float by) {     // in: raw score -> x; by: tanh -> log2 units
+        constexpr float C[5] = {0.999999435f, -0.333282515f, 0.132589832f, -0.0500563026f, 0.0129296324f};
+        float f = in * by;
 #pragma unroll
-    for (int i = 4; i >= 0; --i) r = fma_f32x2(r, t, f32x2(C[i], C[i]));
-    return mul_f32x2(mul_f32x2(x, by), r);
-}
+        for (int i = 0; i < 5; ++i) { c[i] = C[i] * f; f *= in * in; }
+    }
+    __device__ __forceinline__ unsigned long long operator()(unsigned long long x) const {
+        const unsigned long long t = mul_f32x2(x, x);
+        unsigned long long r = f32x2(c[4], c[4]);
+#pragma unroll
+        for (int i = 3; i >= 0; --i) r = fma_f32x2(r, t, f32x2(c[i], c[i]));
+        return mul_f32x2(x, r);
+    }
+};
 
 // MODS: scores are capped, biased or scaled by a negative number.  Calls without have an instance of their own: with the code beside it the
 // 128 scores of a thread no longer fit its registers (2048 tokens over 32k: 1261 us in place of 1132).
@@ -291,10 +300,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                     float most = 0.f;
 #pragma unroll
                     for (int j = 0; j < N; j += 2) most = max_abs(most, __uint_as_float(at(j)), __uint_as_float(at(j + 1)));
-                    if (__all_sync(0xffffffffu, most * fabsf(small) <= 0.75f)) {
-                        const unsigned long long in = f32x2(small, small), by = f32x2(cap2, cap2);
+                    // (a factor of 1e4 and more would take the coefficients towards the end of fp32)
+                    if (__all_sync(0xffffffffu, most * fabsf(small) <= 0.75f && fabsf(small) < 1e4f)) {
+                        const CapSmall capped(small, cap2);
 #pragma unroll
-                        for (int j = 0; j < N; j += 2) put(j, cap_small(mul_f32x2(pair(j), in), by));
+                        for (int j = 0; j < N; j += 2) put(j, capped(pair(j)));
                     } else {
                         const float two = 2.f * scale2 / p.a.softcap;
 #pragma unroll
