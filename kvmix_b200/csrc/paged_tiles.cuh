@@ -141,6 +141,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+
 // softcap * tanh(score / softcap) in log2 units of two raw scores, |score / softcap| <= 0.75: tanh(x) / x as a polynomial in x * x, minimax in relative
 // error (5.7e-7, by a Remez exchange: 2e-5 of an exponent of 30), with the factors of score and softcap in its coefficients.  Six instructions
 // for both where cap_score() takes twelve and four turns of the special function unit.
@@ -152,8 +153,10 @@ struct CapSmall {
 #pragma unroll
         for (int i = 0; i < 5; ++i) { c[i] = C[i] * f; f *= in * in; }
     }
-    __device__ __forceinline__ unsigned long long operator()(unsigned long long x) const {
+    __device__ __forceinline__ unsigned long long operator()(unsigned long long x, float &most) const {         // most: the largest square
         const unsigned long long t = mul_f32x2(x, x);
+        const float2 squares = f32x2_split(t);
+        most = max3(most, squares.x, squares.y);
         unsigned long long r = f32x2(c[4], c[4]);
 #pragma unroll
         for (int i = 3; i >= 0; --i) r = fma_f32x2(r, t, f32x2(c[i], c[i]));
@@ -297,16 +300,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                 };
                 if (cap) {
                     const float small = p.a.softmax_scale / p.a.softcap;
+                    // the polynomial for all first; where a square says that one was too large, the scores are read again.  (A factor of 1e4 and more
+                    // would take the coefficients towards the end of fp32.)
+                    const CapSmall capped(small, cap2);
                     float most = 0.f;
 #pragma unroll
-                    for (int j = 0; j < N; j += 2) most = max_abs(most, __uint_as_float(at(j)), __uint_as_float(at(j + 1)));
-                    // (a factor of 1e4 and more would take the coefficients towards the end of fp32)
-                    if (__all_sync(0xffffffffu, most * fabsf(small) <= 0.75f && fabsf(small) < 1e4f)) {
-                        const CapSmall capped(small, cap2);
-#pragma unroll
-                        for (int j = 0; j < N; j += 2) put(j, capped(pair(j)));
-                    } else {
+                    for (int j = 0; j < N; j += 2) put(j, capped(pair(j), most));
+                    if (!__all_sync(0xffffffffu, most * (small * small) <= 0.75f * 0.75f && fabsf(small) < 1e4f)) {
                         const float two = 2.f * scale2 / p.a.softcap;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) tc_load32(x[c], t_s + half * N + 32 * c);
+                        tc_wait_ld();
 #pragma unroll
                         for (int j = 0; j < N; ++j) at(j) = __float_as_uint(cap_score(__uint_as_float(at(j)), two, cap2));
                     }
