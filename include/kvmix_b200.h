@@ -559,7 +559,8 @@ int kvq_page_write(const kvq_page_book *b, const kvq_page_layer *l, const kvq_pa
  * sequence less than 256 positions before -- and every one that sees a token of its page.
  * GQA: query head h reads kv head h / (nh / Hkv).
  *   q, out [tokens, nh, 128] fp16, strides *_sT, *_sH;  first [tokens], prefix [n] int32, slopes [nh] fp32
- *   max_new: no sequence has more new tokens;  max_tokens: no sequence is longer (both only lay out the work)
+ *   max_new: no sequence has more new tokens;  max_tokens: no sequence is longer;  max_chunks: no more sequences have several new tokens.
+ *   They lay out the work: queries beyond max_new and max_chunks may be left out, max_tokens is a matter of speed only.
  * workspace: kvq_paged_attn_workspace_bytes(...) bytes, not shared by concurrent calls.
  */
 typedef struct {
@@ -568,13 +569,14 @@ typedef struct {
     int64_t q_sT, q_sH, o_sT, o_sH;
     const int32_t *q_start, *rows, *first, *prefix;
     const float *slopes;
-    int32_t n, tokens, nh, max_new, max_tokens, window, causal;
+    int32_t n, tokens, nh, max_new, max_tokens, max_chunks, window, causal;
     float softmax_scale, softcap;
     void *workspace;
     uint64_t workspace_bytes;
 } kvq_paged_attn_args;
 
-uint64_t kvq_paged_attn_workspace_bytes(const kvq_page_layer *l, int32_t n, int32_t tokens, int32_t nh, int32_t max_new, int32_t max_tokens);
+uint64_t kvq_paged_attn_workspace_bytes(const kvq_page_layer *l, int32_t n, int32_t tokens, int32_t nh, int32_t max_new, int32_t max_tokens,
+                                        int32_t max_chunks);
 int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, const kvq_paged_attn_args *a, kvq_stream_t stream);
 
 #ifdef __cplusplus

@@ -110,7 +110,7 @@ class PageWriteArgs(C.Structure):
 class PagedAttnArgs(C.Structure):
     _fields_ = [("q", vp), ("out", vp), ("q_sT", i64), ("q_sH", i64), ("o_sT", i64), ("o_sH", i64),
                 ("q_start", vp), ("rows", vp), ("first", vp), ("prefix", vp), ("slopes", vp),
-                ("n", i32), ("tokens", i32), ("nh", i32), ("max_new", i32), ("max_tokens", i32), ("window", i32), ("causal", i32),
+                ("n", i32), ("tokens", i32), ("nh", i32), ("max_new", i32), ("max_tokens", i32), ("max_chunks", i32), ("window", i32), ("causal", i32),
                 ("softmax_scale", C.c_float), ("softcap", C.c_float), ("workspace", vp), ("workspace_bytes", u64)]
 
 
@@ -168,7 +168,7 @@ def lib():
                           (L.kvq_pages_fork, [blk, vp, vp, i32, vp, vp]), (L.kvq_pages_compact, [blk, vp, vp]),
                           (L.kvq_page_copy, [blk, i32, vp, i32, vp]), (L.kvq_page_write, [blk, blk, blk, vp]), (L.kvq_paged_attn, [blk, blk, blk, vp])):
             fn.restype, fn.argtypes = C.c_int, types
-        L.kvq_paged_attn_workspace_bytes.restype, L.kvq_paged_attn_workspace_bytes.argtypes = u64, [blk] + [i32] * 5
+        L.kvq_paged_attn_workspace_bytes.restype, L.kvq_paged_attn_workspace_bytes.argtypes = u64, [blk] + [i32] * 6
         _lib = L
     return _lib
 

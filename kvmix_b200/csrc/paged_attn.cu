@@ -95,7 +95,7 @@ struct PagedPlan {
     int few_splits, tile_splits, max_tiles;
 };
 
-static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, int max_new, int max_tokens) {
+static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, int max_new, int max_tokens, int max_chunks) {
     PagedPlan r = {};
     const int rep = nh / l.Hkv;
     const int64_t most = (int64_t)max_new * rep;
@@ -116,7 +116,7 @@ static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, 
         const double cost = waves * (rounds + 2) + (s > 1 ? 2 : 0);
         if (cost < best) { best = cost; r.few_splits = s; }
     }
-    int64_t tiles = ((int64_t)tokens * rep) / 256 + n;
+    int64_t tiles = ((int64_t)tokens * rep) / 256 + (r.few && max_chunks < n ? max_chunks : n);     // without the other kernel every sequence is one of chunks
     if (n == 1) tiles = ((int64_t)tokens * rep + 255) / 256;
     r.max_tiles = (int)(tiles < INT32_MAX ? tiles : INT32_MAX);
     // Kernel of tiles: one CTA to an SM, a page a round (some 1.8 us); a CTA's beginning and end count four pages, joining the splits moves
@@ -141,10 +141,11 @@ static uint64_t paged_bytes(const PagedPlan &r, int tokens, int nh) {
 
 }  // namespace kvq
 
-extern "C" uint64_t kvq_paged_attn_workspace_bytes(const kvq_page_layer *l, int32_t n, int32_t tokens, int32_t nh, int32_t max_new, int32_t max_tokens) {
+extern "C" uint64_t kvq_paged_attn_workspace_bytes(const kvq_page_layer *l, int32_t n, int32_t tokens, int32_t nh, int32_t max_new, int32_t max_tokens,
+                                                   int32_t max_chunks) {
     using namespace kvq;
-    if (check_layer(l) || n <= 0 || tokens <= 0 || nh <= 0 || nh % l->Hkv || max_new <= 0 || max_tokens <= 0) return 0;
-    return paged_bytes(paged_plan(*l, n, tokens, nh, max_new, max_tokens), tokens, nh);
+    if (check_layer(l) || n <= 0 || tokens <= 0 || nh <= 0 || nh % l->Hkv || max_new <= 0 || max_tokens <= 0 || max_chunks < 0) return 0;
+    return paged_bytes(paged_plan(*l, n, tokens, nh, max_new, max_tokens, max_chunks), tokens, nh);
 }
 
 extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, const kvq_paged_attn_args *a, kvq_stream_t stream) {
@@ -155,10 +156,10 @@ extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, c
     if (a->n < 0 || a->tokens < 0 || a->nh <= 0 || a->window < 0) return KVQ_ERR_SHAPE;
     if (a->nh % l->Hkv) return KVQ_ERR_HEADS;
     if (a->n == 0 || a->tokens == 0) return KVQ_OK;
-    if (a->max_new <= 0 || a->max_tokens <= 0) return KVQ_ERR_SHAPE;
+    if (a->max_new <= 0 || a->max_tokens <= 0 || a->max_chunks < 0) return KVQ_ERR_SHAPE;
     if (!a->q || !a->out || !a->q_start || !a->rows) return KVQ_ERR_NULL;
     if (!(a->softcap >= 0.f) || !(a->softmax_scale == a->softmax_scale)) return KVQ_ERR_SHAPE;
-    const PagedPlan r = paged_plan(*l, a->n, a->tokens, a->nh, a->max_new, a->max_tokens);
+    const PagedPlan r = paged_plan(*l, a->n, a->tokens, a->nh, a->max_new, a->max_tokens, a->max_chunks);
     const uint64_t need = paged_bytes(r, a->tokens, a->nh);
     if (need && (!a->workspace || a->workspace_bytes < need)) return KVQ_ERR_WORKSPACE;
     if (need && reinterpret_cast<uintptr_t>(a->workspace) % 16) return KVQ_ERR_ALIGN;

@@ -423,7 +423,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
     const int v_grp = v_col >> vr_log2, v_row = min(v_col & ((1 << vr_log2) - 1), R - 1), o_row = o_col & ((1 << vr_log2) - 1), o_grp = o_col >> vr_log2;
     const int o_row1 = VPAIR ? o_row : o_row + 1;
     const uint32_t v_lo = VPAIR && (g & 1) ? 0xffffffffu : 0u;
-    // p * scale * 2^expo: the power of two starts from the first scales (the largest of them becomes 4 to 8) and goes down where one would exceed 256
+    // p * scale * 2^expo: the power of two starts from the first scales (the largest of them becomes 4 to 8) and follows them where a stage's largest
+    // would exceed 256 or stay below 2^-5; the sums so far go along, exactly
     int expo = 32;
 #pragma unroll 1
     for (int k = 0; k < n_mine; ++k) {
@@ -535,9 +536,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
                 uint32_t m2 = 0;
                 for (int w = lane; w < stage_rows * p.v_groups / 2; w += 32) m2 = as_u32(__hmax2(as_h2(m2), as_h2(lds32(c_sc + 4 * w))));
                 const int top = (int)(__reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16)) >> 10 & 31);
-                if (top + expo > 15 + 7) {                        // rare: the first stage, and where scales grow 2^5 fold
+                if (top + expo > 15 + 7 || (top + expo < 10 && top > 0)) {        // rare: the first stage, and where scales grow or shrink some 2^6 fold
                     const int want = min(max(17 - top, -13), 15);
-                    if (want < expo) {
+                    if (want != expo) {
                         const float f = expo == 32 ? 0.f : exp2f((float)(want - expo));
 #pragma unroll
                         for (int m = 0; m < 8; ++m)

@@ -173,13 +173,43 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     // where this CTA's rows are: tiles of later tokens first, they see more
     const int split = blockIdx.x % p.splits, hs = blockIdx.x / p.splits, head = hs % p.l.Hkv;
     int tile = max_tiles - 1 - hs / p.l.Hkv, seq = 0;
-    for (; seq < p.a.n; ++seq) {
-        const int rows = max(0, min(p.a.q_start[seq + 1], p.a.tokens) - max(p.a.q_start[seq], 0)) * p.rep;
-        const int tiles = rows > p.few_rows ? (rows + 2 * kTileRows - 1) / (2 * kTileRows) : 0;
-        if (tile < tiles) break;
-        tile -= tiles;
+    auto tiles_of = [&](int i) {
+        const int rows = max(0, min(p.a.q_start[i + 1], p.a.tokens) - max(p.a.q_start[i], 0)) * p.rep;
+        return rows > p.few_rows ? (rows + 2 * kTileRows - 1) / (2 * kTileRows) : 0;
+    };
+    if (p.a.n <= 8) {
+        for (; seq < p.a.n; ++seq) {
+            const int tiles = tiles_of(seq);
+            if (tile < tiles) break;
+            tile -= tiles;
+        }
+        if (seq == p.a.n) return;
+    } else {                                                      // many sequences, one a thread
+        __shared__ int s_sum[kTileThreads / 32], s_seq, s_tile;
+        if (threadIdx.x == 0) s_seq = -1;
+        for (int at = 0; at < p.a.n; at += kTileThreads) {
+            const int i = at + threadIdx.x, mine = i < p.a.n ? tiles_of(i) : 0;
+            int upto = mine, all = 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                if ((threadIdx.x & 31) >= o) upto += y;
+            }
+            if ((threadIdx.x & 31) == 31) s_sum[threadIdx.x >> 5] = upto;
+            __syncthreads();
+            for (int w = 0; w < kTileThreads / 32; ++w) {
+                all += s_sum[w];
+                if (w < (int)(threadIdx.x >> 5)) upto += s_sum[w];
+            }
+            if (tile >= upto - mine && tile < upto) { s_seq = i; s_tile = tile - (upto - mine); }
+            __syncthreads();
+            if (tile < all) break;
+            tile -= all;
+        }
+        seq = s_seq;
+        if (seq < 0) return;
+        tile = s_tile;
     }
-    if (seq == p.a.n) return;
     const PagedSeq s = paged_seq(p, seq);
     const int row0 = tile * 2 * kTileRows, rows = min(s.n_new * p.rep - row0, 2 * kTileRows), two_tiles = rows > kTileRows;
     const int warp = uniform_warp(), lane = threadIdx.x & 31, wg = warp >> 2;

@@ -31,7 +31,7 @@ _STATUS = {1: "no free fp16 page", 2: "no free packed page", 4: "sequence longer
            "a child that is not empty or also a parent)", 16: "a kernel gave up waiting for its own copies"}
 
 _pack_book, _pack_layer = struct.Struct("@6P4i").pack, struct.Struct("@8P6i").pack
-_pack_write, _pack_attn = struct.Struct("@2P4q2P2i").pack, struct.Struct("@2P4q5P7i2fPQ").pack
+_pack_write, _pack_attn = struct.Struct("@2P4q2P2i").pack, struct.Struct("@2P4q5P8i2fPQ").pack
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
@@ -78,7 +78,7 @@ def page_groups(bits, group):
 
 @functools.lru_cache(maxsize=None)
 def _library():
-    for fmt, cls in (("@6P4i", _lib.PageBookArgs), ("@8P6i", _lib.PageLayerArgs), ("@2P4q2P2i", _lib.PageWriteArgs), ("@2P4q5P7i2fPQ", _lib.PagedAttnArgs)):
+    for fmt, cls in (("@6P4i", _lib.PageBookArgs), ("@8P6i", _lib.PageLayerArgs), ("@2P4q2P2i", _lib.PageWriteArgs), ("@2P4q5P8i2fPQ", _lib.PagedAttnArgs)):
         assert -(-struct.calcsize(fmt) // 8) * 8 == C.sizeof(cls)
     return _lib.lib()
 
@@ -254,7 +254,7 @@ def pages_compact(pages, layers):
 
 @_on_its_device(3)
 def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, prefix=None, first=None, softcap=None, alibi_slopes=None,
-                    softmax_scale=None, max_new=None, max_tokens=None, out=None):
+                    softmax_scale=None, max_new=None, max_tokens=None, max_chunks=None, out=None):
     """Attention of the last tokens of every sequence over its pages.
 
     q [tokens, nh, 128] fp16: tokens [q_start[i], q_start[i+1]) are the last ones of sequence rows[i], whose keys and values are in the
@@ -264,8 +264,9 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
 
     window: sliding window, None or 0 for none.  prefix int32 [n]: the first prefix[i] tokens see each other.  first int32 [tokens]: where the
     token's document begins, for documents packed behind one another.  softcap: scores become softcap * tanh(score / softcap).
-    alibi_slopes fp32 [nh]: slopes[h] * (j - p) is added.  max_new, max_tokens: no sequence has more new tokens, or is longer
-    (host integers that lay out the work; None: whatever fits the tensors).  Tokens that see nothing get zeros.  Cached values have
+    alibi_slopes fp32 [nh]: slopes[h] * (j - p) is added.  max_new, max_tokens, max_chunks: no sequence has more new tokens, none is longer, no
+    more of them have several new tokens (host integers that lay out the work; None: whatever fits the tensors; with many sequences of
+    which few have several tokens the third saves time).  Tokens that see nothing get zeros.  Cached values have
     to be finite: one that is not may reach queries that do not see it (include/kvmix_b200.h).
     Returns [tokens, nh, 128] fp16; rows behind q_start[n] are left as they are."""
     dev, book = _book(pages)
@@ -294,14 +295,15 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     max_new = tokens if max_new is None else min(int(max_new), tokens)
     most = pages.table.shape[1] * PAGE_TOKENS
     max_tokens = most if max_tokens is None else min(int(max_tokens), most)
-    if tokens and n and (max_new <= 0 or max_tokens <= 0):
-        raise RuntimeError("max_new and max_tokens must be positive")
+    max_chunks = n if max_chunks is None else min(int(max_chunks), n)
+    if tokens and n and (max_new <= 0 or max_tokens <= 0 or max_chunks < 0):
+        raise RuntimeError("max_new and max_tokens must be positive, max_chunks not negative")
     L = _library()
-    need = L.kvq_paged_attn_workspace_bytes(block, n, tokens, nh, max_new, max_tokens)
+    need = L.kvq_paged_attn_workspace_bytes(block, n, tokens, nh, max_new, max_tokens, max_chunks)
     ws = pages.count.new_empty((need + 3) // 4) if need else None
     a = _pack_attn(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), _ints(dev, "q_start", q_start, n + 1),
                    _rows(dev, "rows", rows), 0 if first is None else _ints(dev, "first", first, tokens), 0 if prefix is None else _ints(dev, "prefix", prefix, n),
-                   at_slopes, n, tokens, nh, max_new, max_tokens, int(window), int(bool(causal)),
+                   at_slopes, n, tokens, nh, max_new, max_tokens, max_chunks, int(window), int(bool(causal)),
                    1.0 / math.sqrt(128) if softmax_scale is None else softmax_scale, float(softcap), 0 if ws is None else ws.data_ptr(), need)
     _launched(L.kvq_paged_attn(book, block, a, ops.raw_stream()))
     return out
@@ -314,6 +316,7 @@ class PagedStep(NamedTuple):
     tokens: int
     max_new: int
     max_tokens: int
+    max_chunks: int
 
 
 class KVmixPagedCache:
@@ -390,7 +393,8 @@ class KVmixPagedCache:
         pages_extend(at, both[:n], self.book)
         for r, c in zip(rows, counts):
             self.lengths[r] += c
-        return PagedStep(at, both[n:], starts[-1], max(counts, default=0), max((self.lengths[r] for r in rows), default=0))
+        return PagedStep(at, both[n:], starts[-1], max(counts, default=0), max((self.lengths[r] for r in rows), default=0),
+                         sum(c > 1 for c in counts))
 
     def write(self, layer, k, v, step):
         page_write(k, v, step.q_start, step.rows, self.book, self.layers[layer])
@@ -399,7 +403,8 @@ class KVmixPagedCache:
         """Options as ``paged_attention``: causal, window, prefix, first, softcap, alibi_slopes, softmax_scale, out."""
         if q.shape[0] != step.tokens:
             raise RuntimeError("one query for every new token of the step")
-        return paged_attention(q, step.q_start, step.rows, self.book, self.layers[layer], max_new=max(step.max_new, 1), max_tokens=max(step.max_tokens, 1), **options)
+        return paged_attention(q, step.q_start, step.rows, self.book, self.layers[layer], max_new=max(step.max_new, 1), max_tokens=max(step.max_tokens, 1),
+                               max_chunks=step.max_chunks, **options)
 
     def settle(self, rows=None):
         rows = range(len(self.lengths)) if rows is None else rows

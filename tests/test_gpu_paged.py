@@ -388,3 +388,33 @@ def test_pages_beyond_32_bits(cuda):
     x, y = (torch.randn(150, heads, 128, generator=g).half().cuda() for _ in range(2))
     kv.page_write(x, y, starts([150]), small.rows, book, layer)      # positions 50 .. 199
     assert torch.equal(kf[n16 - 1, :, 50:], x[:78].transpose(0, 1)) and torch.equal(vf[0, :, :72], y[78:].transpose(0, 1))
+
+
+@pytest.mark.parametrize("n,chunks", [(9, [8]), (900, [0, 767, 768, 899]), (1600, [1599])])
+def test_few_chunks_among_many_sequences(cuda, n, chunks):
+    """The tile kernel finds its sequences among single tokens, with and without being told how many there are."""
+    lengths, counts = [3] * n, [1] * n
+    for i in chunks:
+        lengths[i], counts[i] = 270, 90
+    c = Cache(lengths, [1 if m == 270 else 0 for m in lengths], 1, 4, 2, 64, seed=n)
+    q = queries(sum(counts), 4)
+    got = attend(c, q, counts, max_new=90, max_chunks=len(chunks))
+    check(c, q, counts, got)
+    assert torch.equal(attend(c, q, counts, max_new=90), got)
+
+
+def test_weights_on_values_of_a_small_scale(cuda):
+    """Pages of large values whose weights are next to nothing before pages of small ones that have them: the small ones keep their precision."""
+    c = Cache([128 * 6], [6], 1, 4, 2, 64, seed=14, outliers=False)
+    ids = c.host["table"][c.host["rows"][0]].tolist()
+    for j, i in enumerate(ids):
+        for t in c.host["v"][1:]:
+            t[i] *= 2.0 ** (6 if j < 4 else -8)
+    c.layer = c.layer._replace(vscale=c.host["v"][1].cuda(), vmn=c.host["v"][2].cuda())
+    slopes = [0.25] * 4                                              # positions 256 and more away: 2^-92
+    q = queries(1, 4)
+    got, (want, _) = attend(c, q, [1], slopes=slopes), plain(c, q, [1], slopes=slopes)
+    err = np.abs(got.double().cpu().numpy() - want)
+    # keys are exact to 2^-20; a weight, its product with a scale and the output are rounded once each (the minima's products share the weight's):
+    # 3 * 2^-11 of codes and minima, which are up to 4 times the values here
+    assert err.max() <= 3 * 2.0 ** -11 * 4 * 2.0 ** -8 * 2, err.max()

@@ -533,3 +533,21 @@ def test_two_streams_read_one_cache(cuda):
             got[i] = kv.paged_attention(q[i], at, row, cache.book, cache.layers[0], max_tokens=1024)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_steps_of_a_cache_lay_out_their_work(cuda):
+    """A step's counts tell how many sequences have several tokens: more query heads a kv head than the kernel of few rows takes, chunks beside
+    single tokens, and a chunk alone give what the calls without such hints give."""
+    gen = torch.Generator().manual_seed(7)
+    cache = kv.KVmixPagedCache([(4, 2)], 1, 128, 6, 600, 12, 24, 64, 128)
+    for counts in ([200, 1, 300], [1, 1, 40], [1, 1, 1], [3, 0, 1], [50, 50, 50]):
+        s = cache.extend([4, 0, 2], counts)
+        k, v = (torch.randn(s.tokens, 1, 128, generator=gen).half().cuda() for _ in range(2))
+        cache.write(0, k, v, s)
+        for heads in (1, 4, 12):
+            q = torch.randn(s.tokens, heads, 128, generator=gen).half().cuda()
+            got, want = cache.attend(0, q, s), kv.paged_attention(q, s.q_start, s.rows, cache.book, cache.layers[0])
+            # other splits sum in another order and may round a weight (2^-11) the other way
+            assert ((got.float() - want.float()).norm(dim=-1) <= 2e-3 * want.float().norm(dim=-1)).all()
+        cache.settle([4, 0, 2])
+    cache.check()

@@ -42,7 +42,7 @@ def layer(**over):
 def attn(**over):
     a = _lib.PagedAttnArgs()
     a.q = a.out = a.q_start = a.rows = 64
-    a.n, a.tokens, a.nh, a.max_new, a.max_tokens, a.softmax_scale = 1, 1, 4, 1, 100, 0.1
+    a.n, a.tokens, a.nh, a.max_new, a.max_tokens, a.max_chunks, a.softmax_scale = 1, 1, 4, 1, 100, 1, 0.1
     for k, v in over.items():
         setattr(a, k, v)
     return bytes(a)
@@ -67,7 +67,7 @@ def test_refusals_need_no_gpu():
         assert L.kvq_page_pack(bad, 64, 1, None) == rc
         assert L.kvq_page_write(book(), bad, bytes(_lib.PageWriteArgs()), None) == rc
         assert L.kvq_paged_attn(book(), bad, attn(), None) == rc
-    for bad, rc in ((attn(nh=3), -6), (attn(q=None), -10), (attn(n=-1), -7), (attn(max_new=0), -7), (attn(window=-1), -7), (attn(softcap=-1.0), -7),
+    for bad, rc in ((attn(nh=3), -6), (attn(q=None), -10), (attn(n=-1), -7), (attn(max_new=0), -7), (attn(max_chunks=-1), -7), (attn(window=-1), -7), (attn(softcap=-1.0), -7),
                     (attn(softcap=float("nan")), -7), (attn(softmax_scale=float("nan")), -7), (attn(tokens=0), 0), (attn(max_tokens=100000), -12)):
         assert L.kvq_paged_attn(book(), layer(), bad, None) == rc
     one = _lib.PageTensor(64, 24)
@@ -81,11 +81,11 @@ def test_workspace_holds_every_split():
         for tokens in (1, 7, 300, 4096):
             for nh, Hkv in ((1, 1), (32, 8), (64, 8), (40, 8)):
                 for length in (1, 128, 5000, 131072):
-                    b = L.kvq_paged_attn_workspace_bytes(layer(Hkv=Hkv), n, tokens, nh, tokens, length)
+                    b = L.kvq_paged_attn_workspace_bytes(layer(Hkv=Hkv), n, tokens, nh, tokens, length, n)
                     assert b % (tokens * nh * 520) == 0
                     splits = b // (tokens * nh * 520)
                     assert splits != 1 and splits <= -(-length // 128)
-    assert L.kvq_paged_attn_workspace_bytes(layer(), 1, 1, 3, 1, 100) == 0
+    assert L.kvq_paged_attn_workspace_bytes(layer(), 1, 1, 3, 1, 100, 1) == 0
 
 
 def test_no_cpu_path():
