@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         if (seq < 0) return;
         tile = s_tile;
     }
-    const PagedSeq s = paged_seq(p, seq);
-    const int row0 = tile * 2 * kTileRows, rows = min(s.n_new * p.rep - row0, 2 * kTileRows), two_tiles = rows > kTileRows;
+    const int q0 = max(p.a.q_start[seq], 0), n_new = min(p.a.q_start[seq + 1], p.a.tokens) - q0;       // as paged_seq has them, which waits for more loads
+    const int row0 = tile * 2 * kTileRows, rows = min(n_new * p.rep - row0, 2 * kTileRows), two_tiles = rows > kTileRows;
     const int warp = uniform_warp(), lane = threadIdx.x & 31, wg = warp >> 2;
 
     const uint32_t base = smem_u32(smem), bars = base + kOffBar;
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
 #pragma unroll
         for (int i = 0; i < 6; ++i) {
             const int row = (threadIdx.x >> 4) + 48 * i, idx = row0 + row, u = idx / p.rep, h = head * p.rep + (idx - u * p.rep);
-            const __half *q = static_cast<const __half *>(p.a.q) + (int64_t)(s.q0 + u) * p.a.q_sT + (int64_t)h * p.a.q_sH + 8 * (threadIdx.x & 15);
+            const __half *q = static_cast<const __half *>(p.a.q) + (int64_t)(q0 + u) * p.a.q_sT + (int64_t)h * p.a.q_sH + 8 * (threadIdx.x & 15);
             qv[i] = make_uint4(0, 0, 0, 0);
             if (row >= rows) continue;
             if (vec) qv[i] = *reinterpret_cast<const uint4 *>(q);
@@ -235,6 +235,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             }
         }
     }
+    const PagedSeq s = paged_seq(p, seq);
     auto bar = [&](int k) { return bars + 8 * k; };
     if (threadIdx.x == 0) {
         for (int k = 0; k < 2; ++k) {
