@@ -79,9 +79,25 @@ __device__ __forceinline__ float rcp_approx(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// softcap * tanh(s / softcap) as softcap * (1 - 2 / (exp(2 s / softcap) + 1)): absolute error 3e-7 * softcap (tanh.approx: 5e-4 * softcap).
-// `two`: 2 log2(e) / softcap * scale.
-__device__ __forceinline__ float cap_score(float raw, float two, float cap) { return cap - 2.f * cap * rcp_approx(exp2_approx(raw * two) + 1.f); }
+// cap * tanh(x), x = score / softcap.  Where |x| <= 0.75: tanh(x) / x as a polynomial in x * x, minimax in relative error (5.7e-7, by a Remez
+// exchange), so that a score keeps its own precision under any cap; beyond: 1 - 2 / (exp(2 x) + 1), whose error of some 2^-23 is
+// small against a tanh of 0.63 and more (of a score of 1 under a cap of 1e5 it would be 0.01).  A NaN stays one.
+constexpr float kCapSmall = 0.75f;
+__device__ __forceinline__ constexpr float cap_poly(int i) {
+    constexpr float C[5] = {0.999999435f, -0.333282515f, 0.132589832f, -0.0500563026f, 0.0129296324f};
+    return C[i];
+}
+__device__ __forceinline__ float cap_small(float x, float cap) {
+    const float t = x * x;
+    float r = cap_poly(4);
+#pragma unroll
+    for (int i = 3; i >= 0; --i) r = fmaf(r, t, cap_poly(i));
+    return x * r * cap;
+}
+__device__ __forceinline__ float cap_score(float x, float cap) {
+    const float large = cap - 2.f * cap * rcp_approx(exp2_approx(x * (2.f * kLog2e)) + 1.f);
+    return fabsf(x) <= kCapSmall ? cap_small(x, cap) : large;
+}
 
 // ---------------------------------------------------------------------------------------------
 // mbarriers.  A wait gives up after two seconds, sets a bit of the status and lets the kernel end.

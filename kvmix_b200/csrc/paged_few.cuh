@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
     float *s_out = reinterpret_cast<float *>(smem + sh.warps + warp * sh.warp_bytes + sh.aside);                // [R][128]
     __half *s_q = reinterpret_cast<__half *>(smem), *s_qs = s_q + R * 128;
     // q by a power of two below 1, so that no product with a scale leaves fp16
-    float2 *s_factor = reinterpret_cast<float2 *>(smem + sh.factor);              // raw scores to log2 units; to cap_score's argument
+    float2 *s_factor = reinterpret_cast<float2 *>(smem + sh.factor);              // raw scores to log2 units; to caps
     for (int r = warp; r < R; r += kFewWarps) {
         const int row = row0 + r;
         float x[4] = {0.f, 0.f, 0.f, 0.f}, top = 0.f;
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
         const float down = __int_as_float((127 - e) << 23), up = __int_as_float((127 + e) << 23), scale2 = p.a.softmax_scale * kLog2e;
 #pragma unroll
         for (int c = 0; c < 4; ++c) s_q[r * 128 + lane + 32 * c] = s_qs[r * 128 + few_slot(lane + 32 * c)] = __float2half_rn(x[c] * down);
-        if (lane == 0) s_factor[r] = make_float2(scale2 * up, p.a.softcap > 0.f ? 2.f * scale2 / p.a.softcap * up : 0.f);
+        if (lane == 0) s_factor[r] = make_float2(scale2 * up, p.a.softcap > 0.f ? p.a.softmax_scale / p.a.softcap * up : 0.f);
     }
     int4 *s_bounds = reinterpret_cast<int4 *>(smem + sh.bounds);  // lowest position, end, position, slope of a row
     if (threadIdx.x < R) {
@@ -294,9 +294,23 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
             float x[4] = {raw.x, raw.y, raw.z, raw.w}, top = -INFINITY;
             const bool whole = b.x <= page_base && b.y >= page_base + kPage && count == kPage;
             const int end = min(b.y, page_base + count);
+            if (p.a.softcap > 0.f) {                              // the polynomial alone wherever it will do
+                bool small = true;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) { x[c] *= by_row.y; small = small && fabsf(x[c]) <= kCapSmall; }
+                if (__all_sync(0xffffffffu, small)) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) x[c] = cap_small(x[c], cap2);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) x[c] = cap_score(x[c], cap2);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[c] *= by_row.x;
+            }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                x[c] = p.a.softcap > 0.f ? cap_score(x[c], by_row.y, cap2) : x[c] * by_row.x;
                 x[c] = fmaf(slope, (float)(j0 + 4 * c - b.z), x[c]);
                 if (!whole && (j0 + 4 * c < b.x || j0 + 4 * c >= end)) x[c] = -INFINITY;
             }

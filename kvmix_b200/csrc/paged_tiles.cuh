@@ -142,16 +142,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// softcap * tanh(score / softcap) in log2 units of two raw scores, |score / softcap| <= 0.75: tanh(x) / x as a polynomial in x * x, minimax in relative
-// error (5.7e-7, by a Remez exchange: 2e-5 of an exponent of 30), with the factors of score and softcap in its coefficients.  Six instructions
-// for both where cap_score() takes twelve and four turns of the special function unit.
+// cap_small() of two raw scores in log2 units, with the factors of score and softcap in its coefficients.  Six instructions
+// for both where cap_score() takes some thirty and four turns of the special function unit.
 struct CapSmall {
     float c[5];
     __device__ __forceinline__ CapSmall(float in, float by) {     // in: raw score -> x; by: tanh -> log2 units
-        constexpr float C[5] = {0.999999435f, -0.333282515f, 0.132589832f, -0.0500563026f, 0.0129296324f};
         float f = in * by;
 #pragma unroll
-        for (int i = 0; i < 5; ++i) { c[i] = C[i] * f; f *= in * in; }
+        for (int i = 0; i < 5; ++i) { c[i] = cap_poly(i) * f; f *= in * in; }
     }
     __device__ __forceinline__ unsigned long long operator()(unsigned long long x, float &most) const {         // most: the largest square
         const unsigned long long t = mul_f32x2(x, x);
@@ -337,13 +335,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                     float most = 0.f;
 #pragma unroll
                     for (int j = 0; j < N; j += 2) put(j, capped(pair(j), most));
-                    if (!__all_sync(0xffffffffu, most * (small * small) <= 0.75f * 0.75f && fabsf(small) < 1e4f)) {
-                        const float two = 2.f * scale2 / p.a.softcap;
+                    if (!__all_sync(0xffffffffu, most * (small * small) <= kCapSmall * kCapSmall && fabsf(small) < 1e4f)) {
 #pragma unroll
                         for (int c = 0; c < 2; ++c) tc_load32(x[c], t_s + half * N + 32 * c);
                         tc_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < N; ++j) at(j) = __float_as_uint(cap_score(__uint_as_float(at(j)), two, cap2));
+                        for (int j = 0; j < N; ++j) at(j) = __float_as_uint(cap_score(__uint_as_float(at(j)) * small, cap2));
                     }
                 }
                 if (bias) {

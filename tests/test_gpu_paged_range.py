@@ -1,0 +1,85 @@
+"""The paged cache over the whole range of its arguments: caps, scales and sizes of keys far from the usual, windows, shared pages, tensors that
+a call has to refuse before it changes anything."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_paged import Cache, attend, queries
+
+pytestmark = pytest.mark.gpu
+
+
+def parts(c, i):
+    """K, V [Hkv, length, 128] of sequence i and what their elements are sums of, |code * scale| + |minimum|, in 64 bits on the device."""
+    K, V = (torch.from_numpy(x).cuda() for x in c.dense(i))
+    kept = c.host
+    signed = kept["k"], kept["v"]
+    c.host = dict(kept, k=(kept["k"][0], kept["k"][1].abs(), kept["k"][2].abs()), v=(kept["v"][0], kept["v"][1].abs(), kept["v"][2].abs()))
+    Ka, Va = (torch.from_numpy(x).cuda().abs() for x in c.dense(i))
+    c.host = dict(kept, k=signed[0], v=signed[1])
+    return K, V, Ka, Va
+
+
+def attention(c, q, counts, exact_keys, scale=None, softcap=0.0, window=0):
+    """Attention from its definition in 64 bits, and a bound of the kernels' roundings that does not grow with the cap:
+    a score    2^-20 of the sum of its terms' sizes (pairs of fp16 or fp16 itself, sums in fp32; 2^-11 more where a key is rounded to fp16) and
+               4e-6 of itself (conversion to log2 units and the cap, some roundings of 2^-24 and a polynomial of 6e-7)
+    an output  three roundings to fp16 of 2^-11: of a weight, of a value or of weight * scale, of the output."""
+    scale = 1 / math.sqrt(128) if scale is None else scale
+    eps, rep, at = 2.0 ** -11, q.shape[1] // c.Hkv, 0
+    out, slack = (torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(2))
+    for i, new in enumerate(counts):
+        n = c.lengths[i]
+        K, V, Ka, Va = parts(c, i)
+        pos, j = torch.arange(n - new, n, device="cuda")[:, None], torch.arange(n, device="cuda")
+        seen = (j <= pos) & (j > pos - window) if window else j <= pos
+        for h in range(q.shape[1]):
+            x, g = q[at:at + new, h].double(), h // rep
+            s = x @ K[g].T * scale
+            if softcap:
+                s = softcap * torch.tanh(s / softcap)
+            p = s.masked_fill(~seen, -math.inf).softmax(-1)
+            rel = x.abs() @ Ka[g].T * abs(scale) * (2.0 ** -20 + (0 if exact_keys else eps)) + s.abs() * 4e-6
+            out[at:at + new, h] = o = p @ V[g]
+            slack[at:at + new, h] = 1.05 * ((p * (rel + 2 * eps)) @ Va[g] + (p * rel).sum(-1, keepdim=True) * o.abs()) + eps * o.abs() + 2.0 ** -24
+        at += new
+    return out, slack
+
+
+def holds(got, want, slack):
+    err = (got.double() - want).abs()
+    assert err.isfinite().all()
+    worst = (err / slack).max().item()
+    assert worst <= 1.0, f"{worst:.2f} times the bound; largest error {err.max().item():.3e}"
+
+
+def rows_hold(got, want, most):
+    err = (got.double() - want).norm(dim=-1) / want.norm(dim=-1).clamp(min=1e-3)
+    assert err.isfinite().all() and err.max() <= most, f"row error {err.max().item():.3e}"
+
+
+# ---- caps ------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("softcap", [1.0, 30.0, 1e4, 1e5, 1e6, 1e9])
+@pytest.mark.parametrize("kb,vb", [(2, 4), (4, 2), (3, 3)])
+def test_caps_of_one_token(cuda, softcap, kb, vb):
+    """A score keeps its own precision, however large the cap is."""
+    c = Cache([700, 301, 1], [4, 2, 0], 2, kb, vb, 32, seed=3)
+    q = queries(3, 4)
+    got, (want, slack) = attend(c, q, [1] * 3, softcap=softcap), attention(c, q, [1] * 3, kb != 3, softcap=softcap)
+    holds(got, want, slack)
+    rows_hold(got, want, 2e-3)                                  # the framework's own tolerance
+
+
+@pytest.mark.parametrize("softcap", [1.0, 1e5, 1e6])
+@pytest.mark.parametrize("new", [1, 100])
+def test_small_scores_beside_large_ones(cuda, softcap, new):
+    """Rows whose scores come near the cap beside rows whose do not (other heads, other tokens): each is as exact as it is alone."""
+    c = Cache([700], [0], 1, 4, 4, 64, seed=6)
+    q = queries(new, 4)
+    scale = softcap / 2e5 if softcap > 1 else 0.2
+    q = (q.float() / (11.3 * scale)).half()                               # scores of 1
+    q[:, 1] *= 1e4 * scale * 11.3 if softcap > 1 else 2                   # scores of some 0.5 to 2 caps
+    got = attend(c, q, [new], softcap=softcap, scale=scale)
+    holds(got, *attention(c, q, [new], True, softcap=softcap, scale=scale))
