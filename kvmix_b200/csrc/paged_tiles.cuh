@@ -142,17 +142,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// cap_small() of two raw scores in log2 units, with the factors of score and softcap in its coefficients.  Six instructions
-// for both where cap_score() takes some thirty and four turns of the special function unit.
+// cap_small() of two raw scores in log2 units.  in: raw score -> x; by: tanh -> log2 units, in the coefficients.  (With `in` there too the higher ones,
+// in^9 and in^7, left fp32 where scale / softcap is small.)  Seven instructions for both where cap_score() takes some thirty and four turns
+// of the special function unit.
 struct CapSmall {
     float c[5];
-    __device__ __forceinline__ CapSmall(float in, float by) {     // in: raw score -> x; by: tanh -> log2 units
-        float f = in * by;
+    unsigned long long in2;
+    __device__ __forceinline__ CapSmall(float in, float by) : in2(f32x2(in, in)) {
 #pragma unroll
-        for (int i = 0; i < 5; ++i) { c[i] = cap_poly(i) * f; f *= in * in; }
+        for (int i = 0; i < 5; ++i) c[i] = cap_poly(i) * by;
     }
-    __device__ __forceinline__ unsigned long long operator()(unsigned long long x, float &most) const {         // most: the largest square
-        const unsigned long long t = mul_f32x2(x, x);
+    __device__ __forceinline__ unsigned long long operator()(unsigned long long raw, float &most) const {       // most: the largest square
+        const unsigned long long x = mul_f32x2(raw, in2), t = mul_f32x2(x, x);
         const float2 squares = f32x2_split(t);
         most = max3(most, squares.x, squares.y);
         unsigned long long r = f32x2(c[4], c[4]);
@@ -329,13 +330,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                 };
                 if (cap) {
                     const float small = p.a.softmax_scale / p.a.softcap;
-                    // the polynomial for all first; where a square says that one was too large, the scores are read again.  (A factor of 1e4 and more
-                    // would take the coefficients towards the end of fp32.)
+                    // the polynomial for all first; where a square says that one was too large, the scores are read again
                     const CapSmall capped(small, cap2);
                     float most = 0.f;
 #pragma unroll
                     for (int j = 0; j < N; j += 2) put(j, capped(pair(j), most));
-                    if (!__all_sync(0xffffffffu, most * (small * small) <= kCapSmall * kCapSmall && fabsf(small) < 1e4f)) {
+                    if (!__all_sync(0xffffffffu, most <= kCapSmall * kCapSmall)) {
 #pragma unroll
                         for (int c = 0; c < 2; ++c) tc_load32(x[c], t_s + half * N + 32 * c);
                         tc_wait_ld();

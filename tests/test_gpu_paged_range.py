@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from test_gpu_paged import Cache, attend, queries
+from test_gpu_paged_book import small
 
 pytestmark = pytest.mark.gpu
 
@@ -59,6 +60,14 @@ def rows_hold(got, want, most):
     assert err.isfinite().all() and err.max() <= most, f"row error {err.max().item():.3e}"
 
 
+def sized(c, k_size):
+    """The same cache with keys of another size."""
+    for t in (*c.host["k"][1:], c.host["kf"]):
+        t.mul_(k_size)
+    c.layer = c.layer._replace(kscale=c.host["k"][1].cuda(), kmn=c.host["k"][2].cuda(), kfull=c.host["kf"].cuda())
+    return c
+
+
 # ---- caps ------------------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("softcap", [1.0, 30.0, 1e4, 1e5, 1e6, 1e9])
@@ -83,3 +92,13 @@ def test_small_scores_beside_large_ones(cuda, softcap, new):
     q[:, 1] *= 1e4 * scale * 11.3 if softcap > 1 else 2                   # scores of some 0.5 to 2 caps
     got = attend(c, q, [new], softcap=softcap, scale=scale)
     holds(got, *attention(c, q, [new], True, softcap=softcap, scale=scale))
+
+
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("scale", [1e-3, 1e-4, 1e-5, 1e-6])
+def test_large_raw_scores_below_the_cap(cuda, new, scale):
+    """Queries and keys so large that their products are 1e4 to 5e7, a small softmax_scale, scores up to the cap's size."""
+    c = sized(Cache([700], [0], 1, 4, 4, 64, seed=7, outliers=False), 60.0)
+    q = (queries(new, 4) * (14 / (scale * 60 * 11.3))).half() if scale > 2e-6 else (queries(new, 4) * 1.2e4).half()
+    assert q.isfinite().all()
+    holds(attend(c, q, [new], softcap=50.0, scale=scale), *attention(c, q, [new], True, softcap=50.0, scale=scale))
