@@ -552,7 +552,7 @@ int kvq_page_write(const kvq_page_book *b, const kvq_page_layer *l, const kvq_pa
  *   max(first[u], p + 1 - window) <= j < max(p + 1, prefix[i]), at most length
  * (first NULL: 0; window 0: no bound; prefix NULL: 0; causal = 0: all from the lower bound on), which covers causal and sliding-window
  * attention, documents packed behind one another (first = the document's start) and prefixes whose tokens all see each other.
- *   s = q.k * softmax_scale;  softcap > 0: s = softcap * tanh(s / softcap);  slopes: s += slopes[h] * (j - p);  out = softmax(s).v
+ *   s = q.k * softmax_scale;  softcap > 0, < 1e30: s = softcap * tanh(s / softcap);  slopes: s += slopes[h] * (j - p);  out = softmax(s).v
  * A row that sees nothing gives zeros.  Positions beyond `length`, pages without a number and rows of q behind q_start[n] are neither
  * read nor written.  Keys that are not finite reach the queries that see them.  Values have to be finite: one that is not reaches the
  * queries that see it, and may reach (a weight of zero times infinity) every query that is worked on with one of those -- new tokens of the same

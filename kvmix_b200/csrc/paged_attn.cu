@@ -1,6 +1,9 @@
 // kvq_paged_attn: checks, the plan of a call, its launches.
 #include "paged_attn.cuh"
 
+#include <cfloat>
+#include <cmath>
+
 namespace kvq {
 
 int paged_few_1(const PagedArgs &p, cudaStream_t st);                            // paged_few_1.cu ..
@@ -158,7 +161,7 @@ extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, c
     if (a->n == 0 || a->tokens == 0) return KVQ_OK;
     if (a->max_new <= 0 || a->max_tokens <= 0 || a->max_chunks < 0) return KVQ_ERR_SHAPE;
     if (!a->q || !a->out || !a->q_start || !a->rows) return KVQ_ERR_NULL;
-    if (!(a->softcap >= 0.f) || !(a->softmax_scale == a->softmax_scale)) return KVQ_ERR_SHAPE;
+    if (!(a->softcap >= 0.f) || !(fabsf(a->softmax_scale) <= FLT_MAX)) return KVQ_ERR_SHAPE;
     const PagedPlan r = paged_plan(*l, a->n, a->tokens, a->nh, a->max_new, a->max_tokens, a->max_chunks);
     const uint64_t need = paged_bytes(r, a->tokens, a->nh);
     if (need && (!a->workspace || a->workspace_bytes < need)) return KVQ_ERR_WORKSPACE;
@@ -171,6 +174,13 @@ extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, c
     p.k_groups = page_groups(l->k_bits, l->group);
     p.v_groups = page_groups(l->v_bits, l->group);
     p.few_rows = r.few_rows;
+    // A cap that no score comes near is none (its square is beyond 1 / fp32's rounding for every score up to 1e26), and one below 1e-30 leaves nothing of
+    // them; what is between keeps products and quotients of caps and scales in fp32's range.
+    if (p.a.softcap >= 1e30f) p.a.softcap = 0.f;
+    if (p.a.softcap > 0.f) {
+        p.a.softcap = fmaxf(p.a.softcap, 1e-30f);
+        p.cap_in = fminf(fmaxf(a->softmax_scale / p.a.softcap, -1e30f), 1e30f);
+    }
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const int most = r.few && r.few_splits > r.tile_splits ? r.few_splits : r.tiles ? r.tile_splits : r.few_splits;
     p.part_out = static_cast<float *>(a->workspace);

@@ -18,6 +18,7 @@ struct PagedArgs {
     kvq_paged_attn_args a;
     int rep, k_groups, v_groups;      // query heads of a kv head; groups of a page's row
     int splits, few_rows;             // few_rows: sequences with at most so many rows are the other kernel's
+    float cap_in;                     // softmax_scale / softcap
     float *part_out;                  // [splits][tokens * nh][128], unnormalised
     float *part_ml;                   // [splits][tokens * nh][2]: the exponents' reference (log2), the weights' sum
 };

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
         const float down = __int_as_float((127 - e) << 23), up = __int_as_float((127 + e) << 23), scale2 = p.a.softmax_scale * kLog2e;
 #pragma unroll
         for (int c = 0; c < 4; ++c) s_q[r * 128 + lane + 32 * c] = s_qs[r * 128 + few_slot(lane + 32 * c)] = __float2half_rn(x[c] * down);
-        if (lane == 0) s_factor[r] = make_float2(scale2 * up, p.a.softcap > 0.f ? p.a.softmax_scale / p.a.softcap * up : 0.f);
+        if (lane == 0) s_factor[r] = make_float2(scale2 * up, p.cap_in * up);
     }
     int4 *s_bounds = reinterpret_cast<int4 *>(smem + sh.bounds);  // lowest position, end, position, slope of a row
     if (threadIdx.x < R) {

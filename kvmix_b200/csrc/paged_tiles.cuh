@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                     at(j + 1) = __float_as_uint(w.y);
                 };
                 if (cap) {
-                    const float small = p.a.softmax_scale / p.a.softcap;
+                    const float small = p.cap_in;
                     // the polynomial for all first; where a square says that one was too large, the scores are read again
                     const CapSmall capped(small, cap2);
                     float most = 0.f;

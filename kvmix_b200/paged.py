@@ -263,7 +263,8 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
         max(first[token], p + 1 - window) <= j < max(p + 1, prefix[i])       (all from the lower bound on where causal is False)
 
     window: sliding window, None or 0 for none.  prefix int32 [n]: the first prefix[i] tokens see each other.  first int32 [tokens]: where the
-    token's document begins, for documents packed behind one another.  softcap: scores become softcap * tanh(score / softcap).
+    token's document begins, for documents packed behind one another.  softcap: scores become softcap * tanh(score / softcap); 1e30 and
+    more, infinity too, is none.
     alibi_slopes fp32 [nh]: slopes[h] * (j - p) is added.  max_new, max_tokens, max_chunks: no sequence has more new tokens, none is longer, no
     more of them have several new tokens (host integers that lay out the work; None: whatever fits the tensors; with many sequences of
     which few have several tokens the third saves time).  Tokens that see nothing get zeros.  Cached values have
@@ -287,6 +288,9 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     window, softcap = window or 0, softcap or 0.0
     if window < 0 or not softcap >= 0.0:
         raise RuntimeError("window and softcap must not be negative")
+    scale = 1.0 / math.sqrt(128) if softmax_scale is None else float(softmax_scale)
+    if not abs(scale) <= 3.4e38:
+        raise RuntimeError("softmax_scale must be a finite number")
     at_slopes = 0
     if alibi_slopes is not None:
         if alibi_slopes.dtype is not torch.float32 or alibi_slopes.shape != (nh,) or alibi_slopes.get_device() != dev or not alibi_slopes.is_contiguous():
@@ -304,7 +308,7 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     a = _pack_attn(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), _ints(dev, "q_start", q_start, n + 1),
                    _rows(dev, "rows", rows), 0 if first is None else _ints(dev, "first", first, tokens), 0 if prefix is None else _ints(dev, "prefix", prefix, n),
                    at_slopes, n, tokens, nh, max_new, max_tokens, max_chunks, int(window), int(bool(causal)),
-                   1.0 / math.sqrt(128) if softmax_scale is None else softmax_scale, float(softcap), 0 if ws is None else ws.data_ptr(), need)
+                   scale, min(float(softcap), 1e38), 0 if ws is None else ws.data_ptr(), need)
     _launched(L.kvq_paged_attn(book, block, a, ops.raw_stream()))
     return out
 

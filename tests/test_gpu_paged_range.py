@@ -102,3 +102,28 @@ def test_large_raw_scores_below_the_cap(cuda, new, scale):
     q = (queries(new, 4) * (14 / (scale * 60 * 11.3))).half() if scale > 2e-6 else (queries(new, 4) * 1.2e4).half()
     assert q.isfinite().all()
     holds(attend(c, q, [new], softcap=50.0, scale=scale), *attention(c, q, [new], True, softcap=50.0, scale=scale))
+
+
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("softcap", [float("inf"), 1e300, 3e38, 1e31])
+def test_a_cap_beyond_all_scores_is_none(cuda, new, softcap):
+    c = Cache([700], [3], 1, 2, 4, 64, seed=8)
+    q = queries(new, 4)
+    assert torch.equal(attend(c, q, [new], softcap=softcap), attend(c, q, [new]))
+
+
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("softcap", [1e-25, 1e-38, 1e-42])
+def test_a_cap_below_all_scores(cuda, new, softcap):
+    """All scores the same to 2^-24: the mean of the values; a query of zeros among them."""
+    c = Cache([300], [1], 1, 4, 4, 64, seed=8)
+    q = queries(new, 4)
+    q[0, 0] = 0
+    holds(attend(c, q, [new], softcap=softcap), *attention(c, q, [new], True, scale=0.0))
+
+
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan"), 1e39])
+def test_scales_that_are_no_numbers(cuda, bad):
+    c = Cache([300], [1], 1, 4, 4, 64, seed=8)
+    with pytest.raises(RuntimeError):
+        attend(c, queries(1, 4), [1], scale=bad)

@@ -105,3 +105,9 @@ def test_layers_of_a_profile():
     cache = kv.KVmixPagedCache(qb, 1, 128, 1, 128, 1, 1, 64, device="cpu")
     assert [(l.k_bits, l.v_bits) for l in cache.layers] == [(qb[i]["k_bits"], qb[i]["v_bits"]) for i in sorted(qb)]
     assert cache.layers[0].kcode.shape[-1] == paged.page_words(cache.layers[0].k_bits)
+
+
+def test_scales_and_caps_that_are_no_numbers():
+    L = paged._library()
+    for bad in (dict(softmax_scale=float("inf")), dict(softmax_scale=-float("inf")), dict(softcap=-float("inf"))):
+        assert L.kvq_paged_attn(book(), layer(), attn(**bad), None) == -7
