@@ -474,8 +474,9 @@ int kvq_decode_attn_static(const kvq_attn_args *a, kvq_stream_t stream);
  *   count    [4]                 free packed pages, free fp16 pages, status, 0
  * A page that several sequences hold is full or packed and never written.
  *
- * count[2], the status, collects KVQ_PAGES_* bits.  A call that cannot be done in full does nothing but set one; while any is set, the
- * calls that change the cache do nothing (lengths and pages stay consistent) until the caller has cleared it.
+ * count[2], the status, collects KVQ_PAGES_* bits.  A call that cannot be done in full does nothing but set one; while such a bit is set, the
+ * calls that change the cache do nothing (lengths and pages stay consistent) until the caller has cleared it.  KVQ_PAGES_STALLED only says
+ * that an attention's output is not to be used: the cache is whole, and calls go on.
  * `rows`: n slots, each at most once in a call.  Stacks are popped and pushed in the order of rows and pages (kvq_pages_extend, _fork,
  * _settle) and of page numbers (pages that come free), so that equal calls give equal numbers.
  */
@@ -484,7 +485,7 @@ int kvq_decode_attn_static(const kvq_attn_args *a, kvq_stream_t stream);
 #define KVQ_PAGES_NO_PACKED 2   /* fewer free packed pages than asked for                                  */
 #define KVQ_PAGES_TOO_LONG 4    /* a sequence would need more than max_pages                               */
 #define KVQ_PAGES_BAD_ROWS 8    /* a row outside the table, named twice, or not as the call wants it       */
-#define KVQ_PAGES_STALLED 16    /* a kernel gave up waiting for its own copies                             */
+#define KVQ_PAGES_STALLED 16    /* an attention gave up waiting for its own copies; holds nothing up        */
 
 typedef struct {
     int32_t *table, *length, *packed, *refs, *free_ids, *count;

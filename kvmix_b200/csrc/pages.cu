@@ -98,7 +98,7 @@ __device__ __forceinline__ void collect(BookShared &s, int32_t *refs, int32_t *s
 
 __global__ void __launch_bounds__(kBookThreads) pages_extend_kernel(kvq_page_book b, const int32_t *rows, const int32_t *counts, int n) {
     __shared__ BookShared s;
-    if (b.count[2]) return;
+    if (refused(b)) return;
     clear_seen(b);
     int bad = 0;
     long long want = 0;
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_extend_kernel(kvq_page_boo
 
 __global__ void __launch_bounds__(kBookThreads) pages_free_kernel(kvq_page_book b, const int32_t *rows, int n) {
     __shared__ BookShared s;
-    if (b.count[2]) return;
+    if (refused(b)) return;
     clear_seen(b);
     bool bad = false;
     for (int i = threadIdx.x; i < n; i += kBookThreads) bad |= !first_seen(b, rows[i]);
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_free_kernel(kvq_page_book 
 __global__ void __launch_bounds__(kBookThreads) pages_settle_kernel(kvq_page_book b, const int32_t *rows, int n, int window, int32_t *moves) {
     __shared__ BookShared s;
     if (threadIdx.x == 0) moves[0] = 0;
-    if (b.count[2]) return;
+    if (refused(b)) return;
     clear_seen(b);
     bool bad = false;
     long long want = 0;
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_settle_kernel(kvq_page_boo
 __global__ void __launch_bounds__(kBookThreads) pages_fork_kernel(kvq_page_book b, const int32_t *parents, const int32_t *children, int n, int32_t *moves) {
     __shared__ BookShared s;
     if (threadIdx.x == 0) moves[0] = 0;
-    if (b.count[2]) return;
+    if (refused(b)) return;
     clear_seen(b);
     bool bad = false;
     for (int i = threadIdx.x; i < n; i += kBookThreads) bad |= !first_seen(b, children[i]);
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_compact_kernel(kvq_page_bo
     __shared__ BookShared s;
     int32_t *moves16 = moves + 4 + 2 * (int64_t)b.n_packed, *to = moves16 + 4 + 2 * (int64_t)b.n_fp16;
     if (threadIdx.x == 0) moves[0] = moves16[0] = 0;
-    if (b.count[2]) return;
+    if (refused(b)) return;
     const int live = close_up(s, b.refs, b.free_ids, b.n_packed, &b.count[0], moves, to);
     const int live16 = close_up(s, b.refs + b.n_packed, b.free_ids + b.n_packed, b.n_fp16, &b.count[1], moves16, to + b.n_packed);
     for (int row = threadIdx.x >> 5; row < b.slots; row += kBookThreads / 32) {
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_compact_kernel(kvq_page_bo
 // New tokens into their pages: a thread takes eight channels of one (token, head), keys and values.
 template <bool VEC>
 __global__ void __launch_bounds__(256) page_write_kernel(const kvq_page_book b, const kvq_page_layer l, const kvq_page_write_args a) {
-    if (b.count[2]) return;
+    if (refused(b)) return;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int c = (int)(i & 15) * 8;
     const int64_t th = i >> 4;

@@ -12,7 +12,8 @@ bit widths, its newest are fp16 (``include/kvmix_b200.h`` has the layouts, which
 
 The bookkeeping (``PageBook``) lives on the device and is changed by kernels only: no call waits for the host, all can be captured in a
 CUDA graph.  A call that cannot be done in full -- no page left, a row named twice -- does nothing but set a bit of ``count[2]``, and
-until that is cleared every call that changes the cache does nothing (``KVmixPagedCache.check`` raises and clears).  The attention is
+until that is cleared every call that changes the cache does nothing (``KVmixPagedCache.check`` raises and clears).  An attention
+that gave up waiting sets a bit too, which holds nothing up: its output is lost, the cache is whole.  The attention is
 exact softmax attention over the dequantised cache: scores are not narrowed to fp16 as ``decode_attention`` does by default.
 """
 import ctypes as C
@@ -28,7 +29,7 @@ from ._lib import check
 
 PAGE_TOKENS = 128
 _STATUS = {1: "no free fp16 page", 2: "no free packed page", 4: "sequence longer than the table", 8: "bad rows (outside the table, named twice, "
-           "a child that is not empty or also a parent)", 16: "a kernel gave up waiting for its own copies"}
+           "a child that is not empty or also a parent)", 16: "an attention gave up waiting for its own copies, its output is not to be used"}
 
 _pack_book, _pack_layer = struct.Struct("@6P4i").pack, struct.Struct("@8P6i").pack
 _pack_write, _pack_attn = struct.Struct("@2P4q2P2i").pack, struct.Struct("@2P4q5P8i2fPQ").pack
@@ -437,7 +438,8 @@ class KVmixPagedCache:
         return tuple(self.book.count[:2].tolist())
 
     def check(self):
-        """Raises if a call since the last check had to be refused, and lets the cache go on from where it was.  Waits for the device."""
+        """Raises if a call since the last check had to be refused or an attention's output is not to be used, and lets the cache go on from where it
+        was.  Waits for the device."""
         status = int(self.book.count[2])
         if status:
             self.book.count[2] = 0

@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from test_gpu_paged import Cache, attend, queries
+import kvmix_b200 as kv
+from test_gpu_paged import P, Cache, attend, queries
 from test_gpu_paged_book import small
 
 pytestmark = pytest.mark.gpu
@@ -127,3 +128,35 @@ def test_scales_that_are_no_numbers(cuda, bad):
     c = Cache([300], [1], 1, 4, 4, 64, seed=8)
     with pytest.raises(RuntimeError):
         attend(c, queries(1, 4), [1], scale=bad)
+
+
+# ---- a stalled wait --------------------------------------------------------------------------------------------------------------------
+
+def test_a_stalled_wait_leaves_the_cache_whole(cuda):
+    """An attention that gave up waiting says so in the status.  Its own output is lost; the layers behind it are written, and later calls work."""
+    gen = torch.Generator().manual_seed(5)
+    cache = kv.KVmixPagedCache([(4, 2), (2, 2), (3, 3)], 2, 128, 3, 700, 8, 10, 64, 128)
+    k, v = (torch.randn(3, 400, 2, 128, generator=gen).half().cuda() for _ in range(2))
+    at = 0
+    for n in (300, 1, 99):
+        s = cache.extend([1], [n])
+        for l in range(3):
+            cache.write(l, k[l, at:at + n], v[l, at:at + n], s)
+            if l == 0:
+                cache.book.count[2] |= 16                       # what a wait of layer 0's attention leaves behind
+        at += n
+        ids = cache.book.table[1].tolist()
+        for l in range(3):
+            packed = int(cache.book.packed[1])
+            for j in range(packed, -(-at // P)):
+                m = min(P, at - j * P)
+                assert torch.equal(cache.layers[l].kfull[ids[j], :, :m], k[l, j * P:j * P + m].transpose(0, 1))
+                assert torch.equal(cache.layers[l].vfull[ids[j], :, :m], v[l, j * P:j * P + m].transpose(0, 1))
+    cache.settle()
+    assert cache.book.packed.tolist() == [0, 2, 0]
+    with pytest.raises(RuntimeError, match="gave up"):
+        cache.check()
+    cache.check()
+    assert cache.lengths == cache.book.length.tolist() == [0, 400, 0]
+    cache.free([1])
+    assert cache.free_pages() == (8, 10)
