@@ -28,6 +28,7 @@ from . import _lib, ops
 from ._lib import check
 
 PAGE_TOKENS = 128
+_MOST = 1 << 30                  # no sequence is longer: wider windows are this one
 _STATUS = {1: "no free fp16 page", 2: "no free packed page", 4: "sequence longer than the table", 8: "bad rows (outside the table, named twice, "
            "a child that is not empty or also a parent)", 16: "an attention gave up waiting for its own copies, its output is not to be used"}
 
@@ -215,7 +216,7 @@ def pages_settle(rows, window, pages, layers):
     moves = pages.count.new_empty(4 + 2 * pages.n_packed)
     blocks, n = [_layer(pages, dev, layer) for layer in layers], rows.numel()
     L, st, at = _library(), ops.raw_stream(), moves.data_ptr()
-    _launched(L.kvq_pages_settle(book, _rows(dev, "rows", rows), n, int(window), at, st))
+    _launched(L.kvq_pages_settle(book, _rows(dev, "rows", rows), n, min(int(window), _MOST), at, st))
     for block in blocks:
         _launched(L.kvq_page_pack(block, at, min(pages.n_packed, n * pages.table.shape[1]), st))
 
@@ -308,7 +309,7 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     ws = pages.count.new_empty((need + 3) // 4) if need else None
     a = _pack_attn(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), _ints(dev, "q_start", q_start, n + 1),
                    _rows(dev, "rows", rows), 0 if first is None else _ints(dev, "first", first, tokens), 0 if prefix is None else _ints(dev, "prefix", prefix, n),
-                   at_slopes, n, tokens, nh, max_new, max_tokens, max_chunks, int(window), int(bool(causal)),
+                   at_slopes, n, tokens, nh, max_new, max_tokens, max_chunks, min(int(window), _MOST), int(bool(causal)),
                    scale, min(float(softcap), 1e38), 0 if ws is None else ws.data_ptr(), need)
     _launched(L.kvq_paged_attn(book, block, a, ops.raw_stream()))
     return out

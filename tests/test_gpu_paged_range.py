@@ -7,7 +7,7 @@ import torch
 
 import kvmix_b200 as kv
 from test_gpu_paged import P, Cache, attend, queries
-from test_gpu_paged_book import small
+from test_gpu_paged_book import ints, small
 
 pytestmark = pytest.mark.gpu
 
@@ -160,3 +160,22 @@ def test_a_stalled_wait_leaves_the_cache_whole(cuda):
     assert cache.lengths == cache.book.length.tolist() == [0, 400, 0]
     cache.free([1])
     assert cache.free_pages() == (8, 10)
+
+
+# ---- windows ---------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 40])
+def test_windows_beyond_32_bits(cuda, window):
+    cache = small()
+    kv.pages_settle(ints(0), window, cache.book, cache.layers)
+    assert not cache.book.packed.any()                          # nothing ends so far back
+    never = kv.KVmixPagedCache([(4, 2)], 1, 128, 1, 512, 4, 4, 64, residual_length=window)
+    never.extend([0], [512])
+    never.settle()
+    assert not never.book.packed.any()
+    q = torch.randn(3, 4, 128, device="cuda").half()
+    for rows in (ints(0), ints(2)):
+        for n in (1, 3):
+            got = kv.paged_attention(q[:n], ints(0, n), rows, cache.book, cache.layers[0], window=window)
+            assert torch.equal(got, kv.paged_attention(q[:n], ints(0, n), rows, cache.book, cache.layers[0]))
+    cache.check()
