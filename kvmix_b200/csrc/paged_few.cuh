@@ -12,7 +12,8 @@ namespace kvq {
 // come from the same place of two words, and a field of 1, 2 or 4 bits is an operand as it stands: masked in place it is the fp16 subnormal
 // code * 2^(position - 24), and the power of two, the same for a whole accumulator, comes off at the end.  Scales go to the other
 // operand, whose columns are (group of the packed axis, query row) pairs:
-//   keys     B = q * scale of a channel's token group, as an exact pair hi + lo of two columns (rounded once it would cost 2^-11 of every term)
+//   keys     B = q * scale of a channel's token group, as a pair hi + lo of two columns: exact to 2^-22 of itself and 2^-25 (the largest of a stage is 2^-6 and
+//            more); rounded once it would cost 2^-11 of every term
 //   values   B = p * scale of a token's channel group, rounded to fp16 as weights are everywhere; a pair as well where columns are left (one
 //            sequence of 1, 2 or 4 rows at groups of 32, 64 or 128: 2.5e-4 of an output's size in place of 3.2e-4, at 2 bits)
 // An accumulator row needs the column of its own group only; what the others hold is not read.  Minima times q or p come from one more MMA
@@ -440,6 +441,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
     // p * scale * 2^expo: the power of two starts from the first scales (the largest of them becomes 4 to 8) and follows them where a stage's largest
     // would exceed 256 or stay below 2^-5; the sums so far go along, exactly
     int expo = 32;
+    // q * scale * 2^lift: 0 wherever a look at some of a stage's scales finds one of 2^-5 or more.  Below that what the pair hi + lo has under 2^-24 would be
+    // lost (5e-3 of a score for 4-bit keys of 1e-4); the largest scale becomes 4 to 8 then, in place, so that usual ones cost the look alone.
+    int lift = 0;
 #pragma unroll 1
     for (int k = 0; k < n_mine; ++k) {
         if (k == ids_base + 32) { fetch_ids(k); produce(); }
@@ -485,6 +489,27 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
             for (int q = 0; q < half_stages; ++q) {
                 const uint32_t c = stage_ready(), c_sc = c + k_cb, c_mn = c_sc + k_sz;
                 if (!ok) break;
+                const int words = stage_rows * p.k_groups / 2;
+                const uint32_t look = lds32(c_sc + 4 * min(lane, words - 1));
+                if (lift || !__any_sync(0xffffffffu, max(look & 0xffffu, look >> 16) >= 0x2800u)) {
+                    uint32_t m2 = 0;
+                    for (int w = lane; w < words; w += 32) m2 = as_u32(__hmax2(as_h2(m2), as_h2(lds32(c_sc + 4 * w))));
+                    const int top = (int)(__reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16)) >> 10 & 31), old = lift;
+                    if (top + lift > 15 + 7 || top + lift < 10) lift = min(max(17 - top, 0), 15);
+                    for (int w = lane; lift && w < words; w += 32)
+                        asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(c_sc + 4 * w), "r"(as_u32(__hmul2(as_h2(lds32(c_sc + 4 * w)), as_h2((uint32_t)(lift + 15) * 0x04000400u)))) : "memory");
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");       // the next copy into this place is the async proxy's
+                    __syncwarp();
+                    if (lift != old) {
+                        const float f = exp2f((float)(lift - old));
+#pragma unroll
+                        for (int n = 0; n < CK; ++n)
+#pragma unroll
+                            for (int m = 0; m < 8; ++m)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) sc[n][m][e] *= f;
+                    }
+                }
                 const __half *q_at = s_qs + q * stage_rows + 4 * t;
 #pragma unroll 1
                 for (int at = 0; at < stage_rows; at += 16) {
@@ -510,6 +535,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
                 stage_done();
             }
             if (!ok) break;
+            const float undo = __int_as_float((127 - lift) << 23);
 #pragma unroll
             for (int n = 0; n < CK; ++n) {
                 const int pair = 4 * n + t, r = pair & ((1 << kr_log2) - 1);
@@ -519,7 +545,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
                     for (int m = 0; m < 8; m += 2) {
                         float v[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = fmaf(sc[n][m + (e >> 1)][2 * (e & 1)] + sc[n][m + (e >> 1)][2 * (e & 1) + 1], few_power<KB>(m + (e >> 1), e & 1), zero);
+                        for (int e = 0; e < 4; ++e) v[e] = fmaf(sc[n][m + (e >> 1)][2 * (e & 1)] + sc[n][m + (e >> 1)][2 * (e & 1) + 1], few_power<KB>(m + (e >> 1), e & 1) * undo, zero);
                         sts_f4(s_s + r * 512 + (16 * g + 2 * m) * 4, v[0], v[1], v[2], v[3]);
                     }
                 }

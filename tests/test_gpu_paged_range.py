@@ -179,3 +179,30 @@ def test_windows_beyond_32_bits(cuda, window):
             got = kv.paged_attention(q[:n], ints(0, n), rows, cache.book, cache.layers[0], window=window)
             assert torch.equal(got, kv.paged_attention(q[:n], ints(0, n), rows, cache.book, cache.layers[0]))
     cache.check()
+
+
+# ---- small keys ------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kb,vb,group", [(2, 2, 32), (4, 4, 64), (1, 4, 128), (4, 2, 128), (3, 3, 128)])
+@pytest.mark.parametrize("rep", [1, 2, 4, 8])
+@pytest.mark.parametrize("k_size", [1e-2, 1e-3, 1e-4, 3e3])
+def test_keys_of_any_size(cuda, kb, vb, group, rep, k_size):
+    """Keys far from 1 and queries that make up for it: scores of the usual size from the smallest fp16 scales, and from large ones."""
+    c = sized(Cache([700], [5], 1, kb, vb, group, seed=5, outliers=False), k_size)
+    q = (queries(1, rep).float() / k_size).half()
+    got, (want, slack) = attend(c, q, [1]), attention(c, q, [1], kb != 3)
+    holds(got, want, slack)
+    rows_hold(got, want, 2e-3)                                  # the framework's own tolerance
+
+
+def test_key_scales_that_grow_along_the_sequence(cuda):
+    """Pages, and channels of a page, whose scales are 2^20 apart."""
+    for rep, kb, group in ((1, 4, 32), (2, 2, 64), (4, 1, 128), (8, 4, 64), (4, 3, 128)):
+        c = Cache([128 * 9], [9], 1, kb, 2, group, seed=8, outliers=False)
+        ids = c.host["table"][c.host["rows"][0]].tolist()
+        for j, i in enumerate(ids):
+            for t in c.host["k"][1:]:
+                t[i] *= 2.0 ** (-12 + 2 * min(j, 8 - j))
+                t[i, :, 64:] *= 2.0 ** (-6 if j % 2 else 4)
+        q = (queries(1, rep).float() * 8).half()
+        holds(attend(sized(c, 1.0), q, [1]), *attention(c, q, [1], kb != 3))
