@@ -29,6 +29,7 @@ from ._lib import check
 
 PAGE_TOKENS = 128
 _MOST = 1 << 30                  # no sequence is longer: wider windows are this one
+_MOST_HEADS = 1 << 15            # what kvq_page_copy takes as one page: 1 GB
 _STATUS = {1: "no free fp16 page", 2: "no free packed page", 4: "sequence longer than the table", 8: "bad rows (outside the table, named twice, "
            "a child that is not empty or also a parent)", 16: "an attention gave up waiting for its own copies, its output is not to be used"}
 
@@ -113,13 +114,17 @@ def _book(pages):
 def _page_tensor(dev, t, dtype, shape):
     # the address is asked for in the same breath: a layer has eight such tensors, a call of many layers hundreds
     if t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous():
-        return t.data_ptr()
-    raise RuntimeError(f"page tensor {tuple(t.shape)} {t.dtype} on {t.device}: contiguous {dtype} {shape} on cuda:{dev} expected")
+        at = t.data_ptr()
+        if not at & 15:                               # here and not by the copies, which come behind bookkeeping that cannot be taken back
+            return at
+    raise RuntimeError(f"page tensor {tuple(t.shape)} {t.dtype} on {t.device}: contiguous {dtype} {shape} on cuda:{dev} at a multiple of 16 bytes expected")
 
 
 def _fp16_pages(pages, dev, layer):
     """Addresses of a layer's fp16 pages."""
     kfull, vfull = layer.kfull, layer.vfull
+    if kfull.shape[1] > _MOST_HEADS:
+        raise RuntimeError(f"pages hold at most {_MOST_HEADS} kv heads")
     shape = (pages.refs.numel() - pages.n_packed, kfull.shape[1], PAGE_TOKENS, 128)
     return _page_tensor(dev, kfull, _f16, shape), _page_tensor(dev, vfull, _f16, shape)
 
@@ -132,6 +137,8 @@ def _layer(pages, dev, layer):
     if group not in (32, 64, 128):
         raise RuntimeError("pages are quantized in groups of 32, 64 or 128")
     n, heads = pages.n_packed, kfull.shape[1]
+    if heads > _MOST_HEADS:
+        raise RuntimeError(f"pages hold at most {_MOST_HEADS} kv heads")
     n16 = pages.refs.numel() - n
     kw, vw, kg, vg = (n, heads, PAGE_TOKENS, page_words(kb)), (n, heads, PAGE_TOKENS, page_words(vb)), (n, heads, PAGE_TOKENS, page_groups(kb, group)), \
         (n, heads, PAGE_TOKENS, page_groups(vb, group))
@@ -245,7 +252,7 @@ def pages_compact(pages, layers):
         _layer(pages, dev, layer)
         for tensors, some in ((packed, (layer.kcode, layer.kscale, layer.kmn, layer.vcode, layer.vscale, layer.vmn)), (fp16, (layer.kfull, layer.vfull))):
             for t in some:
-                tensors += (t.data_ptr(), t.stride(0) * t.element_size())
+                tensors += (t.data_ptr(), t.numel() // max(t.shape[0], 1) * t.element_size())
     moves = pages.count.new_empty(8 + 3 * total)
     _launched(_library().kvq_pages_compact(book, moves.data_ptr(), ops.raw_stream()))
     if n:

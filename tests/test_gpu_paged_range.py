@@ -7,7 +7,7 @@ import torch
 
 import kvmix_b200 as kv
 from test_gpu_paged import P, Cache, attend, queries
-from test_gpu_paged_book import ints, small
+from test_gpu_paged_book import ints, small, snapshot, unchanged
 
 pytestmark = pytest.mark.gpu
 
@@ -206,3 +206,34 @@ def test_key_scales_that_grow_along_the_sequence(cuda):
                 t[i, :, 64:] *= 2.0 ** (-6 if j % 2 else 4)
         q = (queries(1, rep).float() * 8).half()
         holds(attend(sized(c, 1.0), q, [1]), *attention(c, q, [1], kb != 3))
+
+
+# ---- refused before anything is changed ------------------------------------------------------------------------------------------------
+
+def shifted(t):
+    """The same tensor, contiguous, two elements behind a 16-byte boundary."""
+    x = torch.zeros(t.numel() + 8, dtype=t.dtype, device=t.device)[2:2 + t.numel()].view(t.shape)
+    x.copy_(t)
+    assert x.is_contiguous() and x.data_ptr() % 16
+    return x
+
+
+@pytest.mark.parametrize("name", ["kcode", "kscale", "kmn", "kfull", "vcode", "vscale", "vmn", "vfull"])
+def test_misaligned_pages_are_refused_at_once(cuda, name):
+    """Pages that the kernels cannot copy are refused before the bookkeeping hands their numbers on."""
+    cache = small()
+    cache.settle([0])
+    cache.extend([0], [1])
+    cache.free([2])
+    layers = [cache.layers[0], cache.layers[0]._replace(**{name: shifted(getattr(cache.layers[0], name))})]
+    before = snapshot(cache)
+    calls = [lambda: kv.pages_settle(ints(0), 0, cache.book, layers), lambda: kv.pages_compact(cache.book, layers),
+             lambda: kv.page_write(torch.zeros(1, 1, 128, device="cuda").half(), torch.zeros(1, 1, 128, device="cuda").half(), ints(0, 1), ints(0), cache.book, layers[1]),
+             lambda: kv.paged_attention(queries(1, 4), ints(0, 1), ints(0), cache.book, layers[1])]
+    if name in ("kfull", "vfull"):
+        calls.append(lambda: kv.pages_fork(ints(0), ints(3), cache.book, layers))
+    for call in calls:
+        with pytest.raises(RuntimeError):
+            call()
+        unchanged(cache, before)
+    cache.check()
