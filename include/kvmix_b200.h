@@ -472,7 +472,7 @@ int kvq_decode_attn_static(const kvq_attn_args *a, kvq_stream_t stream);
  *   refs     [n_packed + n_fp16] references of every page, fp16 pages behind the packed ones
  *   free_ids [n_packed + n_fp16] the free pages' numbers, two stacks (packed from 0, fp16 from n_packed), the next one to be taken last
  *   count    [4]                 free packed pages, free fp16 pages, status, 0
- * A page that several sequences hold is full or packed and never written.
+ * A page that several sequences hold is full or packed and never written (kvq_page_write leaves tokens out whose page is packed or shared).
  *
  * count[2], the status, collects KVQ_PAGES_* bits.  A call that cannot be done in full does nothing but set one; while such a bit is set, the
  * calls that change the cache do nothing (lengths and pages stay consistent) until the caller has cleared it.  KVQ_PAGES_STALLED only says

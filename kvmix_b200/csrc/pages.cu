@@ -354,13 +354,7 @@ __global__ void __launch_bounds__(256) page_write_kernel(const kvq_page_book b, 
     const int64_t th = i >> 4;
     const int u = (int)(th / l.Hkv), h = (int)(th - (int64_t)u * l.Hkv);
     if (u >= a.tokens || u < a.q_start[0] || u >= a.q_start[a.n]) return;
-    const int s = sequence_of(a.q_start, a.n, u), row = a.rows[s];
-    if (row < 0 || row >= b.slots) return;
-    const int pos = b.length[row] - a.q_start[s + 1] + u, page = pos / kPage;
-    if (pos < 0 || page >= b.max_pages || page < b.packed[row]) return;
-    const int id = b.table[(int64_t)row * b.max_pages + page];
-    if (id < 0 || id >= l.n_fp16) return;
-    const int64_t to = (((int64_t)id * l.Hkv + h) * kPage + pos % kPage) * kHeadDim + c;
+    // asked for first: they land while the token's place is looked up, four loads one behind the other
     const __half *k = static_cast<const __half *>(a.k) + u * a.k_sT + h * a.k_sH + c, *v = static_cast<const __half *>(a.v) + u * a.v_sT + h * a.v_sH + c;
     uint4 x, y;
     if constexpr (VEC) {
@@ -371,6 +365,13 @@ __global__ void __launch_bounds__(256) page_write_kernel(const kvq_page_book b, 
 #pragma unroll
         for (int j = 0; j < 8; ++j) { px[j] = k[j]; py[j] = v[j]; }
     }
+    const int s = sequence_of(a.q_start, a.n, u), row = a.rows[s];
+    if (row < 0 || row >= b.slots) return;
+    const int pos = b.length[row] - a.q_start[s + 1] + u, page = pos / kPage;
+    if (pos < 0 || page >= b.max_pages || page < b.packed[row]) return;
+    const int id = b.table[(int64_t)row * b.max_pages + page];
+    if (id < 0 || id >= min(l.n_fp16, b.n_fp16) || b.refs[b.n_packed + id] > 1) return;      // a page that others hold too stays as it is
+    const int64_t to = (((int64_t)id * l.Hkv + h) * kPage + pos % kPage) * kHeadDim + c;
     *reinterpret_cast<uint4 *>(static_cast<__half *>(l.kfull) + to) = x;
     *reinterpret_cast<uint4 *>(static_cast<__half *>(l.vfull) + to) = y;
 }

@@ -196,7 +196,8 @@ def pages_free(rows, pages):
 @_on_its_device(4)
 def page_write(k, v, q_start, rows, pages, layer):
     """Keys (rotated) and values of new tokens into one layer's fp16 pages.  k, v [tokens, Hkv, 128] fp16, any strides; tokens
-    [q_start[i], q_start[i+1]) are the last ones of sequence rows[i], which ``pages_extend`` has counted already."""
+    [q_start[i], q_start[i+1]) are the last ones of sequence rows[i], which ``pages_extend`` has counted already.  Tokens whose page
+    is packed, or held by another sequence too, are left out."""
     dev, book = _book(pages)
     heads = layer.kfull.shape[1]
     if k.dim() != 3 or k.shape[1:] != (heads, 128) or v.shape != k.shape or k.dtype is not torch.float16 or v.dtype is not torch.float16:

@@ -237,3 +237,28 @@ def test_misaligned_pages_are_refused_at_once(cuda, name):
             call()
         unchanged(cache, before)
     cache.check()
+
+
+# ---- shared pages ----------------------------------------------------------------------------------------------------------------------
+
+def test_shared_pages_are_never_written(cuda):
+    """New tokens that are said to reach back into pages which other sequences hold too: what lies there stays, the rest is written."""
+    gen = torch.Generator().manual_seed(9)
+    cache = kv.KVmixPagedCache([(4, 4)], 2, 128, 3, 700, 2, 10, 64, 1000)
+    k, v = (torch.randn(300, 2, 128, generator=gen).half().cuda() for _ in range(2))
+    cache.write(0, k, v, cache.extend([0], [300]))
+    cache.fork([0], [1])
+    cache.extend([1], [20])
+    x, y = (torch.randn(320, 2, 128, generator=gen).half().cuda() for _ in range(2))
+    kv.page_write(x, y, ints(0, 320), ints(1), cache.book, cache.layers[0])           # 20 of them are new
+    ids, own = cache.book.table[0].tolist(), cache.book.table[1].tolist()
+    assert ids[:2] == own[:2] and ids[2] != own[2]
+    for t, old, new in ((cache.layers[0].kfull, k, x), (cache.layers[0].vfull, v, y)):
+        for j in range(2):
+            assert torch.equal(t[ids[j]], old[j * P:j * P + P].transpose(0, 1))
+        assert torch.equal(t[ids[2], :, :44], old[256:300].transpose(0, 1))
+        assert torch.equal(t[own[2], :, :64], new[256:320].transpose(0, 1))
+    cache.free([0])                                                                   # nobody else holds them now
+    kv.page_write(x, y, ints(0, 320), ints(1), cache.book, cache.layers[0])
+    assert torch.equal(cache.layers[0].kfull[ids[0]], x[:P].transpose(0, 1))
+    cache.check()
