@@ -29,16 +29,19 @@ struct PagedSeq {
     int row, length, packed, q0, n_new, prefix;
     const int32_t *table;
 };
+__device__ __forceinline__ void new_tokens(const PagedArgs &p, int i, int &q0, int &n_new) {
+    q0 = min(max(p.a.q_start[i], 0), p.a.tokens);
+    n_new = min(max(p.a.q_start[i + 1], 0), p.a.tokens) - q0;
+}
 __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs &p, int i) {
     PagedSeq s;
     s.row = p.a.rows[i];
     const bool ok = s.row >= 0 && s.row < p.b.slots;
     const int row = ok ? s.row : 0;
-    s.length = ok ? min(p.b.length[row], p.b.max_pages * kPage) : 0;
-    s.packed = ok ? p.b.packed[row] : 0;
+    s.length = ok ? min(max(p.b.length[row], 0), p.b.max_pages * kPage) : 0;
+    s.packed = ok ? max(p.b.packed[row], 0) : 0;
     s.table = p.b.table + (int64_t)row * p.b.max_pages;
-    s.q0 = max(p.a.q_start[i], 0);
-    s.n_new = min(p.a.q_start[i + 1], p.a.tokens) - s.q0;
+    new_tokens(p, i, s.q0, s.n_new);
     s.prefix = p.a.prefix ? p.a.prefix[i] : 0;
     return s;
 }

@@ -173,7 +173,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     const int split = blockIdx.x % p.splits, hs = blockIdx.x / p.splits, head = hs % p.l.Hkv;
     int tile = max_tiles - 1 - hs / p.l.Hkv, seq = 0;
     auto tiles_of = [&](int i) {
-        const int rows = max(0, min(p.a.q_start[i + 1], p.a.tokens) - max(p.a.q_start[i], 0)) * p.rep;
+        int q0, n_new;
+        new_tokens(p, i, q0, n_new);
+        const int rows = max(0, n_new) * p.rep;
         return rows > p.few_rows ? (rows + 2 * kTileRows - 1) / (2 * kTileRows) : 0;
     };
     if (p.a.n <= 8) {
@@ -209,7 +211,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         if (seq < 0) return;
         tile = s_tile;
     }
-    const int q0 = max(p.a.q_start[seq], 0), n_new = min(p.a.q_start[seq + 1], p.a.tokens) - q0;       // as paged_seq has them, which waits for more loads
+    int q0, n_new;
+    new_tokens(p, seq, q0, n_new);                                // as paged_seq has them, which waits for more loads
     const int row0 = tile * 2 * kTileRows, rows = min(n_new * p.rep - row0, 2 * kTileRows), two_tiles = rows > kTileRows;
     const int warp = uniform_warp(), lane = threadIdx.x & 31, wg = warp >> 2;
 

@@ -55,6 +55,13 @@ __device__ __forceinline__ long long block_sum(BookShared &s, long long v) {
     return s.total;
 }
 
+// The bookkeeping's numbers as they are used: whatever the tensors hold, no index that follows from them leaves a tensor.
+__device__ __forceinline__ int length_of(const kvq_page_book &b, int row) { return min(max(b.length[row], 0), b.max_pages * kPage); }
+__device__ __forceinline__ int packed_of(const kvq_page_book &b, int row) { return min(max(b.packed[row], 0), pages_of(length_of(b, row))); }
+__device__ __forceinline__ int free_packed(const kvq_page_book &b) { return min(max(b.count[0], 0), b.n_packed); }
+__device__ __forceinline__ int free_fp16(const kvq_page_book &b) { return min(max(b.count[1], 0), b.n_fp16); }
+__device__ __forceinline__ bool inside(int id, int n) { return id >= 0 && id < n; }
+
 extern __shared__ uint32_t s_seen[];                              // a bit for every slot
 
 __device__ __forceinline__ void clear_seen(const kvq_page_book &b) {
@@ -73,7 +80,7 @@ __device__ __forceinline__ void drop(int32_t *ref) {
 
 // The pages of a pool that were marked go on its stack in ascending order.
 __device__ __forceinline__ void collect(BookShared &s, int32_t *refs, int32_t *stack, int n, int32_t *n_free) {
-    int at = *n_free, total;
+    int at = min(max(*n_free, 0), n), total;
     for (int base = 0; base < n; base += 4 * kBookThreads) {
         const int p = base + 4 * threadIdx.x;
         bool gone[4];
@@ -89,11 +96,11 @@ __device__ __forceinline__ void collect(BookShared &s, int32_t *refs, int32_t *s
         for (int i = 0; i < 4; ++i)
             if (gone[i]) {
                 refs[p + i] = 0;
-                stack[k++] = p + i;
+                if (k < n) stack[k++] = p + i;
             }
     }
     __syncthreads();
-    if (threadIdx.x == 0) *n_free = at;
+    if (threadIdx.x == 0) *n_free = min(at, n);
 }
 
 __global__ void __launch_bounds__(kBookThreads) pages_extend_kernel(kvq_page_book b, const int32_t *rows, const int32_t *counts, int n) {
@@ -105,13 +112,13 @@ __global__ void __launch_bounds__(kBookThreads) pages_extend_kernel(kvq_page_boo
     for (int i = threadIdx.x; i < n; i += kBookThreads) {
         const int row = rows[i], c = counts[i];
         if (!first_seen(b, row) || c < 0) { bad |= KVQ_PAGES_BAD_ROWS; continue; }
-        const int len = b.length[row];
+        const int len = length_of(b, row);
         if ((long long)len + c > (long long)b.max_pages * kPage) { bad |= KVQ_PAGES_TOO_LONG; continue; }
         want += pages_of(len + c) - pages_of(len);
     }
     bad = (__syncthreads_or(bad & KVQ_PAGES_BAD_ROWS) ? KVQ_PAGES_BAD_ROWS : 0) | (__syncthreads_or(bad & KVQ_PAGES_TOO_LONG) ? KVQ_PAGES_TOO_LONG : 0);
     want = block_sum(s, want);
-    const int n_free = b.count[1];
+    const int n_free = free_fp16(b);
     if (!bad && want > n_free) bad = KVQ_PAGES_NO_FP16;
     if (bad) {
         if (threadIdx.x == 0) atomicOr(&b.count[2], bad);
@@ -123,7 +130,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_extend_kernel(kvq_page_boo
         int need = 0, have = 0, row = 0;
         if (i < n) {
             row = rows[i];
-            const int len = b.length[row], c = counts[i];
+            const int len = length_of(b, row), c = counts[i];
             have = pages_of(len);
             need = pages_of(len + c) - have;
             b.length[row] = len + c;
@@ -137,7 +144,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_extend_kernel(kvq_page_boo
             for (int k = threadIdx.x & 31; k < s.need[r]; k += 32) {
                 const int id = b.free_ids[b.n_packed + n_free - 1 - s.before[r] - k];
                 b.table[(int64_t)s.row[r] * b.max_pages + s.from[r] + k] = id;
-                b.refs[b.n_packed + id] = 1;
+                if (inside(id, b.n_fp16)) b.refs[b.n_packed + id] = 1;
             }
         at += total;
         __syncthreads();
@@ -156,11 +163,11 @@ __global__ void __launch_bounds__(kBookThreads) pages_free_kernel(kvq_page_book 
         return;
     }
     for (int r = threadIdx.x >> 5; r < n; r += kBookThreads / 32) {
-        const int row = rows[r], packed = b.packed[row], held = min(max(pages_of(b.length[row]), packed), b.max_pages);
+        const int row = rows[r], packed = b.packed[row], held = min(max(pages_of(length_of(b, row)), packed), b.max_pages);
         int32_t *t = b.table + (int64_t)row * b.max_pages;
         for (int j = threadIdx.x & 31; j < held; j += 32) {
             const int id = t[j];
-            if (id >= 0 && id < (j < packed ? b.n_packed : b.n_fp16)) drop(b.refs + (j < packed ? id : b.n_packed + id));
+            if (inside(id, j < packed ? b.n_packed : b.n_fp16)) drop(b.refs + (j < packed ? id : b.n_packed + id));
             t[j] = -1;
         }
         __syncwarp();
@@ -178,7 +185,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_settle_kernel(kvq_page_boo
     clear_seen(b);
     bool bad = false;
     long long want = 0;
-    auto due = [&](int row) { return max(0, max(0, b.length[row] - window) / kPage - b.packed[row]); };
+    auto due = [&](int row) { return max(0, max(0, length_of(b, row) - window) / kPage - packed_of(b, row)); };
     for (int i = threadIdx.x; i < n; i += kBookThreads) {
         const int row = rows[i];
         if (first_seen(b, row)) want += due(row);
@@ -186,7 +193,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_settle_kernel(kvq_page_boo
     }
     bad = __syncthreads_or(bad);
     want = block_sum(s, want);
-    const int n_free = b.count[0];
+    const int n_free = free_packed(b);
     if (bad || want > n_free) {
         if (threadIdx.x == 0) atomicOr(&b.count[2], bad ? KVQ_PAGES_BAD_ROWS : KVQ_PAGES_NO_PACKED);
         return;
@@ -199,7 +206,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_settle_kernel(kvq_page_boo
         if (i < n) {
             row = rows[i];
             need = due(row);
-            from = b.packed[row];
+            from = packed_of(b, row);
             b.packed[row] = from + need;
         }
         s.before[threadIdx.x] = at + block_scan(s, need, total);
@@ -214,8 +221,8 @@ __global__ void __launch_bounds__(kBookThreads) pages_settle_kernel(kvq_page_boo
                 moves[4 + 2 * m] = src;
                 moves[5 + 2 * m] = to;
                 *t = to;
-                b.refs[to] = 1;
-                if (src >= 0 && src < b.n_fp16) drop(b.refs + b.n_packed + src);
+                if (inside(to, b.n_packed)) b.refs[to] = 1;
+                if (inside(src, b.n_fp16)) drop(b.refs + b.n_packed + src);
             }
         at += total;
         __syncthreads();
@@ -239,31 +246,32 @@ __global__ void __launch_bounds__(kBookThreads) pages_fork_kernel(kvq_page_book 
         for (int i = threadIdx.x; i < n; i += kBookThreads) {
             const int row = parents[i];
             if (row < 0 || row >= b.slots || (s_seen[row >> 5] >> (row & 31) & 1u) || b.length[children[i]] != 0) bad = true;
-            else want += b.length[row] % kPage != 0;
+            else want += length_of(b, row) % kPage != 0;
         }
         bad = __syncthreads_or(bad);
         want = block_sum(s, want);
-        const int n_free = b.count[1];
+        const int n_free = free_fp16(b);
         if (!bad && want <= n_free) {
             int at = 0, total;
             for (int base = 0; base < n; base += kBookThreads) {
                 const int i = base + threadIdx.x;
-                const int part = i < n && b.length[parents[i]] % kPage != 0;
+                const int part = i < n && length_of(b, parents[i]) % kPage != 0;
                 s.before[threadIdx.x] = at + block_scan(s, part, total);
                 __syncthreads();
                 for (int r = threadIdx.x >> 5; r < min(kBookThreads, n - base); r += kBookThreads / 32) {
-                    const int from = parents[base + r], to = children[base + r], len = b.length[from], packed = b.packed[from];
+                    const int from = parents[base + r], to = children[base + r], len = length_of(b, from), packed = packed_of(b, from);
                     const int32_t *src = b.table + (int64_t)from * b.max_pages;
                     int32_t *dst = b.table + (int64_t)to * b.max_pages;
-                    for (int j = threadIdx.x & 31; j < min(pages_of(len), b.max_pages); j += 32) {
+                    for (int j = threadIdx.x & 31; j < pages_of(len); j += 32) {
                         int id = src[j];
                         if ((j + 1) * kPage > len) {              // not full: a page of its own
                             const int m = s.before[r], own = b.free_ids[b.n_packed + n_free - 1 - m];
-                            moves[4 + 2 * m] = id;
-                            moves[5 + 2 * m] = own;
-                            b.refs[b.n_packed + own] = 1;
+                            const bool both = inside(id, b.n_fp16) && inside(own, b.n_fp16);        // else page 0 onto itself
+                            moves[4 + 2 * m] = both ? id : 0;
+                            moves[5 + 2 * m] = both ? own : 0;
+                            if (inside(own, b.n_fp16)) b.refs[b.n_packed + own] = 1;
                             id = own;
-                        } else if (id >= 0 && id < (j < packed ? b.n_packed : b.n_fp16)) {
+                        } else if (inside(id, j < packed ? b.n_packed : b.n_fp16)) {
                             atomicAdd(b.refs + (j < packed ? id : b.n_packed + id), 1);
                         }
                         dst[j] = id;
@@ -336,7 +344,7 @@ __global__ void __launch_bounds__(kBookThreads) pages_compact_kernel(kvq_page_bo
     const int live16 = close_up(s, b.refs + b.n_packed, b.free_ids + b.n_packed, b.n_fp16, &b.count[1], moves16, to + b.n_packed);
     for (int row = threadIdx.x >> 5; row < b.slots; row += kBookThreads / 32) {
         int32_t *t = b.table + (int64_t)row * b.max_pages;
-        const int packed = b.packed[row], held = min(pages_of(b.length[row]), b.max_pages);
+        const int packed = b.packed[row], held = pages_of(length_of(b, row));
         for (int j = threadIdx.x & 31; j < held; j += 32) {
             const int id = t[j];
             if (j < packed ? id >= live && id < b.n_packed : id >= live16 && id < b.n_fp16) t[j] = to[j < packed ? id : b.n_packed + id];
@@ -367,7 +375,7 @@ __global__ void __launch_bounds__(256) page_write_kernel(const kvq_page_book b, 
     }
     const int s = sequence_of(a.q_start, a.n, u), row = a.rows[s];
     if (row < 0 || row >= b.slots) return;
-    const int pos = b.length[row] - a.q_start[s + 1] + u, page = pos / kPage;
+    const int pos = length_of(b, row) - max(a.q_start[s + 1], 0) + u, page = pos / kPage;
     if (pos < 0 || page >= b.max_pages || page < b.packed[row]) return;
     const int id = b.table[(int64_t)row * b.max_pages + page];
     if (id < 0 || id >= min(l.n_fp16, b.n_fp16) || b.refs[b.n_packed + id] > 1) return;      // a page that others hold too stays as it is

@@ -262,3 +262,60 @@ def test_shared_pages_are_never_written(cuda):
     kv.page_write(x, y, ints(0, 320), ints(1), cache.book, cache.layers[0])
     assert torch.equal(cache.layers[0].kfull[ids[0]], x[:P].transpose(0, 1))
     cache.check()
+
+
+# ---- bookkeeping that holds wrong numbers ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("what", ["length", "packed", "free_ids", "count", "table", "refs"])
+@pytest.mark.parametrize("value", [-1, -2 ** 31, -2 ** 30, 2 ** 31 - 1, 2 ** 30, 5000])
+def test_wrong_numbers_in_the_bookkeeping_stay_inside(cuda, what, value):
+    """Bookkeeping that was never set up, or written over: every call ends without touching anything outside the tensors (they lie in one block, with
+    guards between them)."""
+    sizes = dict(table=(4, 4), length=(4,), packed=(4,), refs=(9,), free_ids=(9,), count=(4,))
+    block = torch.full((4096,), 77, dtype=torch.int32, device="cuda")
+    parts, at = {}, 256
+    for name, shape in sizes.items():
+        n = math.prod(shape)
+        parts[name] = block[at:at + n].view(shape)
+        at += n + 256
+    outside = torch.ones_like(block, dtype=torch.bool)
+    for t in parts.values():
+        start = (t.data_ptr() - block.data_ptr()) // 4
+        outside[start:start + t.numel()] = False
+    cache = kv.KVmixPagedCache([(4, 2)], 1, 128, 4, 512, 4, 5, 64, 0)
+    for call in range(8):
+        for name, t in parts.items():
+            t.copy_(getattr(cache.book, name))
+        book = kv.PageBook(**parts, n_packed=4)
+        kv.pages_extend(ints(0, 1), ints(300, 10), book)
+        kv.pages_settle(ints(0), 130, book, cache.layers)
+        assert int(book.count[2]) == 0
+        if what == "count":
+            book.count[:2] = value
+        else:
+            parts[what].fill_(value)
+        x = torch.zeros(9, 1, 128, device="cuda").half()
+        (lambda: kv.pages_extend(ints(0, 1, 2), ints(100, 0, 1), book), lambda: kv.pages_free(ints(0, 2), book), lambda: kv.pages_settle(ints(0, 1), 0, book, cache.layers),
+         lambda: kv.pages_fork(ints(0, 1), ints(2, 3), book, cache.layers), lambda: kv.pages_compact(book, cache.layers),
+         lambda: kv.page_write(x, x, ints(0, 9), ints(0), book, cache.layers[0]), lambda: kv.paged_attention(queries(9, 4), ints(0, 9), ints(0), book, cache.layers[0]),
+         lambda: kv.paged_attention(queries(1, 4), ints(0, 1), ints(0), book, cache.layers[0]))[call]()
+        torch.cuda.synchronize()
+        assert (block[outside] == 77).all()
+
+
+@pytest.mark.parametrize("bad", [[0, -2 ** 31, 9], [5, -2 ** 31, 9], [2 ** 31 - 1, 9, 9], [0, 2 ** 31 - 1, 2 ** 31 - 1], [-2 ** 31, 3, 9], [9, 4, 0], [-5, 100, 3]])
+def test_wrong_numbers_of_new_tokens_stay_inside(cuda, bad):
+    """q_start that does not ascend, or leads outside q: nothing outside out is written, no page but the sequences' own."""
+    cache = small()
+    block = torch.full((40, 4, 128), 7.0, dtype=torch.half, device="cuda")
+    x = torch.zeros(9, 1, 128, device="cuda").half()
+    own = cache.book.table[[0, 2]].flatten().tolist()
+    for tokens, hints in ((9, {}), (9, dict(max_new=1)), (9, dict(max_new=5, max_chunks=1))):
+        kv.paged_attention(queries(tokens, 4), ints(*bad), ints(0, 2), cache.book, cache.layers[0], out=block[16:16 + tokens], **hints)
+        torch.cuda.synchronize()
+        assert (block[:16] == 7).all() and (block[16 + tokens:] == 7).all()
+    others = [p for p in range(6) if p not in own]
+    before = cache.layers[0].kfull[others].clone()
+    kv.page_write(x, x, ints(*bad), ints(0, 2), cache.book, cache.layers[0])
+    assert torch.equal(cache.layers[0].kfull[others].view(torch.int16), before.view(torch.int16))
+    cache.check()
