@@ -411,6 +411,8 @@ class KVmixPagedCache:
                          sum(c > 1 for c in counts))
 
     def write(self, layer, k, v, step):
+        if k.shape[0] != step.tokens or v.shape[0] != step.tokens:
+            raise RuntimeError("keys and values for every new token of the step")
         page_write(k, v, step.q_start, step.rows, self.book, self.layers[layer])
 
     def attend(self, layer, q, step, **options):

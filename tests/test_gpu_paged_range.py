@@ -239,6 +239,18 @@ def test_misaligned_pages_are_refused_at_once(cuda, name):
     cache.check()
 
 
+def test_a_step_takes_its_own_tokens(cuda):
+    cache = small()
+    s = cache.extend([0], [3])
+    x = torch.zeros(4, 1, 128, device="cuda").half()
+    before = snapshot(cache)
+    for k, v in ((x[:2], x[:2]), (x, x), (x[:3], x)):
+        with pytest.raises(RuntimeError):
+            cache.write(0, k, v, s)
+    unchanged(cache, before)
+    cache.write(0, x[:3], x[:3], s)
+
+
 # ---- shared pages ----------------------------------------------------------------------------------------------------------------------
 
 def test_shared_pages_are_never_written(cuda):
