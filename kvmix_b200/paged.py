@@ -152,6 +152,12 @@ def _rows(dev, name, rows):
     return _ints(dev, name, rows, rows.numel())
 
 
+def _rows_apart(out):
+    """Whether no two of the rows [tokens, heads] of 128 channels share an element (as no layout of one axis inside the other has it)."""
+    (inner, n), (outer, m) = sorted((stride, size) for stride, size in zip(out.stride()[:2], out.shape[:2]))
+    return (n <= 1 or inner >= 128) and (m <= 1 or outer >= (128 if n <= 1 else inner * (n - 1) + 128))
+
+
 def _on_its_device(where):
     """Kernels are launched on the current stream of the tensors' device, whichever is current.  `where`: place of `pages` among the arguments."""
     def wrap(f):
@@ -295,6 +301,8 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
         out = q.new_empty((tokens, nh, 128))
     elif out.shape != q.shape or out.dtype is not _f16 or out.get_device() != dev or out.stride(2) != 1:
         raise RuntimeError("out must be fp16 like q, contiguous along the channels")
+    elif not _rows_apart(out):
+        raise RuntimeError("rows of out must not lie over one another")
     window, softcap = window or 0, softcap or 0.0
     if window < 0 or not softcap >= 0.0:
         raise RuntimeError("window and softcap must not be negative")

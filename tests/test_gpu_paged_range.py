@@ -239,6 +239,20 @@ def test_misaligned_pages_are_refused_at_once(cuda, name):
     cache.check()
 
 
+def test_outputs_that_lie_over_one_another(cuda):
+    c = Cache([300], [1], 1, 4, 4, 64, seed=8)
+    one = torch.zeros(1, 1, 128, dtype=torch.half, device="cuda")
+    flat = torch.zeros(4000, dtype=torch.half, device="cuda")
+    for out in (one.expand(2, 4, 128), torch.zeros(2, 1, 128, dtype=torch.half, device="cuda").expand(2, 4, 128), flat.as_strided((2, 4, 128), (256, 128, 1)),
+                flat.as_strided((2, 4, 128), (1024, 64, 1)), flat.as_strided((2, 4, 128), (128, 200, 1))):
+        with pytest.raises(RuntimeError, match="out"):
+            attend(c, queries(2, 4), [2], out=out)
+    want = attend(c, queries(2, 4), [2])
+    for out in (flat.as_strided((2, 4, 128), (128, 256, 1)), flat.as_strided((2, 4, 128), (600, 130, 1)), torch.zeros(2, 4, 128, dtype=torch.half, device="cuda")):
+        assert torch.equal(attend(c, queries(2, 4), [2], out=out), want)
+    assert attend(c, queries(1, 4), [1], out=flat.as_strided((1, 4, 128), (0, 128, 1))).any()
+
+
 def test_a_step_takes_its_own_tokens(cuda):
     cache = small()
     s = cache.extend([0], [3])
