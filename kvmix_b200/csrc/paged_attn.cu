@@ -37,6 +37,8 @@ static int paged_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
 __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant__ PagedArgs p, int few) {
     const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
+    const int64_t step = p.part_rows;
+    int64_t row;
     int u, h;
     if (few) {
         const int r = (int)(at % kFewRows), head = (int)(at / kFewRows % p.l.Hkv);
@@ -46,17 +48,18 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
         if (s.n_new * p.rep > kFewRows || r >= s.n_new * p.rep) return;
         u = s.q0 + r / p.rep;
         h = head * p.rep + r % p.rep;
+        row = p.part_compact ? at : (int64_t)u * p.a.nh + h;
     } else {
         const int64_t q = at / p.a.nh;
         if (q >= p.a.tokens || q < p.a.q_start[0] || q >= p.a.q_start[p.a.n]) return;
         u = (int)q;
         h = (int)(at - q * p.a.nh);
+        row = at;
         if (p.few_rows) {
             const PagedSeq s = paged_seq(p, sequence_of(p.a.q_start, p.a.n, u));
             if (s.n_new * p.rep <= p.few_rows) return;
         }
     }
-    const int64_t step = (int64_t)p.a.tokens * p.a.nh, row = (int64_t)u * p.a.nh + h;
     float m = -INFINITY, l = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i = lane; i < p.splits; i += 32) m = fmaxf(m, p.part_ml[2 * (i * step + row)]);
@@ -137,9 +140,19 @@ static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, 
     return r;
 }
 
-static uint64_t paged_bytes(const PagedPlan &r, int tokens, int nh) {
-    const int splits = (r.few && r.few_splits > 1) || (r.tiles && r.tile_splits > 1) ? (r.few && r.few_splits > r.tile_splits ? r.few_splits : r.tiles ? r.tile_splits : r.few_splits) : 0;
-    return (uint64_t)splits * tokens * nh * (kHeadDim + 2) * 4;
+// Partial sums of the kernel of few rows lie by rows of q, and beside chunks by kFewRows places of every (sequence, kv head) where those are fewer: a place in
+// every split for the rows of a chunk of 32768 tokens of 32 heads beside a token with 13 splits took 7 GB.
+static bool few_compact(const PagedPlan &r, int n, int Hkv, int tokens, int nh) {
+    return r.tiles && (int64_t)n * Hkv * kFewRows < (int64_t)tokens * nh;
+}
+static int64_t few_part_rows(const PagedPlan &r, int n, int Hkv, int tokens, int nh) {
+    return few_compact(r, n, Hkv, tokens, nh) ? (int64_t)n * Hkv * kFewRows : (int64_t)tokens * nh;
+}
+// Both kernels' partial sums, one after the other in the same place; in whole splits of all rows of q, two at least.
+static uint64_t paged_bytes(const PagedPlan &r, int n, int Hkv, int tokens, int nh) {
+    const int64_t all = (int64_t)tokens * nh, few = r.few && r.few_splits > 1 ? r.few_splits * few_part_rows(r, n, Hkv, tokens, nh) : 0,
+                  tiles = r.tiles && r.tile_splits > 1 ? r.tile_splits * all : 0, most = few > tiles ? few : tiles, units = (most + all - 1) / all;
+    return (uint64_t)(most == 0 ? 0 : units < 2 ? 2 : units) * all * (kHeadDim + 2) * 4;
 }
 
 }  // namespace kvq
@@ -148,7 +161,7 @@ extern "C" uint64_t kvq_paged_attn_workspace_bytes(const kvq_page_layer *l, int3
                                                    int32_t max_chunks) {
     using namespace kvq;
     if (check_layer(l) || n <= 0 || tokens <= 0 || nh <= 0 || nh % l->Hkv || max_new <= 0 || max_tokens <= 0 || max_chunks < 0) return 0;
-    return paged_bytes(paged_plan(*l, n, tokens, nh, max_new, max_tokens, max_chunks), tokens, nh);
+    return paged_bytes(paged_plan(*l, n, tokens, nh, max_new, max_tokens, max_chunks), n, l->Hkv, tokens, nh);
 }
 
 extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, const kvq_paged_attn_args *a, kvq_stream_t stream) {
@@ -163,7 +176,7 @@ extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, c
     if (!a->q || !a->out || !a->q_start || !a->rows) return KVQ_ERR_NULL;
     if (!(a->softcap >= 0.f) || !(fabsf(a->softmax_scale) <= FLT_MAX)) return KVQ_ERR_SHAPE;
     const PagedPlan r = paged_plan(*l, a->n, a->tokens, a->nh, a->max_new, a->max_tokens, a->max_chunks);
-    const uint64_t need = paged_bytes(r, a->tokens, a->nh);
+    const uint64_t need = paged_bytes(r, a->n, l->Hkv, a->tokens, a->nh);
     if (need && (!a->workspace || a->workspace_bytes < need)) return KVQ_ERR_WORKSPACE;
     if (need && reinterpret_cast<uintptr_t>(a->workspace) % 16) return KVQ_ERR_ALIGN;
     PagedArgs p = {};
@@ -182,17 +195,20 @@ extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, c
         p.cap_in = fminf(fmaxf(a->softmax_scale / p.a.softcap, -1e30f), 1e30f);
     }
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const int most = r.few && r.few_splits > r.tile_splits ? r.few_splits : r.tiles ? r.tile_splits : r.few_splits;
     p.part_out = static_cast<float *>(a->workspace);
-    p.part_ml = need ? p.part_out + (uint64_t)most * a->tokens * a->nh * kHeadDim : nullptr;
     if (r.few) {
         p.splits = r.few_splits;
+        p.part_rows = few_part_rows(r, a->n, l->Hkv, a->tokens, a->nh);
+        p.part_compact = few_compact(r, a->n, l->Hkv, a->tokens, a->nh);
+        p.part_ml = p.part_out + p.splits * p.part_rows * kHeadDim;
         if (const int rc = paged_few(p, st)) return rc;
         if (p.splits > 1)
             if (const int rc = paged_merge(p, 1, st)) return rc;
     }
     if (r.tiles) {
         p.splits = r.tile_splits;
+        p.part_rows = (int64_t)a->tokens * a->nh;
+        p.part_ml = p.part_out + p.splits * p.part_rows * kHeadDim;
         if (const int rc = paged_tiles(p, r.max_tiles, st)) return rc;
         if (p.splits > 1)
             if (const int rc = paged_merge(p, 0, st)) return rc;

@@ -19,8 +19,10 @@ struct PagedArgs {
     int rep, k_groups, v_groups;      // query heads of a kv head; groups of a page's row
     int splits, few_rows;             // few_rows: sequences with at most so many rows are the other kernel's
     float cap_in;                     // softmax_scale / softcap
-    float *part_out;                  // [splits][tokens * nh][128], unnormalised
-    float *part_ml;                   // [splits][tokens * nh][2]: the exponents' reference (log2), the weights' sum
+    int64_t part_rows;                // rows of a split's partial sums: those of q, or kFewRows of every (sequence, kv head)
+    bool part_compact;                // the latter
+    float *part_out;                  // [splits][part_rows][128], unnormalised
+    float *part_ml;                   // [splits][part_rows][2]: the exponents' reference (log2), the weights' sum
 };
 
 // Sequence i as every thread sees it: its row of the table, length, packed pages, where its new tokens are.  Numbers that would lead

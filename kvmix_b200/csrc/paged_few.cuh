@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
         if (p.splits == 1) {
             static_cast<__half *>(p.a.out)[(int64_t)u * p.a.o_sT + (int64_t)h * p.a.o_sH + threadIdx.x] = __float2half_rn(l == 0.f ? 0.f : v / l);
         } else {
-            const int64_t at = (int64_t)split * p.a.tokens * p.a.nh + (int64_t)u * p.a.nh + h;
+            const int64_t at = (int64_t)split * p.part_rows + (p.part_compact ? ((int64_t)i * p.l.Hkv + head) * kFewRows + row0 + r : (int64_t)u * p.a.nh + h);
             p.part_out[at * 128 + threadIdx.x] = v;
             if (threadIdx.x == 0) { p.part_ml[2 * at] = m; p.part_ml[2 * at + 1] = l; }
         }

@@ -345,3 +345,16 @@ def test_wrong_numbers_of_new_tokens_stay_inside(cuda, bad):
     kv.page_write(x, x, ints(*bad), ints(0, 2), cache.book, cache.layers[0])
     assert torch.equal(cache.layers[0].kfull[others].view(torch.int16), before.view(torch.int16))
     cache.check()
+
+
+# ---- long sequences, packing under replay ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kb,vb,group", [(2, 2, 64), (3, 3, 128), (4, 4, 32)])
+@pytest.mark.parametrize("counts", [[1, 300, 1, 2], [40, 1, 1, 0], [1, 1, 700, 1]])
+def test_split_single_tokens_beside_chunks(cuda, kb, vb, group, counts):
+    """Single tokens over a long context, in splits, in one call with chunks: each kernel finds its own partial sums."""
+    c = Cache([9000, 4100, 2000, 300], [68, 20, 10, 0], 2, kb, vb, group, seed=kb)
+    q = queries(sum(counts), 8)
+    want, slack = attention(c, q, counts, False)
+    for hints in ({}, dict(max_new=max(counts), max_chunks=2, max_tokens=9000)):
+        holds(attend(c, q, counts, **hints), want, slack)

@@ -111,3 +111,15 @@ def test_scales_and_caps_that_are_no_numbers():
     L = paged._library()
     for bad in (dict(softmax_scale=float("inf")), dict(softmax_scale=-float("inf")), dict(softcap=-float("inf"))):
         assert L.kvq_paged_attn(book(), layer(), attn(**bad), None) == -7
+
+
+def test_workspace_of_a_long_chunk_beside_single_tokens():
+    """Partial sums of single tokens over a long context do not take a place for every row of the chunk beside them in each of their splits."""
+    L = paged._library()
+    for bits in ((2, 2), (3, 2), (4, 4)):
+        for n, tokens, max_new in ((2, 1025, 1024), (2, 8193, 8192), (2, 32769, 32768), (5, 65540, 65536), (30, 20030, 20001)):
+            for chunks in (1, n):
+                b = L.kvq_paged_attn_workspace_bytes(layer(Hkv=8, k_bits=bits[0], v_bits=bits[1]), n, tokens, 32, max_new, 131072, chunks)
+                assert b <= 2 * tokens * 32 * 520, (n, tokens, b)
+    # without a chunk the splits are as many as they pay
+    assert L.kvq_paged_attn_workspace_bytes(layer(Hkv=8), 1, 1, 32, 1, 131072, 1) >= 20 * 32 * 520
