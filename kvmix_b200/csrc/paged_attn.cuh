@@ -41,7 +41,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs &p, int i) {
     const bool ok = s.row >= 0 && s.row < p.b.slots;
     const int row = ok ? s.row : 0;
     s.length = ok ? min(max(p.b.length[row], 0), p.b.max_pages * kPage) : 0;
-    s.packed = ok ? max(p.b.packed[row], 0) : 0;
+    s.packed = ok ? p.b.packed[row] : 0;
     s.table = p.b.table + (int64_t)row * p.b.max_pages;
     new_tokens(p, i, s.q0, s.n_new);
     s.prefix = p.a.prefix ? p.a.prefix[i] : 0;

@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             uint32_t lead;
             asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
             auto same = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
-            const int n_old = same(s.packed - p0), pages = same(np), tiles = same(two_tiles) ? 2 : 1;            // n_old: pages of packed keys
+            const int n_old = same(max(s.packed, 0) - p0), pages = same(np), tiles = same(two_tiles) ? 2 : 1;            // n_old: pages of packed keys
             const uint32_t tm = (uint32_t)same((int)tmem);
             const uint64_t q_desc = tc_desc(base + kOffQ, 16, 1024), k_desc = tc_desc(base + kOffK, 16, 1024), k_mn = tc_desc(base + kOffK, kOperandHalf, 1024),
                            v_desc = tc_desc(base + kOffV, kOperandHalf, 1024);
