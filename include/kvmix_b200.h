@@ -481,6 +481,7 @@ int kvq_decode_attn_static(const kvq_attn_args *a, kvq_stream_t stream);
  * _settle) and of page numbers (pages that come free), so that equal calls give equal numbers.
  */
 #define KVQ_PAGE_TOKENS 128
+extern uint32_t kvq_paged_launch_count;         /* kernels of the paged cache launched by this process so far; a call launches none to four */
 #define KVQ_PAGES_NO_FP16 1     /* fewer free fp16 pages than asked for                                    */
 #define KVQ_PAGES_NO_PACKED 2   /* fewer free packed pages than asked for                                  */
 #define KVQ_PAGES_TOO_LONG 4    /* a sequence would need more than max_pages                               */

@@ -12,7 +12,15 @@ int record_cuda_error(cudaError_t e) {
     g_cuda_error[sizeof(g_cuda_error) - 1] = 0;
     return KVQ_ERR_CUDA;
 }
+
+int count_launch() {
+    const int rc = check_launch();
+    if (rc == KVQ_OK) __atomic_fetch_add(&kvq_paged_launch_count, 1u, __ATOMIC_RELAXED);
+    return rc;
+}
 }  // namespace kvq
+
+extern "C" { uint32_t kvq_paged_launch_count = 0; }
 
 extern "C" int kvq_version(void) { return 107; }   // 105: fused decode step, device-resident state, head-sharded exchange, kvq_prefill, kvq_attn_plan; 106: 3-bit values (ragged_tail); 107: paged cache
 

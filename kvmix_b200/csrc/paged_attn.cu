@@ -91,7 +91,7 @@ static int paged_merge(const PagedArgs &p, int few, cudaStream_t st) {
     const int64_t rows = few ? (int64_t)p.a.n * p.l.Hkv * kFewRows : (int64_t)p.a.tokens * p.a.nh, grid = (rows + 7) / 8;
     if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
     paged_merge_kernel<<<(unsigned)grid, 256, 0, st>>>(p, few);
-    return check_launch();
+    return count_launch();
 }
 
 // How a call is cut.  Either kernel may cut the pages of a sequence into splits, whose partial sums meet in a second launch.

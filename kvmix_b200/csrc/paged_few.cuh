@@ -697,7 +697,7 @@ static int launch_few(const PagedArgs &p, int R, int row_blocks, cudaStream_t st
     const int64_t grid = (int64_t)p.a.n * p.l.Hkv * row_blocks * p.splits;
     if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
     paged_few_kernel<KB, VB, CK><<<(unsigned)grid, kFewWarps * 32, smem, st>>>(p, R, row_blocks, stages, stage_rows, stage_bytes);
-    return check_launch();
+    return count_launch();
 }
 
 template <int KB, int VB>

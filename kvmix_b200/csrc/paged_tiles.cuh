@@ -636,7 +636,7 @@ static int launch_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
     const int64_t rows = (int64_t)p.l.n_fp16 * p.l.Hkv * kPage;
     maps.there = page_map(&maps.k, p.l.kfull, rows) && page_map(&maps.v, p.l.vfull, rows);
     paged_tile_kernel<KB, VB, MODS><<<(unsigned)grid, kTileThreads, kTileSmem, st>>>(p, maps, max_tiles);
-    return check_launch();
+    return count_launch();
 }
 
 template <int KB>

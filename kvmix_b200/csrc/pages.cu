@@ -569,7 +569,7 @@ extern "C" int kvq_pages_extend(const kvq_page_book *b, const int32_t *rows, con
     if (!rows || !counts) return KVQ_ERR_NULL;
     if (const int rc = book_smem(pages_extend_kernel, seen_bytes(*b))) return rc;
     pages_extend_kernel<<<1, kBookThreads, seen_bytes(*b), reinterpret_cast<cudaStream_t>(stream)>>>(*b, rows, counts, n);
-    return check_launch();
+    return count_launch();
 }
 
 extern "C" int kvq_pages_free(const kvq_page_book *b, const int32_t *rows, int32_t n, kvq_stream_t stream) {
@@ -580,7 +580,7 @@ extern "C" int kvq_pages_free(const kvq_page_book *b, const int32_t *rows, int32
     if (!rows) return KVQ_ERR_NULL;
     if (const int rc = book_smem(pages_free_kernel, seen_bytes(*b))) return rc;
     pages_free_kernel<<<1, kBookThreads, seen_bytes(*b), reinterpret_cast<cudaStream_t>(stream)>>>(*b, rows, n);
-    return check_launch();
+    return count_launch();
 }
 
 extern "C" int kvq_pages_settle(const kvq_page_book *b, const int32_t *rows, int32_t n, int32_t window, int32_t *moves, kvq_stream_t stream) {
@@ -590,7 +590,7 @@ extern "C" int kvq_pages_settle(const kvq_page_book *b, const int32_t *rows, int
     if (!moves || (n && !rows)) return KVQ_ERR_NULL;
     if (const int rc = book_smem(pages_settle_kernel, seen_bytes(*b))) return rc;
     pages_settle_kernel<<<1, kBookThreads, seen_bytes(*b), reinterpret_cast<cudaStream_t>(stream)>>>(*b, rows, n, window, moves);
-    return check_launch();
+    return count_launch();
 }
 
 extern "C" int kvq_pages_fork(const kvq_page_book *b, const int32_t *parents, const int32_t *children, int32_t n, int32_t *moves, kvq_stream_t stream) {
@@ -600,7 +600,7 @@ extern "C" int kvq_pages_fork(const kvq_page_book *b, const int32_t *parents, co
     if (!moves || (n && (!parents || !children))) return KVQ_ERR_NULL;
     if (const int rc = book_smem(pages_fork_kernel, seen_bytes(*b))) return rc;
     pages_fork_kernel<<<1, kBookThreads, seen_bytes(*b), reinterpret_cast<cudaStream_t>(stream)>>>(*b, parents, children, n, moves);
-    return check_launch();
+    return count_launch();
 }
 
 extern "C" int kvq_pages_compact(const kvq_page_book *b, int32_t *moves, kvq_stream_t stream) {
@@ -608,7 +608,7 @@ extern "C" int kvq_pages_compact(const kvq_page_book *b, int32_t *moves, kvq_str
     if (const int rc = check_book(b)) return rc;
     if (!moves) return KVQ_ERR_NULL;
     pages_compact_kernel<<<1, kBookThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(*b, moves);
-    return check_launch();
+    return count_launch();
 }
 
 extern "C" int kvq_page_pack(const kvq_page_layer *l, const int32_t *moves, int32_t max_moves, kvq_stream_t stream) {
@@ -625,7 +625,7 @@ extern "C" int kvq_page_pack(const kvq_page_layer *l, const int32_t *moves, int3
         case 3: launch_pack<3>(*l, moves, max_moves, grid, st); break;
         default: launch_pack<4>(*l, moves, max_moves, grid, st); break;
     }
-    return check_launch();
+    return count_launch();
 }
 
 extern "C" int kvq_page_copy(const kvq_page_tensor *tensors, int32_t n, const int32_t *moves, int32_t max_moves, kvq_stream_t stream) {
@@ -644,7 +644,7 @@ extern "C" int kvq_page_copy(const kvq_page_tensor *tensors, int32_t n, const in
     if (!p.n || max_moves <= 0) return KVQ_OK;
     const int64_t units = (int64_t)max_moves * p.first[p.n];
     page_copy_kernel<<<(unsigned)(units < 148 * 8 ? units : 148 * 8), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p, moves, max_moves);
-    return check_launch();
+    return count_launch();
 }
 
 extern "C" int kvq_page_write(const kvq_page_book *b, const kvq_page_layer *l, const kvq_page_write_args *a, kvq_stream_t stream) {
@@ -660,5 +660,5 @@ extern "C" int kvq_page_write(const kvq_page_book *b, const kvq_page_layer *l, c
     const int64_t ctas = ((int64_t)a->tokens * l->Hkv * 16 + 255) / 256;
     if (ctas > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
     (vec ? page_write_kernel<true> : page_write_kernel<false>)<<<(unsigned)ctas, 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(*b, *l, *a);
-    return check_launch();
+    return count_launch();
 }

@@ -7,6 +7,8 @@ namespace kvq {
 constexpr int kPage = KVQ_PAGE_TOKENS;
 constexpr int kPageHalf = kPage * kHeadDim;                       // elements of one head's keys (or values) of a page
 
+int count_launch();                                               // check_launch() of a kernel of the paged cache (api.cu)
+
 __host__ __device__ constexpr int page_words(int bits) { return bits == 3 ? 12 : 4 * bits; }               // per 128 elements
 __host__ __device__ constexpr int page_groups(int bits, int group) { return bits == 3 ? 12 : 128 / group; }
 

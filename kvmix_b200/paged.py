@@ -86,6 +86,12 @@ def _library():
     return _lib.lib()
 
 
+@functools.lru_cache(maxsize=None)
+def _launch_count():
+    """(the library's count of launches, what ops.LAUNCHES has of it)"""
+    return C.c_uint32.in_dll(_library(), "kvq_paged_launch_count"), [0]
+
+
 _i32, _f16 = torch.int32, torch.float16
 
 
@@ -172,10 +178,13 @@ def _on_its_device(where):
     return wrap
 
 
-def _launched(rc, n=1):
+def _launched(rc):
     if rc:
         check(rc)
-    ops.LAUNCHES[0] += n
+    count, seen = _launch_count()
+    now = count.value
+    ops.LAUNCHES[0] += (now - seen[0]) & 0xffffffff
+    seen[0] = now
 
 
 def _copy(tensors, moves, max_moves):

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import kvmix_b200 as kv
+from kvmix_b200 import ops
 from test_gpu_paged import P, Cache, attend, queries
 from test_gpu_paged_book import ints, small, snapshot, unchanged
 
@@ -287,6 +288,33 @@ def test_shared_pages_are_never_written(cuda):
     cache.free([0])                                                                   # nobody else holds them now
     kv.page_write(x, y, ints(0, 320), ints(1), cache.book, cache.layers[0])
     assert torch.equal(cache.layers[0].kfull[ids[0]], x[:P].transpose(0, 1))
+    cache.check()
+
+
+# ---- launches --------------------------------------------------------------------------------------------------------------------------
+
+def test_launches_are_counted_as_they_are(cuda):
+    cache = kv.KVmixPagedCache([(2, 2)] * 3, 1, 128, 4, 9000, 140, 150, 64, 128)
+    x = torch.zeros(8200, 1, 128, device="cuda").half()
+
+    def launches(f, *args, **kw):
+        n = ops.LAUNCHES[0]
+        f(*args, **kw)
+        return ops.LAUNCHES[0] - n
+    b, l = cache.book, cache.layers[0]
+    assert launches(kv.pages_extend, ints(0, 1, 2), ints(8192, 5, 3), b) == 1
+    assert launches(kv.pages_extend, ints(), ints(), b) == 0
+    assert launches(kv.page_write, x[:8200], x[:8200], ints(0, 8192, 8197, 8200), ints(0, 1, 2), b, l) == 1
+    assert launches(kv.pages_settle, ints(0, 1, 2), 128, b, cache.layers) == 4
+    q = queries(9, 4)
+    assert launches(kv.paged_attention, q[:1], ints(0, 1), ints(1), b, l, max_tokens=128) == 1               # whole
+    assert launches(kv.paged_attention, q[:1], ints(0, 1), ints(0), b, l) == 2                                # splits and their join
+    assert launches(kv.paged_attention, q[:9], ints(0, 3, 8, 9), ints(2, 1, 0), b, l, max_new=5, max_tokens=128) == 2      # both kernels
+    assert launches(kv.paged_attention, q[:9], ints(0, 3, 8, 9), ints(2, 1, 0), b, l, max_new=5) == 4
+    assert launches(kv.paged_attention, q[:0], ints(0, 0), ints(0), b, l) == 0
+    assert launches(kv.pages_fork, ints(1), ints(3), b, cache.layers) == 2
+    assert launches(kv.pages_compact, b, cache.layers) == 3
+    assert launches(kv.pages_free, ints(3), b) == 1
     cache.check()
 
 
