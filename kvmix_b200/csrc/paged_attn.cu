@@ -116,7 +116,7 @@ static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, 
     const int64_t pairs = (int64_t)n * l.Hkv * f.row_blocks, slots = 148 * f.ctas;
     double best = 1e30;
     r.few_splits = 1;
-    for (int s = 1; s <= 128 && (s == 1 || s <= pages / 2); ++s) {
+    for (int s = 1; r.few && s <= 128 && (s == 1 || s <= pages / 2); ++s) {
         const double w = (double)(pairs * s) / slots, waves = w <= 1 ? 1 : w < 4 ? (double)((pairs * s + slots - 1) / slots) : w + 0.5;
         const int rounds = ((pages + s - 1) / s + 3) / 4;
         const double cost = waves * (rounds + 2) + (s > 1 ? 2 : 0);
@@ -131,7 +131,7 @@ static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, 
     const int64_t ctas = tiles * l.Hkv;
     best = 1e30;
     r.tile_splits = 1;
-    for (int s = 1; s <= 64 && (s == 1 || s <= pages / 4); ++s) {
+    for (int s = 1; r.tiles && s <= 64 && (s == 1 || s <= pages / 4); ++s) {
         const int64_t waves = (ctas * s + 147) / 148;
         const double joined = s > 1 ? 1.5 + (double)s * tokens * nh * 1040 / 5e6 / 1.8 : 0;
         const double cost = (double)waves * ((pages + s - 1) / s + 4) + joined;

@@ -28,6 +28,7 @@ from . import _lib, ops
 from ._lib import check
 
 PAGE_TOKENS = 128
+_SCALE = 1.0 / math.sqrt(128)
 _MOST = 1 << 30                  # no sequence is longer: wider windows are this one
 _MOST_HEADS = 1 << 15            # what kvq_page_copy takes as one page: 1 GB
 _STATUS = {1: "no free fp16 page", 2: "no free packed page", 4: "sequence longer than the table", 8: "bad rows (outside the table, named twice, "
@@ -35,6 +36,7 @@ _STATUS = {1: "no free fp16 page", 2: "no free packed page", 4: "sequence longer
 
 _pack_book, _pack_layer = struct.Struct("@6P4i").pack, struct.Struct("@8P6i").pack
 _pack_write, _pack_attn = struct.Struct("@2P4q2P2i").pack, struct.Struct("@2P4q5P8i2fPQ").pack
+_addresses = struct.Struct("@8P").unpack_from             # of a layer's argument block
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
@@ -120,17 +122,24 @@ def _book(pages):
 def _page_tensor(dev, t, dtype, shape):
     # the address is asked for in the same breath: a layer has eight such tensors, a call of many layers hundreds
     if t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous():
-        at = t.data_ptr()
-        if not at & 15:                               # here and not by the copies, which come behind bookkeeping that cannot be taken back
-            return at
-    raise RuntimeError(f"page tensor {tuple(t.shape)} {t.dtype} on {t.device}: contiguous {dtype} {shape} on cuda:{dev} at a multiple of 16 bytes expected")
+        return t.data_ptr()
+    raise RuntimeError(f"page tensor {tuple(t.shape)} {t.dtype} on {t.device}: contiguous {dtype} {shape} on cuda:{dev} expected")
+
+
+def _movable(layers, addresses):
+    """What kvq_page_copy and kvq_page_pack would refuse, before the bookkeeping that they come behind and that cannot be taken back."""
+    low = 0
+    for at in addresses:
+        low |= at
+    if low & 15:
+        check(-13)
+    if any(layer.kfull.shape[1] > _MOST_HEADS for layer in layers):
+        raise RuntimeError(f"pages hold at most {_MOST_HEADS} kv heads")
 
 
 def _fp16_pages(pages, dev, layer):
     """Addresses of a layer's fp16 pages."""
     kfull, vfull = layer.kfull, layer.vfull
-    if kfull.shape[1] > _MOST_HEADS:
-        raise RuntimeError(f"pages hold at most {_MOST_HEADS} kv heads")
     shape = (pages.refs.numel() - pages.n_packed, kfull.shape[1], PAGE_TOKENS, 128)
     return _page_tensor(dev, kfull, _f16, shape), _page_tensor(dev, vfull, _f16, shape)
 
@@ -143,8 +152,6 @@ def _layer(pages, dev, layer):
     if group not in (32, 64, 128):
         raise RuntimeError("pages are quantized in groups of 32, 64 or 128")
     n, heads = pages.n_packed, kfull.shape[1]
-    if heads > _MOST_HEADS:
-        raise RuntimeError(f"pages hold at most {_MOST_HEADS} kv heads")
     n16 = pages.refs.numel() - n
     kw, vw, kg, vg = (n, heads, PAGE_TOKENS, page_words(kb)), (n, heads, PAGE_TOKENS, page_words(vb)), (n, heads, PAGE_TOKENS, page_groups(kb, group)), \
         (n, heads, PAGE_TOKENS, page_groups(vb, group))
@@ -238,6 +245,8 @@ def pages_settle(rows, window, pages, layers):
         raise RuntimeError("window must not be negative")
     moves = pages.count.new_empty(4 + 2 * pages.n_packed)
     blocks, n = [_layer(pages, dev, layer) for layer in layers], rows.numel()
+    for block in blocks:
+        _movable((), _addresses(block))
     L, st, at = _library(), ops.raw_stream(), moves.data_ptr()
     _launched(L.kvq_pages_settle(book, _rows(dev, "rows", rows), n, min(int(window), _MOST), at, st))
     for block in blocks:
@@ -254,6 +263,7 @@ def pages_fork(parents, children, pages, layers):
         size = layer.kfull.shape[1] * PAGE_TOKENS * 256
         for at in _fp16_pages(pages, dev, layer):
             tensors += (at, size)
+    _movable(layers, tensors[::2])
     moves = pages.count.new_empty(4 + 2 * n)
     _launched(_library().kvq_pages_fork(book, _rows(dev, "parents", parents), _ints(dev, "children", children, n), n, moves.data_ptr(), ops.raw_stream()))
     _copy(tensors, moves.data_ptr(), n)
@@ -269,6 +279,7 @@ def pages_compact(pages, layers):
         for tensors, some in ((packed, (layer.kcode, layer.kscale, layer.kmn, layer.vcode, layer.vscale, layer.vmn)), (fp16, (layer.kfull, layer.vfull))):
             for t in some:
                 tensors += (t.data_ptr(), t.numel() // max(t.shape[0], 1) * t.element_size())
+    _movable(layers, packed[::2] + fp16[::2])
     moves = pages.count.new_empty(8 + 3 * total)
     _launched(_library().kvq_pages_compact(book, moves.data_ptr(), ops.raw_stream()))
     if n:
@@ -315,8 +326,7 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     window, softcap = window or 0, softcap or 0.0
     if window < 0 or not softcap >= 0.0:
         raise RuntimeError("window and softcap must not be negative")
-    scale = 1.0 / math.sqrt(128) if softmax_scale is None else float(softmax_scale)
-    if not abs(scale) <= 3.4e38:
+    if softmax_scale is not None and not abs(softmax_scale) <= 3.4e38:
         raise RuntimeError("softmax_scale must be a finite number")
     at_slopes = 0
     if alibi_slopes is not None:
@@ -333,9 +343,9 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     need = L.kvq_paged_attn_workspace_bytes(block, n, tokens, nh, max_new, max_tokens, max_chunks)
     ws = pages.count.new_empty((need + 3) // 4) if need else None
     a = _pack_attn(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), _ints(dev, "q_start", q_start, n + 1),
-                   _rows(dev, "rows", rows), 0 if first is None else _ints(dev, "first", first, tokens), 0 if prefix is None else _ints(dev, "prefix", prefix, n),
-                   at_slopes, n, tokens, nh, max_new, max_tokens, max_chunks, min(int(window), _MOST), int(bool(causal)),
-                   scale, min(float(softcap), 1e38), 0 if ws is None else ws.data_ptr(), need)
+                   _ints(dev, "rows", rows, n), 0 if first is None else _ints(dev, "first", first, tokens), 0 if prefix is None else _ints(dev, "prefix", prefix, n),
+                   at_slopes, n, tokens, nh, max_new, max_tokens, max_chunks, min(int(window), _MOST), 1 if causal else 0,
+                   _SCALE if softmax_scale is None else softmax_scale, min(softcap, 1e38), 0 if ws is None else ws.data_ptr(), need)
     _launched(L.kvq_paged_attn(book, block, a, ops.raw_stream()))
     return out
 
