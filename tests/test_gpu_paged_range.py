@@ -377,6 +377,27 @@ def test_wrong_numbers_of_new_tokens_stay_inside(cuda, bad):
 
 # ---- long sequences, packing under replay ------------------------------------------------------------------------------------------------
 
+@pytest.mark.parametrize("kb,vb,group,rep,length", [(3, 2, 128, 4, 131072), (2, 1, 64, 4, 32768), (2, 2, 32, 1, 65433), (4, 4, 64, 8, 40001)])
+def test_one_token_over_a_long_context(cuda, kb, vb, group, rep, length):
+    """The framework's own tolerance, 2e-3 of a row: a weight's and an output's rounding are 2^-11 at most each, and a score's error is 2^-11 of
+    its terms at 3 bits (random signs: 1e-4 of 1) and next to nothing otherwise."""
+    c = Cache([length], [(length - 200) // P], 1, kb, vb, group, seed=length)
+    q = queries(1, rep)
+    got, (want, slack) = attend(c, q, [1]), attention(c, q, [1], kb != 3)
+    holds(got, want, slack)
+    rows_hold(got, want, 2e-3)
+
+
+@pytest.mark.parametrize("kb,vb,group,new,length", [(2, 2, 64, 300, 34816), (4, 4, 32, 129, 20001), (3, 3, 128, 70, 9000)])
+def test_a_chunk_over_a_long_context(cuda, kb, vb, group, new, length):
+    """The same of chunks: keys are rounded to fp16 besides, 2^-12 of an element with random signs: 128 terms of 1 give a score 2e-4 to 5e-4."""
+    c = Cache([length], [(length - new) // P], 1, kb, vb, group, seed=length)
+    q = queries(new, 4)
+    got, (want, slack) = attend(c, q, [new]), attention(c, q, [new], False)
+    holds(got, want, slack)
+    rows_hold(got, want, 2e-3)
+
+
 @pytest.mark.parametrize("kb,vb,group", [(2, 2, 64), (3, 3, 128), (4, 4, 32)])
 @pytest.mark.parametrize("counts", [[1, 300, 1, 2], [40, 1, 1, 0], [1, 1, 700, 1]])
 def test_split_single_tokens_beside_chunks(cuda, kb, vb, group, counts):
@@ -386,3 +407,29 @@ def test_split_single_tokens_beside_chunks(cuda, kb, vb, group, counts):
     want, slack = attention(c, q, counts, False)
     for hints in ({}, dict(max_new=max(counts), max_chunks=2, max_tokens=9000)):
         holds(attend(c, q, counts, **hints), want, slack)
+
+
+def test_replayed_steps_pack_what_is_due(cuda):
+    """A captured step replayed over two boundaries of pages: the packed pages are those that left the window, and are as many as the steps say."""
+    gen = torch.Generator().manual_seed(5)
+    cache = kv.KVmixPagedCache([(2, 2)], 1, 128, 4, 700, 12, 12, 64, 128)
+    rows, prompt = [3, 0, 2], [200, 127, 1]
+    s = cache.extend(rows, prompt)
+    x = torch.randn(s.tokens, 1, 128, generator=gen).half().cuda()
+    cache.write(0, x, x, s)
+    cache.settle(rows)
+    at, ones, begin = ints(*rows), ints(1, 1, 1), ints(0, 1, 2, 3)
+    new = torch.zeros(3, 1, 128, dtype=torch.half, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kv.pages_extend(at, ones, cache.book)
+        kv.page_write(new, new, begin, at, cache.book, cache.layers[0])
+        kv.pages_settle(at, 128, cache.book, cache.layers)
+    for i in range(1, 301):
+        graph.replay()
+        lengths = [127 + i, 0, 1 + i, 200 + i]
+        assert cache.book.length.tolist() == lengths
+        assert cache.book.packed.tolist() == [max(0, n - 128) // 128 for n in lengths], i
+    assert cache.book.packed.tolist() == [2, 0, 1, 2]
+    cache.check()
