@@ -472,11 +472,12 @@ int kvq_decode_attn_static(const kvq_attn_args *a, kvq_stream_t stream);
  *   refs     [n_packed + n_fp16] references of every page, fp16 pages behind the packed ones
  *   free_ids [n_packed + n_fp16] the free pages' numbers, two stacks (packed from 0, fp16 from n_packed), the next one to be taken last
  *   count    [4]                 free packed pages, free fp16 pages, status, 0
- * A page that several sequences hold is full or packed and never written (kvq_page_write leaves tokens out whose page is packed or shared).
+ * A page that several sequences hold is full or packed and never written (kvq_page_write leaves tokens out whose page is packed, shared or not there).
  *
  * count[2], the status, collects KVQ_PAGES_* bits.  A call that cannot be done in full does nothing but set one; while such a bit is set, the
  * calls that change the cache do nothing (lengths and pages stay consistent) until the caller has cleared it.  KVQ_PAGES_STALLED only says
- * that an attention's output is not to be used: the cache is whole, and calls go on.
+ * that an attention's output is not to be used: the cache is whole, and calls go on.  So they do after KVQ_PAGES_NOT_WRITTEN: new tokens of a row
+ * of the table had no place of their sequence's own.
  * `rows`: n slots, each at most once in a call.  Stacks are popped and pushed in the order of rows and pages (kvq_pages_extend, _fork,
  * _settle) and of page numbers (pages that come free), so that equal calls give equal numbers.
  */
@@ -487,6 +488,7 @@ extern uint32_t kvq_paged_launch_count;         /* kernels of the paged cache la
 #define KVQ_PAGES_TOO_LONG 4    /* a sequence would need more than max_pages                               */
 #define KVQ_PAGES_BAD_ROWS 8    /* a row outside the table, named twice, or not as the call wants it       */
 #define KVQ_PAGES_STALLED 16    /* an attention gave up waiting for its own copies; holds nothing up        */
+#define KVQ_PAGES_NOT_WRITTEN 32 /* kvq_page_write left tokens out; holds nothing up                       */
 
 typedef struct {
     int32_t *table, *length, *packed, *refs, *free_ids, *count;

@@ -376,9 +376,11 @@ __global__ void __launch_bounds__(256) page_write_kernel(const kvq_page_book b, 
     const int s = sequence_of(a.q_start, a.n, u), row = a.rows[s];
     if (row < 0 || row >= b.slots) return;
     const int pos = length_of(b, row) - max(a.q_start[s + 1], 0) + u, page = pos / kPage;
-    if (pos < 0 || page >= b.max_pages || page < b.packed[row]) return;
-    const int id = b.table[(int64_t)row * b.max_pages + page];
-    if (id < 0 || id >= min(l.n_fp16, b.n_fp16) || b.refs[b.n_packed + id] > 1) return;      // a page that others hold too stays as it is
+    const int id = pos >= 0 && page < b.max_pages && page >= b.packed[row] ? b.table[(int64_t)row * b.max_pages + page] : -1;
+    if (!inside(id, min(l.n_fp16, b.n_fp16)) || b.refs[b.n_packed + id] > 1) {    // a page that others hold too stays as it is
+        if (c == 0) atomicOr(&b.count[2], KVQ_PAGES_NOT_WRITTEN);
+        return;
+    }
     const int64_t to = (((int64_t)id * l.Hkv + h) * kPage + pos % kPage) * kHeadDim + c;
     *reinterpret_cast<uint4 *>(static_cast<__half *>(l.kfull) + to) = x;
     *reinterpret_cast<uint4 *>(static_cast<__half *>(l.vfull) + to) = y;

@@ -14,9 +14,9 @@ __host__ __device__ constexpr int page_groups(int bits, int group) { return bits
 
 __device__ __forceinline__ int pages_of(int tokens) { return (tokens + kPage - 1) / kPage; }
 
-// Whether a call had to be refused: none changes the cache then.  A wait of the attention that gave up concerns that call's output alone; were
-// the writes behind it left out, tokens that are counted already would be missing in later layers.
-__device__ __forceinline__ bool refused(const kvq_page_book &b) { return b.count[2] & ~KVQ_PAGES_STALLED; }
+// Whether a call had to be refused: none changes the cache then.  A wait of the attention that gave up, and tokens that page_write left out, concern
+// their own call alone; were the writes behind it left out, tokens that are counted already would be missing in later layers.
+__device__ __forceinline__ bool refused(const kvq_page_book &b) { return b.count[2] & ~(KVQ_PAGES_STALLED | KVQ_PAGES_NOT_WRITTEN); }
 
 // Every size that a kernel's index arithmetic relies on.
 inline int check_book(const kvq_page_book *b) {

@@ -13,7 +13,7 @@ bit widths, its newest are fp16 (``include/kvmix_b200.h`` has the layouts, which
 The bookkeeping (``PageBook``) lives on the device and is changed by kernels only: no call waits for the host, all can be captured in a
 CUDA graph.  A call that cannot be done in full -- no page left, a row named twice -- does nothing but set a bit of ``count[2]``, and
 until that is cleared every call that changes the cache does nothing (``KVmixPagedCache.check`` raises and clears).  An attention
-that gave up waiting sets a bit too, which holds nothing up: its output is lost, the cache is whole.  The attention is
+that gave up waiting (its output is lost, the cache is whole) and a ``page_write`` that left tokens out set bits that hold nothing up.  The attention is
 exact softmax attention over the dequantised cache: scores are not narrowed to fp16 as ``decode_attention`` does by default.
 """
 import ctypes as C
@@ -32,7 +32,8 @@ _SCALE = 1.0 / math.sqrt(128)
 _MOST = 1 << 30                  # no sequence is longer: wider windows are this one
 _MOST_HEADS = 1 << 15            # what kvq_page_copy takes as one page: 1 GB
 _STATUS = {1: "no free fp16 page", 2: "no free packed page", 4: "sequence longer than the table", 8: "bad rows (outside the table, named twice, "
-           "a child that is not empty or also a parent)", 16: "an attention gave up waiting for its own copies, its output is not to be used"}
+           "a child that is not empty or also a parent)", 16: "an attention gave up waiting for its own copies, its output is not to be used",
+           32: "new tokens were not written, their page is packed, shared or not there"}
 
 _pack_book, _pack_layer = struct.Struct("@6P4i").pack, struct.Struct("@8P6i").pack
 _pack_write, _pack_attn = struct.Struct("@2P4q2P2i").pack, struct.Struct("@2P4q5P8i2fPQ").pack
@@ -219,7 +220,7 @@ def pages_free(rows, pages):
 def page_write(k, v, q_start, rows, pages, layer):
     """Keys (rotated) and values of new tokens into one layer's fp16 pages.  k, v [tokens, Hkv, 128] fp16, any strides; tokens
     [q_start[i], q_start[i+1]) are the last ones of sequence rows[i], which ``pages_extend`` has counted already.  Tokens whose page
-    is packed, or held by another sequence too, are left out."""
+    is packed, not there or held by another sequence too are left out, and a status bit says so."""
     dev, book = _book(pages)
     heads = layer.kfull.shape[1]
     if k.dim() != 3 or k.shape[1:] != (heads, 128) or v.shape != k.shape or k.dtype is not torch.float16 or v.dtype is not torch.float16:
@@ -476,7 +477,7 @@ class KVmixPagedCache:
         return tuple(self.book.count[:2].tolist())
 
     def check(self):
-        """Raises if a call since the last check had to be refused or an attention's output is not to be used, and lets the cache go on from where it
+        """Raises if a call since the last check had to be refused, left tokens out or lost its output, and lets the cache go on from where it
         was.  Waits for the device."""
         status = int(self.book.count[2])
         if status:

@@ -285,10 +285,32 @@ def test_shared_pages_are_never_written(cuda):
             assert torch.equal(t[ids[j]], old[j * P:j * P + P].transpose(0, 1))
         assert torch.equal(t[ids[2], :, :44], old[256:300].transpose(0, 1))
         assert torch.equal(t[own[2], :, :64], new[256:320].transpose(0, 1))
+    with pytest.raises(RuntimeError, match="not written"):
+        cache.check()
     cache.free([0])                                                                   # nobody else holds them now
     kv.page_write(x, y, ints(0, 320), ints(1), cache.book, cache.layers[0])
     assert torch.equal(cache.layers[0].kfull[ids[0]], x[:P].transpose(0, 1))
     cache.check()
+
+
+def test_tokens_without_a_place_are_reported(cuda):
+    """A step that was not counted, a sequence that is not there, a packed page: page_write says that it left them out, and holds nothing up."""
+    cache = small()
+    x = torch.zeros(300, 1, 128, device="cuda").half()
+    for begin, rows, fine in ((ints(0, 1), ints(1), False), (ints(0, 11), ints(2), False), (ints(0, 10), ints(2), True), (ints(0, 300), ints(0), True)):
+        kv.page_write(x, x, begin, rows, cache.book, cache.layers[0])
+        if fine:
+            cache.check()
+        else:
+            with pytest.raises(RuntimeError, match="not written"):
+                cache.check()
+    cache.settle([0])
+    kv.page_write(x, x, ints(0, 300), ints(0), cache.book, cache.layers[0])            # 256 of them are packed
+    assert int(cache.book.count[2]) == 32
+    cache.extend([0], [1])
+    assert int(cache.book.length[0]) == 301
+    with pytest.raises(RuntimeError, match="not written"):
+        cache.check()
 
 
 # ---- launches --------------------------------------------------------------------------------------------------------------------------
@@ -372,7 +394,7 @@ def test_wrong_numbers_of_new_tokens_stay_inside(cuda, bad):
     before = cache.layers[0].kfull[others].clone()
     kv.page_write(x, x, ints(*bad), ints(0, 2), cache.book, cache.layers[0])
     assert torch.equal(cache.layers[0].kfull[others].view(torch.int16), before.view(torch.int16))
-    cache.check()
+    assert int(cache.book.count[2]) in (0, 32)                                        # tokens without a place are reported, nothing else
 
 
 # ---- long sequences, packing under replay ------------------------------------------------------------------------------------------------
