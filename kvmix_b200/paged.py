@@ -249,7 +249,7 @@ def pages_settle(rows, window, pages, layers):
     for block in blocks:
         _movable((), _addresses(block))
     L, st, at = _library(), ops.raw_stream(), moves.data_ptr()
-    _launched(L.kvq_pages_settle(book, _rows(dev, "rows", rows), n, min(int(window), _MOST), at, st))
+    _launched(L.kvq_pages_settle(book, _rows(dev, "rows", rows), n, int(min(window, _MOST)), at, st))
     for block in blocks:
         _launched(L.kvq_page_pack(block, at, min(pages.n_packed, n * pages.table.shape[1]), st))
 
@@ -345,7 +345,7 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     ws = pages.count.new_empty((need + 3) // 4) if need else None
     a = _pack_attn(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), _ints(dev, "q_start", q_start, n + 1),
                    _ints(dev, "rows", rows, n), 0 if first is None else _ints(dev, "first", first, tokens), 0 if prefix is None else _ints(dev, "prefix", prefix, n),
-                   at_slopes, n, tokens, nh, max_new, max_tokens, max_chunks, min(int(window), _MOST), 1 if causal else 0,
+                   at_slopes, n, tokens, nh, max_new, max_tokens, max_chunks, int(min(window, _MOST)), 1 if causal else 0,
                    _SCALE if softmax_scale is None else softmax_scale, min(softcap, 1e38), 0 if ws is None else ws.data_ptr(), need)
     _launched(L.kvq_paged_attn(book, block, a, ops.raw_stream()))
     return out
@@ -389,7 +389,7 @@ class KVmixPagedCache:
         dev = torch.device(device)
         if dev.type == "cuda" and dev.index is None:
             dev = torch.device("cuda", torch.cuda.current_device())
-        self.window, self.device = int(residual_length), dev
+        self.window, self.device = int(min(residual_length, _MOST)), dev
 
         def packed(bits):
             w, g = page_words(bits), page_groups(bits, group_size)

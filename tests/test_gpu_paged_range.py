@@ -165,7 +165,7 @@ def test_a_stalled_wait_leaves_the_cache_whole(cuda):
 
 # ---- windows ---------------------------------------------------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 40])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 40, float("inf")])
 def test_windows_beyond_32_bits(cuda, window):
     cache = small()
     kv.pages_settle(ints(0), window, cache.book, cache.layers)
