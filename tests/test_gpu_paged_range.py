@@ -455,3 +455,30 @@ def test_replayed_steps_pack_what_is_due(cuda):
         assert cache.book.packed.tolist() == [max(0, n - 128) // 128 for n in lengths], i
     assert cache.book.packed.tolist() == [2, 0, 1, 2]
     cache.check()
+
+
+def test_as_many_rows_as_a_table_may_have(cuda):
+    """2^20 rows: a bit each in shared memory, beyond what a launch has unasked."""
+    n = 1 << 20
+    cache = kv.KVmixPagedCache([(2, 2)], 1, 128, n, 128, 2, 4, 128, 0)
+    rows = [n - 1, 0, 131072]
+    kv.pages_extend(ints(*rows), ints(128, 128, 5), cache.book)
+    assert cache.book.length[rows].tolist() == [128, 128, 5] and int(cache.book.length.sum()) == 261
+    kv.pages_settle(ints(*rows), 0, cache.book, cache.layers)
+    kv.pages_fork(ints(n - 1, 131072), ints(n - 2, 1), cache.book, cache.layers)
+    kv.pages_compact(cache.book, cache.layers)
+    assert cache.book.packed[[n - 1, n - 2, 0, 131072, 1]].tolist() == [1, 1, 1, 0, 0] and cache.free_pages() == (0, 2)
+    kv.pages_free(ints(n - 1, 5, n - 1), cache.book)                                  # named twice
+    with pytest.raises(RuntimeError, match="bad rows"):
+        cache.check()
+    kv.pages_free(ints(n - 1, n - 2, 0, 131072, 1), cache.book)
+    cache.check()
+    assert cache.free_pages() == (2, 4) and not cache.book.length.any()
+
+
+@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("scale", [0.0, 1e-30, -1e-3])
+def test_scales_of_next_to_nothing(cuda, new, scale):
+    c = Cache([300], [1], 2, 4, 2, 64, seed=9)
+    q = queries(new, 4)
+    holds(attend(c, q, [new], scale=scale), *attention(c, q, [new], True, scale=scale))
