@@ -22,7 +22,7 @@ int count_launch() {
 
 extern "C" { uint32_t kvq_paged_launch_count = 0; }
 
-extern "C" int kvq_version(void) { return 107; }   // 105: fused decode step, device-resident state, head-sharded exchange, kvq_prefill, kvq_attn_plan; 106: 3-bit values (ragged_tail); 107: paged cache
+extern "C" int kvq_version(void) { return 108; }   // 105: fused decode step, device-resident state, head-sharded exchange, kvq_prefill, kvq_attn_plan; 106: 3-bit values (ragged_tail); 107: paged cache; 108: status bits that hold nothing up, kvq_paged_launch_count
 
 extern "C" int kvq_features_per_int(int bits) { return (bits >= 1 && bits <= 4) ? kvq::fields_per_word(bits) : 0; }
 

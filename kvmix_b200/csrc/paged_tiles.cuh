@@ -1,4 +1,4 @@
-// Attention of many query rows of a kv head (chunks of prompts, the tokens of a speculative step) over a paged cache, on tcgen05.  A source
+// Attention of many query rows of a kv head (chunks of new tokens, more than 8 query heads a kv head) over a paged cache, on tcgen05.  A source
 // file for each width of the keys (paged_tiles_1.cu ..): their instances build side by side.
 #pragma once
 #include "paged_attn.cuh"
@@ -16,8 +16,8 @@ namespace kvq {
 // 190 us for four capped chunks of 501 tokens); one that fills the operand buffers; a warp that issues the MMAs and a thread that issues
 // copies.  While one tile's scores are worked on, the tensor core multiplies for the other.  TMEM: S0 S1 O0 O1, 128 columns each.
 // Bound: a page is 2048 cycles of MMA and as many of the special function unit (one exponential a score) and takes some 3200; under it the
-// card runs at its power limit (1.5 to 1.6 GHz).  2048 tokens x 32 heads over 34816: 1055 TFLOP/s, 0.65 of the rate measured in bursts and 0.77 of
-// the sustained one.  Tried without gain: a part of the exponentials as polynomials (2 to 20 % slower), weights handed over in quarters.
+// card runs at its power limit (1.5 to 1.6 GHz).  2048 tokens x 32 heads over 34816: 990 to 1050 TFLOP/s from card to card, 0.61 to 0.64 of the rate measured
+// in bursts and 0.73 to 0.77 of the sustained one.  Tried without gain: a part of the exponentials as polynomials (2 to 20 % slower), weights handed over in quarters.
 //
 // Operand buffers hold 128 rows of 128 fp16 as two halves of 64 (128 bytes a row, 16-byte pieces swizzled by the row's number).  Rows are
 // tokens of fp16 pages and of packed values, channels of packed keys: what is contiguous in a row is the contraction axis of fp16 keys (K-major

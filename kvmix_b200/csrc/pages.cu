@@ -555,7 +555,7 @@ static void launch_pack(const kvq_page_layer &l, const int32_t *moves, int max_m
 static size_t seen_bytes(const kvq_page_book &b) { return (size_t)(b.slots + 31) / 32 * 4; }
 
 template <typename K>
-static int book_smem(K kernel, size_t bytes) {                    // beyond the 48 KB that need no asking (393216 slots)
+static int book_smem(K kernel, size_t bytes) {                    // 16 KB (131072 slots) beside BookShared need no asking
     if (bytes <= 16384) return KVQ_OK;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     return e == cudaSuccess ? KVQ_OK : record_cuda_error(e);

@@ -14,7 +14,9 @@ The bookkeeping (``PageBook``) lives on the device and is changed by kernels onl
 CUDA graph.  A call that cannot be done in full -- no page left, a row named twice -- does nothing but set a bit of ``count[2]``, and
 until that is cleared every call that changes the cache does nothing (``KVmixPagedCache.check`` raises and clears).  An attention
 that gave up waiting (its output is lost, the cache is whole) and a ``page_write`` that left tokens out set bits that hold nothing up.  The attention is
-exact softmax attention over the dequantised cache: scores are not narrowed to fp16 as ``decode_attention`` does by default.
+softmax attention over the dequantised cache with scores, softmax and sums in fp32 (scores are not narrowed to fp16 as ``decode_attention`` does by
+default).  What is rounded to fp16 on the way to the tensor cores: weights; for several new tokens (and more than 8 query heads a kv head) dequantised
+keys and values; for one new token those of 3 bits, and weight * scale of a value.
 """
 import ctypes as C
 import functools
