@@ -193,8 +193,10 @@ def _launched(rc):
         check(rc)
     count, seen = _launch_count()
     now = count.value
-    ops.LAUNCHES[0] += (now - seen[0]) & 0xffffffff
-    seen[0] = now
+    new = (now - seen[0]) & 0xffffffff
+    if new < 1 << 31:                                 # else another thread was here between
+        ops.LAUNCHES[0] += new
+        seen[0] = now
 
 
 def _copy(tensors, moves, max_moves):

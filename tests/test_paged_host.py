@@ -123,3 +123,18 @@ def test_workspace_of_a_long_chunk_beside_single_tokens():
                 assert b <= 2 * tokens * 32 * 520, (n, tokens, b)
     # without a chunk the splits are as many as they pay
     assert L.kvq_paged_attn_workspace_bytes(layer(Hkv=8), 1, 1, 32, 1, 131072, 1) >= 20 * 32 * 520
+
+
+def test_launch_counts_of_threads_that_cross():
+    """A thread that read the library's count before another one did, and comes to add it behind that one, adds nothing; the count may wrap."""
+    count, seen = paged._launch_count()
+    kept = count.value, seen[0], kv.ops.LAUNCHES[0]
+    try:
+        for now, had, added in ((5, 3, 2), (5, 6, 0), (1, 2 ** 32 - 2, 3), (2 ** 32 - 1, 2, 0)):
+            count.value, seen[0], before = now, had, kv.ops.LAUNCHES[0]
+            paged._launched(0)
+            assert kv.ops.LAUNCHES[0] - before == added
+            paged._launched(0)
+            assert kv.ops.LAUNCHES[0] - before == added
+    finally:
+        count.value, seen[0], kv.ops.LAUNCHES[0] = kept
