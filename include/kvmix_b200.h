@@ -476,8 +476,8 @@ int kvq_decode_attn_static(const kvq_attn_args *a, kvq_stream_t stream);
  *
  * count[2], the status, collects KVQ_PAGES_* bits.  A call that cannot be done in full does nothing but set one; while such a bit is set, the
  * calls that change the cache do nothing (lengths and pages stay consistent) until the caller has cleared it.  KVQ_PAGES_STALLED only says
- * that an attention's output is not to be used: the cache is whole, and calls go on.  So they do after KVQ_PAGES_NOT_WRITTEN: new tokens of a row
- * of the table had no place of their sequence's own.
+ * that an attention's output is not to be used: the cache is whole, and calls go on.  So they do after KVQ_PAGES_NOT_WRITTEN and KVQ_PAGES_NO_ANGLE: new
+ * tokens of a row of the table had no place of their sequence's own, or no angles.
  * `rows`: n slots, each at most once in a call.  Stacks are popped and pushed in the order of rows and pages (kvq_pages_extend, _fork,
  * _settle) and of page numbers (pages that come free), so that equal calls give equal numbers.
  */
@@ -488,7 +488,8 @@ extern uint32_t kvq_paged_launch_count;         /* kernels of the paged cache la
 #define KVQ_PAGES_TOO_LONG 4    /* a sequence would need more than max_pages                               */
 #define KVQ_PAGES_BAD_ROWS 8    /* a row outside the table, named twice, or not as the call wants it       */
 #define KVQ_PAGES_STALLED 16    /* an attention gave up waiting for its own copies; holds nothing up        */
-#define KVQ_PAGES_NOT_WRITTEN 32 /* kvq_page_write left tokens out; holds nothing up                       */
+#define KVQ_PAGES_NOT_WRITTEN 32 /* kvq_page_write or kvq_page_append left tokens out; holds nothing up    */
+#define KVQ_PAGES_NO_ANGLE 64   /* kvq_page_append left tokens out, their positions are outside the tables; holds nothing up */
 
 typedef struct {
     int32_t *table, *length, *packed, *refs, *free_ids, *count;
@@ -549,6 +550,71 @@ typedef struct {
 } kvq_page_write_args;
 
 int kvq_page_write(const kvq_page_book *b, const kvq_page_layer *l, const kvq_page_write_args *a, kvq_stream_t stream);
+
+/*
+ * The same with the position rotation applied on the way, and queries rotated beside them: keys, values and queries come from the projections.
+ * A head's 128 channels are `parts` (1 or 2) parts of 128 / parts; the first 2 * angles channels of each part are pairs, (i, i + angles) or, interleaved,
+ * (2i, 2i + 1); pair i of a token at position p becomes  (x c - y s, y c + x s),  c = cos[p][i], s = sin[p][i],  in fp32, rounded once to
+ * fp16; the other channels and the values are rounded to fp16.  p: the token's place in its sequence, or positions[token].
+ *   k, v [tokens, Hkv, 128], q [tokens, nh, 128] of `type`, contiguous along the channels, strides *_sT, *_sH;  q_out [tokens, nh, 128] fp16, may be q where that is fp16
+ *   cos, sin [angle_rows][angles] fp32, rows c_sT, s_sT apart;  angles a multiple of 8, at most 64 / parts;  q NULL: keys and values alone
+ * A token whose position is outside the tables is left out, its query too (KVQ_PAGES_NO_ANGLE); one without a place in the pages is left out
+ * as kvq_page_write does (KVQ_PAGES_NOT_WRITTEN), its query is rotated.
+ */
+#define KVQ_F16 0
+#define KVQ_BF16 1
+#define KVQ_F32 2
+typedef struct {
+    const void *k, *v, *q;
+    void *q_out;
+    const float *cos, *sin;
+    int64_t k_sT, k_sH, v_sT, v_sH, q_sT, q_sH, o_sT, o_sH, c_sT, s_sT;
+    const int32_t *q_start, *rows, *positions;
+    int32_t n, tokens, nh, type, angles, angle_rows, parts, interleaved;
+} kvq_page_append_args;
+
+int kvq_page_append(const kvq_page_book *b, const kvq_page_layer *l, const kvq_page_append_args *a, kvq_stream_t stream);
+
+/*
+ * Rows take one another's places, all at once (a step of beam search): rows[i] becomes the sequence that row parent(i) was before the call.  parent(i):
+ * parents[i], or, with beams > 0 (n a multiple of it), rows[i / beams * beams + parents[i]].  A parent may be taken by several rows, by none (its sequence
+ * goes) and may be a row that is not among `rows` (it stays as it is).  Full pages are shared.  A last page that is not full stays with the parent if that goes on
+ * as itself or is not among `rows`, else goes to the first row that takes it; the others get pages of their own, those that the call sets free among
+ * them, and `moves` lists (source, destination, tokens) of those for kvq_page_copy_tails on every layer's kfull and vfull.
+ * moves: int32 [kvq_pages_reorder_moves(b, n)], the triples from moves[4] on, their number in moves[0]; the rest is scratch.
+ */
+uint64_t kvq_pages_reorder_moves(const kvq_page_book *b, int32_t n);
+int kvq_pages_reorder(const kvq_page_book *b, const int32_t *rows, const int32_t *parents, int32_t n, int32_t beams, int32_t *moves, kvq_stream_t stream);
+/* Copies the first tokens of pages [heads][128 tokens][128 channels] of fp16, as `moves` of kvq_pages_reorder has them, in n tensors. */
+int kvq_page_copy_tails(const kvq_page_tensor *tensors, int32_t n, const int32_t *moves, int32_t max_moves, kvq_stream_t stream);
+
+/*
+ * Beam search's selection.  logits [requests * beams, vocabulary] of `type`, rows l_sR elements apart; scores [requests * beams] of the beams so far.
+ *   value(b, t) = scores[b] + (logits[b][t] - log sum_t' exp(logits[b][t']))
+ * The n continuations of a request with the largest values, in that order, equal ones by (beam, token): their values, beams (within the request) and tokens in
+ * out_* [requests, n]; and the first `beams` of them whose token is not among ends[n_ends] in next_* [requests, beams], which is what goes on.
+ * A beam whose score is not finite, or whose logits hold a NaN or +infinity or nothing but -infinity, offers all its tokens at -infinity, and so does every beam
+ * its tokens of -infinity.  n: at least beams * (1 + n_ends) or all there are, and then what is left of next_* is (-infinity, 0, 0).
+ * workspace: kvq_beam_select_workspace_bytes(a) bytes, 16-byte aligned, not shared by concurrent calls.  Two launches.
+ */
+#define KVQ_MOST_BEAMS 64
+#define KVQ_MOST_BEST 128
+typedef struct {
+    const void *logits;
+    int64_t l_sR;
+    const float *scores;
+    const int32_t *ends;
+    float *out_scores;
+    int32_t *out_beams, *out_tokens;
+    float *next_scores;
+    int32_t *next_beams, *next_tokens;
+    int32_t requests, beams, vocabulary, type, n, n_ends;
+    void *workspace;
+    uint64_t workspace_bytes;
+} kvq_beam_args;
+
+uint64_t kvq_beam_select_workspace_bytes(const kvq_beam_args *a);
+int kvq_beam_select(const kvq_beam_args *a, kvq_stream_t stream);
 
 /*
  * Attention of new tokens over a paged cache.  Sequence rows[i]'s last q_start[i+1] - q_start[i] tokens ask (its keys and values, theirs

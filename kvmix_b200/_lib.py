@@ -114,7 +114,21 @@ class PagedAttnArgs(C.Structure):
                 ("softmax_scale", C.c_float), ("softcap", C.c_float), ("workspace", vp), ("workspace_bytes", u64)]
 
 
+class PageAppendArgs(C.Structure):
+    _fields_ = [("k", vp), ("v", vp), ("q", vp), ("q_out", vp), ("cos", vp), ("sin", vp),
+                ("k_sT", i64), ("k_sH", i64), ("v_sT", i64), ("v_sH", i64), ("q_sT", i64), ("q_sH", i64), ("o_sT", i64), ("o_sH", i64),
+                ("c_sT", i64), ("s_sT", i64), ("q_start", vp), ("rows", vp), ("positions", vp),
+                ("n", i32), ("tokens", i32), ("nh", i32), ("type", i32), ("angles", i32), ("angle_rows", i32), ("parts", i32), ("interleaved", i32)]
+
+
+class BeamArgs(C.Structure):
+    _fields_ = [("logits", vp), ("l_sR", i64), ("scores", vp), ("ends", vp), ("out_scores", vp), ("out_beams", vp), ("out_tokens", vp),
+                ("next_scores", vp), ("next_beams", vp), ("next_tokens", vp),
+                ("requests", i32), ("beams", i32), ("vocabulary", i32), ("type", i32), ("n", i32), ("n_ends", i32), ("workspace", vp), ("workspace_bytes", u64)]
+
+
 MAX_PAGE_TENSORS = 256
+MOST_BEAMS, MOST_BEST = 64, 128
 ATTN_WORKSPACE_READY = 1
 
 
@@ -166,8 +180,12 @@ def lib():
         for fn, types in ((L.kvq_pages_extend, [blk, vp, vp, i32, vp]), (L.kvq_pages_free, [blk, vp, i32, vp]),
                           (L.kvq_pages_settle, [blk, vp, i32, i32, vp, vp]), (L.kvq_page_pack, [blk, vp, i32, vp]),
                           (L.kvq_pages_fork, [blk, vp, vp, i32, vp, vp]), (L.kvq_pages_compact, [blk, vp, vp]),
-                          (L.kvq_page_copy, [blk, i32, vp, i32, vp]), (L.kvq_page_write, [blk, blk, blk, vp]), (L.kvq_paged_attn, [blk, blk, blk, vp])):
+                          (L.kvq_page_copy, [blk, i32, vp, i32, vp]), (L.kvq_page_write, [blk, blk, blk, vp]), (L.kvq_paged_attn, [blk, blk, blk, vp]),
+                          (L.kvq_page_append, [blk, blk, blk, vp]), (L.kvq_pages_reorder, [blk, vp, vp, i32, i32, vp, vp]),
+                          (L.kvq_page_copy_tails, [blk, i32, vp, i32, vp]), (L.kvq_beam_select, [blk, vp])):
             fn.restype, fn.argtypes = C.c_int, types
+        L.kvq_pages_reorder_moves.restype, L.kvq_pages_reorder_moves.argtypes = u64, [blk, i32]
+        L.kvq_beam_select_workspace_bytes.restype, L.kvq_beam_select_workspace_bytes.argtypes = u64, [blk]
         L.kvq_paged_attn_workspace_bytes.restype, L.kvq_paged_attn_workspace_bytes.argtypes = u64, [blk] + [i32] * 6
         _lib = L
     return _lib
@@ -177,7 +195,8 @@ EXPORTS = ["kvq_version", "kvq_error_string", "kvq_last_cuda_error", "kvq_featur
            "kvq_quant_lastdim", "kvq_append_kv", "kvq_gemv", "kvq_decode_attn", "kvq_decode_attn_workspace_bytes",
            "kvq_decode_attn_static", "kvq_decode_attn_plan", "kvq_decode_attn_workspace_init", "kvq_prefill", "kvq_peer_wait", "kvq_peer_wait_next", "kvq_append_k", "kvq_append_v",
            "kvq_pages_extend", "kvq_pages_free", "kvq_pages_settle", "kvq_page_pack", "kvq_pages_fork", "kvq_pages_compact", "kvq_page_copy", "kvq_page_write",
-           "kvq_paged_attn", "kvq_paged_attn_workspace_bytes"]
+           "kvq_paged_attn", "kvq_paged_attn_workspace_bytes", "kvq_page_append", "kvq_pages_reorder", "kvq_pages_reorder_moves", "kvq_page_copy_tails",
+           "kvq_beam_select", "kvq_beam_select_workspace_bytes"]
 
 
 def check(rc):

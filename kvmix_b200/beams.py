@@ -1,0 +1,82 @@
+"""Beam search's selection on the device: which tokens continue which beams.
+
+``KVmixPagedCache.advance`` calls it and lets the cache's rows follow.  No upstream counterpart: upstream decodes greedily or samples.
+"""
+import ctypes as C
+import struct
+from typing import NamedTuple
+
+import torch
+
+from . import _lib, ops
+from ._lib import check
+
+_pack = struct.Struct("@Pq8P6iPQ").pack
+_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+class BeamStep(NamedTuple):
+    """The n best continuations of every request, best first -- ``scores`` fp32, ``beams`` (within the request) and ``tokens`` int32, [requests, n] each -- and
+    the first of them that do not end, [requests, beams] each, which is what goes on."""
+    scores: torch.Tensor
+    beams: torch.Tensor
+    tokens: torch.Tensor
+    next_scores: torch.Tensor
+    next_beams: torch.Tensor
+    next_tokens: torch.Tensor
+
+
+def beam_select(logits, scores, beams, n=None, ends=None):
+    """The best continuations of every request over its beams and the vocabulary, in two launches that read the logits once.
+
+    logits [requests * beams, vocabulary] fp16, bf16 or fp32, any row stride; scores fp32 [requests * beams], the beams' so far.  A continuation's score is
+    scores[beam] + log_softmax(logits[beam])[token]; the ``n`` best of a request (None: twice the beams, or beams * (1 + number of ends) where that is more; at most 128, beams at
+    most 64) come in order, equal ones by (beam, token).  ends: int32 tensor of tokens that end a sequence; n must leave ``beams`` others.  Sums of exponentials are kept in
+    64 bits across threads, so that the order of two beams' continuations does not hang on them.
+    A beam offers -infinity everywhere where its score is not finite (a beam that is not there: -infinity), its logits hold a NaN or +infinity, or all of
+    them are masked (-infinity)."""
+    dev = logits.get_device()
+    if dev < 0:
+        raise RuntimeError("kvmix_b200 operators need CUDA tensors (there is no CPU path)")
+    if logits.dim() != 2 or logits.dtype not in _TYPES:
+        raise RuntimeError("beam_select takes logits [requests * beams, vocabulary], fp16, bf16 or fp32")
+    rows, vocabulary = logits.shape
+    if not 0 < beams <= _lib.MOST_BEAMS or rows % beams or not 0 < vocabulary < 1 << 31:
+        raise RuntimeError(f"rows come in groups of `beams`, at most {_lib.MOST_BEAMS}")
+    if scores.dtype is not torch.float32 or scores.numel() != rows or scores.get_device() != dev or not scores.is_contiguous():
+        raise RuntimeError(f"scores must be contiguous float32 [{rows}] on cuda:{dev}")
+    n_ends, at_ends = 0, 0
+    if ends is not None:
+        if ends.dtype is not torch.int32 or ends.dim() != 1 or ends.get_device() != dev or not ends.is_contiguous():
+            raise RuntimeError(f"ends must be a contiguous int32 tensor on cuda:{dev}")
+        n_ends, at_ends = ends.numel(), ends.data_ptr()
+    all_of_them, needed = beams * vocabulary, beams * (1 + n_ends)
+    n = min(max(2 * beams, needed), all_of_them) if n is None else int(n)
+    if not min(needed, all_of_them) <= n <= min(all_of_them, _lib.MOST_BEST):
+        raise RuntimeError(f"n must be {min(needed, all_of_them)} to {min(all_of_them, _lib.MOST_BEST)} for {beams} beams and {n_ends} ends")
+    if logits.stride(1) != 1 and vocabulary > 1:
+        logits = logits.contiguous()
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _select(logits, scores, beams, n, n_ends, at_ends)
+    return _select(logits, scores, beams, n, n_ends, at_ends)
+
+
+def _select(logits, scores, beams, n, n_ends, at_ends):
+    rows, vocabulary = logits.shape
+    requests, L = rows // beams, _lib.lib()
+    assert struct.calcsize("@Pq8P6iPQ") == C.sizeof(_lib.BeamArgs)
+    out = scores.new_empty(3 * requests * (n + beams), dtype=torch.int32)
+    parts = [t.view(requests, -1) for t in out.split([requests * n] * 3 + [requests * beams] * 3)] if requests else [out.new_empty(0, w) for w in (n, n, n, beams, beams, beams)]
+    parts[0], parts[3] = parts[0].view(torch.float32), parts[3].view(torch.float32)
+
+    def block(at, size):
+        return _pack(logits.data_ptr(), logits.stride(0), scores.data_ptr(), at_ends, *[t.data_ptr() for t in parts], requests, beams, vocabulary, _TYPES[logits.dtype], n,
+                     n_ends, at, size)
+
+    if requests:
+        need = L.kvq_beam_select_workspace_bytes(block(0, 0))
+        workspace = out.new_empty((need + 3) // 4)
+        check(L.kvq_beam_select(block(workspace.data_ptr(), need), ops.raw_stream()))
+        ops.LAUNCHES[0] += 2
+    return BeamStep(*parts)

@@ -55,13 +55,6 @@ __device__ __forceinline__ long long block_sum(BookShared &s, long long v) {
     return s.total;
 }
 
-// The bookkeeping's numbers as they are used: whatever the tensors hold, no index that follows from them leaves a tensor.
-__device__ __forceinline__ int length_of(const kvq_page_book &b, int row) { return min(max(b.length[row], 0), b.max_pages * kPage); }
-__device__ __forceinline__ int packed_of(const kvq_page_book &b, int row) { return min(max(b.packed[row], 0), pages_of(length_of(b, row))); }
-__device__ __forceinline__ int free_packed(const kvq_page_book &b) { return min(max(b.count[0], 0), b.n_packed); }
-__device__ __forceinline__ int free_fp16(const kvq_page_book &b) { return min(max(b.count[1], 0), b.n_fp16); }
-__device__ __forceinline__ bool inside(int id, int n) { return id >= 0 && id < n; }
-
 extern __shared__ uint32_t s_seen[];                              // a bit for every slot
 
 __device__ __forceinline__ void clear_seen(const kvq_page_book &b) {
@@ -352,6 +345,153 @@ __global__ void __launch_bounds__(kBookThreads) pages_compact_kernel(kvq_page_bo
     }
 }
 
+// Rows take one another's sequences.  A page at the same place of both lists keeps its references as they are, so that what beams share costs a
+// look at two numbers.  References are added before any is taken; how many pages come free is known before anything is written, and where they do not
+// suffice for the copies the references go back.  New lists and lengths stand in `moves` meanwhile: every row may be read as a parent until all have been.
+// Scratch behind the triples: keeper [slots], the row that keeps a parent's last page (-1: the parent itself); length, packed pages [n]; lists
+// [n][max_pages].
+__global__ void __launch_bounds__(kBookThreads) pages_reorder_kernel(kvq_page_book b, const int32_t *rows, const int32_t *parents, int n, int beams, int32_t *moves) {
+    __shared__ BookShared s;
+    if (threadIdx.x == 0) moves[0] = 0;
+    if (refused(b)) return;
+    int32_t *keeper = moves + 4 + 3 * (int64_t)n, *length = keeper + b.slots, *packed = length + n, *lists = packed + n;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto parent_of = [&](int i) {                                 // -1: none
+        const int p = parents[i], row = beams > 0 ? p >= 0 && p < beams ? rows[i / beams * beams + p] : -1 : p;
+        return row >= 0 && row < b.slots ? row : -1;
+    };
+    auto seen = [&](int row) { return s_seen[row >> 5] >> (row & 31) & 1u; };
+    clear_seen(b);
+    bool bad = false;
+    for (int i = threadIdx.x; i < n; i += kBookThreads) {
+        const int p = parent_of(i);
+        bad |= !first_seen(b, rows[i]) || p < 0;
+        if (p >= 0) keeper[p] = INT32_MAX;
+    }
+    if (__syncthreads_or(bad)) {
+        if (threadIdx.x == 0) atomicOr(&b.count[2], KVQ_PAGES_BAD_ROWS);
+        return;
+    }
+    for (int i = threadIdx.x; i < n; i += kBookThreads) {
+        const int p = parent_of(i);
+        atomicMin(keeper + p, p == rows[i] || !seen(p) ? -1 : i);
+    }
+    __syncthreads();
+    // What becomes of row i: its lists' entries [0, held) and those of its parent [0, taken), the last of which is copied or not
+    struct Change { int row, parent, held, old_packed, taken, new_packed; bool copy; };
+    auto change_of = [&](int i) {
+        Change c;
+        c.row = rows[i];
+        c.parent = parent_of(i);
+        const int len = length_of(b, c.parent);
+        c.held = pages_of(length_of(b, c.row));
+        c.old_packed = packed_of(b, c.row);
+        c.taken = pages_of(len);
+        c.new_packed = packed_of(b, c.parent);
+        c.copy = c.parent != c.row && len % kPage && c.taken > c.new_packed && __ldcg(keeper + c.parent) != i;
+        return c;
+    };
+    auto ref_of = [&](int id, bool is_packed) { return inside(id, is_packed ? b.n_packed : b.n_fp16) ? b.refs + (is_packed ? id : b.n_packed + id) : nullptr; };
+    // f(place, old page or -1, new page or -1) for every page that row i loses or takes, the copied one left out of the latter
+    auto each = [&](int i, const Change &c, auto f) {
+        const int32_t *was = b.table + (int64_t)c.row * b.max_pages, *now = b.table + (int64_t)c.parent * b.max_pages;
+        for (int j = lane; j < max(c.held, c.taken); j += 32) {
+            const int o = j < c.held ? was[j] : -1, t = j < c.taken ? now[j] : -1;
+            const bool taken = j < c.taken && !(c.copy && j == c.taken - 1), same = taken && o == t && (j < c.old_packed) == (j < c.new_packed);
+            f(j, t, j < c.held && !same ? ref_of(o, j < c.old_packed) : nullptr, taken && !same ? ref_of(t, j < c.new_packed) : nullptr);
+        }
+    };
+    long long copies = 0, gone = 0;
+    for (int i = warp; i < n; i += kBookThreads / 32) {
+        const Change c = change_of(i);
+        if (c.parent == c.row) continue;
+        each(i, c, [&](int j, int t, int32_t *, int32_t *more) {
+            if (more) atomicAdd(more, 1);
+            if (j < c.taken) lists[(int64_t)i * b.max_pages + j] = t;
+        });
+        if (lane == 0) {
+            length[i] = length_of(b, c.parent);
+            packed[i] = c.new_packed;
+            copies += c.copy;
+        }
+    }
+    __syncthreads();
+    for (int i = warp; i < n; i += kBookThreads / 32) {
+        const Change c = change_of(i);
+        if (c.parent == c.row) continue;
+        each(i, c, [&](int j, int, int32_t *less, int32_t *) {
+            if (less && atomicSub(less, 1) == 1) gone += j >= c.old_packed;
+        });
+    }
+    copies = block_sum(s, copies);
+    __syncthreads();
+    gone = block_sum(s, gone);
+    const bool enough = copies <= free_fp16(b) + gone;
+    for (int i = warp; i < n; i += kBookThreads / 32) {
+        const Change c = change_of(i);
+        if (c.parent == c.row) continue;
+        each(i, c, [&](int, int, int32_t *less, int32_t *more) {
+            if (enough) {
+                if (less) atomicCAS(less, 0, kGone);
+            } else {
+                if (less) atomicAdd(less, 1);
+                if (more) atomicSub(more, 1);
+            }
+        });
+    }
+    if (!enough) {
+        if (threadIdx.x == 0) atomicOr(&b.count[2], KVQ_PAGES_NO_FP16);
+        return;
+    }
+    __syncthreads();
+    collect(s, b.refs, b.free_ids, b.n_packed, &b.count[0]);
+    collect(s, b.refs + b.n_packed, b.free_ids + b.n_packed, b.n_fp16, &b.count[1]);
+    __syncthreads();
+    const int n_free = free_fp16(b);
+    int at = 0, total;
+    for (int base = 0; base < n; base += kBookThreads) {
+        const int i = base + threadIdx.x;
+        bool changes = false, copy = false;
+        if (i < n) {
+            const int row = rows[i], p = parent_of(i);
+            changes = p != row;
+            copy = changes && length[i] % kPage && pages_of(length[i]) > packed[i] && __ldcg(keeper + p) != i;
+        }
+        s.before[threadIdx.x] = at + block_scan(s, copy, total);
+        s.need[threadIdx.x] = changes ? copy ? 2 : 1 : 0;
+        __syncthreads();
+        for (int r = warp; r < min(kBookThreads, n - base); r += kBookThreads / 32) {
+            if (!s.need[r]) continue;
+            const int i = base + r, row = rows[i], len = length[i], taken = pages_of(len), held = pages_of(length_of(b, row));
+            int32_t *t = b.table + (int64_t)row * b.max_pages;
+            for (int j = lane; j < max(taken, held); j += 32) {
+                int id = j < taken ? lists[(int64_t)i * b.max_pages + j] : -1;
+                if (s.need[r] == 2 && j == taken - 1) {
+                    const int m = s.before[r], own = n_free - 1 - m >= 0 ? b.free_ids[b.n_packed + n_free - 1 - m] : -1;
+                    const bool both = inside(id, b.n_fp16) && inside(own, b.n_fp16);
+                    moves[4 + 3 * m] = both ? id : 0;
+                    moves[5 + 3 * m] = both ? own : 0;
+                    moves[6 + 3 * m] = both ? len % kPage : 0;
+                    if (inside(own, b.n_fp16)) b.refs[b.n_packed + own] = 1;
+                    id = own;
+                }
+                t[j] = id;
+            }
+            __syncwarp();
+            if (lane == 0) {
+                b.length[row] = len;
+                b.packed[row] = packed[i];
+            }
+        }
+        at += total;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        moves[0] = at;
+        b.count[1] = max(n_free - at, 0);
+    }
+}
+
 // ---------------------------------------------------------------------------------------------
 // New tokens into their pages: a thread takes eight channels of one (token, head), keys and values.
 template <bool VEC>
@@ -417,6 +557,32 @@ __global__ void __launch_bounds__(256) page_copy_kernel(const __grid_constant__ 
             if ((int)threadIdx.x + 256 * i < n) x[i] = src[threadIdx.x + 256 * i];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
+            if ((int)threadIdx.x + 256 * i < n) dst[threadIdx.x + 256 * i] = x[i];
+    }
+}
+
+// The first tokens of pages: a unit is one head of a page of one tensor, its tokens lie side by side.
+__global__ void __launch_bounds__(256) page_copy_tails_kernel(const __grid_constant__ PageTensors p, const int32_t *moves, int max_moves) {
+    const int heads = p.first[p.n];
+    const int64_t units = (int64_t)min(moves[0], max_moves) * heads;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int m = (int)(u / heads), head = (int)(u - (int64_t)m * heads);
+        int lo = 0, hi = p.n;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (p.first[mid] <= head) lo = mid;
+            else hi = mid;
+        }
+        char *base = static_cast<char *>(p.t[lo].base) + (int64_t)(head - p.first[lo]) * (kPageHalf * 2);
+        const uint4 *src = reinterpret_cast<const uint4 *>(base + (int64_t)moves[4 + 3 * m] * p.t[lo].page_bytes);
+        uint4 *dst = reinterpret_cast<uint4 *>(base + (int64_t)moves[5 + 3 * m] * p.t[lo].page_bytes);
+        const int n = moves[6 + 3 * m] * (kHeadDim * 2 / 16);     // at most 2032
+        uint4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if ((int)threadIdx.x + 256 * i < n) x[i] = src[threadIdx.x + 256 * i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
             if ((int)threadIdx.x + 256 * i < n) dst[threadIdx.x + 256 * i] = x[i];
     }
 }
@@ -646,6 +812,41 @@ extern "C" int kvq_page_copy(const kvq_page_tensor *tensors, int32_t n, const in
     if (!p.n || max_moves <= 0) return KVQ_OK;
     const int64_t units = (int64_t)max_moves * p.first[p.n];
     page_copy_kernel<<<(unsigned)(units < 148 * 8 ? units : 148 * 8), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p, moves, max_moves);
+    return count_launch();
+}
+
+extern "C" uint64_t kvq_pages_reorder_moves(const kvq_page_book *b, int32_t n) {
+    using namespace kvq;
+    if (check_book(b) || n < 0) return 0;
+    return 4 + (uint64_t)n * (5 + (uint64_t)b->max_pages) + b->slots;
+}
+
+extern "C" int kvq_pages_reorder(const kvq_page_book *b, const int32_t *rows, const int32_t *parents, int32_t n, int32_t beams, int32_t *moves, kvq_stream_t stream) {
+    using namespace kvq;
+    if (const int rc = check_book(b)) return rc;
+    if (n < 0 || n > b->slots || beams < 0 || (beams > 0 && n % beams)) return KVQ_ERR_SHAPE;
+    if (!moves || (n && (!rows || !parents))) return KVQ_ERR_NULL;
+    if (const int rc = book_smem(pages_reorder_kernel, seen_bytes(*b))) return rc;
+    pages_reorder_kernel<<<1, kBookThreads, seen_bytes(*b), reinterpret_cast<cudaStream_t>(stream)>>>(*b, rows, parents, n, beams, moves);
+    return count_launch();
+}
+
+extern "C" int kvq_page_copy_tails(const kvq_page_tensor *tensors, int32_t n, const int32_t *moves, int32_t max_moves, kvq_stream_t stream) {
+    using namespace kvq;
+    if (n < 0 || n > KVQ_MAX_PAGE_TENSORS) return KVQ_ERR_SHAPE;
+    if (!moves || (n && !tensors)) return KVQ_ERR_NULL;
+    PageTensors p = {};
+    for (int i = 0; i < n; ++i) {
+        if (!tensors[i].base || tensors[i].page_bytes <= 0) continue;         // an empty pool
+        if (reinterpret_cast<uintptr_t>(tensors[i].base) % 16) return KVQ_ERR_ALIGN;
+        if (tensors[i].page_bytes % (kPageHalf * 2) || tensors[i].page_bytes > (1LL << 30)) return KVQ_ERR_SHAPE;
+        p.t[p.n] = tensors[i];
+        p.first[p.n + 1] = p.first[p.n] + (int)(tensors[i].page_bytes / (kPageHalf * 2));
+        ++p.n;
+    }
+    if (!p.n || max_moves <= 0) return KVQ_OK;
+    const int64_t units = (int64_t)max_moves * p.first[p.n];
+    page_copy_tails_kernel<<<(unsigned)(units < 148 * 8 ? units : 148 * 8), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p, moves, max_moves);
     return count_launch();
 }
 

@@ -16,7 +16,14 @@ __device__ __forceinline__ int pages_of(int tokens) { return (tokens + kPage - 1
 
 // Whether a call had to be refused: none changes the cache then.  A wait of the attention that gave up, and tokens that page_write left out, concern
 // their own call alone; were the writes behind it left out, tokens that are counted already would be missing in later layers.
-__device__ __forceinline__ bool refused(const kvq_page_book &b) { return b.count[2] & ~(KVQ_PAGES_STALLED | KVQ_PAGES_NOT_WRITTEN); }
+__device__ __forceinline__ bool refused(const kvq_page_book &b) { return b.count[2] & ~(KVQ_PAGES_STALLED | KVQ_PAGES_NOT_WRITTEN | KVQ_PAGES_NO_ANGLE); }
+
+// The bookkeeping's numbers as they are used: whatever the tensors hold, no index that follows from them leaves a tensor.
+__device__ __forceinline__ int length_of(const kvq_page_book &b, int row) { return min(max(b.length[row], 0), b.max_pages * kPage); }
+__device__ __forceinline__ int packed_of(const kvq_page_book &b, int row) { return min(max(b.packed[row], 0), pages_of(length_of(b, row))); }
+__device__ __forceinline__ int free_packed(const kvq_page_book &b) { return min(max(b.count[0], 0), b.n_packed); }
+__device__ __forceinline__ int free_fp16(const kvq_page_book &b) { return min(max(b.count[1], 0), b.n_fp16); }
+__device__ __forceinline__ bool inside(int id, int n) { return id >= 0 && id < n; }
 
 // Every size that a kernel's index arithmetic relies on.
 inline int check_book(const kvq_page_book *b) {

@@ -8,12 +8,14 @@ bit widths, its newest are fp16 (``include/kvmix_b200.h`` has the layouts, which
     pages_extend     new tokens' pages                    page_write       their keys and values, layer by layer
     paged_attention  one new token or chunks of them      pages_settle     full pages that leave the fp16 window are quantized
     pages_fork       a sequence branches                  pages_free       a sequence goes
-    pages_compact    pages in use move together           KVmixPagedCache  all of them with the tensors they work on
+    pages_compact    pages in use move together           pages_reorder    rows take one another's sequences (beam search)
+    page_append      page_write with the position rotation, for queries too
+    KVmixPagedCache  all of them with the tensors they work on
 
 The bookkeeping (``PageBook``) lives on the device and is changed by kernels only: no call waits for the host, all can be captured in a
 CUDA graph.  A call that cannot be done in full -- no page left, a row named twice -- does nothing but set a bit of ``count[2]``, and
 until that is cleared every call that changes the cache does nothing (``KVmixPagedCache.check`` raises and clears).  An attention
-that gave up waiting (its output is lost, the cache is whole) and a ``page_write`` that left tokens out set bits that hold nothing up.  The attention is
+that gave up waiting (its output is lost, the cache is whole) and a ``page_write`` or ``page_append`` that left tokens out set bits that hold nothing up.  The attention is
 softmax attention over the dequantised cache with scores, softmax and sums in fp32 (scores are not narrowed to fp16 as ``decode_attention`` does by
 default).  What is rounded to fp16 on the way to the tensor cores: weights; for several new tokens (and more than 8 query heads a kv head) dequantised
 keys and values; for one new token those of 3 bits, and weight * scale of a value.
@@ -28,6 +30,7 @@ import torch
 
 from . import _lib, ops
 from ._lib import check
+from .beams import beam_select
 
 PAGE_TOKENS = 128
 _SCALE = 1.0 / math.sqrt(128)
@@ -35,10 +38,12 @@ _MOST = 1 << 30                  # no sequence is longer: wider windows are this
 _MOST_HEADS = 1 << 15            # what kvq_page_copy takes as one page: 1 GB
 _STATUS = {1: "no free fp16 page", 2: "no free packed page", 4: "sequence longer than the table", 8: "bad rows (outside the table, named twice, "
            "a child that is not empty or also a parent)", 16: "an attention gave up waiting for its own copies, its output is not to be used",
-           32: "new tokens were not written, their page is packed, shared or not there"}
+           32: "new tokens were not written, their page is packed, shared or not there", 64: "new tokens were not written, their positions are "
+           "outside the tables of angles"}
 
 _pack_book, _pack_layer = struct.Struct("@6P4i").pack, struct.Struct("@8P6i").pack
 _pack_write, _pack_attn = struct.Struct("@2P4q2P2i").pack, struct.Struct("@2P4q5P8i2fPQ").pack
+_pack_append = struct.Struct("@6P10q3P8i").pack
 _addresses = struct.Struct("@8P").unpack_from             # of a layer's argument block
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
@@ -86,7 +91,8 @@ def page_groups(bits, group):
 
 @functools.lru_cache(maxsize=None)
 def _library():
-    for fmt, cls in (("@6P4i", _lib.PageBookArgs), ("@8P6i", _lib.PageLayerArgs), ("@2P4q2P2i", _lib.PageWriteArgs), ("@2P4q5P8i2fPQ", _lib.PagedAttnArgs)):
+    for fmt, cls in (("@6P4i", _lib.PageBookArgs), ("@8P6i", _lib.PageLayerArgs), ("@2P4q2P2i", _lib.PageWriteArgs), ("@2P4q5P8i2fPQ", _lib.PagedAttnArgs),
+                     ("@6P10q3P8i", _lib.PageAppendArgs)):
         assert -(-struct.calcsize(fmt) // 8) * 8 == C.sizeof(cls)
     return _lib.lib()
 
@@ -98,6 +104,7 @@ def _launch_count():
 
 
 _i32, _f16 = torch.int32, torch.float16
+_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
 def _ints(dev, name, t, n):
@@ -199,11 +206,12 @@ def _launched(rc):
         seen[0] = now
 
 
-def _copy(tensors, moves, max_moves):
-    """Whole pages of tensors given as (address, bytes of a page), from and to the numbers in `moves`."""
+def _copy(tensors, moves, max_moves, how=None):
+    """Pages of tensors given as (address, bytes of a page), from and to the numbers in `moves`: whole, or as `how` copies them."""
+    how = how or _library().kvq_page_copy
     for at in range(0, len(tensors), 2 * _lib.MAX_PAGE_TENSORS):
         some = tensors[at:at + 2 * _lib.MAX_PAGE_TENSORS]
-        _launched(_library().kvq_page_copy(struct.pack("@" + "Pq" * (len(some) // 2), *some), len(some) // 2, moves, max_moves, ops.raw_stream()))
+        _launched(how(struct.pack("@" + "Pq" * (len(some) // 2), *some), len(some) // 2, moves, max_moves, ops.raw_stream()))
 
 
 @_on_its_device(2)
@@ -241,6 +249,55 @@ def page_write(k, v, q_start, rows, pages, layer):
     _launched(_library().kvq_page_write(book, _layer(pages, dev, layer), a, ops.raw_stream()))
 
 
+@_on_its_device(6)
+def page_append(k, v, cos, sin, q_start, rows, pages, layer, q=None, q_out=None, positions=None, interleaved=False, parts=1):
+    """``page_write`` of keys and values from the projections: keys are rotated by their positions' angles on the way, and so are the step's queries.
+
+    k, v [tokens, Hkv, 128], q [tokens, nh, 128]: fp16, bf16 or fp32, one type, any strides.  cos, sin fp32 [positions, angles], contiguous along the angles, angles a
+    multiple of 8: pair i of a head's channels, (i, i + angles) or, interleaved, (2i, 2i + 1), is turned by angle i of the token's row; channels from 2 * angles on stay.
+    parts = 2: the two halves of a head are turned each for itself (``paged_differential_attention``), angles up to 32 then.  A token's row is its
+    place in the sequence, or positions[token] (int32 [tokens]).  Rotations are fp32 products and sums, rounded once to fp16.
+    Tokens that ``page_write`` would leave out are left out; those whose position is outside the tables too, their queries with them, and a
+    status bit says so.  Returns the queries, fp16 (q_out where it is given, which may be q itself; None without q); rows behind q_start[n] are left as they are."""
+    dev, book = _book(pages)
+    heads, tokens = layer.kfull.shape[1], k.shape[0]
+    if k.dim() != 3 or k.shape[1:] != (heads, 128) or v.shape != k.shape or v.dtype is not k.dtype or k.dtype not in _TYPES:
+        raise RuntimeError(f"page_append takes keys and values [tokens, {heads}, 128] of one type, fp16, bf16 or fp32")
+    if q is None:
+        if q_out is not None:
+            raise RuntimeError("q_out without q")
+    elif q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != 128 or q.dtype is not k.dtype:
+        raise RuntimeError(f"queries must be [{tokens}, heads, 128] of the keys' type")
+    if any(t.get_device() != dev for t in (k, v, cos, sin) + (() if q is None else (q,))):
+        raise RuntimeError(f"keys, values, queries and angles must be on cuda:{dev}")
+    if cos.dim() != 2 or sin.shape != cos.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or (cos.numel() and (cos.stride(1) != 1 or sin.stride(1) != 1)):
+        raise RuntimeError("cos and sin must be float32 [positions, angles], contiguous along the angles")
+    angle_rows, angles = cos.shape
+    if parts not in (1, 2) or angles % 8 or not 0 < angles <= 64 // parts:
+        raise RuntimeError("angles must be a multiple of 8, at most 64 / parts; parts 1 or 2")
+    if k.stride(2) != 1:
+        k = k.contiguous()
+    if v.stride(2) != 1:
+        v = v.contiguous()
+    at_q = at_out = nh = 0
+    strides = (0, 0, 0, 0)
+    if q is not None:
+        nh = q.shape[1]
+        if q_out is None:
+            q_out = q.new_empty(q.shape, dtype=_f16)
+        elif q_out.shape != q.shape or q_out.dtype is not _f16 or q_out.get_device() != dev or q_out.stride(2) != 1 or not _rows_apart(q_out):
+            raise RuntimeError("q_out must be fp16 like q, contiguous along the channels, its rows apart")
+        if q.stride(2) != 1:
+            q = q.contiguous()
+        at_q, at_out, strides = q.data_ptr(), q_out.data_ptr(), (q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1))
+    n = rows.numel()
+    a = _pack_append(k.data_ptr(), v.data_ptr(), at_q, at_out, cos.data_ptr(), sin.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), *strides,
+                     cos.stride(0), sin.stride(0), _ints(dev, "q_start", q_start, n + 1), _rows(dev, "rows", rows),
+                     0 if positions is None else _ints(dev, "positions", positions, tokens), n, tokens, nh, _TYPES[k.dtype], angles, angle_rows, parts, 1 if interleaved else 0)
+    _launched(_library().kvq_page_append(book, _layer(pages, dev, layer), a, ops.raw_stream()))
+    return q_out
+
+
 @_on_its_device(2)
 def pages_settle(rows, window, pages, layers):
     """Full pages that end ``window`` tokens or more before their sequence's end are quantized in every layer and their fp16 pages given
@@ -272,6 +329,30 @@ def pages_fork(parents, children, pages, layers):
     moves = pages.count.new_empty(4 + 2 * n)
     _launched(_library().kvq_pages_fork(book, _rows(dev, "parents", parents), _ints(dev, "children", children, n), n, moves.data_ptr(), ops.raw_stream()))
     _copy(tensors, moves.data_ptr(), n)
+
+
+@_on_its_device(2)
+def pages_reorder(rows, parents, pages, layers, beams=None):
+    """Rows take one another's sequences, all at once: row rows[i] becomes what row parents[i] was before the call (int32 [n] each, no row twice).  With ``beams``, n
+    is a multiple of it and parents[i] counts within i's group of that many rows, as ``beam_select`` gives it.  A parent may be taken by several rows, by
+    none (its sequence goes), and may be a row that is not among them (it stays).  Full pages are shared; of a last page that is not full one taker keeps the page,
+    the others get pages of their own with its tokens, for which the pages that the call sets free serve too."""
+    dev, book = _book(pages)
+    parents, n, tensors = parents.reshape(-1), rows.numel(), []
+    if beams is not None and (beams <= 0 or n % beams):
+        raise RuntimeError("rows must come in groups of `beams`")
+    if n > pages.table.shape[0]:
+        raise RuntimeError("more rows than the table has")
+    for layer in layers:
+        size = layer.kfull.shape[1] * PAGE_TOKENS * 256
+        for at in _fp16_pages(pages, dev, layer):
+            tensors += (at, size)
+    _movable(layers, tensors[::2])
+    L = _library()
+    moves = pages.count.new_empty(L.kvq_pages_reorder_moves(book, n))
+    at = moves.data_ptr()
+    _launched(L.kvq_pages_reorder(book, _rows(dev, "rows", rows), _ints(dev, "parents", parents, n), n, beams or 0, at, ops.raw_stream()))
+    _copy(tensors, at, n, L.kvq_page_copy_tails)
 
 
 @_on_its_device(0)
@@ -377,6 +458,7 @@ class KVmixPagedCache:
             out = cache.attend(l, q, step)             # [tokens, nh, 128]; options as paged_attention
         cache.settle(rows)                             # full pages behind the window are quantized
 
+    ``append`` takes keys and queries as the projections give them and rotates both; ``advance`` ends a step of beam search.
     ``lengths`` mirrors the lengths on the host (it lays out the work); ``check()`` raises if a call had to be refused."""
 
     def __init__(self, layers, kv_heads, head_dim, max_seqs, max_tokens, packed_pages, fp16_pages, group_size, residual_length=128, device="cuda"):
@@ -454,6 +536,15 @@ class KVmixPagedCache:
         return paged_attention(q, step.q_start, step.rows, self.book, self.layers[layer], max_new=max(step.max_new, 1), max_tokens=max(step.max_tokens, 1),
                                max_chunks=step.max_chunks, **options)
 
+    def append(self, layer, k, v, cos, sin, step, q=None, **options):
+        """``write`` of keys that are not rotated yet, and the step's queries rotated: returns them.  Options as ``page_append``: q_out, positions, interleaved,
+        parts."""
+        if k.shape[0] != step.tokens or v.shape[0] != step.tokens or (q is not None and q.shape[0] != step.tokens):
+            raise RuntimeError("keys, values and queries for every new token of the step")
+        if options.get("positions") is None and cos.shape[0] < step.max_tokens:
+            raise RuntimeError(f"angles for {cos.shape[0]} positions, the step has tokens up to {step.max_tokens}")
+        return page_append(k, v, cos, sin, step.q_start, step.rows, self.book, self.layers[layer], q=q, **options)
+
     def settle(self, rows=None):
         rows = range(len(self.lengths)) if rows is None else rows
         pages_settle(self._row_tensor(rows)[1], self.window, self.book, self.layers)
@@ -466,6 +557,36 @@ class KVmixPagedCache:
         pages_fork(at, to, self.book, self.layers)
         for p, c in zip(parents, children):
             self.lengths[c] = self.lengths[p]
+
+    def reorder(self, rows, parents, beams=None):
+        """Row rows[i] becomes what row parents[i] was (``pages_reorder``).  With ``beams``, parents are the beams within each group of that many rows: a list or,
+        as ``beam_select`` returns them, int32 on the device; the rows of a group then have one length."""
+        rows, at = self._row_tensor(rows)
+        if beams is not None and (beams <= 0 or len(rows) % beams):
+            raise RuntimeError("rows must come in groups of `beams`")
+        if isinstance(parents, torch.Tensor):
+            if beams is None or parents.numel() != len(rows):
+                raise RuntimeError("parents on the device are beams within groups of rows, one a row")
+            if any(self.lengths[r] != self.lengths[rows[i // beams * beams]] for i, r in enumerate(rows)):
+                raise RuntimeError("the rows of a group must have one length where parents are on the device")
+            pages_reorder(at, parents, self.book, self.layers, beams)
+            return
+        parents = [int(p) for p in parents]
+        if len(parents) != len(rows) or any(not 0 <= p < (len(self.lengths) if beams is None else beams) for p in parents):
+            raise RuntimeError("one parent for every row")
+        if beams is not None:
+            parents = [rows[i // beams * beams + p] for i, p in enumerate(parents)]
+        pages_reorder(at, self._row_tensor(parents, distinct=False)[1], self.book, self.layers)
+        lengths = [self.lengths[p] for p in parents]
+        for r, n in zip(rows, lengths):
+            self.lengths[r] = n
+
+    def advance(self, rows, logits, scores, beams, **options):
+        """The end of a step of beam search: the best continuations of every group of ``beams`` rows (``beam_select``, whose options these are), which the rows
+        then hold (``reorder``).  Returns the ``BeamStep``: its next_tokens are the next step's."""
+        chosen = beam_select(logits, scores, beams, **options)
+        self.reorder(rows, chosen.next_beams, beams)
+        return chosen
 
     def free(self, rows):
         rows, at = self._row_tensor(rows)
