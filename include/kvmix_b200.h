@@ -649,6 +649,23 @@ uint64_t kvq_paged_attn_workspace_bytes(const kvq_page_layer *l, int32_t n, int3
                                         int32_t max_chunks);
 int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, const kvq_paged_attn_args *a, kvq_stream_t stream);
 
+/*
+ * Differential attention over the same pages: a head's 128 channels of q and k are two halves of 64, (q1, q2) and (k1, k2), and
+ *   out = (softmax(s1) - lambdas[h] * softmax(s2)) . v,   s1 = q1.k1 * softmax_scale, s2 = q2.k2 * softmax_scale,
+ * both capped, biased and masked as kvq_paged_attn says; then, with norm_weight [128], out = out / sqrt(mean(out^2) + norm_eps) * norm_weight.  The two attentions
+ * stay in fp32 until their difference is rounded.  lambdas [nh], norm_weight [128] or NULL: fp32, device memory.
+ * workspace: kvq_paged_diff_attn_workspace_bytes(...) bytes.
+ */
+typedef struct {
+    kvq_paged_attn_args a;
+    const float *lambdas, *norm_weight;
+    float norm_eps;
+} kvq_paged_diff_args;
+
+uint64_t kvq_paged_diff_attn_workspace_bytes(const kvq_page_layer *l, int32_t n, int32_t tokens, int32_t nh, int32_t max_new, int32_t max_tokens,
+                                             int32_t max_chunks);
+int kvq_paged_diff_attn(const kvq_page_book *b, const kvq_page_layer *l, const kvq_paged_diff_args *a, kvq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -114,6 +114,10 @@ class PagedAttnArgs(C.Structure):
                 ("softmax_scale", C.c_float), ("softcap", C.c_float), ("workspace", vp), ("workspace_bytes", u64)]
 
 
+class PagedDiffArgs(C.Structure):
+    _fields_ = [("a", PagedAttnArgs), ("lambdas", vp), ("norm_weight", vp), ("norm_eps", C.c_float)]
+
+
 class PageAppendArgs(C.Structure):
     _fields_ = [("k", vp), ("v", vp), ("q", vp), ("q_out", vp), ("cos", vp), ("sin", vp),
                 ("k_sT", i64), ("k_sH", i64), ("v_sT", i64), ("v_sH", i64), ("q_sT", i64), ("q_sH", i64), ("o_sT", i64), ("o_sH", i64),
@@ -180,13 +184,14 @@ def lib():
         for fn, types in ((L.kvq_pages_extend, [blk, vp, vp, i32, vp]), (L.kvq_pages_free, [blk, vp, i32, vp]),
                           (L.kvq_pages_settle, [blk, vp, i32, i32, vp, vp]), (L.kvq_page_pack, [blk, vp, i32, vp]),
                           (L.kvq_pages_fork, [blk, vp, vp, i32, vp, vp]), (L.kvq_pages_compact, [blk, vp, vp]),
-                          (L.kvq_page_copy, [blk, i32, vp, i32, vp]), (L.kvq_page_write, [blk, blk, blk, vp]), (L.kvq_paged_attn, [blk, blk, blk, vp]),
+                          (L.kvq_page_copy, [blk, i32, vp, i32, vp]), (L.kvq_page_write, [blk, blk, blk, vp]), (L.kvq_paged_attn, [blk, blk, blk, vp]), (L.kvq_paged_diff_attn, [blk, blk, blk, vp]),
                           (L.kvq_page_append, [blk, blk, blk, vp]), (L.kvq_pages_reorder, [blk, vp, vp, i32, i32, vp, vp]),
                           (L.kvq_page_copy_tails, [blk, i32, vp, i32, vp]), (L.kvq_beam_select, [blk, vp])):
             fn.restype, fn.argtypes = C.c_int, types
         L.kvq_pages_reorder_moves.restype, L.kvq_pages_reorder_moves.argtypes = u64, [blk, i32]
         L.kvq_beam_select_workspace_bytes.restype, L.kvq_beam_select_workspace_bytes.argtypes = u64, [blk]
-        L.kvq_paged_attn_workspace_bytes.restype, L.kvq_paged_attn_workspace_bytes.argtypes = u64, [blk] + [i32] * 6
+        for fn in (L.kvq_paged_attn_workspace_bytes, L.kvq_paged_diff_attn_workspace_bytes):
+            fn.restype, fn.argtypes = u64, [blk] + [i32] * 6
         _lib = L
     return _lib
 
@@ -196,7 +201,7 @@ EXPORTS = ["kvq_version", "kvq_error_string", "kvq_last_cuda_error", "kvq_featur
            "kvq_decode_attn_static", "kvq_decode_attn_plan", "kvq_decode_attn_workspace_init", "kvq_prefill", "kvq_peer_wait", "kvq_peer_wait_next", "kvq_append_k", "kvq_append_v",
            "kvq_pages_extend", "kvq_pages_free", "kvq_pages_settle", "kvq_page_pack", "kvq_pages_fork", "kvq_pages_compact", "kvq_page_copy", "kvq_page_write",
            "kvq_paged_attn", "kvq_paged_attn_workspace_bytes", "kvq_page_append", "kvq_pages_reorder", "kvq_pages_reorder_moves", "kvq_page_copy_tails",
-           "kvq_beam_select", "kvq_beam_select_workspace_bytes"]
+           "kvq_beam_select", "kvq_beam_select_workspace_bytes", "kvq_paged_diff_attn", "kvq_paged_diff_attn_workspace_bytes"]
 
 
 def check(rc):

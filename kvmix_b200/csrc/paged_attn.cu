@@ -1,4 +1,4 @@
-// kvq_paged_attn: checks, the plan of a call, its launches.
+// kvq_paged_attn and kvq_paged_diff_attn: checks, the plan of a call, its launches.
 #include "paged_attn.cuh"
 
 #include <cfloat>
@@ -14,8 +14,24 @@ int paged_tiles_1(const PagedArgs &p, int max_tiles, cudaStream_t st);          
 int paged_tiles_2(const PagedArgs &p, int max_tiles, cudaStream_t st);
 int paged_tiles_3(const PagedArgs &p, int max_tiles, cudaStream_t st);
 int paged_tiles_4(const PagedArgs &p, int max_tiles, cudaStream_t st);
+int paged_diff_few_1(const PagedArgs &p, cudaStream_t st);                       // paged_diff_few_1.cu ..
+int paged_diff_few_2(const PagedArgs &p, cudaStream_t st);
+int paged_diff_few_3(const PagedArgs &p, cudaStream_t st);
+int paged_diff_few_4(const PagedArgs &p, cudaStream_t st);
+int paged_diff_tiles_1(const PagedArgs &p, int max_tiles, cudaStream_t st);      // paged_diff_tiles_1.cu ..
+int paged_diff_tiles_2(const PagedArgs &p, int max_tiles, cudaStream_t st);
+int paged_diff_tiles_3(const PagedArgs &p, int max_tiles, cudaStream_t st);
+int paged_diff_tiles_4(const PagedArgs &p, int max_tiles, cudaStream_t st);
 
 static int paged_few(const PagedArgs &p, cudaStream_t st) {
+    if (p.lambdas) {
+        switch (p.l.k_bits) {
+            case 1: return paged_diff_few_1(p, st);
+            case 2: return paged_diff_few_2(p, st);
+            case 3: return paged_diff_few_3(p, st);
+            default: return paged_diff_few_4(p, st);
+        }
+    }
     switch (p.l.k_bits) {
         case 1: return paged_few_1(p, st);
         case 2: return paged_few_2(p, st);
@@ -24,6 +40,14 @@ static int paged_few(const PagedArgs &p, cudaStream_t st) {
     }
 }
 static int paged_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
+    if (p.lambdas) {
+        switch (p.l.k_bits) {
+            case 1: return paged_diff_tiles_1(p, max_tiles, st);
+            case 2: return paged_diff_tiles_2(p, max_tiles, st);
+            case 3: return paged_diff_tiles_3(p, max_tiles, st);
+            default: return paged_diff_tiles_4(p, max_tiles, st);
+        }
+    }
     switch (p.l.k_bits) {
         case 1: return paged_tiles_1(p, max_tiles, st);
         case 2: return paged_tiles_2(p, max_tiles, st);
@@ -32,10 +56,11 @@ static int paged_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
     }
 }
 
-// Partial sums of the splits -> outputs, in the splits' order: a row a warp.  `few`: rows of the kernel of few rows, kFewRows places for every (sequence,
-// kv head); else rows of q, of which those that the kernel of tiles had are joined.
+// Partial sums of the splits -> outputs, in the splits' order: a row a warp, or a head's two rows.  `few`: rows of the kernel of few rows, kFewRows places
+// for every (sequence, kv head); else rows of q, of which those that the kernel of tiles had are joined.
+template <bool DIFF>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant__ PagedArgs p, int few) {
-    const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t at = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (DIFF ? 2 : 1);
     const int lane = threadIdx.x & 31;
     const int64_t step = p.part_rows;
     int64_t row;
@@ -60,24 +85,44 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
             if (s.n_new * p.rep <= p.few_rows) return;
         }
     }
-    float m = -INFINITY, l = 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = lane; i < p.splits; i += 32) m = fmaxf(m, p.part_ml[2 * (i * step + row)]);
-    m = warp_max(m);
-    for (int base = 0; base < p.splits; base += 8) {              // eight splits' loads under way at once: one by one each waits for L2
-        float2 ml[8];
-        float4 x[8];
+    auto join = [&](int64_t row, float &l) {
+        float m = -INFINITY;
+        l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = lane; i < p.splits; i += 32) m = fmaxf(m, p.part_ml[2 * (i * step + row)]);
+        m = warp_max(m);
+        for (int base = 0; base < p.splits; base += 8) {          // eight splits' loads under way at once: one by one each waits for L2
+            float2 ml[8];
+            float4 x[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int64_t at_i = (int64_t)min(base + k, p.splits - 1) * step + row;
-            ml[k] = *reinterpret_cast<const float2 *>(p.part_ml + 2 * at_i);
-            x[k] = *reinterpret_cast<const float4 *>(p.part_out + at_i * 128 + 4 * lane);
-        }
+            for (int k = 0; k < 8; ++k) {
+                const int64_t at_i = (int64_t)min(base + k, p.splits - 1) * step + row;
+                ml[k] = *reinterpret_cast<const float2 *>(p.part_ml + 2 * at_i);
+                x[k] = *reinterpret_cast<const float4 *>(p.part_out + at_i * 128 + 4 * lane);
+            }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float f = base + k < p.splits ? part_factor(ml[k].x, ml[k].y, m) : 0.f;
-            if (f != 0.f) { l += f * ml[k].y; v.x += f * x[k].x; v.y += f * x[k].y; v.z += f * x[k].z; v.w += f * x[k].w; }
+            for (int k = 0; k < 8; ++k) {
+                const float f = base + k < p.splits ? part_factor(ml[k].x, ml[k].y, m) : 0.f;
+                if (f != 0.f) { l += f * ml[k].y; v.x += f * x[k].x; v.y += f * x[k].y; v.z += f * x[k].z; v.w += f * x[k].w; }
+            }
         }
+        return v;
+    };
+    float l;
+    float4 v = join(row, l);
+    if constexpr (DIFF) {
+        float l2;
+        float4 w = join(row + 1, l2);
+        h >>= 1;
+        const float lambda = p.lambdas[h];
+        auto one = [&](float a, float b) { return diff_of(l == 0.f ? 0.f : a / l, l2 == 0.f ? 0.f : b / l2, lambda); };
+        v = make_float4(one(v.x, w.x), one(v.y, w.y), one(v.z, w.z), one(v.w, w.w));
+        if (p.norm_weight) {
+            const float by = diff_norm(p, warp_sum(v.x * v.x + v.y * v.y + (v.z * v.z + v.w * v.w)));
+            const float *weight = p.norm_weight + 4 * lane;
+            v = make_float4(v.x * (by * weight[0]), v.y * (by * weight[1]), v.z * (by * weight[2]), v.w * (by * weight[3]));
+        }
+        l = 1.f;
     }
     __half *out = static_cast<__half *>(p.a.out) + (int64_t)u * p.a.o_sT + (int64_t)h * p.a.o_sH + 4 * lane;
     auto put = [&](int c, float x) { out[c] = __float2half_rn(l == 0.f ? 0.f : x / l); };
@@ -90,7 +135,8 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
 static int paged_merge(const PagedArgs &p, int few, cudaStream_t st) {
     const int64_t rows = few ? (int64_t)p.a.n * p.l.Hkv * kFewRows : (int64_t)p.a.tokens * p.a.nh, grid = (rows + 7) / 8;
     if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
-    paged_merge_kernel<<<(unsigned)grid, 256, 0, st>>>(p, few);
+    if (p.lambdas) paged_merge_kernel<true><<<(unsigned)((grid + 1) / 2), 256, 0, st>>>(p, few);
+    else paged_merge_kernel<false><<<(unsigned)grid, 256, 0, st>>>(p, few);
     return count_launch();
 }
 
@@ -101,7 +147,7 @@ struct PagedPlan {
     int few_splits, tile_splits, max_tiles;
 };
 
-static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, int max_new, int max_tokens, int max_chunks) {
+static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, int max_new, int max_tokens, int max_chunks, bool diff) {
     PagedPlan r = {};
     const int rep = nh / l.Hkv;
     const int64_t most = (int64_t)max_new * rep;
@@ -112,7 +158,7 @@ static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, 
     const int pages = (max_tokens + kPage - 1) / kPage;
     // Kernel of few rows: the splits that take the fewest rounds of pages (four warps a CTA), over all waves of CTAs; a CTA's beginning and
     // end count two rounds, the launch that joins the splits another two.
-    const FewShape f = few_shape(l, rep, max_new);
+    const FewShape f = diff ? diff_shape(l, rep, max_new) : few_shape(l, rep, max_new);
     const int64_t pairs = (int64_t)n * l.Hkv * f.row_blocks, slots = 148 * f.ctas;
     double best = 1e30;
     r.few_splits = 1;
@@ -161,29 +207,46 @@ extern "C" uint64_t kvq_paged_attn_workspace_bytes(const kvq_page_layer *l, int3
                                                    int32_t max_chunks) {
     using namespace kvq;
     if (check_layer(l) || n <= 0 || tokens <= 0 || nh <= 0 || nh % l->Hkv || max_new <= 0 || max_tokens <= 0 || max_chunks < 0) return 0;
-    return paged_bytes(paged_plan(*l, n, tokens, nh, max_new, max_tokens, max_chunks), n, l->Hkv, tokens, nh);
+    return paged_bytes(paged_plan(*l, n, tokens, nh, max_new, max_tokens, max_chunks, false), n, l->Hkv, tokens, nh);
 }
 
-extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, const kvq_paged_attn_args *a, kvq_stream_t stream) {
+extern "C" uint64_t kvq_paged_diff_attn_workspace_bytes(const kvq_page_layer *l, int32_t n, int32_t tokens, int32_t nh, int32_t max_new, int32_t max_tokens,
+                                                        int32_t max_chunks) {
     using namespace kvq;
+    if (check_layer(l) || n <= 0 || tokens <= 0 || nh <= 0 || nh > INT32_MAX / 2 || nh % l->Hkv || max_new <= 0 || max_tokens <= 0 || max_chunks < 0) return 0;
+    return paged_bytes(paged_plan(*l, n, tokens, 2 * nh, max_new, max_tokens, max_chunks, true), n, l->Hkv, tokens, 2 * nh);
+}
+
+namespace kvq {
+
+// a->nh counts heads; two rows each where `diff` is given
+static int attend(const kvq_page_book *b, const kvq_page_layer *l, const kvq_paged_attn_args *a, const kvq_paged_diff_args *diff, kvq_stream_t stream) {
     if (const int rc = check_book(b)) return rc;
     if (const int rc = check_layer(l)) return rc;
     if (!a) return KVQ_ERR_NULL;
     if (a->n < 0 || a->tokens < 0 || a->nh <= 0 || a->window < 0) return KVQ_ERR_SHAPE;
     if (a->nh % l->Hkv) return KVQ_ERR_HEADS;
+    if (diff && a->nh > INT32_MAX / 2) return KVQ_ERR_UNSUPPORTED;
+    const int nh = diff ? 2 * a->nh : a->nh;
     if (a->n == 0 || a->tokens == 0) return KVQ_OK;
     if (a->max_new <= 0 || a->max_tokens <= 0 || a->max_chunks < 0) return KVQ_ERR_SHAPE;
     if (!a->q || !a->out || !a->q_start || !a->rows) return KVQ_ERR_NULL;
     if (!(a->softcap >= 0.f) || !(fabsf(a->softmax_scale) <= FLT_MAX)) return KVQ_ERR_SHAPE;
-    const PagedPlan r = paged_plan(*l, a->n, a->tokens, a->nh, a->max_new, a->max_tokens, a->max_chunks);
-    const uint64_t need = paged_bytes(r, a->n, l->Hkv, a->tokens, a->nh);
+    const PagedPlan r = paged_plan(*l, a->n, a->tokens, nh, a->max_new, a->max_tokens, a->max_chunks, diff);
+    const uint64_t need = paged_bytes(r, a->n, l->Hkv, a->tokens, nh);
     if (need && (!a->workspace || a->workspace_bytes < need)) return KVQ_ERR_WORKSPACE;
     if (need && reinterpret_cast<uintptr_t>(a->workspace) % 16) return KVQ_ERR_ALIGN;
     PagedArgs p = {};
     p.b = *b;
     p.l = *l;
     p.a = *a;
-    p.rep = a->nh / l->Hkv;
+    p.a.nh = nh;
+    p.rep = nh / l->Hkv;
+    if (diff) {
+        p.lambdas = diff->lambdas;
+        p.norm_weight = diff->norm_weight;
+        p.norm_eps = diff->norm_eps;
+    }
     p.k_groups = page_groups(l->k_bits, l->group);
     p.v_groups = page_groups(l->v_bits, l->group);
     p.few_rows = r.few_rows;
@@ -198,8 +261,8 @@ extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, c
     p.part_out = static_cast<float *>(a->workspace);
     if (r.few) {
         p.splits = r.few_splits;
-        p.part_rows = few_part_rows(r, a->n, l->Hkv, a->tokens, a->nh);
-        p.part_compact = few_compact(r, a->n, l->Hkv, a->tokens, a->nh);
+        p.part_rows = few_part_rows(r, a->n, l->Hkv, a->tokens, nh);
+        p.part_compact = few_compact(r, a->n, l->Hkv, a->tokens, nh);
         p.part_ml = p.part_out + p.splits * p.part_rows * kHeadDim;
         if (const int rc = paged_few(p, st)) return rc;
         if (p.splits > 1)
@@ -207,11 +270,25 @@ extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, c
     }
     if (r.tiles) {
         p.splits = r.tile_splits;
-        p.part_rows = (int64_t)a->tokens * a->nh;
+        p.part_rows = (int64_t)a->tokens * nh;
         p.part_ml = p.part_out + p.splits * p.part_rows * kHeadDim;
         if (const int rc = paged_tiles(p, r.max_tiles, st)) return rc;
         if (p.splits > 1)
             if (const int rc = paged_merge(p, 0, st)) return rc;
     }
     return KVQ_OK;
+}
+
+}  // namespace kvq
+
+extern "C" int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, const kvq_paged_attn_args *a, kvq_stream_t stream) {
+    return kvq::attend(b, l, a, nullptr, stream);
+}
+
+extern "C" int kvq_paged_diff_attn(const kvq_page_book *b, const kvq_page_layer *l, const kvq_paged_diff_args *a, kvq_stream_t stream) {
+    using namespace kvq;
+    if (!a) return KVQ_ERR_NULL;
+    if (a->a.n > 0 && a->a.tokens > 0 && !a->lambdas) return KVQ_ERR_NULL;
+    if (a->norm_weight && !(a->norm_eps >= 0.f && a->norm_eps <= FLT_MAX)) return KVQ_ERR_SHAPE;
+    return attend(b, l, &a->a, a, stream);
 }

@@ -23,7 +23,14 @@ struct PagedArgs {
     bool part_compact;                // the latter
     float *part_out;                  // [splits][part_rows][128], unnormalised
     float *part_ml;                   // [splits][part_rows][2]: the exponents' reference (log2), the weights' sum
+    // Differential attention: a query head is two rows, one for each half of its channels, next to each other; a.nh and rep count them apart
+    // everywhere, slopes and outputs are those of query heads.
+    const float *lambdas, *norm_weight;                           // [query heads]; [128] or NULL
+    float norm_eps;
 };
+// What becomes of a head's two attentions over the values, channel by channel; then its norm over the channels, where there is one: x * diff_norm() * weight
+__device__ __forceinline__ float diff_of(float a, float b, float lambda) { return fmaf(-lambda, b, a); }
+__device__ __forceinline__ float diff_norm(const PagedArgs &p, float squares) { return rsqrtf(fmaf(squares, 1.f / kHeadDim, p.norm_eps)); }
 
 // Sequence i as every thread sees it: its row of the table, length, packed pages, where its new tokens are.  Numbers that would lead
 // outside anything are made harmless.
@@ -70,6 +77,22 @@ inline FewShape few_shape(const kvq_page_layer &l, int rep, int max_new) {
     } else if (f.rows > rows) {
         f.rows = rows < 1 ? 1 : rows;
     }
+    f.row_blocks = (rows + f.rows - 1) / f.rows;
+    return f;
+}
+
+// The same where heads are two rows each: a channel belongs to one half of the keys, so B's columns of a k-step hold that half's rows alone, and the columns of
+// one set that hold the keys of a head's two rows twice as hi and lo are as many as those that hold both rows' weights.  Two sets where
+// one does not hold all rows.
+inline FewShape diff_shape(const kvq_page_layer &l, int rep, int max_new) {
+    const int64_t most = (int64_t)max_new * rep;
+    const int rows = most < kFewRows ? (int)most : kFewRows, ng = kHeadDim / l.group;
+    FewShape f = {kFewRows, 1, 1, 3};
+    if (l.k_bits != 3 || l.v_bits != 3) {
+        if (rows > 8 / ng) f.key_sets = 2;
+        f.rows = 8 * f.key_sets / ng;
+    }
+    if (f.rows > rows) f.rows = rows;
     f.row_blocks = (rows + f.rows - 1) / f.rows;
     return f;
 }

@@ -154,8 +154,10 @@ struct FewShared {
     }
 };
 
-template <int KB, int VB, int CK>
-__global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 ? 3 : 4)
+// DIFF: heads are two rows each (PagedArgs), R is even; CK counts the sets of columns of keys and of values, and the score columns of a k-step are those of
+// the rows whose half it is in: a page's scores come half by half.
+template <int KB, int VB, int CK, bool DIFF>
+__global__ void __launch_bounds__(kFewWarps * 32, DIFF || KB == 3 || VB == 3 || CK == 2 ? 3 : 4)
     paged_few_kernel(const __grid_constant__ PagedArgs p, int R, int row_blocks, int stages, int stage_rows, int stage_bytes) {
     extern __shared__ __align__(128) char smem[];
     const FewShared sh(R, stages, stage_bytes);
@@ -181,9 +183,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
         const int row = row0 + r;
         float x[4] = {0.f, 0.f, 0.f, 0.f}, top = 0.f;
         if (r < rows) {
-            const __half *q = static_cast<const __half *>(p.a.q) + (int64_t)(s.q0 + row / p.rep) * p.a.q_sT + (int64_t)(head * p.rep + row % p.rep) * p.a.q_sH;
+            const __half *q = static_cast<const __half *>(p.a.q) + (int64_t)(s.q0 + row / p.rep) * p.a.q_sT + (int64_t)((head * p.rep + row % p.rep) >> (DIFF ? 1 : 0)) * p.a.q_sH;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) { x[c] = __half2float(q[lane + 32 * c]); top = fmaxf(top, fabsf(x[c])); }
+            for (int c = 0; c < 4; ++c) {
+                if (DIFF && (c >> 1) != (row & 1)) continue;      // the other half's channels: zero
+                x[c] = __half2float(q[lane + 32 * c]);
+                top = fmaxf(top, fabsf(x[c]));
+            }
         }
         top = warp_max_f32(top);
         const int e = top > 0.f && top < INFINITY ? (__float_as_int(top) >> 23 & 255) - 126 : 0;
@@ -199,7 +205,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
         const int row = row0 + threadIdx.x;
         if ((int)threadIdx.x < rows) {
             paged_bounds(p, s, row / p.rep, pos, lo, hi);
-            if (p.a.slopes) slope = p.a.slopes[head * p.rep + row % p.rep] * kLog2e;
+            if (p.a.slopes) slope = p.a.slopes[(head * p.rep + row % p.rep) >> (DIFF ? 1 : 0)] * kLog2e;
         }
         s_bounds[threadIdx.x] = make_int4(lo, hi, pos, __float_as_int(slope));
     }
@@ -427,16 +433,29 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
     const float aside_ref = ref;
 
     // ---- packed pages
-    float out[VT][4], out_mn[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int VN = DIFF && VB != 3 ? CK : 1;                  // sets of columns
+    float out[VN][VT][4], out_mn[VN][4];
 #pragma unroll
-    for (int m = 0; m < VT; ++m)
+    for (int n = 0; n < VN; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[m][e] = 0.f;
+        for (int e = 0; e < 4; ++e) {
+            out_mn[n][e] = 0.f;
+#pragma unroll
+            for (int m = 0; m < VT; ++m) out[n][m][e] = 0.f;
+        }
     // values' columns: group and row of B's column g, and of the accumulators' columns 2t, 2t + 1 (VPAIR: hi and lo of one row)
-    constexpr bool VPAIR = KB != 3 && VB != 3 && CK == 1;
-    const int vr_log2 = VB == 3 ? 3 : (VPAIR ? 2 : 3) - ng_log2, v_col = VPAIR ? g >> 1 : g, o_col = VPAIR ? t : 2 * t;
-    const int v_grp = v_col >> vr_log2, v_row = min(v_col & ((1 << vr_log2) - 1), R - 1), o_row = o_col & ((1 << vr_log2) - 1), o_grp = o_col >> vr_log2;
-    const int o_row1 = VPAIR ? o_row : o_row + 1;
+    constexpr bool VPAIR = !DIFF && KB != 3 && VB != 3 && CK == 1;
+    const int vr_log2 = VB == 3 ? 3 : (VPAIR ? 2 : 2 + VN) - ng_log2;
+    int v_grp[VN], v_row[VN], o_grp[VN], o_row[VN];
+#pragma unroll
+    for (int n = 0; n < VN; ++n) {
+        const int v_col = VPAIR ? g >> 1 : 8 * n + g, o_col = VPAIR ? t : 8 * n + 2 * t;
+        v_grp[n] = v_col >> vr_log2;
+        v_row[n] = min(v_col & ((1 << vr_log2) - 1), R - 1);
+        o_grp[n] = o_col >> vr_log2;
+        o_row[n] = o_col & ((1 << vr_log2) - 1);
+    }
+    auto o_row1 = [&](int n) { return VPAIR ? o_row[n] : o_row[n] + 1; };
     const uint32_t v_lo = VPAIR && (g & 1) ? 0xffffffffu : 0u;
     // p * scale * 2^expo: the power of two starts from the first scales (the largest of them becomes 4 to 8) and follows them where a stage's largest
     // would exceed 256 or stay below 2^-5; the sums so far go along, exactly
@@ -470,49 +489,82 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
             dense_scores(sc, [&](int m, int e) { return few_element<3>(g, m, e); });
         } else {
             float sc[CK][8][4], z[CK][4];
-            int row[CK], grp[CK];                                 // of B's column g of each set: pairs (hi, lo) of (group, row)
+            int row[CK], grp[CK];                                 // of B's column g of each set: pairs (hi, lo) of (group, row); DIFF: a head, in place of a row
             const int kr_log2 = 1 + CK - ng_log2;                 // log2 of the rows that 4 CK pairs hold
+            auto clear = [&]() {
+#pragma unroll
+                for (int n = 0; n < CK; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        z[n][e] = 0.f;
+#pragma unroll
+                        for (int m = 0; m < 8; ++m) sc[n][m][e] = 0.f;
+                    }
+            };
 #pragma unroll
             for (int n = 0; n < CK; ++n) {
                 const int pair = 4 * n + (g >> 1);
                 row[n] = pair & ((1 << kr_log2) - 1);
+                if (DIFF) row[n] = min(2 * row[n], R - 2);
                 grp[n] = pair >> kr_log2;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    z[n][e] = 0.f;
-#pragma unroll
-                    for (int m = 0; m < 8; ++m) sc[n][m][e] = 0.f;
-                }
             }
+            clear();
             const uint32_t lo_mask = g & 1 ? 0xffffffffu : 0u;
-#pragma unroll 1
-            for (int q = 0; q < half_stages; ++q) {
-                const uint32_t c = stage_ready(), c_sc = c + k_cb, c_mn = c_sc + k_sz;
-                if (!ok) break;
-                const int words = stage_rows * p.k_groups / 2;
-                const uint32_t look = lds32(c_sc + 4 * min(lane, words - 1));
-                if (lift || !__any_sync(0xffffffffu, max(look & 0xffffu, look >> 16) >= 0x2800u)) {
-                    uint32_t m2 = 0;
-                    for (int w = lane; w < words; w += 32) m2 = as_u32(__hmax2(as_h2(m2), as_h2(lds32(c_sc + 4 * w))));
-                    const int top = (int)(__reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16)) >> 10 & 31), old = lift;
-                    if (top + lift > 15 + 7 || top + lift < 10) lift = min(max(17 - top, 0), 15);
-                    for (int w = lane; lift && w < words; w += 32)
-                        asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(c_sc + 4 * w), "r"(as_u32(__hmul2(as_h2(lds32(c_sc + 4 * w)), as_h2((uint32_t)(lift + 15) * 0x04000400u)))) : "memory");
-                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");       // the next copy into this place is the async proxy's
-                    __syncwarp();
-                    if (lift != old) {
-                        const float f = exp2f((float)(lift - old));
+            // scores of the rows of half `which`, or of all
+            auto put_scores = [&](int which) {
+                const float undo = __int_as_float((127 - lift) << 23);
 #pragma unroll
-                        for (int n = 0; n < CK; ++n)
+                for (int n = 0; n < CK; ++n) {
+                    const int pair = 4 * n + t, head_of = pair & ((1 << kr_log2) - 1), r = DIFF ? 2 * head_of + which : head_of;
+                    const float zero = __shfl_sync(0xffffffffu, z[n][0], 4 * own_group + t);
+                    if (pair >> kr_log2 == own_group && r < rows) {
 #pragma unroll
-                            for (int m = 0; m < 8; ++m)
+                        for (int m = 0; m < 8; m += 2) {
+                            float v[4];
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) sc[n][m][e] *= f;
+                            for (int e = 0; e < 4; ++e) v[e] = fmaf(sc[n][m + (e >> 1)][2 * (e & 1)] + sc[n][m + (e >> 1)][2 * (e & 1) + 1], few_power<KB>(m + (e >> 1), e & 1) * undo, zero);
+                            sts_f4(s_s + r * 512 + (16 * g + 2 * m) * 4, v[0], v[1], v[2], v[3]);
+                        }
                     }
                 }
-                const __half *q_at = s_qs + q * stage_rows + 4 * t;
+            };
+            // a stage, or half a stage where that holds both halves
+            const int run = DIFF ? min(stage_rows, 64) : stage_rows, runs = DIFF ? max(half_stages, 2) : half_stages;
+            uint32_t c = 0;
 #pragma unroll 1
-                for (int at = 0; at < stage_rows; at += 16) {
+            for (int q = 0; q < runs; ++q) {
+                const int in_stage = DIFF && stage_rows == kPage ? q * run : 0;
+                if (!DIFF || in_stage == 0) {
+                    c = stage_ready();
+                    if (!ok) break;
+                }
+                const uint32_t c_sc = c + k_cb, c_mn = c_sc + k_sz;
+                if (!DIFF || in_stage == 0) {
+                    const int words = stage_rows * p.k_groups / 2;
+                    const uint32_t look = lds32(c_sc + 4 * min(lane, words - 1));
+                    if (lift || !__any_sync(0xffffffffu, max(look & 0xffffu, look >> 16) >= 0x2800u)) {
+                        uint32_t m2 = 0;
+                        for (int w = lane; w < words; w += 32) m2 = as_u32(__hmax2(as_h2(m2), as_h2(lds32(c_sc + 4 * w))));
+                        const int top = (int)(__reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16)) >> 10 & 31), old = lift;
+                        if (top + lift > 15 + 7 || top + lift < 10) lift = min(max(17 - top, 0), 15);
+                        for (int w = lane; lift && w < words; w += 32)
+                            asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(c_sc + 4 * w), "r"(as_u32(__hmul2(as_h2(lds32(c_sc + 4 * w)), as_h2((uint32_t)(lift + 15) * 0x04000400u)))) : "memory");
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");       // the next copy into this place is the async proxy's
+                        __syncwarp();
+                        if (lift != old) {
+                            const float f = exp2f((float)(lift - old));
+#pragma unroll
+                            for (int n = 0; n < CK; ++n)
+#pragma unroll
+                                for (int m = 0; m < 8; ++m)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) sc[n][m][e] *= f;
+                        }
+                    }
+                }
+                const __half *q_at = s_qs + q * run - in_stage + 4 * t + (DIFF ? (q * run >> 6) * 128 : 0);
+#pragma unroll 1
+                for (int at = in_stage; at < in_stage + run; at += 16) {
                     const FewWords<KB> a(c, at, g, t);
                     uint32_t mn[2], b[CK][2];
                     few_pairs(c_mn, at, t, p.k_groups, g & (p.k_groups - 1), mn);              // rows beyond the groups are not read
@@ -532,31 +584,24 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
                         for (int n = 0; n < CK; ++n) mma16816(sc[n][m], a0, a1, a2, a3, b[n][0], b[n][1]);
                     }
                 }
-                stage_done();
-            }
-            if (!ok) break;
-            const float undo = __int_as_float((127 - lift) << 23);
-#pragma unroll
-            for (int n = 0; n < CK; ++n) {
-                const int pair = 4 * n + t, r = pair & ((1 << kr_log2) - 1);
-                const float zero = __shfl_sync(0xffffffffu, z[n][0], 4 * own_group + t);
-                if (pair >> kr_log2 == own_group && r < rows) {
-#pragma unroll
-                    for (int m = 0; m < 8; m += 2) {
-                        float v[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = fmaf(sc[n][m + (e >> 1)][2 * (e & 1)] + sc[n][m + (e >> 1)][2 * (e & 1) + 1], few_power<KB>(m + (e >> 1), e & 1) * undo, zero);
-                        sts_f4(s_s + r * 512 + (16 * g + 2 * m) * 4, v[0], v[1], v[2], v[3]);
-                    }
+                if (!DIFF || in_stage + run == stage_rows) stage_done();
+                if (DIFF && (q + 1) * run == 64) {
+                    put_scores(0);
+                    clear();
                 }
             }
+            if (!ok) break;
+            put_scores(1);
         }
         if (softmax_page(page_at(k) * kPage, kPage)) {
-            rescale(out, o_row, o_row1);
-            if constexpr (VB != 3) {
-                const float a0 = __shfl_sync(0xffffffffu, alpha, o_row), a1 = __shfl_sync(0xffffffffu, alpha, o_row1);
-                out_mn[0] *= a0;
-                out_mn[1] *= a1;
+#pragma unroll
+            for (int n = 0; n < VN; ++n) {
+                rescale(out[n], o_row[n], o_row1(n));
+                if constexpr (VB != 3) {
+                    const float a0 = __shfl_sync(0xffffffffu, alpha, o_row[n]), a1 = __shfl_sync(0xffffffffu, alpha, o_row1(n));
+                    out_mn[n][0] *= a0;
+                    out_mn[n][1] *= a1;
+                }
             }
         }
 #pragma unroll 1
@@ -569,7 +614,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
                 for (int at = 0; at < stage_rows; at += 16) {
                     uint32_t b0, b1;
                     weights(min(g, R - 1), step0 + at / 16, b0, b1);
-                    few_step3(out, c, c_sc, c_mn, at, g, t, b0, b1);
+                    few_step3(out[0], c, c_sc, c_mn, at, g, t, b0, b1);
                 }
             } else {
                 // the exponent of the stage's largest scale: its scales are stage_rows * groups / 32 a lane, two at a time
@@ -581,9 +626,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
                     if (want != expo) {
                         const float f = expo == 32 ? 0.f : exp2f((float)(want - expo));
 #pragma unroll
-                        for (int m = 0; m < 8; ++m)
+                        for (int n = 0; n < VN; ++n)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) out[m][e] *= f;
+                            for (int m = 0; m < 8; ++m)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) out[n][m][e] *= f;
                         expo = want;
                     }
                 }
@@ -591,22 +638,30 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
 #pragma unroll 1
                 for (int at = 0; at < stage_rows; at += 16) {
                     const FewWords<VB> a(c, at, g, t);
-                    uint32_t b0, b1, mn[2], sv[2];
-                    weights(v_row, step0 + at / 16, b0, b1);
+                    uint32_t b[VN][2], mn[2];
                     few_pairs(c_mn, at, t, p.v_groups, g & (p.v_groups - 1), mn);
-                    few_pairs(c_sc, at, t, p.v_groups, v_grp, sv);
-                    const __half2 s0 = __hmul2(as_h2(sv[0]), by), s1 = __hmul2(as_h2(sv[1]), by);
-                    if constexpr (VPAIR) {
-                        mma16816(out_mn, mn[0], 0u, mn[1], 0u, b0 & ~v_lo, b1 & ~v_lo);
-                        b0 = hilo(as_h2(b0), s0, v_lo);
-                        b1 = hilo(as_h2(b1), s1, v_lo);
-                    } else {
-                        mma16816(out_mn, mn[0], 0u, mn[1], 0u, b0, b1);
-                        b0 = as_u32(__hmul2(as_h2(b0), s0));
-                        b1 = as_u32(__hmul2(as_h2(b1), s1));
+#pragma unroll
+                    for (int n = 0; n < VN; ++n) {
+                        uint32_t sv[2];
+                        weights(v_row[n], step0 + at / 16, b[n][0], b[n][1]);
+                        few_pairs(c_sc, at, t, p.v_groups, v_grp[n], sv);
+                        const __half2 s0 = __hmul2(as_h2(sv[0]), by), s1 = __hmul2(as_h2(sv[1]), by);
+                        if constexpr (VPAIR) {
+                            mma16816(out_mn[n], mn[0], 0u, mn[1], 0u, b[n][0] & ~v_lo, b[n][1] & ~v_lo);
+                            b[n][0] = hilo(as_h2(b[n][0]), s0, v_lo);
+                            b[n][1] = hilo(as_h2(b[n][1]), s1, v_lo);
+                        } else {
+                            mma16816(out_mn[n], mn[0], 0u, mn[1], 0u, b[n][0], b[n][1]);
+                            b[n][0] = as_u32(__hmul2(as_h2(b[n][0]), s0));
+                            b[n][1] = as_u32(__hmul2(as_h2(b[n][1]), s1));
+                        }
                     }
 #pragma unroll
-                    for (int m = 0; m < 8; ++m) mma16816(out[m], a.a(m, 0), a.a(m, 1), a.a(m, 2), a.a(m, 3), b0, b1);
+                    for (int m = 0; m < 8; ++m) {
+                        const uint32_t a0 = a.a(m, 0), a1 = a.a(m, 1), a2 = a.a(m, 2), a3 = a.a(m, 3);
+#pragma unroll
+                        for (int n = 0; n < VN; ++n) mma16816(out[n][m], a0, a1, a2, a3, b[n][0], b[n][1]);
+                    }
                 }
             }
             stage_done();
@@ -630,22 +685,24 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int c = few_element<3>(g, m, e);
-                if (c >= 0 && 2 * t < rows) add(2 * t, c, out[m][2 * e], f0);
-                if (c >= 0 && 2 * t + 1 < rows) add(2 * t + 1, c, out[m][2 * e + 1], f1);
+                if (c >= 0 && 2 * t < rows) add(2 * t, c, out[0][m][2 * e], f0);
+                if (c >= 0 && 2 * t + 1 < rows) add(2 * t + 1, c, out[0][m][2 * e + 1], f1);
             }
     } else {
-        const float f0 = __shfl_sync(0xffffffffu, aside_by, o_row), f1 = __shfl_sync(0xffffffffu, aside_by, o_row1);
-        const float z0 = __shfl_sync(0xffffffffu, out_mn[0], 4 * own_group + t), z1 = __shfl_sync(0xffffffffu, out_mn[1], 4 * own_group + t);
         const float undo = expo == 32 ? 0.f : exp2f((float)-expo);
-        if (o_grp == own_group) {
+#pragma unroll
+        for (int n = 0; n < VN; ++n) {
+            const float f0 = __shfl_sync(0xffffffffu, aside_by, o_row[n]), f1 = __shfl_sync(0xffffffffu, aside_by, o_row1(n));
+            const float z0 = __shfl_sync(0xffffffffu, out_mn[n][0], 4 * own_group + t), z1 = __shfl_sync(0xffffffffu, out_mn[n][1], 4 * own_group + t);
+            if (o_grp[n] != own_group) continue;
 #pragma unroll
             for (int m = 0; m < 8; ++m)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int c = few_element<1>(g, m, e);
                     const float f = few_power<VB>(m, e) * undo;
-                    if (o_row < rows) add(o_row, c, fmaf(VPAIR ? out[m][2 * e] + out[m][2 * e + 1] : out[m][2 * e], f, z0), f0);
-                    if (!VPAIR && o_row1 < rows) add(o_row1, c, fmaf(out[m][2 * e + 1], f, z1), f1);
+                    if (o_row[n] < rows) add(o_row[n], c, fmaf(VPAIR ? out[n][m][2 * e] + out[n][m][2 * e + 1] : out[n][m][2 * e], f, z0), f0);
+                    if (!VPAIR && o_row1(n) < rows) add(o_row1(n), c, fmaf(out[n][m][2 * e + 1], f, z1), f1);
                 }
         }
     }
@@ -656,9 +713,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
         for (int j = 0; j < 32; ++j) l += __uint_as_float(lds32(s_sum + lane * 128 + 4 * j));
     if (lane < rows) asm volatile("st.shared.v2.f32 [%0], {%1, %2};\n" ::"r"(s_s + lane * 8), "f"(ref), "f"(l) : "memory");
     __syncthreads();
-    for (int r = 0; r < rows; ++r) {
-        float m = -INFINITY, v = 0.f;
-        l = 0.f;
+    auto join = [&](int r, float &m, float &v) {                  // the warps' parts of row r, this thread's channel: reference, sum; l: the weights' sum
+        m = -INFINITY;
+        v = l = 0.f;
         auto part = [&](int w) { return reinterpret_cast<const float *>(smem + sh.warps + w * sh.warp_bytes + sh.scores) + 2 * r; };
 #pragma unroll
         for (int w = 0; w < kFewWarps; ++w) m = fmaxf(m, part(w)[0]);
@@ -668,6 +725,36 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
             l += f * part(w)[1];
             if (f != 0.f) v += f * reinterpret_cast<const float *>(smem + sh.warps + w * sh.warp_bytes + sh.aside)[r * 128 + threadIdx.x];
         }
+    };
+    if (DIFF && p.splits == 1) {
+        __shared__ float s_squares[kFewRows / 2][kFewWarps];
+        float y[kFewRows / 2];
+#pragma unroll
+        for (int k = 0; k < kFewRows / 2; ++k) {
+            if (2 * k >= rows) break;
+            float m, a, b;
+            join(2 * k, m, a);
+            a = l == 0.f ? 0.f : a / l;
+            join(2 * k + 1, m, b);
+            b = l == 0.f ? 0.f : b / l;
+            y[k] = diff_of(a, b, p.lambdas[(head * p.rep + (row0 + 2 * k) % p.rep) >> 1]);
+            const float squares = warp_sum(y[k] * y[k]);
+            if (lane == 0) s_squares[k][warp] = squares;
+        }
+        __syncthreads();
+        const float weight = p.norm_weight ? p.norm_weight[threadIdx.x] : 1.f;
+#pragma unroll
+        for (int k = 0; k < kFewRows / 2; ++k) {
+            if (2 * k >= rows) break;
+            const int u = s.q0 + (row0 + 2 * k) / p.rep, h = (head * p.rep + (row0 + 2 * k) % p.rep) >> 1;
+            if (p.norm_weight) y[k] *= diff_norm(p, s_squares[k][0] + s_squares[k][1] + s_squares[k][2] + s_squares[k][3]) * weight;
+            static_cast<__half *>(p.a.out)[(int64_t)u * p.a.o_sT + (int64_t)h * p.a.o_sH + threadIdx.x] = __float2half_rn(y[k]);
+        }
+        return;
+    }
+    for (int r = 0; r < rows; ++r) {
+        float m, v;
+        join(r, m, v);
         const int u = s.q0 + (row0 + r) / p.rep, h = head * p.rep + (row0 + r) % p.rep;
         if (p.splits == 1) {
             static_cast<__half *>(p.a.out)[(int64_t)u * p.a.o_sT + (int64_t)h * p.a.o_sH + threadIdx.x] = __float2half_rn(l == 0.f ? 0.f : v / l);
@@ -679,10 +766,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, KB == 3 || VB == 3 || CK == 2 
     }
 }
 
-template <int KB, int VB, int CK>
+template <int KB, int VB, int CK, bool DIFF>
 static int launch_few(const PagedArgs &p, int R, int row_blocks, cudaStream_t st) {
     const int k_row = 4 * page_words(KB) + 4 * p.k_groups, v_row = 4 * page_words(VB) + 4 * p.v_groups, row = k_row > v_row ? k_row : v_row;
-    const int ctas = KB == 3 || VB == 3 || CK == 2 ? 3 : 4;
+    const int ctas = DIFF || KB == 3 || VB == 3 || CK == 2 ? 3 : 4;
     // what 227 KB leave each of the CTAs of an SM (1 KB of each is the system's): two stages at least, of as many rows as that allows (a stage costs some
     // 100 instructions besides its rows)
     const int room = (227 * 1024 / ctas - 1024 - FewShared(R, 0, 0).total) / kFewWarps;
@@ -692,29 +779,29 @@ static int launch_few(const PagedArgs &p, int R, int row_blocks, cudaStream_t st
     int stages = room / stage_bytes;
     stages = stages < 2 ? 2 : stages > kMaxStages ? kMaxStages : stages;
     const size_t smem = FewShared(R, stages, stage_bytes).total;
-    const cudaError_t e = cudaFuncSetAttribute(paged_few_kernel<KB, VB, CK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = cudaFuncSetAttribute(paged_few_kernel<KB, VB, CK, DIFF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return record_cuda_error(e);
     const int64_t grid = (int64_t)p.a.n * p.l.Hkv * row_blocks * p.splits;
     if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
-    paged_few_kernel<KB, VB, CK><<<(unsigned)grid, kFewWarps * 32, smem, st>>>(p, R, row_blocks, stages, stage_rows, stage_bytes);
+    paged_few_kernel<KB, VB, CK, DIFF><<<(unsigned)grid, kFewWarps * 32, smem, st>>>(p, R, row_blocks, stages, stage_rows, stage_bytes);
     return count_launch();
 }
 
-template <int KB, int VB>
+template <int KB, int VB, bool DIFF>
 static int launch_few(const PagedArgs &p, cudaStream_t st) {
-    const FewShape f = few_shape(p.l, p.rep, p.a.max_new);
-    if constexpr (KB != 3)
-        if (f.key_sets == 2) return launch_few<KB, VB, 2>(p, f.rows, f.row_blocks, st);
-    return launch_few<KB, VB, 1>(p, f.rows, f.row_blocks, st);
+    const FewShape f = DIFF ? diff_shape(p.l, p.rep, p.a.max_new) : few_shape(p.l, p.rep, p.a.max_new);
+    if constexpr (DIFF ? KB != 3 || VB != 3 : KB != 3)
+        if (f.key_sets == 2) return launch_few<KB, VB, 2, DIFF>(p, f.rows, f.row_blocks, st);
+    return launch_few<KB, VB, 1, DIFF>(p, f.rows, f.row_blocks, st);
 }
 
-template <int KB>
+template <int KB, bool DIFF = false>
 static int launch_few(const PagedArgs &p, cudaStream_t st) {
     switch (p.l.v_bits) {
-        case 1: return launch_few<KB, 1>(p, st);
-        case 2: return launch_few<KB, 2>(p, st);
-        case 3: return launch_few<KB, 3>(p, st);
-        default: return launch_few<KB, 4>(p, st);
+        case 1: return launch_few<KB, 1, DIFF>(p, st);
+        case 2: return launch_few<KB, 2, DIFF>(p, st);
+        case 3: return launch_few<KB, 3, DIFF>(p, st);
+        default: return launch_few<KB, 4, DIFF>(p, st);
     }
 }
 

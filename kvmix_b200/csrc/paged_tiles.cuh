@@ -165,7 +165,9 @@ struct CapSmall {
 
 // MODS: scores are capped, biased or scaled by a negative number.  Calls without have an instance of their own: with the code beside it the
 // 128 scores of a thread no longer fit its registers (2048 tokens over 32k: 1261 us in place of 1132).
-template <int KB, int VB, bool MODS>
+// DIFF: heads are two rows each (PagedArgs); the two tiles are the two maps of the same 128 rows -- (token, query head) pairs --, a map's scores the product of
+// half the channels, and the map of the second half hands its part of the output over in shared memory.
+template <int KB, int VB, bool MODS, bool DIFF>
 __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ PagedMaps maps, int max_tiles) {
     extern __shared__ __align__(1024) char smem[];
     __shared__ uint32_t s_tmem;
@@ -213,18 +215,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     }
     int q0, n_new;
     new_tokens(p, seq, q0, n_new);                                // as paged_seq has them, which waits for more loads
-    const int row0 = tile * 2 * kTileRows, rows = min(n_new * p.rep - row0, 2 * kTileRows), two_tiles = rows > kTileRows;
+    const int rep = DIFF ? p.rep / 2 : p.rep, tile_rows = DIFF ? kTileRows : 2 * kTileRows;
+    const int row0 = tile * tile_rows, rows = min(n_new * rep - row0, tile_rows), two_tiles = DIFF || rows > kTileRows;
     const int warp = uniform_warp(), lane = threadIdx.x & 31, wg = warp >> 2;
 
     const uint32_t base = smem_u32(smem), bars = base + kOffBar;
     // Q, 16 threads a row, asked for before anything that does not have to come first: a row a thread, after the barrier, the same loads took 6 us
     // of a CTA that has some 30 us of pages
-    uint4 qv[6];
+    constexpr int kTurns = DIFF ? 3 : 6;
+    uint4 qv[kTurns];
     {
         const bool vec = (reinterpret_cast<uintptr_t>(p.a.q) % 16 | p.a.q_sT % 8 | p.a.q_sH % 8) == 0;
 #pragma unroll
-        for (int i = 0; i < 6; ++i) {
-            const int row = (threadIdx.x >> 4) + 48 * i, idx = row0 + row, u = idx / p.rep, h = head * p.rep + (idx - u * p.rep);
+        for (int i = 0; i < kTurns; ++i) {
+            const int row = (threadIdx.x >> 4) + 48 * i, idx = row0 + row, u = idx / rep, h = head * rep + (idx - u * rep);
             const __half *q = static_cast<const __half *>(p.a.q) + (int64_t)(q0 + u) * p.a.q_sT + (int64_t)h * p.a.q_sH + 8 * (threadIdx.x & 15);
             qv[i] = make_uint4(0, 0, 0, 0);
             if (row >= rows) continue;
@@ -262,7 +266,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     // the pages that any row sees: bounds of the first and last tokens hold for those between, unless they are given token by token
     int first = INT32_MAX, last = 0;
     {
-        const int u0 = row0 / p.rep, u1 = (row0 + rows - 1) / p.rep;
+        const int u0 = row0 / rep, u1 = (row0 + rows - 1) / rep;
         for (int u = u0 + threadIdx.x; u <= u1; u += kTileThreads) {
             int pos, lo, hi;
             paged_bounds(p, s, u, pos, lo, hi);
@@ -273,9 +277,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         __shared__ int s_first[kTileThreads / 32], s_last[kTileThreads / 32];
         if (lane == 0) { s_first[warp] = first; s_last[warp] = last; }
 #pragma unroll
-        for (int i = 0; i < 6; ++i) {
+        for (int i = 0; i < kTurns; ++i) {
             const int row = (threadIdx.x >> 4) + 48 * i;
-            if (row < 2 * kTileRows) sts128(operand_at(base + kOffQ + (row >> 7) * kOperandBytes, row & 127, threadIdx.x & 15), qv[i].x, qv[i].y, qv[i].z, qv[i].w);
+            if (row < tile_rows) sts128(operand_at(base + kOffQ + (row >> 7) * kOperandBytes, row & 127, threadIdx.x & 15), qv[i].x, qv[i].y, qv[i].z, qv[i].w);
         }
         fence_async();
         tc_fence_before();
@@ -302,8 +306,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         // ------------------------------------------------------------------ softmax, 64 columns of one row a thread
         asm volatile("setmaxnreg.inc.sync.aligned.u32 88;\n");
         constexpr int N = 64;
-        const int tile_of = wg >> 1, half = wg & 1, r = threadIdx.x & 127, idx = row0 + tile_of * kTileRows + r, u = idx / p.rep, h = head * p.rep + (idx - u * p.rep);
-        const bool mine = tile_of * kTileRows + r < rows;
+        const int tile_of = wg >> 1, half = wg & 1, r = threadIdx.x & 127, at_row = DIFF ? r : tile_of * kTileRows + r, idx = row0 + at_row, u = idx / rep,
+                  h = head * rep + (idx - u * rep);
+        const bool mine = at_row < rows;
         if (tile_of == 0 || two_tiles) {
             int pos = 0, lo = 0, hi = 0;
             if (mine) paged_bounds(p, s, u, pos, lo, hi);
@@ -427,8 +432,72 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             l = half ? __uint_as_float(lds32(other_top)) + l : l + __uint_as_float(lds32(other_top));
             const float inv = l == 0.f ? 0.f : 1.f / l;
             __half *out = static_cast<__half *>(p.a.out) + (int64_t)(s.q0 + u) * p.a.o_sT + (int64_t)h * p.a.o_sH + half * N;
-            const int64_t part = (int64_t)split * p.a.tokens * p.a.nh + (int64_t)(s.q0 + u) * p.a.nh + h;
+            const int64_t part = (int64_t)split * p.a.tokens * p.a.nh + (int64_t)(s.q0 + u) * p.a.nh + (DIFF ? 2 * h + tile_of : h);
             const bool vec = (reinterpret_cast<uintptr_t>(p.a.out) % 16 | p.a.o_sT % 8 | p.a.o_sH % 8) == 0;
+            if (DIFF && p.splits == 1) {
+                // The operand buffers are free: no copy and no product is under way.  A row's 16-byte pieces are mixed by its number.
+                float *const other = reinterpret_cast<float *>(smem + kOffK);
+                auto piece = [&](int k) { return reinterpret_cast<float4 *>(other + r * 128) + ((half * (N / 4) + k) ^ (r & 31)); };
+                auto column = [&](uint32_t v) { return np == 0 || l == 0.f ? 0.f : __uint_as_float(v) * inv; };
+                if (tile_of == 1) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[16];
+                        if (np > 0) {
+                            tc_load16(o, t_o + 16 * c);
+                            tc_wait_ld();
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) *piece(4 * c + j) = make_float4(column(o[4 * j]), column(o[4 * j + 1]), column(o[4 * j + 2]), column(o[4 * j + 3]));
+                    }
+                }
+                asm volatile("bar.sync 4, 512;\n" ::: "memory");
+                if (tile_of == 0) {
+                    const float lambda = mine ? p.lambdas[h] : 0.f;
+                    float y[N], squares = 0.f;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[16];
+                        if (np > 0) {
+                            tc_load16(o, t_o + 16 * c);
+                            tc_wait_ld();
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float4 b = *piece(4 * c + j);
+                            const float second[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float v = diff_of(column(o[4 * j + k]), second[k], lambda);
+                                y[16 * c + 4 * j + k] = v;
+                                squares = fmaf(v, v, squares);
+                            }
+                        }
+                    }
+                    if (p.norm_weight) {
+                        const uint32_t turn = 4 * kTileRows * 4;  // the place that the sums of weights are not in
+                        asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(my_top + turn), "f"(squares) : "memory");
+                        pair_meets();
+                        const float more = __uint_as_float(lds32(other_top + turn)), by = diff_norm(p, half ? more + squares : squares + more);
+#pragma unroll
+                        for (int j = 0; j < N; ++j) y[j] *= by * p.norm_weight[half * N + j];
+                    }
+                    if (mine) {
+                        if (vec) {
+#pragma unroll
+                            for (int j = 0; j < N / 8; ++j) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) w[k] = as_u32(__floats2half2_rn(y[8 * j + 2 * k], y[8 * j + 2 * k + 1]));
+                                reinterpret_cast<uint4 *>(out)[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < N; ++j) out[j] = __float2half_rn(y[j]);
+                        }
+                    }
+                }
+            } else {
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 uint32_t o[16];
@@ -456,6 +525,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                         for (int j = 0; j < 16; ++j) out[16 * c + j] = __ushort_as_half((unsigned short)(w[j >> 1] >> (16 * (j & 1))));
                     }
                 }
+            }
             }
             if (mine && half == 0 && p.splits > 1) {
                 p.part_ml[2 * part] = m;
@@ -519,16 +589,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             auto wait = [&](int b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar(b), parity, status)); };
             bool ok = true;
             // the address fields of descriptors count 16 bytes, and no operand's end carries out of them
-            auto scores = [&](int it, int w) {                    // S[w] = Q[w] K^T of page `it`
-                const uint64_t q = q_desc + w * (kOperandBytes / 16);
+            auto scores = [&](int it, int w) {                    // S[w] = Q[w] K^T of page `it`; DIFF: of the channels of half w
+                constexpr int STEPS = DIFF ? 4 : 8;
+                const uint64_t q = q_desc + w * ((DIFF ? kOperandHalf : kOperandBytes) / 16);
                 const uint32_t stage = (it & 1) * (kOperandBytes / 16);
                 if (it < n_old) {
+                    const uint64_t k = k_mn + stage + (DIFF ? w * 512 : 0);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) tc_mma(tm + w * 128, q + (e >> 2) * (kOperandHalf / 16) + (e & 3) * 2, k_mn + stage + e * 128, kIdescMn, e > 0, lead);
+                    for (int e = 0; e < STEPS; ++e) tc_mma(tm + w * 128, q + (e >> 2) * (kOperandHalf / 16) + (e & 3) * 2, k + e * 128, kIdescMn, e > 0, lead);
                 } else {
+                    const uint64_t k = k_desc + stage + (DIFF ? w * (kOperandHalf / 16) : 0);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        tc_mma(tm + w * 128, q + (e >> 2) * (kOperandHalf / 16) + (e & 3) * 2, k_desc + stage + (e >> 2) * (kOperandHalf / 16) + (e & 3) * 2, kIdesc, e > 0, lead);
+                    for (int e = 0; e < STEPS; ++e)
+                        tc_mma(tm + w * 128, q + (e >> 2) * (kOperandHalf / 16) + (e & 3) * 2, k + (e >> 2) * (kOperandHalf / 16) + (e & 3) * 2, kIdesc, e > 0, lead);
                 }
                 tc_commit(bar(kBarS + w), lead);
             };
@@ -625,9 +698,9 @@ static bool page_map(CUtensorMap *map, void *base, int64_t rows) {
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int KB, int VB, bool MODS>
+template <int KB, int VB, bool MODS, bool DIFF>
 static int launch_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_tile_kernel<KB, VB, MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem);
+    const cudaError_t e = cudaFuncSetAttribute(paged_tile_kernel<KB, VB, MODS, DIFF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem);
     if (e != cudaSuccess) return record_cuda_error(e);
     const int64_t grid = (int64_t)max_tiles * p.l.Hkv * p.splits;
     if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
@@ -635,17 +708,17 @@ static int launch_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
     PagedMaps maps = {};
     const int64_t rows = (int64_t)p.l.n_fp16 * p.l.Hkv * kPage;
     maps.there = page_map(&maps.k, p.l.kfull, rows) && page_map(&maps.v, p.l.vfull, rows);
-    paged_tile_kernel<KB, VB, MODS><<<(unsigned)grid, kTileThreads, kTileSmem, st>>>(p, maps, max_tiles);
+    paged_tile_kernel<KB, VB, MODS, DIFF><<<(unsigned)grid, kTileThreads, kTileSmem, st>>>(p, maps, max_tiles);
     return count_launch();
 }
 
-template <int KB>
+template <int KB, bool DIFF = false>
 static int launch_tiles(const PagedArgs &p, int max_tiles, bool mods, cudaStream_t st) {
     switch (p.l.v_bits) {
-        case 1: return mods ? launch_tiles<KB, 1, true>(p, max_tiles, st) : launch_tiles<KB, 1, false>(p, max_tiles, st);
-        case 2: return mods ? launch_tiles<KB, 2, true>(p, max_tiles, st) : launch_tiles<KB, 2, false>(p, max_tiles, st);
-        case 3: return mods ? launch_tiles<KB, 3, true>(p, max_tiles, st) : launch_tiles<KB, 3, false>(p, max_tiles, st);
-        default: return mods ? launch_tiles<KB, 4, true>(p, max_tiles, st) : launch_tiles<KB, 4, false>(p, max_tiles, st);
+        case 1: return mods ? launch_tiles<KB, 1, true, DIFF>(p, max_tiles, st) : launch_tiles<KB, 1, false, DIFF>(p, max_tiles, st);
+        case 2: return mods ? launch_tiles<KB, 2, true, DIFF>(p, max_tiles, st) : launch_tiles<KB, 2, false, DIFF>(p, max_tiles, st);
+        case 3: return mods ? launch_tiles<KB, 3, true, DIFF>(p, max_tiles, st) : launch_tiles<KB, 3, false, DIFF>(p, max_tiles, st);
+        default: return mods ? launch_tiles<KB, 4, true, DIFF>(p, max_tiles, st) : launch_tiles<KB, 4, false, DIFF>(p, max_tiles, st);
     }
 }
 

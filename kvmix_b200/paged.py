@@ -10,6 +10,7 @@ bit widths, its newest are fp16 (``include/kvmix_b200.h`` has the layouts, which
     pages_fork       a sequence branches                  pages_free       a sequence goes
     pages_compact    pages in use move together           pages_reorder    rows take one another's sequences (beam search)
     page_append      page_write with the position rotation, for queries too
+    paged_differential_attention  the difference of two softmax maps, over the same pages
     KVmixPagedCache  all of them with the tensors they work on
 
 The bookkeeping (``PageBook``) lives on the device and is changed by kernels only: no call waits for the host, all can be captured in a
@@ -43,6 +44,7 @@ _STATUS = {1: "no free fp16 page", 2: "no free packed page", 4: "sequence longer
 
 _pack_book, _pack_layer = struct.Struct("@6P4i").pack, struct.Struct("@8P6i").pack
 _pack_write, _pack_attn = struct.Struct("@2P4q2P2i").pack, struct.Struct("@2P4q5P8i2fPQ").pack
+_pack_diff = struct.Struct("@2P4q5P8i2fPQ2Pf").pack
 _pack_append = struct.Struct("@6P10q3P8i").pack
 _addresses = struct.Struct("@8P").unpack_from             # of a layer's argument block
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
@@ -92,7 +94,7 @@ def page_groups(bits, group):
 @functools.lru_cache(maxsize=None)
 def _library():
     for fmt, cls in (("@6P4i", _lib.PageBookArgs), ("@8P6i", _lib.PageLayerArgs), ("@2P4q2P2i", _lib.PageWriteArgs), ("@2P4q5P8i2fPQ", _lib.PagedAttnArgs),
-                     ("@6P10q3P8i", _lib.PageAppendArgs)):
+                     ("@6P10q3P8i", _lib.PageAppendArgs), ("@2P4q5P8i2fPQ2Pf", _lib.PagedDiffArgs)):
         assert -(-struct.calcsize(fmt) // 8) * 8 == C.sizeof(cls)
     return _lib.lib()
 
@@ -392,9 +394,38 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     which few have several tokens the third saves time).  Tokens that see nothing get zeros.  Cached values have
     to be finite: one that is not may reach queries that do not see it (include/kvmix_b200.h).
     Returns [tokens, nh, 128] fp16; rows behind q_start[n] are left as they are."""
+    return _attend(q, q_start, rows, pages, layer, causal, window, prefix, first, softcap, alibi_slopes, _SCALE if softmax_scale is None else softmax_scale, max_new, max_tokens,
+                   max_chunks, out, None)
+
+
+@_on_its_device(4)
+def paged_differential_attention(q, lambdas, q_start, rows, pages, layer, causal=True, window=None, prefix=None, first=None, softcap=None, alibi_slopes=None,
+                                 softmax_scale=None, norm_weight=None, norm_eps=1e-5, max_new=None, max_tokens=None, max_chunks=None, out=None):
+    """The difference of two softmax maps over the pages of every sequence: a head's 128 channels of q and of the cached keys are two halves of 64,
+
+        out = (softmax(q1 k1^T * scale) - lambdas[head] * softmax(q2 k2^T * scale)) v,   then out / sqrt(mean(out^2) + norm_eps) * norm_weight
+
+    lambdas fp32 [nh]; norm_weight fp32 [128], or None for no norm; softmax_scale None: 1 / 8.  Everything else is as ``paged_attention`` has it, for both maps
+    alike.  Both attentions are fp32 until their difference (normed) is rounded; keys, values and weights are rounded on the way as there.  Keys that ``page_append``
+    rotates want parts=2."""
+    dev, nh = pages.table.get_device(), q.shape[1] if q.dim() == 3 else 0
+    if lambdas.dtype is not torch.float32 or lambdas.shape != (nh,) or lambdas.get_device() != dev or not lambdas.is_contiguous():
+        raise RuntimeError(f"lambdas must be float32 [{nh}] on cuda:{dev}")
+    at_weight = 0
+    if norm_weight is not None:
+        if norm_weight.dtype is not torch.float32 or norm_weight.shape != (128,) or norm_weight.get_device() != dev or not norm_weight.is_contiguous():
+            raise RuntimeError(f"norm_weight must be float32 [128] on cuda:{dev}")
+        if not 0.0 <= norm_eps <= 3.4e38:
+            raise RuntimeError("norm_eps must not be negative")
+        at_weight = norm_weight.data_ptr()
+    return _attend(q, q_start, rows, pages, layer, causal, window, prefix, first, softcap, alibi_slopes, 0.125 if softmax_scale is None else softmax_scale, max_new, max_tokens,
+                   max_chunks, out, (lambdas.data_ptr(), at_weight, norm_eps))
+
+
+def _attend(q, q_start, rows, pages, layer, causal, window, prefix, first, softcap, alibi_slopes, softmax_scale, max_new, max_tokens, max_chunks, out, diff):
     dev, book = _book(pages)
     if q.dim() != 3 or q.dtype is not _f16 or q.get_device() != dev or q.shape[2] != 128:
-        raise RuntimeError(f"paged_attention takes fp16 queries [tokens, heads, 128] on cuda:{dev}")
+        raise RuntimeError(f"attention over pages takes fp16 queries [tokens, heads, 128] on cuda:{dev}")
     tokens, nh, _ = q.shape
     n = rows.numel()
     block = _layer(pages, dev, layer)
@@ -412,7 +443,7 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     window, softcap = window or 0, softcap or 0.0
     if window < 0 or not softcap >= 0.0:
         raise RuntimeError("window and softcap must not be negative")
-    if softmax_scale is not None and not abs(softmax_scale) <= 3.4e38:
+    if not abs(softmax_scale) <= 3.4e38:
         raise RuntimeError("softmax_scale must be a finite number")
     at_slopes = 0
     if alibi_slopes is not None:
@@ -426,13 +457,16 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     if tokens and n and (max_new <= 0 or max_tokens <= 0 or max_chunks < 0):
         raise RuntimeError("max_new and max_tokens must be positive, max_chunks not negative")
     L = _library()
-    need = L.kvq_paged_attn_workspace_bytes(block, n, tokens, nh, max_new, max_tokens, max_chunks)
+    need = (L.kvq_paged_diff_attn_workspace_bytes if diff else L.kvq_paged_attn_workspace_bytes)(block, n, tokens, nh, max_new, max_tokens, max_chunks)
     ws = pages.count.new_empty((need + 3) // 4) if need else None
-    a = _pack_attn(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), _ints(dev, "q_start", q_start, n + 1),
+    a = (q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), _ints(dev, "q_start", q_start, n + 1),
                    _ints(dev, "rows", rows, n), 0 if first is None else _ints(dev, "first", first, tokens), 0 if prefix is None else _ints(dev, "prefix", prefix, n),
                    at_slopes, n, tokens, nh, max_new, max_tokens, max_chunks, int(min(window, _MOST)), 1 if causal else 0,
-                   _SCALE if softmax_scale is None else softmax_scale, min(softcap, 1e38), 0 if ws is None else ws.data_ptr(), need)
-    _launched(L.kvq_paged_attn(book, block, a, ops.raw_stream()))
+                   softmax_scale, min(softcap, 1e38), 0 if ws is None else ws.data_ptr(), need)
+    if diff:
+        _launched(L.kvq_paged_diff_attn(book, block, _pack_diff(*a, *diff), ops.raw_stream()))
+    else:
+        _launched(L.kvq_paged_attn(book, block, _pack_attn(*a), ops.raw_stream()))
     return out
 
 
@@ -535,6 +569,13 @@ class KVmixPagedCache:
             raise RuntimeError("one query for every new token of the step")
         return paged_attention(q, step.q_start, step.rows, self.book, self.layers[layer], max_new=max(step.max_new, 1), max_tokens=max(step.max_tokens, 1),
                                max_chunks=step.max_chunks, **options)
+
+    def attend_differential(self, layer, q, lambdas, step, **options):
+        """Options as ``paged_differential_attention``: norm_weight, norm_eps and those of ``attend``."""
+        if q.shape[0] != step.tokens:
+            raise RuntimeError("one query for every new token of the step")
+        return paged_differential_attention(q, lambdas, step.q_start, step.rows, self.book, self.layers[layer], max_new=max(step.max_new, 1),
+                                            max_tokens=max(step.max_tokens, 1), max_chunks=step.max_chunks, **options)
 
     def append(self, layer, k, v, cos, sin, step, q=None, **options):
         """``write`` of keys that are not rotated yet, and the step's queries rotated: returns them.  Options as ``page_append``: q_out, positions, interleaved,

@@ -15,14 +15,14 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def test_argument_blocks_match_the_header():
-    names = ["kvq_page_append_args", "kvq_beam_args"]
+    names = ["kvq_page_append_args", "kvq_beam_args", "kvq_paged_diff_args"]
     src = '#include <stdio.h>\n#include "kvmix_b200.h"\nint main(void){ printf("%s %%d %%d", %s, KVQ_MOST_BEAMS, KVQ_MOST_BEST); return 0; }\n' % (
         " ".join(["%zu"] * len(names)), ", ".join("sizeof(%s)" % n for n in names))
     with tempfile.TemporaryDirectory() as d:
         open(os.path.join(d, "s.c"), "w").write(src)
         subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), os.path.join(d, "s.c"), "-o", os.path.join(d, "s")])
         sizes = [int(x) for x in subprocess.check_output([os.path.join(d, "s")]).split()]
-    assert sizes == [ctypes.sizeof(_lib.PageAppendArgs), ctypes.sizeof(_lib.BeamArgs), _lib.MOST_BEAMS, _lib.MOST_BEST]
+    assert sizes == [ctypes.sizeof(_lib.PageAppendArgs), ctypes.sizeof(_lib.BeamArgs), ctypes.sizeof(_lib.PagedDiffArgs), _lib.MOST_BEAMS, _lib.MOST_BEST]
     paged._library()
 
 
@@ -96,6 +96,34 @@ def test_no_cpu_path():
     cache = kv.KVmixPagedCache([(4, 2)], 1, 128, 2, 256, 1, 2, 64, device="cpu")
     i, x, t = torch.zeros(1, dtype=torch.int32), torch.zeros(1, 1, 128).half(), torch.zeros(4, 64)
     for call in (lambda: kv.page_append(x, x, t, t, i, i, cache.book, cache.layers[0]), lambda: kv.pages_reorder(i, i, cache.book, cache.layers),
-                 lambda: kv.beam_select(t, torch.zeros(4), 2)):
+                 lambda: kv.beam_select(t, torch.zeros(4), 2), lambda: kv.paged_differential_attention(x, t[0, :1], i, i, cache.book, cache.layers[0])):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def diff(over=None, **own):
+    a = _lib.PagedDiffArgs()
+    a.a.q = a.a.out = a.a.q_start = a.a.rows = a.lambdas = 64
+    a.a.n, a.a.tokens, a.a.nh, a.a.max_new, a.a.max_tokens, a.a.max_chunks, a.a.softmax_scale, a.norm_eps = 1, 1, 4, 1, 100, 1, 0.1, 1e-5
+    for k, v in (over or {}).items():
+        setattr(a.a, k, v)
+    for k, v in own.items():
+        setattr(a, k, v)
+    return bytes(a)
+
+
+def test_refused_differential_attention():
+    L = paged._library()
+    for bad, rc in ((diff(dict(nh=3)), -6), (diff(dict(nh=2 ** 30 + 2 ** 29)), -11), (diff(dict(q=None)), -10), (diff(dict(n=-1)), -7), (diff(dict(max_new=0)), -7), (diff(dict(tokens=0)), 0),
+                    (diff(dict(max_tokens=100000)), -12), (diff(lambdas=None), -10), (diff(norm_weight=64, norm_eps=-1.0), -7), (diff(norm_weight=64, norm_eps=float("nan")), -7),
+                    (diff(norm_weight=64, norm_eps=float("inf")), -7), (diff(dict(softcap=-1.0)), -7), (None, -10)):
+        assert L.kvq_paged_diff_attn(book(), layer(), bad, None) == rc
+    assert L.kvq_paged_diff_attn(book(count=None), layer(), diff(), None) == -10
+    assert L.kvq_paged_diff_attn(book(), layer(group=16), diff(), None) == -11
+    for n in (1, 3, 64):
+        for tokens in (1, 7, 300, 4096):
+            for nh, Hkv in ((1, 1), (32, 8), (64, 8), (40, 8)):
+                for length in (1, 128, 5000, 131072):
+                    b = L.kvq_paged_diff_attn_workspace_bytes(layer(Hkv=Hkv), n, tokens, nh, tokens, length, n)
+                    assert b % (2 * tokens * nh * 520) == 0 and b // (2 * tokens * nh * 520) != 1
+    assert L.kvq_paged_diff_attn_workspace_bytes(layer(), 1, 1, 3, 1, 100, 1) == 0
