@@ -3,6 +3,7 @@
 ``KVmixPagedCache.advance`` calls it and lets the cache's rows follow.  No upstream counterpart: upstream decodes greedily or samples.
 """
 import ctypes as C
+import functools
 import struct
 from typing import NamedTuple
 
@@ -12,6 +13,7 @@ from . import _lib, ops
 from ._lib import check
 
 _pack = struct.Struct("@Pq8P6iPQ").pack
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
@@ -56,27 +58,31 @@ def beam_select(logits, scores, beams, n=None, ends=None):
         raise RuntimeError(f"n must be {min(needed, all_of_them)} to {min(all_of_them, _lib.MOST_BEST)} for {beams} beams and {n_ends} ends")
     if logits.stride(1) != 1 and vocabulary > 1:
         logits = logits.contiguous()
-    if dev != torch.cuda.current_device():
+    if dev != _current_device():
         with torch.cuda.device(dev):
             return _select(logits, scores, beams, n, n_ends, at_ends)
     return _select(logits, scores, beams, n, n_ends, at_ends)
 
 
-def _select(logits, scores, beams, n, n_ends, at_ends):
-    rows, vocabulary = logits.shape
-    requests, L = rows // beams, _lib.lib()
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes(requests, beams, vocabulary, kind, n, n_ends):
     assert struct.calcsize("@Pq8P6iPQ") == C.sizeof(_lib.BeamArgs)
-    out = scores.new_empty(3 * requests * (n + beams), dtype=torch.int32)
-    parts = [t.view(requests, -1) for t in out.split([requests * n] * 3 + [requests * beams] * 3)] if requests else [out.new_empty(0, w) for w in (n, n, n, beams, beams, beams)]
-    parts[0], parts[3] = parts[0].view(torch.float32), parts[3].view(torch.float32)
+    return _lib.lib().kvq_beam_select_workspace_bytes(_pack(*[0] * 10, requests, beams, vocabulary, kind, n, n_ends, 0, 0))
 
-    def block(at, size):
-        return _pack(logits.data_ptr(), logits.stride(0), scores.data_ptr(), at_ends, *[t.data_ptr() for t in parts], requests, beams, vocabulary, _TYPES[logits.dtype], n,
-                     n_ends, at, size)
 
+def _select(logits, scores, beams, n, n_ends, at_ends):
+    (rows, vocabulary), kind = logits.shape, _TYPES[logits.dtype]
+    requests = rows // beams
+    best, going = scores.new_empty((requests, n)), scores.new_empty((requests, beams))
+    best_beams, going_beams = torch.empty_like(best, dtype=torch.int32), torch.empty_like(going, dtype=torch.int32)
+    best_tokens, going_tokens = torch.empty_like(best_beams), torch.empty_like(going_beams)
     if requests:
-        need = L.kvq_beam_select_workspace_bytes(block(0, 0))
-        workspace = out.new_empty((need + 3) // 4)
-        check(L.kvq_beam_select(block(workspace.data_ptr(), need), ops.raw_stream()))
+        need = _workspace_bytes(requests, beams, vocabulary, kind, n, n_ends)
+        workspace = scores.new_empty((need + 3) // 4)
+        a = _pack(logits.data_ptr(), logits.stride(0), scores.data_ptr(), at_ends, best.data_ptr(), best_beams.data_ptr(), best_tokens.data_ptr(), going.data_ptr(),
+                  going_beams.data_ptr(), going_tokens.data_ptr(), requests, beams, vocabulary, kind, n, n_ends, workspace.data_ptr(), need)
+        rc = _lib._lib.kvq_beam_select(a, ops.raw_stream())            # loaded: _workspace_bytes asked it
+        if rc:
+            check(rc)
         ops.LAUNCHES[0] += 2
-    return BeamStep(*parts)
+    return BeamStep(best, best_beams, best_tokens, going, going_beams, going_tokens)

@@ -8,7 +8,7 @@
 // A candidate within a beam is one 64-bit key, the logit in an order of unsigned numbers above the complement of the token: keys are
 // all different, the largest is the best and ties go to the lowest token, in whatever order threads come.
 // Sums are fp32 within a thread (some hundred terms) and 64-bit from there: which of two beams goes on may hang on the last bits of their sums.
-#include "common.cuh"
+#include "quant_core.cuh"
 
 #include <cuda_bf16.h>
 
@@ -17,7 +17,7 @@ namespace kvq {
 using u64 = unsigned long long;
 constexpr int kScanThreads = 256, kTurn = 16;                     // elements a thread takes at a time
 constexpr int kMostBest = KVQ_MOST_BEST, kMostBeams = KVQ_MOST_BEAMS, kMostParts = 32;
-constexpr int kKeys = kMostBest * kTurn + 64;                     // of a first turn no more pass: n groups of threads have a key that reaches the threshold
+constexpr int kKeys = 16 * kMostBest;                             // room for what reaches a part's threshold
 constexpr float kLog2 = 1.4426950408889634f;
 
 struct BeamArgs {
@@ -56,151 +56,207 @@ __device__ __forceinline__ void floats(uint4 v, float *x) {
     }
 }
 
-// A part of a row.  The first turn's threshold: of the groups of threads (four lanes, or one where n is large) the n-th best has a key that n elements reach.
+// exp(x - top) of a thread's elements under its own running maximum.  The difference comes first: times log2 e it may lose bits only of itself, whatever
+// the logits are added to, and the type's lowest value stays a number.
+__device__ __forceinline__ float max3_of(float a, float b, float c) {             // what is not a number is left out
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+struct RunningSum {
+    float top = -INFINITY, sum = 0.f;
+    __device__ __forceinline__ void add(const float (&v)[kTurn], float now) {          // now: the maximum with these
+        const float from = now == -INFINITY ? 0.f : now;
+        const u64 by = f32x2(kLog2, kLog2), off = f32x2(-from, -from);
+        u64 more[2] = {f32x2(sum * beam_exp2((top - from) * kLog2), 0.f), 0ull};
+#pragma unroll
+        for (int e = 0; e < kTurn; e += 2) {
+            const float2 d = f32x2_split(mul_f32x2(add_f32x2(f32x2(v[e], v[e + 1]), off), by));
+            more[e >> 1 & 1] = add_f32x2(more[e >> 1 & 1], f32x2(beam_exp2(d.x), beam_exp2(d.y)));
+        }
+        const float2 all = f32x2_split(add_f32x2(more[0], more[1]));
+        sum = all.x + all.y;
+        top = now;
+    }
+};
+
+// A part of a row, 4096 elements a turn.  The pass over it keeps a thread's sum, its maximum and where that came first, and nothing else.  Of the groups of threads (eight
+// lanes, fewer where n is large) the n-th best then has a key that n elements reach at least, and none of the n best is in a thread whose best does not reach
+// it: what the others hold -- those of some 1.1 n threads -- is read once more, from L2, and what reaches the threshold goes to shared memory.  Should
+// there be no room for all of it (rows that were made for that), the n best of what there was room for give a higher threshold.
 // Which thread has which token follows from the token alone, not from the row's alignment: rows alike have sums alike, to the last bit, and ties between
 // beams stay ties.  Rows that are not 16-byte aligned are therefore read element by element (VEC false).
-// What reaches it goes to shared memory, some 1.1 n of the first turn's 4096, and in later turns n a turn; every 48 beyond n, the n best
-// of them give the next threshold.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const __grid_constant__ BeamArgs p) {
-    constexpr int E = 16 / sizeof(T), U = kTurn / E;
+__global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid_constant__ BeamArgs p) {
+    constexpr int E = 16 / sizeof(T), U = kTurn / E, kStep = U * kScanThreads;         // pieces of 16 bytes a turn
     __shared__ u64 s_key[kKeys], s_best[kScanThreads], s_from;
     __shared__ double s_sum[kScanThreads / 32];
     __shared__ float s_top[kScanThreads / 32];
-    __shared__ int s_count;
+    __shared__ int s_count, s_threads, s_thread[kScanThreads];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.a.n, V = p.a.vocabulary;
     const int part = blockIdx.x % p.parts;
     const int64_t row = blockIdx.x / p.parts;
     const T *x = static_cast<const T *>(p.a.logits) + row * p.a.l_sR;
     const int pieces = V / E + (V % E != 0), lo = (int)((int64_t)pieces * part / p.parts), hi = (int)((int64_t)pieces * (part + 1) / p.parts);
-    float top = -INFINITY, sum = 0.f;
+    const int whole = VEC ? min(hi, V / E) : lo;                  // pieces before it are 16 bytes that are all there, aligned
+    auto load = [&](int piece) {                                  // elements that are not there: whatever
+        uint4 to = make_uint4(0, 0, 0, 0);
+        if (piece < whole) {
+            to = reinterpret_cast<const uint4 *>(x)[piece];
+        } else if (piece < hi) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (piece * (int64_t)E + e < V) reinterpret_cast<T *>(&to)[e] = x[(int64_t)piece * E + e];
+        }
+        return to;
+    };
+    auto here = [&](int piece) { return piece < whole ? E : piece < hi ? min(E, V - piece * E) : 0; };
 
-    uint4 next[U];
-    auto load = [&](int at) {
+    RunningSum sum;
+    int first = INT32_MAX;                                        // the piece in which the maximum came first
+    auto turn = [&](int at, const uint4 (&raw)[U], bool full) {
+        float v[kTurn], most[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int piece = at + u * kScanThreads + tid;
-            if (piece >= hi) continue;
-            if (VEC && (piece + 1) * (int64_t)E <= V) {
-                next[u] = reinterpret_cast<const uint4 *>(x)[piece];
-            } else {
+            floats<T>(raw[u], v + u * E);
+            if (!full) {
+                const int some = here(at + u * kScanThreads + tid);
 #pragma unroll
                 for (int e = 0; e < E; ++e)
-                    if (piece * (int64_t)E + e < V) reinterpret_cast<T *>(&next[u])[e] = x[(int64_t)piece * E + e];
+                    if (e >= some) v[u * E + e] = -INFINITY;
+                if (some && first == INT32_MAX) first = at + u * kScanThreads + tid;           // where there is nothing but -infinity
             }
+            most[u] = fmaxf(v[u * E], v[u * E + 1]);
+#pragma unroll
+            for (int e = 2; e < E; e += 2) most[u] = max3_of(most[u], v[u * E + e], v[u * E + e + 1]);
         }
-    };
-    if (tid == 0) { s_count = 0; s_from = 0; }
-    auto compact = [&]() {                                        // the n best of what is kept, in order
-        const int kept = min(s_count, kKeys);
-        for (int i = tid; i < kept; i += kScanThreads) {
-            const u64 key = s_key[i];
-            int rank = 0;
-            for (int j = 0; j < kept; ++j) rank += s_key[j] > key;
-            if (rank < n) s_best[rank] = key;
-        }
-        __syncthreads();
-        if (tid < min(kept, n)) s_key[tid] = s_best[tid];
-        if (tid == 0) {
-            s_count = min(kept, n);
-            if (kept >= n) s_from = s_best[n - 1] + 1;
-        }
-        __syncthreads();
-    };
-    load(lo);
-    for (int at = lo; at == lo || at < hi; at += U * kScanThreads) {
-        float v[kTurn], most = -INFINITY;
-        uint32_t pending = 0;
+        float now = sum.top;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int piece = at + u * kScanThreads + tid, there = piece < hi ? (int)min((int64_t)E, V - (int64_t)piece * E) : 0;
-            floats<T>(next[u], v + u * E);
-            pending |= ((1u << there) - 1u) << (u * E);
+            if (most[u] > now) first = at + u * kScanThreads + tid;
+            now = fmaxf(now, most[u]);
+        }
+        sum.add(v, now);
+    };
+    const int turns = (whole - lo) / kStep, rest = lo + turns * kStep;                 // turns that are all there
+    {
+        const uint4 *vec = reinterpret_cast<const uint4 *>(x) + lo + tid;
+        uint4 next[2][U];
+        auto ask = [&](uint4 (&to)[U], int k) {
+            if (k >= turns) return;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                if (e >= there) v[u * E + e] = -INFINITY;
-                most = fmaxf(most, v[u * E + e]);
+            for (int u = 0; u < U; ++u) to[u] = vec[k * kStep + u * kScanThreads];
+        };
+        ask(next[0], 0);
+        ask(next[1], 1);
+        if (turns > 0) first = lo + tid;
+        for (int k = 0; k < turns; k += 2) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (k + h >= turns) break;
+                uint4 raw[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) raw[u] = next[h][u];
+                ask(next[h], k + h + 2);
+                turn(lo + (k + h) * kStep, raw, true);
             }
         }
-        load(at + U * kScanThreads);
-        const float now = fmaxf(top, most), ref = now == -INFINITY ? 0.f : now;
-        float more[2] = {sum * beam_exp2((top - ref) * kLog2), 0.f};
-#pragma unroll
-        for (int e = 0; e < kTurn; ++e) more[e & 1] += beam_exp2((v[e] - ref) * kLog2);
-        sum = more[0] + more[1];
-        top = now;
-        auto token = [&](int e) { return (at + (e / E) * kScanThreads + tid) * E + e % E; };
-        if (at == lo) {
-            u64 best = 0;
-#pragma unroll
-            for (int e = 0; e < kTurn; ++e)
-                if (pending >> e & 1) best = max(best, beam_key(v[e], token(e)));
-            const bool fours = n <= 32;
-            if (fours) {
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-            }
-            const int groups = fours ? kScanThreads / 4 : kScanThreads;
-            if (!fours || (lane & 3) == 0) s_best[fours ? tid >> 2 : tid] = best;
-            __syncthreads();
-            if (tid < groups) {
-                const u64 mine = s_best[tid];
-                int rank = 0;
-#pragma unroll 8
-                for (int j = 0; j < groups; ++j) rank += s_best[j] > mine;
-                if (rank == n - 1 && mine) s_from = mine;
-            }
-            __syncthreads();
-        }
-        bool again;
-        do {                                                      // more than once where there is no room for all that pass
-            const u64 from = s_from;
-            bool full = false;
-            if (most >= from_ordered((uint32_t)(from >> 32)) || from == 0) {
-#pragma unroll
-                for (int e = 0; e < kTurn; ++e)
-                    if (pending >> e & 1) {
-                        const u64 key = beam_key(v[e], token(e));
-                        if (key >= from) {
-                            const int place = atomicAdd(&s_count, 1);
-                            if (place < kKeys) s_key[place] = key;
-                            full |= place >= n + 48;
-                            if (place < kKeys) pending &= ~(1u << e);
-                        } else {
-                            pending &= ~(1u << e);
-                        }
-                    }
-            } else {
-                pending = 0;
-            }
-            again = __syncthreads_or(full);
-            if (again) {
-                compact();
-                again = __syncthreads_or(pending != 0);
-            }
-        } while (again);
     }
-    __syncthreads();
-    compact();
-    const int64_t at = row * p.parts + part;
-    if (tid < n) p.keys[at * n + tid] = tid < s_count ? s_key[tid] : 0;
-    const float all = warp_max(top);
+    if (tid == 0) { s_from = 0; s_threads = s_count = 0; }
+    for (int at = rest; at < hi; at += kStep) {
+        uint4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = load(at + u * kScanThreads + tid);
+        turn(at, raw, false);
+    }
+
+    const u64 mine = first == INT32_MAX ? 0 : beam_key(sum.top, first);
+    const int width = n <= 16 ? 8 : n <= 32 ? 4 : 1, groups = kScanThreads / width;    // threads of a group
+    u64 best = mine;
+    for (int o = 1; o < width; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane % width == 0) s_best[tid / width] = best;
+    const float all = warp_max(sum.top);
     if (lane == 0) s_top[warp] = all;
     __syncthreads();
-    float best = s_top[0];
+    {                                                             // the n-th best of the groups, a vote for each
+        u64 held[kScanThreads / 32];
 #pragma unroll
-    for (int w = 1; w < kScanThreads / 32; ++w) best = fmaxf(best, s_top[w]);
-    double d = sum == 0.f ? 0.0 : (double)sum * (double)beam_exp2((top - best) * kLog2);
+        for (int k = 0; k < kScanThreads / 32; ++k) held[k] = 32 * k < groups ? s_best[32 * k + lane] : 0;
+        for (int g = warp; g < groups; g += kScanThreads / 32) {
+            const u64 one = s_best[g];
+            int rank = 0;
+#pragma unroll
+            for (int k = 0; k < kScanThreads / 32; ++k)
+                if (32 * k < groups) rank += __popc(__ballot_sync(0xffffffffu, held[k] > one));
+            if (lane == 0 && rank == n - 1 && one) s_from = one;
+        }
+    }
+    float top = s_top[0];
+#pragma unroll
+    for (int w = 1; w < kScanThreads / 32; ++w) top = fmaxf(top, s_top[w]);
+    double d = sum.sum == 0.f ? 0.0 : (double)sum.sum * (double)beam_exp2((sum.top - top) * kLog2);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
     if (lane == 0) s_sum[warp] = d;
     __syncthreads();
-    if (tid == 0) {
+    const int64_t out = row * p.parts + part;
+    if (tid == kScanThreads - 1) {
         d = 0.0;
+#pragma unroll
         for (int w = 0; w < kScanThreads / 32; ++w) d += s_sum[w];
-        p.sums[at] = d;
-        p.tops[at] = best;
+        p.sums[out] = d;
+        p.tops[out] = top;
     }
+    // keys of pieces here: a token's place behind its piece's
+    if (mine && mine >= s_from) s_thread[atomicAdd(&s_threads, 1)] = tid;
+    u64 from = s_from;
+    const u64 from_piece = from;
+    const float from_x = from_ordered((uint32_t)(from >> 32));
+    bool lost;
+    do {
+        __syncthreads();
+        lost = false;
+        const int each = (hi - lo + kScanThreads - 1) / kScanThreads;                  // pieces of a thread
+        for (int i = warp; i < s_threads; i += kScanThreads / 32)
+            for (int j = lane; j < each; j += 32) {
+                const int piece = lo + j * kScanThreads + s_thread[i], some = here(piece);
+                const uint4 raw = load(piece);
+                float v[E];
+                floats<T>(raw, v);
+                uint32_t reach = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e) reach |= v[e] < from_x ? 0u : 1u << e;     // from_x is no number where everything does
+                reach &= (1u << some) - 1u;
+                while (reach) {
+                    const int e = __ffs(reach) - 1;
+                    reach &= reach - 1;
+                    float one = v[0];
+#pragma unroll
+                    for (int k = 1; k < E; ++k) one = k == e ? v[k] : one;
+                    const u64 key = beam_key(one, piece * E + e);
+                    if (beam_key(one, piece) < from_piece || (from != from_piece && key < from)) continue;
+                    const int place = atomicAdd(&s_count, 1);
+                    if (place < kKeys) s_key[place] = key;
+                    else lost = true;
+                }
+            }
+        lost = __syncthreads_or(lost);
+        const int kept = min(s_count, kKeys);
+        for (int i = tid; i < kept; i += kScanThreads) {
+            const u64 key = s_key[i];
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < kept; ++j) rank += s_key[j] > key;
+            if (rank < n) s_best[rank] = key;
+        }
+        __syncthreads();
+        if (lost) {
+            from = s_best[n - 1];
+            if (tid == 0) s_count = 0;
+        } else if (tid < n) {
+            p.keys[out * n + tid] = tid < kept ? s_best[tid] : 0;
+        }
+    } while (lost);
 }
 
 // The largest of the lanes' keys; `lane_of`: the first lane that has it.
@@ -216,9 +272,132 @@ __device__ __forceinline__ u64 ordered64(double x) {              // as ordered(
     return u ^ ((long long)u < 0 ? ~0ull : 1ull << 63);
 }
 
-// A CTA a request.  A warp joins a beam's parts: its sum, and the n best of sorted lists, one a lane, by looking n times which head is the best.  Then
-// one warp joins the beams alike, two a lane, and lists those that do not end.
-__global__ void __launch_bounds__(256) beam_join_kernel(const __grid_constant__ BeamArgs p) {
+// The sum of a beam's exponentials from its parts', a lane each: score minus its logarithm, which a logit is added to; not finite where the beam offers nothing.
+__device__ __forceinline__ double beam_base(const BeamArgs &p, int64_t row, int lane, double &all) {
+    const float my_top = lane < p.parts ? p.tops[row * p.parts + lane] : -INFINITY, top = warp_max(my_top);
+    double sum = lane < p.parts ? p.sums[row * p.parts + lane] : 0.0;
+    if (sum != 0.0) sum *= (double)expf(my_top - top);             // 2^-23: as exact as the terms
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    all = (double)top + log(sum);
+    return (double)p.a.scores[row];
+}
+__device__ __forceinline__ void put_best(const BeamArgs &p, int64_t at, float value, int beam, int token) {
+    p.a.out_scores[at] = value;
+    p.a.out_beams[at] = beam;
+    p.a.out_tokens[at] = token;
+}
+__device__ __forceinline__ void put_next(const BeamArgs &p, int64_t at, float value, int beam, int token) {
+    p.a.next_scores[at] = value;
+    p.a.next_beams[at] = beam;
+    p.a.next_tokens[at] = token;
+}
+
+// Few candidates: a CTA a request, a thread a candidate -- beam, part, place in the part's sorted list.  The n-th best
+// of the first ceil(n / lists) of every list bounds the n-th best of all, and so does every list's last (beams' scores may lie far apart), so that hardly more
+// than n are left to be counted against each other, 32 by a vote.  What counts
+// here is the chain of dependent instructions (some 300, at eight cycles each): both launches for 4 beams of 32000 tokens, 8.2 us so, 11.0 by beam_merge_kernel.
+constexpr int kFewCandidates = 512;
+__global__ void __launch_bounds__(kFewCandidates) beam_count_kernel(const __grid_constant__ BeamArgs p) {
+    __shared__ double s_all[kMostBeams], s_score[kMostBeams];
+    __shared__ u64 s_value[kFewCandidates], s_place[kFewCandidates], s_from;       // ordered values; (beam, token)
+    __shared__ uint32_t s_goes[(kMostBest + 31) / 32];
+    __shared__ int s_left;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5, n = p.a.n, K = p.a.beams, list = p.parts * n, all = K * list;
+    const int beam = min(tid / list, K - 1), i = tid - beam * list;
+    const u64 key = tid < all ? p.keys[((int64_t)blockIdx.x * K + beam) * list + i] : 0;
+    for (int b = warp; b < K; b += warps) {
+        double sum;
+        const double score = beam_base(p, (int64_t)blockIdx.x * K + b, lane, sum);
+        if (lane == 0) { s_all[b] = sum; s_score[b] = score; }
+    }
+    if (tid < (kMostBest + 31) / 32) s_goes[tid] = 0;
+    if (tid == 0) { s_left = 0; s_from = 0; }
+    __syncthreads();
+    double value = -INFINITY;
+    int token = (int)~(uint32_t)key;
+    bool there = key != 0;
+    if (tid < all) {
+        if (!isfinite(s_all[beam]) || !isfinite(s_score[beam])) {
+            token = i;                                            // its first tokens, once
+            there = i < n && i < p.a.vocabulary;
+        } else if (there) {
+            value = s_score[beam] + ((double)from_ordered((uint32_t)(key >> 32)) - s_all[beam]);
+        }
+    }
+    there &= tid < all;
+    const u64 mine = there ? ordered64(value) : 0, place = (u64)beam << 32 | (uint32_t)token;
+    const int lists = K * p.parts, firsts = (n + lists - 1) / lists, heads = lists * firsts;
+    if (heads <= 32) {
+        s_value[tid] = mine;
+        __syncthreads();
+        const u64 head = lane < heads ? s_value[lane / firsts * n + lane % firsts] : 0, last = lane < lists ? s_value[lane * n + n - 1] : 0;
+        int whose;
+        const u64 full = warp_best(last, whose);                  // n reach it in its own list
+        for (int h = warp; h < heads; h += warps) {
+            const u64 one = __shfl_sync(0xffffffffu, head, h);
+            const int better = __popc(__ballot_sync(0xffffffffu, head > one)), reach = __popc(__ballot_sync(0xffffffffu, head >= one));
+            if (lane == 0 && better < n && reach >= n) s_from = max(one, full);  // the n-th best; several may be it
+        }
+        __syncthreads();
+    }
+    int slot = -1;
+    if (there && mine >= s_from) {
+        slot = atomicAdd(&s_left, 1);
+        s_place[slot] = place;
+    }
+    const int keep = slot;
+    __syncthreads();
+    if (keep >= 0) s_value[keep] = mine;
+    __shared__ int s_rank[kFewCandidates];
+    __syncthreads();
+    const int left = s_left;
+    for (int base = 0; base < left; base += 128) {                // 128 of them stand in a warp's registers
+        u64 held[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) held[k] = base + 32 * k + lane < left ? s_value[base + 32 * k + lane] : 0;
+        for (int m = warp; m < left; m += warps) {
+            const u64 v = s_value[m], at = s_place[m];
+            int rank = 0, alike = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (base + 32 * k >= left) break;
+                rank += __popc(__ballot_sync(0xffffffffu, held[k] > v));
+                alike += __popc(__ballot_sync(0xffffffffu, held[k] == v));
+            }
+            if (alike > 1 || (alike == 1 && (m < base || m >= base + 128))) {          // equal ones by their places
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int j = base + 32 * k + lane;
+                    rank += __popc(__ballot_sync(0xffffffffu, j < left && held[k] == v && s_place[min(j, left - 1)] < at));
+                }
+            }
+            if (lane == 0) s_rank[m] = base ? s_rank[m] + rank : rank;
+        }
+    }
+    __syncthreads();
+    const int rank = keep >= 0 ? s_rank[keep] : n;
+    if (rank < n) {
+        put_best(p, (int64_t)blockIdx.x * n + rank, (float)value, beam, token);
+        bool ends = false;
+        for (int e = 0; e < p.a.n_ends; ++e) ends |= p.a.ends[e] == token;
+        if (!ends) atomicOr(&s_goes[rank >> 5], 1u << (rank & 31));
+    }
+    __syncthreads();
+    int before = 0, going = 0;                                    // those that go on and are better; all
+#pragma unroll
+    for (int w = 0; w < (kMostBest + 31) / 32; ++w) {
+        const uint32_t bits = s_goes[w];
+        before += __popc(w < rank >> 5 ? bits : w == rank >> 5 ? bits & ((1u << (rank & 31)) - 1u) : 0u);
+        going += __popc(bits);
+    }
+    if (rank < n && (s_goes[rank >> 5] >> (rank & 31) & 1u) && before < K) put_next(p, (int64_t)blockIdx.x * K + before, (float)value, beam, token);
+    for (int k = going + tid; k < K; k += blockDim.x) put_next(p, (int64_t)blockIdx.x * K + k, -INFINITY, 0, 0);       // everything else ends
+}
+
+// Many: a CTA a request.  A warp joins a beam's parts, sorted lists, one a lane, by looking n times which head is the best.  Then one warp joins the beams
+// alike, two a lane, and lists those that do not end.
+__global__ void __launch_bounds__(256) beam_merge_kernel(const __grid_constant__ BeamArgs p) {
     extern __shared__ __align__(16) u64 s_join[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, n = p.a.n, K = p.a.beams, parts = p.parts;
     double *s_value = reinterpret_cast<double *>(s_join);         // [K][n]
@@ -227,13 +406,8 @@ __global__ void __launch_bounds__(256) beam_join_kernel(const __grid_constant__ 
     for (int b = warp; b < K; b += warps) {
         const int64_t row = (int64_t)blockIdx.x * K + b;
         for (int i = lane; i < parts * n; i += 32) s_list[i] = p.keys[row * parts * n + i];
-        const float score = p.a.scores[row], my_top = lane < parts ? p.tops[row * parts + lane] : -INFINITY;
-        const float top = warp_max(my_top);
-        double sum = lane < parts ? p.sums[row * parts + lane] : 0.0;
-        if (sum != 0.0) sum *= exp((double)my_top - (double)top);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const double all = (double)top + log(sum);
+        double all;
+        const double score = beam_base(p, row, lane, all);
         const bool alive = isfinite(all) && isfinite(score);
         __syncwarp();
         int at = 0;
@@ -244,7 +418,7 @@ __global__ void __launch_bounds__(256) beam_join_kernel(const __grid_constant__ 
             if (alive) {
                 const u64 best = warp_best(mine, whose);
                 token = (int)~(uint32_t)best;
-                if (best) value = (double)score + ((double)from_ordered((uint32_t)(best >> 32)) - all);
+                if (best) value = score + ((double)from_ordered((uint32_t)(best >> 32)) - all);
                 else token = INT32_MAX;                           // a vocabulary of fewer than n
                 if (lane == whose) mine = ++at < n ? s_list[lane * n + at] : 0;
             } else if (i >= p.a.vocabulary) {
@@ -277,28 +451,20 @@ __global__ void __launch_bounds__(256) beam_join_kernel(const __grid_constant__ 
         for (int e = lane + 32; e < p.a.n_ends; e += 32) ends |= p.a.ends[e] == token;
         ends = __any_sync(0xffffffffu, ends);
         if (lane == 0) {
-            p.a.out_scores[out + i] = value;
-            p.a.out_beams[out + i] = b;
-            p.a.out_tokens[out + i] = token;
-            if (!ends && going < K) {
-                p.a.next_scores[go + going] = value;
-                p.a.next_beams[go + going] = b;
-                p.a.next_tokens[go + going] = token;
-            }
+            put_best(p, out + i, value, b, token);
+            if (!ends && going < K) put_next(p, go + going, value, b, token);
         }
         going += !ends;
     }
-    for (int i = going + lane; i < K; i += 32) {                  // everything else ends
-        p.a.next_scores[go + i] = -INFINITY;
-        p.a.next_beams[go + i] = 0;
-        p.a.next_tokens[go + i] = 0;
-    }
+    for (int i = going + lane; i < K; i += 32) put_next(p, go + i, -INFINITY, 0, 0);           // everything else ends
 }
 
-// Parts of a row: enough CTAs for all SMs, whole first turns; 1024 keys of a beam at most are joined.
+// Parts of a row: a part of its own costs some 4 us of beginning and end beside 0.4 us a turn, so one CTA an SM where rows are few and four where they are many
+// (16 rows of 128256: 11.0 us in 8 parts, 14.0 in 32; 128 of 32000: 12.0 in one, 16.2 in 4; 256 of 128256: 25.4 in 2, 28.3 in 4).  1024 keys of a beam at
+// most are joined.
 static int beam_parts(const kvq_beam_args &a) {
     const int64_t rows = (int64_t)a.requests * a.beams;
-    int64_t parts = (4 * 148 + rows - 1) / rows;
+    int64_t parts = (rows <= 148 ? 148 : 4 * 148) / (rows > 0 ? rows : 1);
     const int64_t most = (a.vocabulary + kScanThreads * kTurn - 1) / (kScanThreads * kTurn);
     if (parts > most) parts = most;
     if (parts > kMostParts) parts = kMostParts;
@@ -345,10 +511,15 @@ extern "C" int kvq_beam_select(const kvq_beam_args *a, kvq_stream_t stream) {
     else if (a->type == KVQ_BF16) scan(beam_scan_kernel<__nv_bfloat16, true>, beam_scan_kernel<__nv_bfloat16, false>);
     else scan(beam_scan_kernel<__half, true>, beam_scan_kernel<__half, false>);
     if (const int rc = check_launch()) return rc;
+    const int64_t lists = (int64_t)a->beams * p.parts, candidates = lists * a->n, heads = (a->n + lists - 1) / lists * lists;
+    if (candidates <= 128 || (candidates <= kFewCandidates && heads <= 32)) {
+        beam_count_kernel<<<(unsigned)a->requests, candidates <= 256 ? 256 : kFewCandidates, 0, st>>>(p);
+        return check_launch();
+    }
     const int warps = a->beams < 8 ? a->beams : 8, pairs = a->beams * a->n;
     const size_t smem = (size_t)pairs * 8 + (size_t)(pairs + 1) / 2 * 8 + (size_t)warps * p.parts * a->n * 8;
-    const cudaError_t e = cudaFuncSetAttribute(beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     if (e != cudaSuccess) return record_cuda_error(e);
-    beam_join_kernel<<<(unsigned)a->requests, 32 * warps, smem, st>>>(p);
+    beam_merge_kernel<<<(unsigned)a->requests, 32 * warps, smem, st>>>(p);
     return check_launch();
 }
