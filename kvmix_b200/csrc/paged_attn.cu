@@ -145,6 +145,7 @@ struct PagedPlan {
     bool few, tiles;                  // which kernels are launched
     int few_rows;                     // sequences with more rows are the kernel of tiles'
     int few_splits, tile_splits, max_tiles;
+    FewShape shape;                   // of the kernel of few rows, differential attention
 };
 
 static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, int max_new, int max_tokens, int max_chunks, bool diff) {
@@ -158,15 +159,28 @@ static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, 
     const int pages = (max_tokens + kPage - 1) / kPage;
     // Kernel of few rows: the splits that take the fewest rounds of pages (four warps a CTA), over all waves of CTAs; a CTA's beginning and
     // end count two rounds, the launch that joins the splits another two.
-    const FewShape f = diff ? diff_shape(l, rep, max_new) : few_shape(l, rep, max_new);
-    const int64_t pairs = (int64_t)n * l.Hkv * f.row_blocks, slots = 148 * f.ctas;
-    double best = 1e30;
+    auto splits = [&](const FewShape &f, double round, double &least) {
+        const int64_t pairs = (int64_t)n * l.Hkv * f.row_blocks, slots = 148 * f.ctas;
+        int r = 1;
+        least = 1e30;
+        for (int s = 1; s <= 128 && (s == 1 || s <= pages / 2); ++s) {
+            const double w = (double)(pairs * s) / slots, waves = w <= 1 ? 1 : w < 4 ? (double)((pairs * s + slots - 1) / slots) : w + 0.5;
+            const int rounds = ((pages + s - 1) / s + 3) / 4;
+            const double cost = waves * (rounds * round + 2) + (s > 1 ? 2 : 0);
+            if (cost < least) { least = cost; r = s; }
+        }
+        return r;
+    };
+    double best;
     r.few_splits = 1;
-    for (int s = 1; r.few && s <= 128 && (s == 1 || s <= pages / 2); ++s) {
-        const double w = (double)(pairs * s) / slots, waves = w <= 1 ? 1 : w < 4 ? (double)((pairs * s + slots - 1) / slots) : w + 0.5;
-        const int rounds = ((pages + s - 1) / s + 3) / 4;
-        const double cost = waves * (rounds + 2) + (s > 1 ? 2 : 0);
-        if (cost < best) { best = cost; r.few_splits = s; }
+    if (r.few && !diff) r.few_splits = splits(few_shape(l, rep, max_new), 1, best);
+    // Differential attention: fewer rows to a CTA while that leaves SMs to do them (one token over 777 tokens, 8 heads of 4: 18 us by two rows, 37 by eight), else as
+    // many as the columns hold, what a page costs beside its rows being as much as five rows.
+    double least = 1e30;
+    for (int most = 2; r.few && diff && most <= kFewRows; most *= 2) {
+        const FewShape f = diff_shape(l, rep, max_new, most);
+        const int s = splits(f, 0.7 * (1 + f.rows / 5.0), best);
+        if (best < 0.97 * least) { least = best; r.few_splits = s; r.shape = f; }
     }
     int64_t tiles = ((int64_t)tokens * rep) / 256 + (r.few && max_chunks < n ? max_chunks : n);     // without the other kernel every sequence is one of chunks
     if (n == 1) tiles = ((int64_t)tokens * rep + 255) / 256;
@@ -246,6 +260,7 @@ static int attend(const kvq_page_book *b, const kvq_page_layer *l, const kvq_pag
         p.lambdas = diff->lambdas;
         p.norm_weight = diff->norm_weight;
         p.norm_eps = diff->norm_eps;
+        p.few_shape = r.shape;
     }
     p.k_groups = page_groups(l->k_bits, l->group);
     p.v_groups = page_groups(l->v_bits, l->group);

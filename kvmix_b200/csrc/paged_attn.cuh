@@ -12,6 +12,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // kernel of tiles.
 constexpr int kFewRows = 8;
 
+// How the kernel of few rows takes them: rows to a CTA, blocks of them to a (sequence, kv head); sets of key columns; CTAs of an SM
+struct FewShape { int rows, row_blocks, key_sets, ctas; };
+
 struct PagedArgs {
     kvq_page_book b;
     kvq_page_layer l;
@@ -27,6 +30,7 @@ struct PagedArgs {
     // everywhere, slopes and outputs are those of query heads.
     const float *lambdas, *norm_weight;                           // [query heads]; [128] or NULL
     float norm_eps;
+    FewShape few_shape;
 };
 // What becomes of a head's two attentions over the values, channel by channel; then its norm over the channels, where there is one: x * diff_norm() * weight
 __device__ __forceinline__ float diff_of(float a, float b, float lambda) { return fmaf(-lambda, b, a); }
@@ -65,7 +69,6 @@ __device__ __forceinline__ void paged_bounds(const PagedArgs &p, const PagedSeq 
 
 // A CTA of the kernel of few rows: as many query rows as the columns of an MMA hold with all groups (keys twice, as hi and lo, in one or two
 // sets of columns); CTAs of an SM.
-struct FewShape { int rows, row_blocks, key_sets, ctas; };
 inline FewShape few_shape(const kvq_page_layer &l, int rep, int max_new) {
     const int64_t most = (int64_t)max_new * rep;
     const int rows = most < kFewRows ? (int)most : kFewRows, ng = kHeadDim / l.group;
@@ -81,17 +84,13 @@ inline FewShape few_shape(const kvq_page_layer &l, int rep, int max_new) {
     return f;
 }
 
-// The same where heads are two rows each: a channel belongs to one half of the keys, so B's columns of a k-step hold that half's rows alone, and the columns of
-// one set that hold the keys of a head's two rows twice as hi and lo are as many as those that hold both rows' weights.  Two sets where
-// one does not hold all rows.
-inline FewShape diff_shape(const kvq_page_layer &l, int rep, int max_new) {
-    const int64_t most = (int64_t)max_new * rep;
-    const int rows = most < kFewRows ? (int)most : kFewRows, ng = kHeadDim / l.group;
-    FewShape f = {kFewRows, 1, 1, 3};
-    if (l.k_bits != 3 || l.v_bits != 3) {
-        if (rows > 8 / ng) f.key_sets = 2;
-        f.rows = 8 * f.key_sets / ng;
-    }
+// The same where heads are two rows each, for `most` rows at most to a CTA (even): the columns of a k-step hold the keys of half the rows twice, as hi and lo, and
+// the weights of all of them once.
+inline FewShape diff_shape(const kvq_page_layer &l, int rep, int max_new, int most) {
+    const int64_t all = (int64_t)max_new * rep;
+    const int rows = all < kFewRows ? (int)all : kFewRows, ng = kHeadDim / l.group;
+    FewShape f = {l.k_bits == 3 && l.v_bits == 3 ? kFewRows : 8 / ng, 1, 1, 3};
+    if (f.rows > most) f.rows = most;
     if (f.rows > rows) f.rows = rows;
     f.row_blocks = (rows + f.rows - 1) / f.rows;
     return f;

@@ -154,8 +154,8 @@ struct FewShared {
     }
 };
 
-// DIFF: heads are two rows each (PagedArgs), R is even; CK counts the sets of columns of keys and of values, and the score columns of a k-step are those of
-// the rows whose half it is in: a page's scores come half by half.
+// DIFF: heads are two rows each (PagedArgs), R is even, CK is 1.  A channel belongs to one half of the keys, so the score columns of a k-step are those of the
+// rows whose half it is in, and a page's scores come half by half: a head's two rows take as many products with the keys as one row of 128 channels.
 template <int KB, int VB, int CK, bool DIFF>
 __global__ void __launch_bounds__(kFewWarps * 32, DIFF || KB == 3 || VB == 3 || CK == 2 ? 3 : 4)
     paged_few_kernel(const __grid_constant__ PagedArgs p, int R, int row_blocks, int stages, int stage_rows, int stage_bytes) {
@@ -433,29 +433,16 @@ __global__ void __launch_bounds__(kFewWarps * 32, DIFF || KB == 3 || VB == 3 || 
     const float aside_ref = ref;
 
     // ---- packed pages
-    constexpr int VN = DIFF && VB != 3 ? CK : 1;                  // sets of columns
-    float out[VN][VT][4], out_mn[VN][4];
+    float out[VT][4], out_mn[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int n = 0; n < VN; ++n)
+    for (int m = 0; m < VT; ++m)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            out_mn[n][e] = 0.f;
-#pragma unroll
-            for (int m = 0; m < VT; ++m) out[n][m][e] = 0.f;
-        }
+        for (int e = 0; e < 4; ++e) out[m][e] = 0.f;
     // values' columns: group and row of B's column g, and of the accumulators' columns 2t, 2t + 1 (VPAIR: hi and lo of one row)
     constexpr bool VPAIR = !DIFF && KB != 3 && VB != 3 && CK == 1;
-    const int vr_log2 = VB == 3 ? 3 : (VPAIR ? 2 : 2 + VN) - ng_log2;
-    int v_grp[VN], v_row[VN], o_grp[VN], o_row[VN];
-#pragma unroll
-    for (int n = 0; n < VN; ++n) {
-        const int v_col = VPAIR ? g >> 1 : 8 * n + g, o_col = VPAIR ? t : 8 * n + 2 * t;
-        v_grp[n] = v_col >> vr_log2;
-        v_row[n] = min(v_col & ((1 << vr_log2) - 1), R - 1);
-        o_grp[n] = o_col >> vr_log2;
-        o_row[n] = o_col & ((1 << vr_log2) - 1);
-    }
-    auto o_row1 = [&](int n) { return VPAIR ? o_row[n] : o_row[n] + 1; };
+    const int vr_log2 = VB == 3 ? 3 : (VPAIR ? 2 : 3) - ng_log2, v_col = VPAIR ? g >> 1 : g, o_col = VPAIR ? t : 2 * t;
+    const int v_grp = v_col >> vr_log2, v_row = min(v_col & ((1 << vr_log2) - 1), R - 1), o_row = o_col & ((1 << vr_log2) - 1), o_grp = o_col >> vr_log2;
+    const int o_row1 = VPAIR ? o_row : o_row + 1;
     const uint32_t v_lo = VPAIR && (g & 1) ? 0xffffffffu : 0u;
     // p * scale * 2^expo: the power of two starts from the first scales (the largest of them becomes 4 to 8) and follows them where a stage's largest
     // would exceed 256 or stay below 2^-5; the sums so far go along, exactly
@@ -594,14 +581,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, DIFF || KB == 3 || VB == 3 || 
             put_scores(1);
         }
         if (softmax_page(page_at(k) * kPage, kPage)) {
-#pragma unroll
-            for (int n = 0; n < VN; ++n) {
-                rescale(out[n], o_row[n], o_row1(n));
-                if constexpr (VB != 3) {
-                    const float a0 = __shfl_sync(0xffffffffu, alpha, o_row[n]), a1 = __shfl_sync(0xffffffffu, alpha, o_row1(n));
-                    out_mn[n][0] *= a0;
-                    out_mn[n][1] *= a1;
-                }
+            rescale(out, o_row, o_row1);
+            if constexpr (VB != 3) {
+                const float a0 = __shfl_sync(0xffffffffu, alpha, o_row), a1 = __shfl_sync(0xffffffffu, alpha, o_row1);
+                out_mn[0] *= a0;
+                out_mn[1] *= a1;
             }
         }
 #pragma unroll 1
@@ -614,7 +598,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, DIFF || KB == 3 || VB == 3 || 
                 for (int at = 0; at < stage_rows; at += 16) {
                     uint32_t b0, b1;
                     weights(min(g, R - 1), step0 + at / 16, b0, b1);
-                    few_step3(out[0], c, c_sc, c_mn, at, g, t, b0, b1);
+                    few_step3(out, c, c_sc, c_mn, at, g, t, b0, b1);
                 }
             } else {
                 // the exponent of the stage's largest scale: its scales are stage_rows * groups / 32 a lane, two at a time
@@ -626,11 +610,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, DIFF || KB == 3 || VB == 3 || 
                     if (want != expo) {
                         const float f = expo == 32 ? 0.f : exp2f((float)(want - expo));
 #pragma unroll
-                        for (int n = 0; n < VN; ++n)
+                        for (int m = 0; m < 8; ++m)
 #pragma unroll
-                            for (int m = 0; m < 8; ++m)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) out[n][m][e] *= f;
+                            for (int e = 0; e < 4; ++e) out[m][e] *= f;
                         expo = want;
                     }
                 }
@@ -638,30 +620,22 @@ __global__ void __launch_bounds__(kFewWarps * 32, DIFF || KB == 3 || VB == 3 || 
 #pragma unroll 1
                 for (int at = 0; at < stage_rows; at += 16) {
                     const FewWords<VB> a(c, at, g, t);
-                    uint32_t b[VN][2], mn[2];
+                    uint32_t b0, b1, mn[2], sv[2];
+                    weights(v_row, step0 + at / 16, b0, b1);
                     few_pairs(c_mn, at, t, p.v_groups, g & (p.v_groups - 1), mn);
-#pragma unroll
-                    for (int n = 0; n < VN; ++n) {
-                        uint32_t sv[2];
-                        weights(v_row[n], step0 + at / 16, b[n][0], b[n][1]);
-                        few_pairs(c_sc, at, t, p.v_groups, v_grp[n], sv);
-                        const __half2 s0 = __hmul2(as_h2(sv[0]), by), s1 = __hmul2(as_h2(sv[1]), by);
-                        if constexpr (VPAIR) {
-                            mma16816(out_mn[n], mn[0], 0u, mn[1], 0u, b[n][0] & ~v_lo, b[n][1] & ~v_lo);
-                            b[n][0] = hilo(as_h2(b[n][0]), s0, v_lo);
-                            b[n][1] = hilo(as_h2(b[n][1]), s1, v_lo);
-                        } else {
-                            mma16816(out_mn[n], mn[0], 0u, mn[1], 0u, b[n][0], b[n][1]);
-                            b[n][0] = as_u32(__hmul2(as_h2(b[n][0]), s0));
-                            b[n][1] = as_u32(__hmul2(as_h2(b[n][1]), s1));
-                        }
+                    few_pairs(c_sc, at, t, p.v_groups, v_grp, sv);
+                    const __half2 s0 = __hmul2(as_h2(sv[0]), by), s1 = __hmul2(as_h2(sv[1]), by);
+                    if constexpr (VPAIR) {
+                        mma16816(out_mn, mn[0], 0u, mn[1], 0u, b0 & ~v_lo, b1 & ~v_lo);
+                        b0 = hilo(as_h2(b0), s0, v_lo);
+                        b1 = hilo(as_h2(b1), s1, v_lo);
+                    } else {
+                        mma16816(out_mn, mn[0], 0u, mn[1], 0u, b0, b1);
+                        b0 = as_u32(__hmul2(as_h2(b0), s0));
+                        b1 = as_u32(__hmul2(as_h2(b1), s1));
                     }
 #pragma unroll
-                    for (int m = 0; m < 8; ++m) {
-                        const uint32_t a0 = a.a(m, 0), a1 = a.a(m, 1), a2 = a.a(m, 2), a3 = a.a(m, 3);
-#pragma unroll
-                        for (int n = 0; n < VN; ++n) mma16816(out[n][m], a0, a1, a2, a3, b[n][0], b[n][1]);
-                    }
+                    for (int m = 0; m < 8; ++m) mma16816(out[m], a.a(m, 0), a.a(m, 1), a.a(m, 2), a.a(m, 3), b0, b1);
                 }
             }
             stage_done();
@@ -685,24 +659,22 @@ __global__ void __launch_bounds__(kFewWarps * 32, DIFF || KB == 3 || VB == 3 || 
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int c = few_element<3>(g, m, e);
-                if (c >= 0 && 2 * t < rows) add(2 * t, c, out[0][m][2 * e], f0);
-                if (c >= 0 && 2 * t + 1 < rows) add(2 * t + 1, c, out[0][m][2 * e + 1], f1);
+                if (c >= 0 && 2 * t < rows) add(2 * t, c, out[m][2 * e], f0);
+                if (c >= 0 && 2 * t + 1 < rows) add(2 * t + 1, c, out[m][2 * e + 1], f1);
             }
     } else {
+        const float f0 = __shfl_sync(0xffffffffu, aside_by, o_row), f1 = __shfl_sync(0xffffffffu, aside_by, o_row1);
+        const float z0 = __shfl_sync(0xffffffffu, out_mn[0], 4 * own_group + t), z1 = __shfl_sync(0xffffffffu, out_mn[1], 4 * own_group + t);
         const float undo = expo == 32 ? 0.f : exp2f((float)-expo);
-#pragma unroll
-        for (int n = 0; n < VN; ++n) {
-            const float f0 = __shfl_sync(0xffffffffu, aside_by, o_row[n]), f1 = __shfl_sync(0xffffffffu, aside_by, o_row1(n));
-            const float z0 = __shfl_sync(0xffffffffu, out_mn[n][0], 4 * own_group + t), z1 = __shfl_sync(0xffffffffu, out_mn[n][1], 4 * own_group + t);
-            if (o_grp[n] != own_group) continue;
+        if (o_grp == own_group) {
 #pragma unroll
             for (int m = 0; m < 8; ++m)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int c = few_element<1>(g, m, e);
                     const float f = few_power<VB>(m, e) * undo;
-                    if (o_row[n] < rows) add(o_row[n], c, fmaf(VPAIR ? out[n][m][2 * e] + out[n][m][2 * e + 1] : out[n][m][2 * e], f, z0), f0);
-                    if (!VPAIR && o_row1(n) < rows) add(o_row1(n), c, fmaf(out[n][m][2 * e + 1], f, z1), f1);
+                    if (o_row < rows) add(o_row, c, fmaf(VPAIR ? out[m][2 * e] + out[m][2 * e + 1] : out[m][2 * e], f, z0), f0);
+                    if (!VPAIR && o_row1 < rows) add(o_row1, c, fmaf(out[m][2 * e + 1], f, z1), f1);
                 }
         }
     }
@@ -789,8 +761,9 @@ static int launch_few(const PagedArgs &p, int R, int row_blocks, cudaStream_t st
 
 template <int KB, int VB, bool DIFF>
 static int launch_few(const PagedArgs &p, cudaStream_t st) {
-    const FewShape f = DIFF ? diff_shape(p.l, p.rep, p.a.max_new) : few_shape(p.l, p.rep, p.a.max_new);
-    if constexpr (DIFF ? KB != 3 || VB != 3 : KB != 3)
+    if constexpr (DIFF) return launch_few<KB, VB, 1, DIFF>(p, p.few_shape.rows, p.few_shape.row_blocks, st);
+    const FewShape f = few_shape(p.l, p.rep, p.a.max_new);
+    if constexpr (KB != 3 && !DIFF)
         if (f.key_sets == 2) return launch_few<KB, VB, 2, DIFF>(p, f.rows, f.row_blocks, st);
     return launch_few<KB, VB, 1, DIFF>(p, f.rows, f.row_blocks, st);
 }

@@ -262,41 +262,44 @@ def page_append(k, v, cos, sin, q_start, rows, pages, layer, q=None, q_out=None,
     Tokens that ``page_write`` would leave out are left out; those whose position is outside the tables too, their queries with them, and a
     status bit says so.  Returns the queries, fp16 (q_out where it is given, which may be q itself; None without q); rows behind q_start[n] are left as they are."""
     dev, book = _book(pages)
-    heads, tokens = layer.kfull.shape[1], k.shape[0]
-    if k.dim() != 3 or k.shape[1:] != (heads, 128) or v.shape != k.shape or v.dtype is not k.dtype or k.dtype not in _TYPES:
+    kfull, kind, shape = layer.kfull, k.dtype, k.shape
+    heads = kfull.shape[1]
+    if len(shape) != 3 or shape[1] != heads or shape[2] != 128 or v.shape != shape or v.dtype is not kind or kind not in _TYPES:
         raise RuntimeError(f"page_append takes keys and values [tokens, {heads}, 128] of one type, fp16, bf16 or fp32")
-    if q is None:
-        if q_out is not None:
-            raise RuntimeError("q_out without q")
-    elif q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != 128 or q.dtype is not k.dtype:
-        raise RuntimeError(f"queries must be [{tokens}, heads, 128] of the keys' type")
-    if any(t.get_device() != dev for t in (k, v, cos, sin) + (() if q is None else (q,))):
+    if k.get_device() != dev or v.get_device() != dev or cos.get_device() != dev or sin.get_device() != dev or (q is not None and q.get_device() != dev):
         raise RuntimeError(f"keys, values, queries and angles must be on cuda:{dev}")
-    if cos.dim() != 2 or sin.shape != cos.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or (cos.numel() and (cos.stride(1) != 1 or sin.stride(1) != 1)):
-        raise RuntimeError("cos and sin must be float32 [positions, angles], contiguous along the angles")
-    angle_rows, angles = cos.shape
+    if cos.dim() != 2 or sin.shape != cos.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
+        raise RuntimeError("cos and sin must be float32 [positions, angles]")
+    tokens, (angle_rows, angles), (c_sT, c_s), (s_sT, s_s) = shape[0], cos.shape, cos.stride(), sin.stride()
     if parts not in (1, 2) or angles % 8 or not 0 < angles <= 64 // parts:
         raise RuntimeError("angles must be a multiple of 8, at most 64 / parts; parts 1 or 2")
+    if c_s != 1 or s_s != 1:
+        raise RuntimeError("cos and sin must be contiguous along the angles")
     if k.stride(2) != 1:
         k = k.contiguous()
     if v.stride(2) != 1:
         v = v.contiguous()
-    at_q = at_out = nh = 0
-    strides = (0, 0, 0, 0)
+    at_q = at_out = nh = q_sT = q_sH = o_sT = o_sH = 0
     if q is not None:
+        if q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != 128 or q.dtype is not kind:
+            raise RuntimeError(f"queries must be [{tokens}, heads, 128] of the keys' type")
         nh = q.shape[1]
         if q_out is None:
-            q_out = q.new_empty(q.shape, dtype=_f16)
+            q_out = q.new_empty((tokens, nh, 128)) if kind is _f16 else q.new_empty((tokens, nh, 128), dtype=_f16)
         elif q_out.shape != q.shape or q_out.dtype is not _f16 or q_out.get_device() != dev or q_out.stride(2) != 1 or not _rows_apart(q_out):
             raise RuntimeError("q_out must be fp16 like q, contiguous along the channels, its rows apart")
         if q.stride(2) != 1:
             q = q.contiguous()
-        at_q, at_out, strides = q.data_ptr(), q_out.data_ptr(), (q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1))
-    n = rows.numel()
-    a = _pack_append(k.data_ptr(), v.data_ptr(), at_q, at_out, cos.data_ptr(), sin.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), *strides,
-                     cos.stride(0), sin.stride(0), _ints(dev, "q_start", q_start, n + 1), _rows(dev, "rows", rows),
-                     0 if positions is None else _ints(dev, "positions", positions, tokens), n, tokens, nh, _TYPES[k.dtype], angles, angle_rows, parts, 1 if interleaved else 0)
-    _launched(_library().kvq_page_append(book, _layer(pages, dev, layer), a, ops.raw_stream()))
+        at_q, at_out, (q_sT, q_sH, _), (o_sT, o_sH, _) = q.data_ptr(), q_out.data_ptr(), q.stride(), q_out.stride()
+    elif q_out is not None:
+        raise RuntimeError("q_out without q")
+    n, (k_sT, k_sH, _), (v_sT, v_sH, _) = rows.numel(), k.stride(), v.stride()
+    at_k, at_v = _fp16_pages(pages, dev, layer)
+    block = _pack_layer(0, 0, 0, at_k, 0, 0, 0, at_v, heads, layer.k_bits, layer.v_bits, layer.group, 0, kfull.shape[0])        # packed pages are not touched
+    a = _pack_append(k.data_ptr(), v.data_ptr(), at_q, at_out, cos.data_ptr(), sin.data_ptr(), k_sT, k_sH, v_sT, v_sH, q_sT, q_sH, o_sT, o_sH, c_sT, s_sT,
+                     _ints(dev, "q_start", q_start, n + 1), _ints(dev, "rows", rows, n), 0 if positions is None else _ints(dev, "positions", positions, tokens), n, tokens, nh,
+                     _TYPES[kind], angles, angle_rows, parts, 1 if interleaved else 0)
+    _launched(_library().kvq_page_append(book, block, a, ops.raw_stream()))
     return q_out
 
 
