@@ -31,7 +31,9 @@ struct PagedArgs {
     const float *lambdas, *norm_weight;                           // [query heads]; [128] or NULL
     float norm_eps;
     FewShape few_shape;
+    int max_tiles, n_whole;           // kernel of tiles: (tile, kv head) pairs in the order of CTAs, of which the first n_whole are not cut
 };
+constexpr int kMostCutSequences = 8;                              // the launch that joins the splits of some tiles counts tiles sequence by sequence
 // What becomes of a head's two attentions over the values, channel by channel; then its norm over the channels, where there is one: x * diff_norm() * weight
 __device__ __forceinline__ float diff_of(float a, float b, float lambda) { return fmaf(-lambda, b, a); }
 __device__ __forceinline__ float diff_norm(const PagedArgs &p, float squares) { return rsqrtf(fmaf(squares, 1.f / kHeadDim, p.norm_eps)); }

@@ -172,7 +172,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     extern __shared__ __align__(1024) char smem[];
     __shared__ uint32_t s_tmem;
     // where this CTA's rows are: tiles of later tokens first, they see more
-    const int split = blockIdx.x % p.splits, hs = blockIdx.x / p.splits, head = hs % p.l.Hkv;
+    const bool whole = DIFF && (int)blockIdx.x < p.n_whole;
+    auto splits = [&]() { return DIFF && whole ? 1 : p.splits; };
+    const unsigned cta = blockIdx.x - (DIFF ? p.n_whole : 0);
+    const int split = DIFF && whole ? 0 : cta % p.splits, hs = DIFF && whole ? blockIdx.x : cta / p.splits + (DIFF ? p.n_whole : 0), head = hs % p.l.Hkv;
     int tile = max_tiles - 1 - hs / p.l.Hkv, seq = 0;
     auto tiles_of = [&](int i) {
         int q0, n_new;
@@ -289,7 +292,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         for (int w = 0; w < kTileThreads / 32; ++w) { first = min(first, s_first[w]); last = max(last, s_last[w]); }
     }
     const uint32_t tmem = s_tmem;
-    const int p_lo = first < last ? first / kPage : 0, p_hi = first < last ? pages_of(last) : 0, per = (p_hi - p_lo + p.splits - 1) / p.splits;
+    const int p_lo = first < last ? first / kPage : 0, p_hi = first < last ? pages_of(last) : 0, per = (p_hi - p_lo + splits() - 1) / splits();
     const int p0 = p_lo + split * per, np = max(0, min(p_hi, p0 + per) - p0);
     int32_t *const status = &p.b.count[2];
     auto page_id = [&](int page) {
@@ -434,7 +437,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             __half *out = static_cast<__half *>(p.a.out) + (int64_t)(s.q0 + u) * p.a.o_sT + (int64_t)h * p.a.o_sH + half * N;
             const int64_t part = (int64_t)split * p.a.tokens * p.a.nh + (int64_t)(s.q0 + u) * p.a.nh + (DIFF ? 2 * h + tile_of : h);
             const bool vec = (reinterpret_cast<uintptr_t>(p.a.out) % 16 | p.a.o_sT % 8 | p.a.o_sH % 8) == 0;
-            if (DIFF && p.splits == 1) {
+            if (DIFF && splits() == 1) {
                 // The operand buffers are free: no copy and no product is under way.  A row's 16-byte pieces are mixed by its number.
                 float *const other = reinterpret_cast<float *>(smem + kOffK);
                 auto piece = [&](int k) { return reinterpret_cast<float4 *>(other + r * 128) + ((half * (N / 4) + k) ^ (r & 31)); };
@@ -510,7 +513,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
                     if (np == 0 || l == 0.f) o[j] = 0;
-                if (p.splits > 1) {
+                if (splits() > 1) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) reinterpret_cast<uint4 *>(p.part_out + part * 128 + half * N + 16 * c)[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                 } else {
@@ -527,7 +530,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
                 }
             }
             }
-            if (mine && half == 0 && p.splits > 1) {
+            if (mine && half == 0 && splits() > 1) {
                 p.part_ml[2 * part] = m;
                 p.part_ml[2 * part + 1] = l;
             }
@@ -702,7 +705,7 @@ template <int KB, int VB, bool MODS, bool DIFF>
 static int launch_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
     const cudaError_t e = cudaFuncSetAttribute(paged_tile_kernel<KB, VB, MODS, DIFF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTileSmem);
     if (e != cudaSuccess) return record_cuda_error(e);
-    const int64_t grid = (int64_t)max_tiles * p.l.Hkv * p.splits;
+    const int64_t grid = p.n_whole + ((int64_t)max_tiles * p.l.Hkv - p.n_whole) * p.splits;
     if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
     if (grid == 0) return KVQ_OK;
     PagedMaps maps = {};
