@@ -210,7 +210,7 @@ static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, 
         if (cost < 0.85 * best) { best = cost; r.tile_splits = s; }
     }
     // Differential attention: what is left of a last round of CTAs may be cut alone, where tiles are alike because what is new is little (a chunk of 2048 over
-    // 32k tokens, 512 tiles of 148 at a time: 2021 us whole, CUTUS with the last 68 halved).
+    // 32k tokens, 512 tiles of 148 at a time: 2021 us whole, 1777 with the last 68 halved).
     if (diff && r.tiles && r.tile_splits == 1 && n <= kMostCutSequences && ctas > 148 && ctas < INT32_MAX && (int64_t)max_new * 4 <= max_tokens) {
         const int rest = (int)(ctas % 148);
         double least = 0.96 * (double)((ctas + 147) / 148);
