@@ -171,24 +171,35 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
     }
 
     const u64 mine = first == INT32_MAX ? 0 : beam_key(sum.top, first);
-    const int width = n <= 16 ? 8 : n <= 32 ? 4 : 1, groups = kScanThreads / width;    // threads of a group
-    u64 best = mine;
-    for (int o = 1; o < width; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane % width == 0) s_best[tid / width] = best;
     const float all = warp_max(sum.top);
     if (lane == 0) s_top[warp] = all;
-    __syncthreads();
-    {                                                             // the n-th best of the groups, a vote for each
-        u64 held[kScanThreads / 32];
-#pragma unroll
-        for (int k = 0; k < kScanThreads / 32; ++k) held[k] = 32 * k < groups ? s_best[32 * k + lane] : 0;
+    if (n <= 32) {                                                // groups of eight or four lanes
+        const int width = n <= 16 ? 8 : 4, groups = kScanThreads / width;
+        u64 best = mine;
+        for (int o = 1; o < width; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+        if (lane % width == 0) s_best[tid / width] = best;
+        __syncthreads();
+        const u64 held[2] = {s_best[lane], groups > 32 ? s_best[32 + lane] : 0};
         for (int g = warp; g < groups; g += kScanThreads / 32) {
             const u64 one = s_best[g];
-            int rank = 0;
-#pragma unroll
-            for (int k = 0; k < kScanThreads / 32; ++k)
-                if (32 * k < groups) rank += __popc(__ballot_sync(0xffffffffu, held[k] > one));
+            const int rank = __popc(__ballot_sync(0xffffffffu, held[0] > one)) + __popc(__ballot_sync(0xffffffffu, held[1] > one));
             if (lane == 0 && rank == n - 1 && one) s_from = one;
+        }
+    } else {                                                      // an eighth of n of every warp's lanes; the least of the warps' thresholds has n above it
+        const int want = (n + kScanThreads / 32 - 1) / (kScanThreads / 32);
+        u64 nth = 0;
+#pragma unroll 8
+        for (int g = 0; g < 32; ++g) {
+            const u64 one = __shfl_sync(0xffffffffu, mine, g);
+            if (__popc(__ballot_sync(0xffffffffu, mine > one)) == want - 1 && one) nth = one;
+        }
+        if (lane == 0) s_best[warp] = nth;
+        __syncthreads();
+        if (tid == 0) {
+            u64 least = s_best[0];
+#pragma unroll
+            for (int w = 1; w < kScanThreads / 32; ++w) least = min(least, s_best[w]);
+            s_from = least;
         }
     }
     float top = s_top[0];
@@ -242,12 +253,11 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
             }
         lost = __syncthreads_or(lost);
         const int kept = min(s_count, kKeys);
-        for (int i = tid; i < kept; i += kScanThreads) {
+        for (int i = warp; i < kept; i += kScanThreads / 32) {    // a vote counts those that are better
             const u64 key = s_key[i];
             int rank = 0;
-#pragma unroll 4
-            for (int j = 0; j < kept; ++j) rank += s_key[j] > key;
-            if (rank < n) s_best[rank] = key;
+            for (int j = lane; j < (kept + 31) / 32 * 32; j += 32) rank += __popc(__ballot_sync(0xffffffffu, (j < kept ? s_key[j] : 0) > key));
+            if (lane == 0 && rank < n) s_best[rank] = key;
         }
         __syncthreads();
         if (lost) {
@@ -271,6 +281,7 @@ __device__ __forceinline__ u64 ordered64(double x) {              // as ordered(
     const u64 u = (u64)__double_as_longlong(x + 0.0);
     return u ^ ((long long)u < 0 ? ~0ull : 1ull << 63);
 }
+__device__ __forceinline__ double from_ordered64(u64 u) { return __longlong_as_double((long long)(u ^ ((long long)u < 0 ? 1ull << 63 : ~0ull))); }
 
 // The sum of a beam's exponentials from its parts', a lane each: score minus its logarithm, which a logit is added to; not finite where the beam offers nothing.
 __device__ __forceinline__ double beam_base(const BeamArgs &p, int64_t row, int lane, double &all) {
@@ -293,178 +304,146 @@ __device__ __forceinline__ void put_next(const BeamArgs &p, int64_t at, float va
     p.a.next_tokens[at] = token;
 }
 
-// Few candidates: a CTA a request, a thread a candidate -- beam, part, place in the part's sorted list.  The n-th best
-// of the first ceil(n / lists) of every list bounds the n-th best of all, and so does every list's last (beams' scores may lie far apart), so that hardly more
-// than n are left to be counted against each other, 32 by a vote.  What counts
-// here is the chain of dependent instructions (some 300, at eight cycles each): both launches for 4 beams of 32000 tokens, 8.2 us so, 11.0 by beam_merge_kernel.
-constexpr int kFewCandidates = 512;
-__global__ void __launch_bounds__(kFewCandidates) beam_count_kernel(const __grid_constant__ BeamArgs p) {
+// A CTA a request: of all its candidates -- beam, part, place in the part's sorted list -- those that reach a bound are counted against each other, 32 by a
+// vote.  The bound: the n-th best of the first ceil(n / lists) of every list, or, as beams' scores may lie far apart, what n of one beam or
+// list reach; hardly more than n reach both.  Should there be no room for all that do, the n best of what there was room for give
+// a higher one.  What counts here is the chain of dependent instructions (some 300, at eight cycles each): both launches for 4 beams of 32000
+// tokens 8.9 us, 11.0 where beams and parts were merged by looking n times which list's head is the best.
+constexpr int kJoined = 1024;
+__global__ void __launch_bounds__(512) beam_join_kernel(const __grid_constant__ BeamArgs p) {
     __shared__ double s_all[kMostBeams], s_score[kMostBeams];
-    __shared__ u64 s_value[kFewCandidates], s_place[kFewCandidates], s_from;       // ordered values; (beam, token)
+    __shared__ u64 s_value[kJoined], s_place[kJoined], s_from, s_full[16];         // ordered values; (beam, token)
     __shared__ uint32_t s_goes[(kMostBest + 31) / 32];
-    __shared__ int s_left;
+    __shared__ int s_left, s_best[kMostBest];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5, n = p.a.n, K = p.a.beams, list = p.parts * n, all = K * list;
-    const int beam = min(tid / list, K - 1), i = tid - beam * list;
-    const u64 key = tid < all ? p.keys[((int64_t)blockIdx.x * K + beam) * list + i] : 0;
+    const u64 *keys = p.keys + (int64_t)blockIdx.x * all;
+    const u64 mine_first = tid < all ? keys[tid] : 0;             // asked for early
+    // n of a beam reach the n-th best of the first ceil(n / parts) of its lists, and n of a list its last one.  The former is closer where n is large and takes longer (16 beams,
+    // n = 48, 4 parts of 128256 tokens, both launches: 44 and 61 us; 4 beams, n = 8: 10.2 and 8.9).
+    const bool by_beams = n > 16 && p.parts > 1;
+    u64 full = 0, unused;
     for (int b = warp; b < K; b += warps) {
         double sum;
         const double score = beam_base(p, (int64_t)blockIdx.x * K + b, lane, sum);
         if (lane == 0) { s_all[b] = sum; s_score[b] = score; }
+        if (by_beams) {                                           // 159 of its keys at most
+            const int each = (n + p.parts - 1) / p.parts, some = p.parts * each;
+            u64 held[5], nth = 0;
+#pragma unroll
+            for (int k = 0; k < 5; ++k) {
+                const int e = 32 * k + lane;
+                held[k] = e < some ? keys[b * list + e / each * n + e % each] : 0;
+            }
+#pragma unroll
+            for (int k = 0; k < 5; ++k)
+                for (int e = 0; e < min(32, some - 32 * k); ++e) {
+                    const u64 one = __shfl_sync(0xffffffffu, held[k], e);
+                    int rank = 0;
+#pragma unroll
+                    for (int h = 0; h < 5; ++h)
+                        if (32 * h < some) rank += __popc(__ballot_sync(0xffffffffu, held[h] > one));
+                    if (rank == n - 1 && one) nth = one;
+                }
+            if (nth && isfinite(sum) && isfinite(score)) full = max(full, ordered64(score + ((double)from_ordered((uint32_t)(nth >> 32)) - sum)));
+        }
     }
     if (tid < (kMostBest + 31) / 32) s_goes[tid] = 0;
     if (tid == 0) { s_left = 0; s_from = 0; }
     __syncthreads();
-    double value = -INFINITY;
-    int token = (int)~(uint32_t)key;
-    bool there = key != 0;
-    if (tid < all) {
-        if (!isfinite(s_all[beam]) || !isfinite(s_score[beam])) {
-            token = i;                                            // its first tokens, once
-            there = i < n && i < p.a.vocabulary;
-        } else if (there) {
-            value = s_score[beam] + ((double)from_ordered((uint32_t)(key >> 32)) - s_all[beam]);
-        }
+    // candidate c's value, in order, and its place; 0: there is none
+    auto candidate = [&](int c, u64 key, u64 &place) -> u64 {
+        const int beam = c / list, i = c - beam * list;
+        const bool alive = isfinite(s_all[beam]) && isfinite(s_score[beam]);
+        const int token = alive ? (int)~(uint32_t)key : i;        // a beam that offers nothing: its first tokens, once
+        place = (u64)beam << 32 | (uint32_t)token;
+        if (alive ? key == 0 : i >= n || i >= p.a.vocabulary) return 0;
+        return ordered64(alive ? s_score[beam] + ((double)from_ordered((uint32_t)(key >> 32)) - s_all[beam]) : -INFINITY);
+    };
+    const int lists = K * p.parts, firsts = (n + lists - 1) / lists, heads = lists * firsts;       // 192 + 128 heads at most (beam_parts)
+    for (int h = tid; h < heads; h += blockDim.x) s_value[h] = candidate(h / firsts * n + h % firsts, keys[h / firsts * n + h % firsts], unused);
+    int whose;
+    if (!by_beams) {
+        for (int l = tid; l < lists; l += blockDim.x) full = max(full, candidate(l * n + n - 1, keys[l * n + n - 1], unused));
+        if (32 * warp < lists) full = warp_best(full, whose);
     }
-    there &= tid < all;
-    const u64 mine = there ? ordered64(value) : 0, place = (u64)beam << 32 | (uint32_t)token;
-    const int lists = K * p.parts, firsts = (n + lists - 1) / lists, heads = lists * firsts;
-    if (heads <= 32) {
-        s_value[tid] = mine;
-        __syncthreads();
-        const u64 head = lane < heads ? s_value[lane / firsts * n + lane % firsts] : 0, last = lane < lists ? s_value[lane * n + n - 1] : 0;
-        int whose;
-        const u64 full = warp_best(last, whose);                  // n reach it in its own list
-        for (int h = warp; h < heads; h += warps) {
-            const u64 one = __shfl_sync(0xffffffffu, head, h);
-            const int better = __popc(__ballot_sync(0xffffffffu, head > one)), reach = __popc(__ballot_sync(0xffffffffu, head >= one));
-            if (lane == 0 && better < n && reach >= n) s_from = max(one, full);  // the n-th best; several may be it
-        }
-        __syncthreads();
-    }
-    int slot = -1;
-    if (there && mine >= s_from) {
-        slot = atomicAdd(&s_left, 1);
-        s_place[slot] = place;
-    }
-    const int keep = slot;
+    if (lane == 0) s_full[warp] = full;
     __syncthreads();
-    if (keep >= 0) s_value[keep] = mine;
-    __shared__ int s_rank[kFewCandidates];
+    for (int h = warp; h < heads; h += warps) {
+        const u64 one = s_value[h];
+        int better = 0, reach = 0;
+        for (int j = lane; j < (heads + 31) / 32 * 32; j += 32) {
+            const u64 other = j < heads ? s_value[j] : 0;
+            better += __popc(__ballot_sync(0xffffffffu, other > one));
+            reach += __popc(__ballot_sync(0xffffffffu, j < heads && other >= one));
+        }
+        if (lane == 0 && better < n && reach >= n) s_from = one;  // several may be the n-th best
+    }
+    for (int w = 0; w < warps; ++w) full = max(full, s_full[w]);
     __syncthreads();
-    const int left = s_left;
-    for (int base = 0; base < left; base += 128) {                // 128 of them stand in a warp's registers
-        u64 held[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) held[k] = base + 32 * k + lane < left ? s_value[base + 32 * k + lane] : 0;
+    u64 from = max(s_from, full), from_place = ~0ull;             // what reaches it: better, or as good and its place not behind
+    int left;
+    for (;;) {
+        bool lost = false;
+        for (int c = tid; c < all; c += blockDim.x) {
+            u64 place;
+            const u64 value = candidate(c, c == tid ? mine_first : keys[c], place);
+            if (value == 0 || value < from || (value == from && place > from_place)) continue;
+            const int slot = atomicAdd(&s_left, 1);
+            if (slot < kJoined) {
+                s_value[slot] = value;
+                s_place[slot] = place;
+            } else {
+                lost = true;
+            }
+        }
+        lost = __syncthreads_or(lost);
+        left = min(s_left, kJoined);
         for (int m = warp; m < left; m += warps) {
             const u64 v = s_value[m], at = s_place[m];
-            int rank = 0, alike = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (base + 32 * k >= left) break;
-                rank += __popc(__ballot_sync(0xffffffffu, held[k] > v));
-                alike += __popc(__ballot_sync(0xffffffffu, held[k] == v));
+            int rank = 0;
+            for (int j = lane; j < (left + 31) / 32 * 32; j += 32) {
+                const u64 other = j < left ? s_value[j] : 0;
+                rank += __popc(__ballot_sync(0xffffffffu, other > v));
+                if (__popc(__ballot_sync(0xffffffffu, other == v)) > (m >> 5 == j >> 5)) rank += __popc(__ballot_sync(0xffffffffu, other == v && s_place[min(j, left - 1)] < at));
             }
-            if (alike > 1 || (alike == 1 && (m < base || m >= base + 128))) {          // equal ones by their places
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int j = base + 32 * k + lane;
-                    rank += __popc(__ballot_sync(0xffffffffu, j < left && held[k] == v && s_place[min(j, left - 1)] < at));
-                }
-            }
-            if (lane == 0) s_rank[m] = base ? s_rank[m] + rank : rank;
+            if (lane == 0 && rank < n) s_best[rank] = m;
         }
+        __syncthreads();
+        if (!lost) break;
+        from = s_value[s_best[n - 1]];
+        from_place = s_place[s_best[n - 1]];
+        __syncthreads();
+        if (tid == 0) s_left = 0;
+        __syncthreads();
     }
-    __syncthreads();
-    const int rank = keep >= 0 ? s_rank[keep] : n;
-    if (rank < n) {
-        put_best(p, (int64_t)blockIdx.x * n + rank, (float)value, beam, token);
+    const bool chosen = tid < min(n, left);
+    const u64 place = chosen ? s_place[s_best[tid]] : 0, value = chosen ? s_value[s_best[tid]] : 0;
+    const int beam = (int)(place >> 32), token = (int)(uint32_t)place;
+    const float score = (float)from_ordered64(value);
+    if (chosen) {
+        put_best(p, (int64_t)blockIdx.x * n + tid, score, beam, token);
         bool ends = false;
         for (int e = 0; e < p.a.n_ends; ++e) ends |= p.a.ends[e] == token;
-        if (!ends) atomicOr(&s_goes[rank >> 5], 1u << (rank & 31));
+        if (!ends) atomicOr(&s_goes[tid >> 5], 1u << lane);
     }
     __syncthreads();
     int before = 0, going = 0;                                    // those that go on and are better; all
 #pragma unroll
     for (int w = 0; w < (kMostBest + 31) / 32; ++w) {
         const uint32_t bits = s_goes[w];
-        before += __popc(w < rank >> 5 ? bits : w == rank >> 5 ? bits & ((1u << (rank & 31)) - 1u) : 0u);
+        before += __popc(w < warp ? bits : w == warp ? bits & ((1u << lane) - 1u) : 0u);
         going += __popc(bits);
     }
-    if (rank < n && (s_goes[rank >> 5] >> (rank & 31) & 1u) && before < K) put_next(p, (int64_t)blockIdx.x * K + before, (float)value, beam, token);
+    if (chosen && (s_goes[warp] >> lane & 1u) && before < K) put_next(p, (int64_t)blockIdx.x * K + before, score, beam, token);
     for (int k = going + tid; k < K; k += blockDim.x) put_next(p, (int64_t)blockIdx.x * K + k, -INFINITY, 0, 0);       // everything else ends
 }
 
-// Many: a CTA a request.  A warp joins a beam's parts, sorted lists, one a lane, by looking n times which head is the best.  Then one warp joins the beams
-// alike, two a lane, and lists those that do not end.
-__global__ void __launch_bounds__(256) beam_merge_kernel(const __grid_constant__ BeamArgs p) {
-    extern __shared__ __align__(16) u64 s_join[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, n = p.a.n, K = p.a.beams, parts = p.parts;
-    double *s_value = reinterpret_cast<double *>(s_join);         // [K][n]
-    int *s_token = reinterpret_cast<int *>(s_value + K * n);      // [K][n]
-    u64 *s_list = reinterpret_cast<u64 *>(s_token + (K * n + 1) / 2 * 2) + warp * parts * n;
-    for (int b = warp; b < K; b += warps) {
-        const int64_t row = (int64_t)blockIdx.x * K + b;
-        for (int i = lane; i < parts * n; i += 32) s_list[i] = p.keys[row * parts * n + i];
-        double all;
-        const double score = beam_base(p, row, lane, all);
-        const bool alive = isfinite(all) && isfinite(score);
-        __syncwarp();
-        int at = 0;
-        u64 mine = lane < parts ? s_list[lane * n] : 0;
-        for (int i = 0; i < n; ++i) {
-            int whose, token = i;
-            double value = -INFINITY;
-            if (alive) {
-                const u64 best = warp_best(mine, whose);
-                token = (int)~(uint32_t)best;
-                if (best) value = score + ((double)from_ordered((uint32_t)(best >> 32)) - all);
-                else token = INT32_MAX;                           // a vocabulary of fewer than n
-                if (lane == whose) mine = ++at < n ? s_list[lane * n + at] : 0;
-            } else if (i >= p.a.vocabulary) {
-                token = INT32_MAX;
-            }
-            if (lane == 0) { s_value[b * n + i] = value; s_token[b * n + i] = token; }
-        }
-        __syncwarp();
-    }
-    __syncthreads();
-    if (warp != 0) return;
-    const int64_t out = (int64_t)blockIdx.x * n, go = (int64_t)blockIdx.x * K;
-    const int end = lane < p.a.n_ends ? p.a.ends[lane] : 0;
-    int at[2] = {0, 0}, going = 0;
-    // A place of none (a beam's list is at its end) is 0, below the key of -infinity.
-    auto key_of = [&](int k) { return 2 * lane + k < K && at[k] < n && s_token[(2 * lane + k) * n + at[k]] != INT32_MAX ? ordered64(s_value[(2 * lane + k) * n + at[k]]) : 0ull; };
-    u64 mine[2] = {key_of(0), key_of(1)};
-    for (int i = 0; i < n; ++i) {
-        int whose;
-        const u64 best = warp_best(max(mine[0], mine[1]), whose);
-        const bool second = mine[0] != best;
-        const int k = __shfl_sync(0xffffffffu, (int)second, whose), place = __shfl_sync(0xffffffffu, second ? at[1] : at[0], whose), b = 2 * whose + k;
-        const float value = (float)s_value[b * n + place];
-        const int token = s_token[b * n + place];
-        if (lane == whose) {
-            if (second) { ++at[1]; mine[1] = key_of(1); }
-            else { ++at[0]; mine[0] = key_of(0); }
-        }
-        bool ends = lane < p.a.n_ends && end == token;
-        for (int e = lane + 32; e < p.a.n_ends; e += 32) ends |= p.a.ends[e] == token;
-        ends = __any_sync(0xffffffffu, ends);
-        if (lane == 0) {
-            put_best(p, out + i, value, b, token);
-            if (!ends && going < K) put_next(p, go + going, value, b, token);
-        }
-        going += !ends;
-    }
-    for (int i = going + lane; i < K; i += 32) put_next(p, go + i, -INFINITY, 0, 0);           // everything else ends
-}
-
-// Parts of a row: a part of its own costs some 4 us of beginning and end beside 0.4 us a turn, so one CTA an SM where rows are few and four where they are many
-// (16 rows of 128256: 11.0 us in 8 parts, 14.0 in 32; 128 of 32000: 12.0 in one, 16.2 in 4; 256 of 128256: 25.4 in 2, 28.3 in 4).  1024 keys of a beam at
-// most are joined.
+// Parts of a row: a part of its own costs some 4 us of beginning and end beside 0.4 us a turn, so one CTA an SM, two where there are six million logits and few are wanted, and four where
+// rows are many (32 rows of 128256: 11.8 us in 4 parts, 14.7 in 16; 128 of 32000: 12.0 in one, 13.2 in 2; 128 of 128256: 24.6 in one, 20.6 in 2; 256: 25.4 in 2,
+// 28.3 in 4).  1024 keys of a beam at most are joined.
 static int beam_parts(const kvq_beam_args &a) {
     const int64_t rows = (int64_t)a.requests * a.beams;
-    int64_t parts = (rows <= 148 ? 148 : 4 * 148) / (rows > 0 ? rows : 1);
+    int64_t parts = (rows > 148 ? 4 * 148 : rows * a.vocabulary >= 6 << 20 && a.n <= 32 ? 2 * 148 : 148) / (rows > 0 ? rows : 1);
     const int64_t most = (a.vocabulary + kScanThreads * kTurn - 1) / (kScanThreads * kTurn);
     if (parts > most) parts = most;
     if (parts > kMostParts) parts = kMostParts;
@@ -511,15 +490,6 @@ extern "C" int kvq_beam_select(const kvq_beam_args *a, kvq_stream_t stream) {
     else if (a->type == KVQ_BF16) scan(beam_scan_kernel<__nv_bfloat16, true>, beam_scan_kernel<__nv_bfloat16, false>);
     else scan(beam_scan_kernel<__half, true>, beam_scan_kernel<__half, false>);
     if (const int rc = check_launch()) return rc;
-    const int64_t lists = (int64_t)a->beams * p.parts, candidates = lists * a->n, heads = (a->n + lists - 1) / lists * lists;
-    if (candidates <= 128 || (candidates <= kFewCandidates && heads <= 32)) {
-        beam_count_kernel<<<(unsigned)a->requests, candidates <= 256 ? 256 : kFewCandidates, 0, st>>>(p);
-        return check_launch();
-    }
-    const int warps = a->beams < 8 ? a->beams : 8, pairs = a->beams * a->n;
-    const size_t smem = (size_t)pairs * 8 + (size_t)(pairs + 1) / 2 * 8 + (size_t)warps * p.parts * a->n * 8;
-    const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-    if (e != cudaSuccess) return record_cuda_error(e);
-    beam_merge_kernel<<<(unsigned)a->requests, 32 * warps, smem, st>>>(p);
+    beam_join_kernel<<<(unsigned)a->requests, a->beams * p.parts * a->n <= 512 ? 256 : 512, 0, st>>>(p);
     return check_launch();
 }
