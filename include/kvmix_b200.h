@@ -653,7 +653,7 @@ int kvq_paged_attn(const kvq_page_book *b, const kvq_page_layer *l, const kvq_pa
  * Differential attention over the same pages: a head's 128 channels of q and k are two halves of 64, (q1, q2) and (k1, k2), and
  *   out = (softmax(s1) - lambdas[h] * softmax(s2)) . v,   s1 = q1.k1 * softmax_scale, s2 = q2.k2 * softmax_scale,
  * both capped, biased and masked as kvq_paged_attn says; then, with norm_weight [128], out = out / sqrt(mean(out^2) + norm_eps) * norm_weight.  The two attentions
- * stay in fp32 until their difference is rounded.  lambdas [nh], norm_weight [128] or NULL: fp32, device memory.
+ * stay in fp32 until their difference is rounded; a row that sees nothing gives zeros.  lambdas [nh] (finite), norm_weight [128] or NULL: fp32, device memory.
  * workspace: kvq_paged_diff_attn_workspace_bytes(...) bytes.
  */
 typedef struct {

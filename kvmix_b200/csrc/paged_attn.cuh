@@ -34,9 +34,10 @@ struct PagedArgs {
     int max_tiles, n_whole;           // kernel of tiles: (tile, kv head) pairs in the order of CTAs, of which the first n_whole are not cut
 };
 constexpr int kMostCutSequences = 8;                              // the launch that joins the splits of some tiles counts tiles sequence by sequence
-// What becomes of a head's two attentions over the values, channel by channel; then its norm over the channels, where there is one: x * diff_norm() * weight
+// What becomes of a head's two attentions over the values, channel by channel; then its norm over the channels, where there is one: x * diff_norm() * weight.
+// Nothing at all stays nothing, whatever norm_eps.
 __device__ __forceinline__ float diff_of(float a, float b, float lambda) { return fmaf(-lambda, b, a); }
-__device__ __forceinline__ float diff_norm(const PagedArgs &p, float squares) { return rsqrtf(fmaf(squares, 1.f / kHeadDim, p.norm_eps)); }
+__device__ __forceinline__ float diff_norm(const PagedArgs &p, float squares) { return squares == 0.f ? 0.f : rsqrtf(fmaf(squares, 1.f / kHeadDim, p.norm_eps)); }
 
 // Sequence i as every thread sees it: its row of the table, length, packed pages, where its new tokens are.  Numbers that would lead
 // outside anything are made harmless.

@@ -381,7 +381,7 @@ def pages_compact(pages, layers):
 
 @_on_its_device(3)
 def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, prefix=None, first=None, softcap=None, alibi_slopes=None,
-                    softmax_scale=None, max_new=None, max_tokens=None, max_chunks=None, out=None):
+                    softmax_scale=None, max_new=None, max_tokens=None, max_chunks=None, out=None, _diff=None):
     """Attention of the last tokens of every sequence over its pages.
 
     q [tokens, nh, 128] fp16: tokens [q_start[i], q_start[i+1]) are the last ones of sequence rows[i], whose keys and values are in the
@@ -397,35 +397,6 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     which few have several tokens the third saves time).  Tokens that see nothing get zeros.  Cached values have
     to be finite: one that is not may reach queries that do not see it (include/kvmix_b200.h).
     Returns [tokens, nh, 128] fp16; rows behind q_start[n] are left as they are."""
-    return _attend(q, q_start, rows, pages, layer, causal, window, prefix, first, softcap, alibi_slopes, _SCALE if softmax_scale is None else softmax_scale, max_new, max_tokens,
-                   max_chunks, out, None)
-
-
-@_on_its_device(4)
-def paged_differential_attention(q, lambdas, q_start, rows, pages, layer, causal=True, window=None, prefix=None, first=None, softcap=None, alibi_slopes=None,
-                                 softmax_scale=None, norm_weight=None, norm_eps=1e-5, max_new=None, max_tokens=None, max_chunks=None, out=None):
-    """The difference of two softmax maps over the pages of every sequence: a head's 128 channels of q and of the cached keys are two halves of 64,
-
-        out = (softmax(q1 k1^T * scale) - lambdas[head] * softmax(q2 k2^T * scale)) v,   then out / sqrt(mean(out^2) + norm_eps) * norm_weight
-
-    lambdas fp32 [nh]; norm_weight fp32 [128], or None for no norm; softmax_scale None: 1 / 8.  Everything else is as ``paged_attention`` has it, for both maps
-    alike.  Both attentions are fp32 until their difference (normed) is rounded; keys, values and weights are rounded on the way as there.  Keys that ``page_append``
-    rotates want parts=2."""
-    dev, nh = pages.table.get_device(), q.shape[1] if q.dim() == 3 else 0
-    if lambdas.dtype is not torch.float32 or lambdas.shape != (nh,) or lambdas.get_device() != dev or not lambdas.is_contiguous():
-        raise RuntimeError(f"lambdas must be float32 [{nh}] on cuda:{dev}")
-    at_weight = 0
-    if norm_weight is not None:
-        if norm_weight.dtype is not torch.float32 or norm_weight.shape != (128,) or norm_weight.get_device() != dev or not norm_weight.is_contiguous():
-            raise RuntimeError(f"norm_weight must be float32 [128] on cuda:{dev}")
-        if not 0.0 <= norm_eps <= 3.4e38:
-            raise RuntimeError("norm_eps must not be negative")
-        at_weight = norm_weight.data_ptr()
-    return _attend(q, q_start, rows, pages, layer, causal, window, prefix, first, softcap, alibi_slopes, 0.125 if softmax_scale is None else softmax_scale, max_new, max_tokens,
-                   max_chunks, out, (lambdas.data_ptr(), at_weight, norm_eps))
-
-
-def _attend(q, q_start, rows, pages, layer, causal, window, prefix, first, softcap, alibi_slopes, softmax_scale, max_new, max_tokens, max_chunks, out, diff):
     dev, book = _book(pages)
     if q.dim() != 3 or q.dtype is not _f16 or q.get_device() != dev or q.shape[2] != 128:
         raise RuntimeError(f"attention over pages takes fp16 queries [tokens, heads, 128] on cuda:{dev}")
@@ -446,7 +417,7 @@ def _attend(q, q_start, rows, pages, layer, causal, window, prefix, first, softc
     window, softcap = window or 0, softcap or 0.0
     if window < 0 or not softcap >= 0.0:
         raise RuntimeError("window and softcap must not be negative")
-    if not abs(softmax_scale) <= 3.4e38:
+    if softmax_scale is not None and not abs(softmax_scale) <= 3.4e38:
         raise RuntimeError("softmax_scale must be a finite number")
     at_slopes = 0
     if alibi_slopes is not None:
@@ -460,17 +431,41 @@ def _attend(q, q_start, rows, pages, layer, causal, window, prefix, first, softc
     if tokens and n and (max_new <= 0 or max_tokens <= 0 or max_chunks < 0):
         raise RuntimeError("max_new and max_tokens must be positive, max_chunks not negative")
     L = _library()
-    need = (L.kvq_paged_diff_attn_workspace_bytes if diff else L.kvq_paged_attn_workspace_bytes)(block, n, tokens, nh, max_new, max_tokens, max_chunks)
+    need = (L.kvq_paged_diff_attn_workspace_bytes if _diff else L.kvq_paged_attn_workspace_bytes)(block, n, tokens, nh, max_new, max_tokens, max_chunks)
     ws = pages.count.new_empty((need + 3) // 4) if need else None
     a = (q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), _ints(dev, "q_start", q_start, n + 1),
-                   _ints(dev, "rows", rows, n), 0 if first is None else _ints(dev, "first", first, tokens), 0 if prefix is None else _ints(dev, "prefix", prefix, n),
-                   at_slopes, n, tokens, nh, max_new, max_tokens, max_chunks, int(min(window, _MOST)), 1 if causal else 0,
-                   softmax_scale, min(softcap, 1e38), 0 if ws is None else ws.data_ptr(), need)
-    if diff:
-        _launched(L.kvq_paged_diff_attn(book, block, _pack_diff(*a, *diff), ops.raw_stream()))
+         _ints(dev, "rows", rows, n), 0 if first is None else _ints(dev, "first", first, tokens), 0 if prefix is None else _ints(dev, "prefix", prefix, n),
+         at_slopes, n, tokens, nh, max_new, max_tokens, max_chunks, int(min(window, _MOST)), 1 if causal else 0,
+         _SCALE if softmax_scale is None else softmax_scale, min(softcap, 1e38), 0 if ws is None else ws.data_ptr(), need)
+    if _diff:
+        _launched(L.kvq_paged_diff_attn(book, block, _pack_diff(*a, *_diff), ops.raw_stream()))
     else:
         _launched(L.kvq_paged_attn(book, block, _pack_attn(*a), ops.raw_stream()))
     return out
+
+
+@_on_its_device(4)
+def paged_differential_attention(q, lambdas, q_start, rows, pages, layer, causal=True, window=None, prefix=None, first=None, softcap=None, alibi_slopes=None,
+                                 softmax_scale=None, norm_weight=None, norm_eps=1e-5, max_new=None, max_tokens=None, max_chunks=None, out=None):
+    """The difference of two softmax maps over the pages of every sequence: a head's 128 channels of q and of the cached keys are two halves of 64,
+
+        out = (softmax(q1 k1^T * scale) - lambdas[head] * softmax(q2 k2^T * scale)) v,   then out / sqrt(mean(out^2) + norm_eps) * norm_weight
+
+    lambdas fp32 [nh], finite; norm_weight fp32 [128], or None for no norm (a token that sees nothing gets zeros with one too); softmax_scale
+    None: 1 / 8.  Everything else is as ``paged_attention`` has it, for both maps alike.  Both attentions are fp32 until their difference (normed) is rounded; keys, values and weights are rounded on the way as there.  Keys that ``page_append``
+    rotates want parts=2."""
+    dev, nh = pages.table.get_device(), q.shape[1] if q.dim() == 3 else 0
+    if lambdas.dtype is not torch.float32 or lambdas.shape != (nh,) or lambdas.get_device() != dev or not lambdas.is_contiguous():
+        raise RuntimeError(f"lambdas must be float32 [{nh}] on cuda:{dev}")
+    at_weight = 0
+    if norm_weight is not None:
+        if norm_weight.dtype is not torch.float32 or norm_weight.shape != (128,) or norm_weight.get_device() != dev or not norm_weight.is_contiguous():
+            raise RuntimeError(f"norm_weight must be float32 [128] on cuda:{dev}")
+        if not 0.0 <= norm_eps <= 3.4e38:
+            raise RuntimeError("norm_eps must not be negative")
+        at_weight = norm_weight.data_ptr()
+    return paged_attention.__wrapped__(q, q_start, rows, pages, layer, causal, window, prefix, first, softcap, alibi_slopes, 0.125 if softmax_scale is None else softmax_scale,
+                                       max_new, max_tokens, max_chunks, out, (lambdas.data_ptr(), at_weight, norm_eps))
 
 
 class PagedStep(NamedTuple):

@@ -113,6 +113,38 @@ def test_masks_and_numbers_that_are_none(cuda, kind):
     assert (got.scores[1, :].isfinite()).any()
 
 
+def test_more_that_reach_a_bound_than_there_is_room_for(cuda):
+    """Beams that offer nothing, or the same: 64 of them, 128 wanted."""
+    x = torch.zeros(128, 500, device="cuda")
+    for scores in (torch.zeros(128), torch.full((128,), -math.inf), torch.where(torch.arange(128) % 3 == 0, -1.0, -math.inf)):
+        got, want = check(x, scores.cuda(), 64, 128), definition(x, scores.cuda(), 64, 128, ())
+        for r in range(2):
+            assert list(zip(got.beams[r].tolist(), got.tokens[r].tolist())) == [w[1:] for w in want[r][:128]]
+    x[:] = -math.inf
+    x[:, 77] = 1.0
+    check(x, torch.zeros(128).cuda(), 64, 128)
+
+
+def test_a_row_made_to_overflow_a_part(cuda):
+    """All of a part's large logits in the pieces of few threads, each thread's above the next one's: thousands reach the first threshold."""
+    V = 131072
+    token = torch.arange(V)
+    thread = token // 4 % 256                                    # pieces of four fp32 numbers, 256 threads by turns
+    for chosen in (thread % 2 == 0, thread < 128, thread % 8 == 5):
+        x = torch.where(chosen, thread + (token * 2654435761 % 2 ** 20).float() / 2 ** 20, -5.0 + token * 1e-6)
+        for n in (128, 100, 40, 8):
+            check(torch.stack([x, x.flip(0) * 0.9]).float().cuda(), torch.tensor([-1.0, -1.5]).cuda(), 2, n)
+
+
+@pytest.mark.parametrize("beams,n", [(16, 17), (16, 48), (40, 40), (64, 64), (64, 128), (3, 128)])
+def test_many_lists(cuda, beams, n):
+    """Beams' scores close together and far apart, many parts and few."""
+    for V in (700, 9000, 60000):
+        x, scores = inputs(2 * beams, V, torch.bfloat16, V + n)
+        for spread in (0.0, 1.0, 100.0):
+            check(x, scores * spread, beams, n)
+
+
 def test_first_step_of_a_request(cuda):
     """One beam is all there is: every continuation is its own."""
     x, _ = inputs(8, 3000, torch.float32, 7)
@@ -400,6 +432,21 @@ def test_more_rows_than_threads(cuda):
     sim.extend(rows, counts)
     for _ in range(2):
         parents = [rng.choice(rows) for _ in rows]
+        cache.reorder(rows, parents)
+        sim.reorder(rows, parents)
+        sim.same(cache.book)
+    cache.check()
+
+
+def test_lists_beyond_the_registers(cuda):
+    """Few rows of many pages: more of them than the CTA's threads hold."""
+    cache = kv.KVmixPagedCache([(2, 2)], 1, 128, 8, 128 * 1100, 1, 4400, 64, 10 ** 7)
+    sim = Order(8, 1100, 1, 4400)
+    rows = [6, 1, 3, 0, 7]
+    for r, n in zip(rows, (1100 * 128, 900 * 128 + 7, 128 * 500, 128 * 1000 + 1, 0)):
+        cache.extend([r], [n])
+        sim.extend([r], [n])
+    for parents in ([6, 1, 3, 0, 7], [1, 6, 0, 3, 7], [3, 3, 3, 3, 3], [6, 7, 7, 7, 1], [0, 0, 0, 0, 0]):
         cache.reorder(rows, parents)
         sim.reorder(rows, parents)
         sim.same(cache.book)

@@ -42,7 +42,7 @@ class Case:
     def __init__(self, past, new, heads=4, kv_heads=2, kind=torch.float16, angles=64, parts=1, seed=0, behind=0, wide=0, max_tokens=1024, size=1.0):
         self.gen = torch.Generator().manual_seed(seed)
         n = len(new)
-        self.cache = kv.KVmixPagedCache([(4, 2)], kv_heads, 128, n + 1, max_tokens, 8, 16 + 10 * n, 64)
+        self.cache = kv.KVmixPagedCache([(4, 2)], kv_heads, 128, n + 1, max_tokens, 8, 16 + (max_tokens // 100) * n, 64)
         self.rows = torch.randperm(n + 1, generator=self.gen).tolist()[:n]
         self.cache.extend(self.rows, past)
         for t in (self.cache.layers[0].kfull, self.cache.layers[0].vfull):
@@ -89,6 +89,33 @@ def test_rotation(cuda, kind, angles, parts, interleaved):
 @pytest.mark.parametrize("heads,kv_heads,new", [(1, 1, [1]), (32, 8, [1] * 40), (40, 8, [700, 1, 3]), (8, 1, [129]), (5, 5, [0, 1, 0])])
 def test_head_layouts(cuda, heads, kv_heads, new):
     c = Case([(37 * i) % 260 for i in range(len(new))], new, heads, kv_heads, seed=heads)
+    got = c.call(q=c.q)
+    want, bound = turned(c.q, c.cos[c.pos], c.sin[c.pos], 1, False)
+    assert ((got.double() - want).abs() <= bound).all()
+    c.holds()
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(0, 1), (1, 1), (2, 1), (7, 3), (33, 1), (31, 2), (100, 20), (6, 5), (64, 64)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rows_of_a_token(cuda, heads, kv_heads, interleaved):
+    """Any number of rows a token: places that are left empty, several tokens at once, several turns."""
+    for new in ([3], [37, 1, 90], [400]):
+        c = Case([11 * i for i in range(len(new))], new, max(heads, 1), kv_heads, seed=heads + kv_heads, behind=2)
+        if heads == 0:
+            assert c.call(interleaved=interleaved) is None
+            assert c.call(interleaved=interleaved, q=c.q[:, :0]).shape == (sum(new) + 2, 0, 128)
+        else:
+            out = torch.full(c.q.shape, 7.0, dtype=torch.float16, device="cuda")
+            c.call(q=c.q, q_out=out, interleaved=interleaved)
+            n = sum(new)
+            want, bound = turned(c.q[:n], c.cos[c.pos], c.sin[c.pos], 1, interleaved)
+            assert ((out[:n].double() - want).abs() <= bound).all() and (out[n:] == 7).all()
+        c.holds(interleaved=interleaved)
+
+
+def test_many_tokens(cuda):
+    """Several tokens a place of a CTA: more than 148 * 8 * 4 tokens."""
+    c = Case([0, 200], [9001, 3000], 2, 1, seed=14, max_tokens=9100)
     got = c.call(q=c.q)
     want, bound = turned(c.q, c.cos[c.pos], c.sin[c.pos], 1, False)
     assert ((got.double() - want).abs() <= bound).all()

@@ -143,6 +143,41 @@ def test_splits_are_joined(cuda):
     assert kv.paged._library().kvq_paged_diff_attn_workspace_bytes(kv.paged._layer(c.book, 0, c.layer), 1, 10, 4, 10, 9000, 1) >= 2 * 80 * 520
 
 
+@pytest.mark.parametrize("counts,lengths,packed,cut", [([700], [4000], [20], True), ([650, 1, 300], [5000, 700, 2900], [30, 4, 10], False),
+                                                       ([500, 0, 2, 510, 1], [4300, 10, 4000, 4200, 3000], [33, 0, 31, 0, 23], False),
+                                                       ([400, 1, 230], [5000, 700, 2900], [30, 4, 10], True), ([300, 0, 2, 250, 1], [4300, 10, 4000, 4200, 3000], [33, 0, 31, 0, 23], True)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_tiles_that_are_left_of_a_round_are_cut(cuda, counts, lengths, packed, cut, norm):
+    """More tiles than SMs, over contexts that are long beside what is new: those of the last round are cut and joined, the others are not."""
+    Hkv, rep = 8, 4
+    c = Cache(lengths, packed, Hkv, 4, 2, 64, seed=21)
+    q, lam = queries(sum(counts), Hkv * rep), torch.linspace(0.1, 0.9, Hkv * rep).cuda()
+    before = kv.ops.LAUNCHES[0]
+    got = call(c, q, lam, counts, norm_weight=NORM.cuda() if norm else None, max_new=max(counts), max_tokens=max(lengths))
+    if cut:
+        assert kv.ops.LAUNCHES[0] - before >= (2 if len(counts) == 1 else 3)      # tiles and the join, and where there are single tokens theirs
+    at = 0
+    for i, new in enumerate(counts):
+        K, V = (torch.from_numpy(x).cuda() for x in c.dense(i))
+        pos, j = torch.arange(lengths[i] - new, lengths[i], device="cuda")[:, None], torch.arange(lengths[i], device="cuda")
+        for h in range(Hkv * rep if new else 0):
+            x, g = q[at:at + new, h].double(), h // rep
+            maps = [(x[:, o:o + 64] @ K[g][:, o:o + 64].T / 8).masked_fill(j > pos, -math.inf).softmax(-1) for o in (0, 64)]
+            # a key, a weight and a value are rounded to fp16 once each, 2^-11 of themselves (test_gpu_paged has the bound)
+            slack = 0.0
+            for m, o, by in zip(maps, (0, 64), (1.0, float(lam[h]))):
+                rel = x[:, o:o + 64].abs() @ K[g][:, o:o + 64].abs().T / 8 * 2.0 ** -11 + 1e-5 + 2 * 2.0 ** -11
+                slack = slack + 1.05 * by * ((m * rel) @ V[g].abs() + (m * rel).sum(-1, keepdim=True) * (m @ V[g]).abs())
+            want = (maps[0] - lam[h].double() * maps[1]) @ V[g]
+            if norm:
+                by = 1 / (want.square().mean(-1, keepdim=True) + 1e-5).sqrt()
+                grow = (want.abs() * slack).mean(-1, keepdim=True) * by ** 2
+                slack, want = NORM.cuda().abs() * by * 1.1 * (slack + want.abs() * grow), want * by * NORM.cuda()
+            err = (got[at:at + new, h].double() - want).abs()
+            assert (err <= slack + 2.0 ** -10 * want.abs() + 1e-5).all(), (i, h)
+        at += new
+
+
 # ---- rows that see nothing, weights that cancel, numbers that are none ----------------------------------------------------------------------
 
 @pytest.mark.parametrize("counts", [[1, 1], [100, 1]])
@@ -152,10 +187,7 @@ def test_rows_that_see_nothing(cuda, counts):
     for eps in (1e-5, 0.0):
         got = call(c, queries(sum(counts), 4), torch.full((4,), 0.5).cuda(), counts, first=first, norm_weight=NORM.cuda(), norm_eps=eps)
         none = torch.tensor([f > 0 for f in first]).cuda()
-        if eps:
-            assert (got[none] == 0).all() and got.isfinite().all() and (got[~none] != 0).any()
-        else:
-            assert got[none].isnan().all() or (got[none] == 0).all()       # 0 / 0, as the formula has it
+        assert (got[none] == 0).all() and got.isfinite().all() and (got[~none] != 0).any()
     assert (call(c, queries(sum(counts), 4), torch.full((4,), 0.5).cuda(), counts, first=first)[none] == 0).all()
 
 
