@@ -166,7 +166,10 @@ struct CapSmall {
 // MODS: scores are capped, biased or scaled by a negative number.  Calls without have an instance of their own: with the code beside it the
 // 128 scores of a thread no longer fit its registers (2048 tokens over 32k: 1261 us in place of 1132).
 // DIFF: heads are two rows each (PagedArgs); the two tiles are the two maps of the same 128 rows -- (token, query head) pairs --, a map's scores the product of
-// half the channels, and the map of the second half hands its part of the output over in shared memory.
+// half the channels, and the map of the second half hands its part of the output over in shared memory.  A page is as many exponentials as with two tiles of
+// rows and three quarters of the products, and takes as long (some 3000 cycles; 59 % of the special function unit, 44 % of the tensor core over fp16 pages).  Softmax threads
+// have 96 registers (512 x 96 + 128 x 56 + 128 x 40 is what the CTA was launched with): 1777 -> 1727 us for a chunk of 2048 over 32k tokens.  Half a page a turn, so that
+// scores are there before weights are done: 2225 us.
 template <int KB, int VB, bool MODS, bool DIFF>
 __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ PagedMaps maps, int max_tiles) {
     extern __shared__ __align__(1024) char smem[];
@@ -307,7 +310,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
 
     if (wg < 4) {
         // ------------------------------------------------------------------ softmax, 64 columns of one row a thread
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 88;\n");
+        if constexpr (DIFF) asm volatile("setmaxnreg.inc.sync.aligned.u32 96;\n");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 88;\n");
         constexpr int N = 64;
         const int tile_of = wg >> 1, half = wg & 1, r = threadIdx.x & 127, at_row = DIFF ? r : tile_of * kTileRows + r, idx = row0 + at_row, u = idx / rep,
                   h = head * rep + (idx - u * rep);
@@ -539,6 +543,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
     } else if (wg == 4) {
         // ------------------------------------------------------------------ operands: job 2i is page i's keys, 2i + 1 its values.  Packed
         // ones are unpacked here, and the fp16 page that holds the sequence's end is copied here, with zeros behind the end.
+        if constexpr (DIFF) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;\n");
         const int r = threadIdx.x & 127;
         bool ok = true;
         uint32_t tails = 0;
@@ -580,7 +585,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
         }
     } else {
         // ------------------------------------------------------------------ MMAs
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
+        if constexpr (DIFF) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
         if (warp == 20) {
             uint32_t lead;
             asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(lead));
