@@ -306,10 +306,12 @@ __device__ __forceinline__ void put_next(const BeamArgs &p, int64_t at, float va
 
 // A CTA a request: of all its candidates -- beam, part, place in the part's sorted list -- those that reach a bound are counted against each other, 32 by a
 // vote.  The bound: the n-th best of the first ceil(n / lists) of every list, or, as beams' scores may lie far apart, what n of one beam or
-// list reach; hardly more than n reach both.  Should there be no room for all that do, the n best of what there was room for give
+// list reach: BY_BEAMS, the n-th best of the first ceil(n / parts) of a beam's lists, closer where n is large and longer to find (16 beams, n = 48, 4 parts of 128256
+// tokens, both launches: 44 us, and 61 by the lists' last ones; 4 beams, n = 8: 10.2 and 8.9); hardly more than n reach both.  Should there be no room for all that do, the n best of what there was room for give
 // a higher one.  What counts here is the chain of dependent instructions (some 300, at eight cycles each): both launches for 4 beams of 32000
 // tokens 8.9 us, 11.0 where beams and parts were merged by looking n times which list's head is the best.
 constexpr int kJoined = 1024;
+template <bool BY_BEAMS>
 __global__ void __launch_bounds__(512) beam_join_kernel(const __grid_constant__ BeamArgs p) {
     __shared__ double s_all[kMostBeams], s_score[kMostBeams];
     __shared__ u64 s_value[kJoined], s_place[kJoined], s_from, s_full[16];         // ordered values; (beam, token)
@@ -318,15 +320,13 @@ __global__ void __launch_bounds__(512) beam_join_kernel(const __grid_constant__ 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5, n = p.a.n, K = p.a.beams, list = p.parts * n, all = K * list;
     const u64 *keys = p.keys + (int64_t)blockIdx.x * all;
     const u64 mine_first = tid < all ? keys[tid] : 0;             // asked for early
-    // n of a beam reach the n-th best of the first ceil(n / parts) of its lists, and n of a list its last one.  The former is closer where n is large and takes longer (16 beams,
-    // n = 48, 4 parts of 128256 tokens, both launches: 44 and 61 us; 4 beams, n = 8: 10.2 and 8.9).
-    const bool by_beams = n > 16 && p.parts > 1;
+    const float per_list = 1.f / list;                            // c / list = (c + 0.5) * this for every c here (below 2^22)
     u64 full = 0, unused;
     for (int b = warp; b < K; b += warps) {
         double sum;
         const double score = beam_base(p, (int64_t)blockIdx.x * K + b, lane, sum);
         if (lane == 0) { s_all[b] = sum; s_score[b] = score; }
-        if (by_beams) {                                           // 159 of its keys at most
+        if constexpr (BY_BEAMS) {                                 // 159 of its keys at most
             const int each = (n + p.parts - 1) / p.parts, some = p.parts * each;
             u64 held[5], nth = 0;
 #pragma unroll
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(512) beam_join_kernel(const __grid_constant__ 
     __syncthreads();
     // candidate c's value, in order, and its place; 0: there is none
     auto candidate = [&](int c, u64 key, u64 &place) -> u64 {
-        const int beam = c / list, i = c - beam * list;
+        const int beam = (int)((c + 0.5f) * per_list), i = c - beam * list;
         const bool alive = isfinite(s_all[beam]) && isfinite(s_score[beam]);
         const int token = alive ? (int)~(uint32_t)key : i;        // a beam that offers nothing: its first tokens, once
         place = (u64)beam << 32 | (uint32_t)token;
@@ -360,9 +360,12 @@ __global__ void __launch_bounds__(512) beam_join_kernel(const __grid_constant__ 
         return ordered64(alive ? s_score[beam] + ((double)from_ordered((uint32_t)(key >> 32)) - s_all[beam]) : -INFINITY);
     };
     const int lists = K * p.parts, firsts = (n + lists - 1) / lists, heads = lists * firsts;       // 192 + 128 heads at most (beam_parts)
-    for (int h = tid; h < heads; h += blockDim.x) s_value[h] = candidate(h / firsts * n + h % firsts, keys[h / firsts * n + h % firsts], unused);
+    for (int h = tid; h < heads; h += blockDim.x) {
+        const int c = firsts == 1 ? h * n : h / firsts * n + h % firsts;
+        s_value[h] = candidate(c, keys[c], unused);
+    }
     int whose;
-    if (!by_beams) {
+    if constexpr (!BY_BEAMS) {
         for (int l = tid; l < lists; l += blockDim.x) full = max(full, candidate(l * n + n - 1, keys[l * n + n - 1], unused));
         if (32 * warp < lists) full = warp_best(full, whose);
     }
@@ -490,6 +493,8 @@ extern "C" int kvq_beam_select(const kvq_beam_args *a, kvq_stream_t stream) {
     else if (a->type == KVQ_BF16) scan(beam_scan_kernel<__nv_bfloat16, true>, beam_scan_kernel<__nv_bfloat16, false>);
     else scan(beam_scan_kernel<__half, true>, beam_scan_kernel<__half, false>);
     if (const int rc = check_launch()) return rc;
-    beam_join_kernel<<<(unsigned)a->requests, a->beams * p.parts * a->n <= 512 ? 256 : 512, 0, st>>>(p);
+    const unsigned threads = a->beams * p.parts * a->n <= 512 ? 256 : 512;
+    if (a->n > 16 && p.parts > 1) beam_join_kernel<true><<<(unsigned)a->requests, threads, 0, st>>>(p);
+    else beam_join_kernel<false><<<(unsigned)a->requests, threads, 0, st>>>(p);
     return check_launch();
 }
