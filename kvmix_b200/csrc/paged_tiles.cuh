@@ -97,20 +97,33 @@ __device__ __forceinline__ void unpack_row(uint32_t raw, uint32_t to, int r) {
 #pragma unroll
     for (int k = 0; k < W; k += 4) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(w[k]), "=r"(w[k + 1]), "=r"(w[k + 2]), "=r"(w[k + 3]) : "r"(codes + 4 * k));
     uint32_t sc[NG], lo[NG];                                      // both halves alike
-#pragma unroll
-    for (int k = 0; k < NG; ++k) { sc[k] = lds16(scale + 2 * k) * 0x10001u; lo[k] = lds16(mn + 2 * k) * 0x10001u; }
     uint32_t out[4];
     if constexpr (BITS == 3) {
-        auto code = [&](int i) { return i % 11 < 10 ? (w[i / 11] >> (3 * (i % 11))) & 7u : w[i / 11] >> 30; };
+        // Twelve scales and minima in six wide loads: loads wait in one queue with the exponentials of the other warps, some 40 cycles each.  Words hold eleven fields: neighbours
+        // stand at the same place of a word's half and of the half three bits on, and every other word begins in mid-pair.  (2048 tokens over 16k, K3V3: 622 -> 508 us, two
+        // maps 1124 -> 844, against a load a scale and a shift and a mask a field.  The other widths have few scales; wide loads there cost as much as they gave.)
+        uint32_t x[2][NG / 2];
+#pragma unroll
+        for (int k = 0; k < NG; k += 2)
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n" : "=r"(x[k >= NG / 2][k % (NG / 2)]), "=r"(x[k >= NG / 2][k % (NG / 2) + 1]) : "r"((k < NG / 2 ? scale : mn) + 4 * (k % (NG / 2))));
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+            sc[k] = prmt(x[0][k / 2], 0, k & 1 ? 0x3232 : 0x1010);
+            lo[k] = prmt(x[1][k / 2], 0, k & 1 ? 0x3232 : 0x1010);
+        }
 #pragma unroll
         for (int i = 0; i < 64; ++i) {
-            const int a = 2 * i / 11, b = (2 * i + 1) / 11;
-            const __half2 x = __hsub2(as_h2(code(2 * i) | code(2 * i + 1) << 16 | 0x64006400u), as_h2(0x64006400u));
+            const int a = 2 * i / 11, b = (2 * i + 1) / 11, f = 2 * i % 11, by = 3 * (f & 1) + (f < 6 ? 0 : 18), at = 3 * f - by, pos = a != b || at == 0 ? 0 : 6;
+            const uint32_t pair = a != b ? prmt(w[a] >> 30, w[b], 0x5410) : prmt(w[a] >> by, w[a] >> (by + 3), 0x5410), expo = (uint32_t)(25 - pos) << 10;
+            uint32_t v;
+            asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(a == b && at == 12 ? pair >> 6 : pair), "r"((7u << pos) * 0x10001u), "r"(expo * 0x10001u));
             const uint32_t s2 = a == b ? sc[a] : prmt(sc[a], sc[b], 0x5410), l2 = a == b ? lo[a] : prmt(lo[a], lo[b], 0x5410);
-            out[i & 3] = as_u32(__hfma2(x, as_h2(s2), as_h2(l2)));
+            out[i & 3] = as_u32(__hfma2(__hsub2(as_h2(v), as_h2(expo * 0x10001u)), as_h2(s2), as_h2(l2)));
             if ((i & 3) == 3) sts128(operand_at(to, r, i >> 2), out[0], out[1], out[2], out[3]);
         }
     } else {
+#pragma unroll
+        for (int k = 0; k < NG; ++k) { sc[k] = lds16(scale + 2 * k) * 0x10001u; lo[k] = lds16(mn + 2 * k) * 0x10001u; }
         constexpr int PAIRS = 8 / BITS, DIRECT = (10 - BITS) / (2 * BITS) + 1;      // pairs of neighbours in a half word; in reach without a shift
 #pragma unroll
         for (int i = 0; i < 64; ++i) {                            // elements 2i, 2i + 1
