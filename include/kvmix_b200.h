@@ -559,7 +559,7 @@ int kvq_page_write(const kvq_page_book *b, const kvq_page_layer *l, const kvq_pa
  *   k, v [tokens, Hkv, 128], q [tokens, nh, 128] of `type`, contiguous along the channels, strides *_sT, *_sH;  q_out [tokens, nh, 128] fp16, may be q where that is fp16
  *   cos, sin [angle_rows][angles] fp32, rows c_sT, s_sT apart;  angles a multiple of 8, at most 64 / parts;  q NULL: keys and values alone
  * A token whose position is outside the tables is left out, its query too (KVQ_PAGES_NO_ANGLE); one without a place in the pages is left out
- * as kvq_page_write does (KVQ_PAGES_NOT_WRITTEN), its query is rotated.
+ * as kvq_page_write does (KVQ_PAGES_NOT_WRITTEN), its query is rotated.  While an earlier call stands refused (count[2]) nothing is written, q_out neither.
  */
 #define KVQ_F16 0
 #define KVQ_BF16 1

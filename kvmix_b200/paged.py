@@ -260,7 +260,8 @@ def page_append(k, v, cos, sin, q_start, rows, pages, layer, q=None, q_out=None,
     parts = 2: the two halves of a head are turned each for itself (``paged_differential_attention``), angles up to 32 then.  A token's row is its
     place in the sequence, or positions[token] (int32 [tokens]).  Rotations are fp32 products and sums, rounded once to fp16.
     Tokens that ``page_write`` would leave out are left out; those whose position is outside the tables too, their queries with them, and a
-    status bit says so.  Returns the queries, fp16 (q_out where it is given, which may be q itself; None without q); rows behind q_start[n] are left as they are."""
+    status bit says so.  Returns the queries, fp16 (q_out where it is given, which may be q itself; None without q); rows behind q_start[n] are left as they are, and
+    all of them while an earlier call stands refused."""
     dev, book = _book(pages)
     kfull, kind, shape = layer.kfull, k.dtype, k.shape
     heads = kfull.shape[1]
@@ -490,7 +491,8 @@ class KVmixPagedCache:
             out = cache.attend(l, q, step)             # [tokens, nh, 128]; options as paged_attention
         cache.settle(rows)                             # full pages behind the window are quantized
 
-    ``append`` takes keys and queries as the projections give them and rotates both; ``advance`` ends a step of beam search.
+    ``append`` is ``write`` of keys as the projections give them, and rotates the queries too; ``attend_differential`` is the difference of two
+    attentions; ``advance`` ends a step of beam search (``beam_select``, then ``reorder``).
     ``lengths`` mirrors the lengths on the host (it lays out the work); ``check()`` raises if a call had to be refused."""
 
     def __init__(self, layers, kv_heads, head_dim, max_seqs, max_tokens, packed_pages, fp16_pages, group_size, residual_length=128, device="cuda"):
