@@ -43,7 +43,7 @@ def check(logits, scores, beams, n=None, ends=()):
             slack = off + 2.0 ** -23 * abs(v) if math.isfinite(v) else 0.0
             assert mine[i][0] == v or abs(mine[i][0] - v) <= slack, (r, i, mine[i], want[i])
             near = [w[1:] for w in want if w[0] == v or abs(w[0] - v) <= 2 * slack]
-            if v == -math.inf or len(near) == 1 or len({w[1] for w in near}) == 1:        # one beam's continuations are compared exactly
+            if v == -math.inf or len(near) == 1 or len({w[0] for w in near}) == 1:        # one beam's continuations are compared exactly
                 assert mine[i][1:] == want[i][1:], (r, i, mine[i], want[i])
             else:
                 assert mine[i][1:] in near
