@@ -8,6 +8,7 @@
 // A candidate within a beam is one 64-bit key, the logit in an order of unsigned numbers above the complement of the token: keys are
 // all different, the largest is the best and ties go to the lowest token, in whatever order threads come.
 // Sums are fp32 within a thread (some hundred terms) and 64-bit from there: which of two beams goes on may hang on the last bits of their sums.
+#include "beam_reach.cuh"
 #include "quant_core.cuh"
 
 #include <cuda_bf16.h>
@@ -83,7 +84,7 @@ struct RunningSum {
 // A part of a row, 4096 elements a turn.  The pass over it keeps a thread's sum, its maximum and where that came first, and nothing else.  Of the groups of threads (eight
 // lanes, fewer where n is large) the n-th best then has a key that n elements reach at least, and none of the n best is in a thread whose best does not reach
 // it: what the others hold -- those of some 1.1 n threads -- is read once more, from L2, and what reaches the threshold goes to shared memory.  Should
-// there be no room for all of it (rows that were made for that), the n best of what there was room for give a higher threshold.
+// there be no room for all of it (rows that were made for that), the n best of what there was room for give a higher threshold (Reach).
 // Which thread has which token follows from the token alone, not from the row's alignment: rows alike have sums alike, to the last bit, and ties between
 // beams stay ties.  Rows that are not 16-byte aligned are therefore read element by element (VEC false).
 template <typename T, bool VEC>
@@ -220,9 +221,8 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
     }
     // keys of pieces here: a token's place behind its piece's
     if (mine && mine >= s_from) s_thread[atomicAdd(&s_threads, 1)] = tid;
-    u64 from = s_from;
-    const u64 from_piece = from;
-    const float from_x = from_ordered((uint32_t)(from >> 32));
+    Reach reaches(s_from);
+    const float from_x = from_ordered((uint32_t)(reaches.by_piece >> 32));
     bool lost;
     do {
         __syncthreads();
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
 #pragma unroll
                     for (int k = 1; k < E; ++k) one = k == e ? v[k] : one;
                     const u64 key = beam_key(one, piece * E + e);
-                    if (beam_key(one, piece) < from_piece || (from != from_piece && key < from)) continue;
+                    if (!reaches.takes(beam_key(one, piece), key)) continue;
                     const int place = atomicAdd(&s_count, 1);
                     if (place < kKeys) s_key[place] = key;
                     else lost = true;
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
         }
         __syncthreads();
         if (lost) {
-            from = s_best[n - 1];
+            reaches.raise(s_best[n - 1]);
             if (tid == 0) s_count = 0;
         } else if (tid < n) {
             p.keys[out * n + tid] = tid < kept ? s_best[tid] : 0;
