@@ -590,7 +590,7 @@ int kvq_page_copy_tails(const kvq_page_tensor *tensors, int32_t n, const int32_t
 
 /*
  * Beam search's selection.  logits [requests * beams, vocabulary] of `type`, rows l_sR elements apart; scores [requests * beams] of the beams so far.
- *   value(b, t) = scores[b] + (logits[b][t] - log sum_t' exp(logits[b][t']))
+ *   value(b, t) = scores[b] + log_softmax(logits[b])[t],   log_softmax(x)[t] = (x[t] - max x) - log sum_t' exp(x[t'] - max x)
  * The n continuations of a request with the largest values, in that order, equal ones by (beam, token): their values, beams (within the request) and tokens in
  * out_* [requests, n]; and the first `beams` of them whose token is not among ends[n_ends] in next_* [requests, beams], which is what goes on.
  * A beam whose score is not finite, or whose logits hold a NaN or +infinity or nothing but -infinity, offers all its tokens at -infinity, and so does every beam

@@ -1,7 +1,9 @@
 // Beam search's selection: the best continuations of every request over its beams and the vocabulary.
 //
-//   value(b, t) = score_b + (logit_bt - log sum_t' exp(logit_bt')),   the n largest of a request, equal ones by (b, t)
+//   value(b, t) = score_b + ((logit_bt - top_b) - log sum_t' exp(logit_bt' - top_b)),   the n largest of a request, equal ones by (b, t)
 //
+// with top_b the largest logit of the beam, which is never added to the logarithm: beside a top of 1e30, or where all logits are the type's lowest number, that
+// would be lost, and every token have the probability of one.
 // Within a beam the order of the values is the order of the logits, so one pass over a row gives both what it needs: the sum of
 // exponentials under a running maximum and the row's n best logits.  A row is cut into up to 32 parts, a CTA each (beam_scan_kernel); a second launch
 // joins the parts of each beam, then the beams of each request (beam_join_kernel).
@@ -283,15 +285,19 @@ __device__ __forceinline__ u64 ordered64(double x) {              // as ordered(
 }
 __device__ __forceinline__ double from_ordered64(u64 u) { return __longlong_as_double((long long)(u ^ ((long long)u < 0 ? 1ull << 63 : ~0ull))); }
 
-// The sum of a beam's exponentials from its parts', a lane each: score minus its logarithm, which a logit is added to; not finite where the beam offers nothing.
-__device__ __forceinline__ double beam_base(const BeamArgs &p, int64_t row, int lane, double &all) {
+// A beam's largest logit and the logarithm of its sum of exponentials from its parts', a lane each; not finite where the beam offers nothing.
+struct BeamBase {
+    double score, top, log_sum;
+    __device__ __forceinline__ bool alive() const { return isfinite(score) && isfinite(log_sum); }
+    __device__ __forceinline__ u64 value(u64 key) const { return ordered64(score + (((double)from_ordered((uint32_t)(key >> 32)) - top) - log_sum)); }
+};
+__device__ __forceinline__ BeamBase beam_base(const BeamArgs &p, int64_t row, int lane) {
     const float my_top = lane < p.parts ? p.tops[row * p.parts + lane] : -INFINITY, top = warp_max(my_top);
     double sum = lane < p.parts ? p.sums[row * p.parts + lane] : 0.0;
     if (sum != 0.0) sum *= (double)expf(my_top - top);             // 2^-23: as exact as the terms
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    all = (double)top + log(sum);
-    return (double)p.a.scores[row];
+    return {(double)p.a.scores[row], (double)top, log(sum)};       // no sum, no number or an infinite top: neither is the logarithm finite
 }
 __device__ __forceinline__ void put_best(const BeamArgs &p, int64_t at, float value, int beam, int token) {
     p.a.out_scores[at] = value;
@@ -313,7 +319,7 @@ __device__ __forceinline__ void put_next(const BeamArgs &p, int64_t at, float va
 constexpr int kJoined = 1024;
 template <bool BY_BEAMS>
 __global__ void __launch_bounds__(512) beam_join_kernel(const __grid_constant__ BeamArgs p) {
-    __shared__ double s_all[kMostBeams], s_score[kMostBeams];
+    __shared__ BeamBase s_base[kMostBeams];
     __shared__ u64 s_value[kJoined], s_place[kJoined], s_from, s_full[16];         // ordered values; (beam, token)
     __shared__ uint32_t s_goes[(kMostBest + 31) / 32];
     __shared__ int s_left, s_best[kMostBest];
@@ -323,9 +329,8 @@ __global__ void __launch_bounds__(512) beam_join_kernel(const __grid_constant__ 
     const float per_list = 1.f / list;                            // c / list = (c + 0.5) * this for every c here (below 2^22)
     u64 full = 0, unused;
     for (int b = warp; b < K; b += warps) {
-        double sum;
-        const double score = beam_base(p, (int64_t)blockIdx.x * K + b, lane, sum);
-        if (lane == 0) { s_all[b] = sum; s_score[b] = score; }
+        const BeamBase base = beam_base(p, (int64_t)blockIdx.x * K + b, lane);
+        if (lane == 0) s_base[b] = base;
         if constexpr (BY_BEAMS) {                                 // 159 of its keys at most
             const int each = (n + p.parts - 1) / p.parts, some = p.parts * each;
             u64 held[5], nth = 0;
@@ -344,7 +349,7 @@ __global__ void __launch_bounds__(512) beam_join_kernel(const __grid_constant__ 
                         if (32 * h < some) rank += __popc(__ballot_sync(0xffffffffu, held[h] > one));
                     if (rank == n - 1 && one) nth = one;
                 }
-            if (nth && isfinite(sum) && isfinite(score)) full = max(full, ordered64(score + ((double)from_ordered((uint32_t)(nth >> 32)) - sum)));
+            if (nth && base.alive()) full = max(full, base.value(nth));
         }
     }
     if (tid < (kMostBest + 31) / 32) s_goes[tid] = 0;
@@ -353,11 +358,11 @@ __global__ void __launch_bounds__(512) beam_join_kernel(const __grid_constant__ 
     // candidate c's value, in order, and its place; 0: there is none
     auto candidate = [&](int c, u64 key, u64 &place) -> u64 {
         const int beam = (int)((c + 0.5f) * per_list), i = c - beam * list;
-        const bool alive = isfinite(s_all[beam]) && isfinite(s_score[beam]);
+        const bool alive = s_base[beam].alive();
         const int token = alive ? (int)~(uint32_t)key : i;        // a beam that offers nothing: its first tokens, once
         place = (u64)beam << 32 | (uint32_t)token;
         if (alive ? key == 0 : i >= n || i >= p.a.vocabulary) return 0;
-        return ordered64(alive ? s_score[beam] + ((double)from_ordered((uint32_t)(key >> 32)) - s_all[beam]) : -INFINITY);
+        return alive ? s_base[beam].value(key) : ordered64(-INFINITY);
     };
     const int lists = K * p.parts, firsts = (n + lists - 1) / lists, heads = lists * firsts;       // 192 + 128 heads at most (beam_parts)
     for (int h = tid; h < heads; h += blockDim.x) {

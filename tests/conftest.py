@@ -12,6 +12,18 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (run on a B200)")
 
 
+# A row of 20000 logits that are all the type's lowest number (bf16 and fp32: -3.4e38) has log-probabilities of -log 20000 = -9.9.  The definition there,
+# x - logsumexp(x) in 64 bits, gives 0: beside 3.4e38 the 9.9 are less than half a unit of the last place (2^127 * 2^-53 = 2^74).  The test runs as it is and has
+# to fail; test_gpu_beam_edges.py runs the same rows with the logarithm kept apart from the maximum.
+_LOSES_THE_LOGARITHM = {"test_gpu_beams.py::test_masks_and_numbers_that_are_none[kind%d]" % i for i in (1, 2)}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        if item.nodeid.split("/")[-1] in _LOSES_THE_LOGARITHM:
+            item.add_marker(pytest.mark.xfail(strict=True, raises=AssertionError, reason="its definition gives 0 for -log V beside logits of -3.4e38"))
+
+
 @pytest.fixture(scope="session")
 def cuda():
     import torch
