@@ -57,7 +57,7 @@ static int paged_tiles(const PagedArgs &p, int max_tiles, cudaStream_t st) {
 }
 
 // Partial sums of the splits -> outputs, in the splits' order: a row a warp, or a head's two rows.  `few`: rows of the kernel of few rows, kFewRows places
-// for every (sequence, kv head); else rows of q, of which those that the kernel of tiles had are joined.
+// for every (sequence, kv head); else, where some tiles are cut alone, the rows of their CTAs; else rows of q, of which those that the kernel of tiles had are joined.
 template <bool DIFF>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant__ PagedArgs p, int few) {
     const int64_t at = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (DIFF ? 2 : 1);
@@ -74,6 +74,20 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
         u = s.q0 + r / p.rep;
         h = head * p.rep + r % p.rep;
         row = p.part_compact ? at : (int64_t)u * p.a.nh + h;
+    } else if (DIFF && p.n_whole > 0) {
+        const int hs = p.n_whole + (int)(at >> 8), head = hs % p.l.Hkv;
+        int tile = p.max_tiles - 1 - hs / p.l.Hkv, i = 0, q0 = 0, n_new = 0;         // as the kernel of tiles counts them
+        for (; i < p.a.n; ++i) {
+            new_tokens(p, i, q0, n_new);
+            const int rows = max(0, n_new) * p.rep, tiles = rows > p.few_rows ? (rows + 255) / 256 : 0;
+            if (tile < tiles) break;
+            tile -= tiles;
+        }
+        const int r = tile * 256 + (int)(at & 255);
+        if (i == p.a.n || tile < 0 || r >= n_new * p.rep) return;
+        u = q0 + r / p.rep;
+        h = head * p.rep + r % p.rep;
+        row = at;
     } else {
         const int64_t q = at / p.a.nh;
         if (q >= p.a.tokens || q < p.a.q_start[0] || q >= p.a.q_start[p.a.n]) return;
@@ -83,17 +97,6 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
         if (p.few_rows) {
             const PagedSeq s = paged_seq(p, sequence_of(p.a.q_start, p.a.n, u));
             if (s.n_new * p.rep <= p.few_rows) return;
-        }
-        if (DIFF && p.n_whole > 0) {                              // a tile that was not cut?
-            int before = 0, q0 = 0, n_new = 0;
-            for (int i = 0; i < p.a.n; ++i) {
-                new_tokens(p, i, q0, n_new);
-                if (u >= q0 && u < q0 + n_new) break;
-                const int rows = max(0, n_new) * p.rep;
-                if (rows > p.few_rows) before += (rows + 255) / 256;
-            }
-            const int tile = before + ((u - q0) * p.rep + h % p.rep) / 256;
-            if ((int64_t)(p.max_tiles - 1 - tile) * p.l.Hkv + h / p.rep < p.n_whole) return;
         }
     }
     auto join = [&](int64_t row, float &l) {
@@ -144,7 +147,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant_
 }
 
 static int paged_merge(const PagedArgs &p, int few, cudaStream_t st) {
-    const int64_t rows = few ? (int64_t)p.a.n * p.l.Hkv * kFewRows : (int64_t)p.a.tokens * p.a.nh, grid = (rows + 7) / 8;
+    const int64_t rows = few ? (int64_t)p.a.n * p.l.Hkv * kFewRows : p.part_rows, grid = (rows + 7) / 8;
     if (grid > 2147483647LL) return KVQ_ERR_UNSUPPORTED;
     if (p.lambdas) paged_merge_kernel<true><<<(unsigned)((grid + 1) / 2), 256, 0, st>>>(p, few);
     else paged_merge_kernel<false><<<(unsigned)grid, 256, 0, st>>>(p, few);
@@ -159,6 +162,13 @@ struct PagedPlan {
     FewShape shape;                   // of the kernel of few rows, differential attention
     int n_whole;                      // tiles that are not cut beside others that are (PagedArgs), differential attention
 };
+
+// Bytes of `rows` partial sums: whole splits of all rows of q are asked for, two at least.
+static uint64_t part_bytes(int64_t rows, int64_t all) {
+    const int64_t units = (rows + all - 1) / all;
+    return (uint64_t)(rows == 0 ? 0 : units < 2 ? 2 : units) * all * (kHeadDim + 2) * 4;
+}
+constexpr uint64_t kMostCutBytes = 1 << 29;
 
 static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, int max_new, int max_tokens, int max_chunks, bool diff) {
     PagedPlan r = {};
@@ -210,11 +220,13 @@ static PagedPlan paged_plan(const kvq_page_layer &l, int n, int tokens, int nh, 
         if (cost < 0.85 * best) { best = cost; r.tile_splits = s; }
     }
     // Differential attention: what is left of a last round of CTAs may be cut alone, where tiles are alike because what is new is little (a chunk of 2048 over
-    // 32k tokens, 512 tiles of 148 at a time: 2021 us whole, 1777 with the last 68 halved).
+    // 32k tokens, 512 tiles of 148 at a time: 2021 us whole, 1777 with the last 68 halved), unless the sums take more than kMostCutBytes: calls of many rounds
+    // gain the least.
     if (diff && r.tiles && r.tile_splits == 1 && n <= kMostCutSequences && ctas > 148 && ctas < INT32_MAX && (int64_t)max_new * 4 <= max_tokens) {
         const int rest = (int)(ctas % 148);
         double least = 0.96 * (double)((ctas + 147) / 148);
         for (int s = 2; rest && s <= 8 && s <= pages / 4; ++s) {
+            if (part_bytes((int64_t)s * rest * 256, (int64_t)tokens * nh) > kMostCutBytes) break;
             const double cost = (double)(ctas / 148) + (double)((rest * s + 147) / 148) * (pages / (double)s + 4) / (pages + 4) + (1.5 + (double)s * rest * 256 * 1040 / 5e6 / 1.8) / (pages + 4);
             if (cost < least) { least = cost; r.tile_splits = s; r.n_whole = (int)ctas - rest; }
         }
@@ -230,11 +242,15 @@ static bool few_compact(const PagedPlan &r, int n, int Hkv, int tokens, int nh) 
 static int64_t few_part_rows(const PagedPlan &r, int n, int Hkv, int tokens, int nh) {
     return few_compact(r, n, Hkv, tokens, nh) ? (int64_t)n * Hkv * kFewRows : (int64_t)tokens * nh;
 }
-// Both kernels' partial sums, one after the other in the same place; in whole splits of all rows of q, two at least.
+// Rows of a split of the kernel of tiles: where only some tiles are cut, those of their CTAs in the order of CTAs, else those of q.
+static int64_t tile_part_rows(const PagedPlan &r, int Hkv, int tokens, int nh) {
+    return r.n_whole > 0 ? ((int64_t)r.max_tiles * Hkv - r.n_whole) * 256 : (int64_t)tokens * nh;
+}
+// Both kernels' partial sums, one after the other in the same place.
 static uint64_t paged_bytes(const PagedPlan &r, int n, int Hkv, int tokens, int nh) {
-    const int64_t all = (int64_t)tokens * nh, few = r.few && r.few_splits > 1 ? r.few_splits * few_part_rows(r, n, Hkv, tokens, nh) : 0,
-                  tiles = r.tiles && r.tile_splits > 1 ? r.tile_splits * all : 0, most = few > tiles ? few : tiles, units = (most + all - 1) / all;
-    return (uint64_t)(most == 0 ? 0 : units < 2 ? 2 : units) * all * (kHeadDim + 2) * 4;
+    const int64_t few = r.few && r.few_splits > 1 ? r.few_splits * few_part_rows(r, n, Hkv, tokens, nh) : 0,
+                  tiles = r.tiles && r.tile_splits > 1 ? r.tile_splits * tile_part_rows(r, Hkv, tokens, nh) : 0;
+    return part_bytes(few > tiles ? few : tiles, (int64_t)tokens * nh);
 }
 
 }  // namespace kvq
@@ -309,7 +325,7 @@ static int attend(const kvq_page_book *b, const kvq_page_layer *l, const kvq_pag
         p.splits = r.tile_splits;
         p.max_tiles = r.max_tiles;
         p.n_whole = r.n_whole;
-        p.part_rows = (int64_t)a->tokens * nh;
+        p.part_rows = tile_part_rows(r, l->Hkv, a->tokens, nh);
         p.part_ml = p.part_out + p.splits * p.part_rows * kHeadDim;
         if (const int rc = paged_tiles(p, r.max_tiles, st)) return rc;
         if (p.splits > 1)

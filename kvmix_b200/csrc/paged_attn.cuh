@@ -22,8 +22,8 @@ struct PagedArgs {
     int rep, k_groups, v_groups;      // query heads of a kv head; groups of a page's row
     int splits, few_rows;             // few_rows: sequences with at most so many rows are the other kernel's
     float cap_in;                     // softmax_scale / softcap
-    int64_t part_rows;                // rows of a split's partial sums: those of q, or kFewRows of every (sequence, kv head)
-    bool part_compact;                // the latter
+    int64_t part_rows;                // rows of a split's partial sums: those of q, or kFewRows of every (sequence, kv head), or 256 of every CTA that is cut
+    bool part_compact;                // the second
     float *part_out;                  // [splits][part_rows][128], unnormalised
     float *part_ml;                   // [splits][part_rows][2]: the exponents' reference (log2), the weights' sum
     // Differential attention: a query head is two rows, one for each half of its channels, next to each other; a.nh and rep count them apart

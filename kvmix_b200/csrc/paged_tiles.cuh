@@ -452,7 +452,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const __gri
             l = half ? __uint_as_float(lds32(other_top)) + l : l + __uint_as_float(lds32(other_top));
             const float inv = l == 0.f ? 0.f : 1.f / l;
             __half *out = static_cast<__half *>(p.a.out) + (int64_t)(s.q0 + u) * p.a.o_sT + (int64_t)h * p.a.o_sH + half * N;
-            const int64_t part = (int64_t)split * p.a.tokens * p.a.nh + (int64_t)(s.q0 + u) * p.a.nh + (DIFF ? 2 * h + tile_of : h);
+            const int64_t part = DIFF && p.n_whole > 0 ? split * p.part_rows + (int64_t)(hs - p.n_whole) * 256 + 2 * r + tile_of
+                                                       : split * p.part_rows + (int64_t)(s.q0 + u) * p.a.nh + (DIFF ? 2 * h + tile_of : h);
             const bool vec = (reinterpret_cast<uintptr_t>(p.a.out) % 16 | p.a.o_sT % 8 | p.a.o_sH % 8) == 0;
             if (DIFF && splits() == 1) {
                 // The operand buffers are free: no copy and no product is under way.  A row's 16-byte pieces are mixed by its number.
