@@ -382,7 +382,7 @@ def pages_compact(pages, layers):
 
 @_on_its_device(3)
 def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, prefix=None, first=None, softcap=None, alibi_slopes=None,
-                    softmax_scale=None, max_new=None, max_tokens=None, max_chunks=None, out=None, _diff=None):
+                    softmax_scale=None, max_new=None, max_tokens=None, max_chunks=None, out=None):
     """Attention of the last tokens of every sequence over its pages.
 
     q [tokens, nh, 128] fp16: tokens [q_start[i], q_start[i+1]) are the last ones of sequence rows[i], whose keys and values are in the
@@ -398,6 +398,12 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     which few have several tokens the third saves time).  Tokens that see nothing get zeros.  Cached values have
     to be finite: one that is not may reach queries that do not see it (include/kvmix_b200.h).
     Returns [tokens, nh, 128] fp16; rows behind q_start[n] are left as they are."""
+    return _attend(q, q_start, rows, pages, layer, causal, window, prefix, first, softcap, alibi_slopes, _SCALE if softmax_scale is None else softmax_scale, max_new, max_tokens,
+                   max_chunks, out)
+
+
+def _attend(q, q_start, rows, pages, layer, causal, window, prefix, first, softcap, alibi_slopes, softmax_scale, max_new, max_tokens, max_chunks, out, diff=None):
+    """``paged_attention``, or with diff -- addresses of lambdas and of the norm's weight, its eps -- the differential one."""
     dev, book = _book(pages)
     if q.dim() != 3 or q.dtype is not _f16 or q.get_device() != dev or q.shape[2] != 128:
         raise RuntimeError(f"attention over pages takes fp16 queries [tokens, heads, 128] on cuda:{dev}")
@@ -418,7 +424,7 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     window, softcap = window or 0, softcap or 0.0
     if window < 0 or not softcap >= 0.0:
         raise RuntimeError("window and softcap must not be negative")
-    if softmax_scale is not None and not abs(softmax_scale) <= 3.4e38:
+    if not abs(softmax_scale) <= 3.4e38:
         raise RuntimeError("softmax_scale must be a finite number")
     at_slopes = 0
     if alibi_slopes is not None:
@@ -432,14 +438,14 @@ def paged_attention(q, q_start, rows, pages, layer, causal=True, window=None, pr
     if tokens and n and (max_new <= 0 or max_tokens <= 0 or max_chunks < 0):
         raise RuntimeError("max_new and max_tokens must be positive, max_chunks not negative")
     L = _library()
-    need = (L.kvq_paged_diff_attn_workspace_bytes if _diff else L.kvq_paged_attn_workspace_bytes)(block, n, tokens, nh, max_new, max_tokens, max_chunks)
+    need = (L.kvq_paged_diff_attn_workspace_bytes if diff else L.kvq_paged_attn_workspace_bytes)(block, n, tokens, nh, max_new, max_tokens, max_chunks)
     ws = pages.count.new_empty((need + 3) // 4) if need else None
     a = (q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), _ints(dev, "q_start", q_start, n + 1),
          _ints(dev, "rows", rows, n), 0 if first is None else _ints(dev, "first", first, tokens), 0 if prefix is None else _ints(dev, "prefix", prefix, n),
          at_slopes, n, tokens, nh, max_new, max_tokens, max_chunks, int(min(window, _MOST)), 1 if causal else 0,
-         _SCALE if softmax_scale is None else softmax_scale, min(softcap, 1e38), 0 if ws is None else ws.data_ptr(), need)
-    if _diff:
-        _launched(L.kvq_paged_diff_attn(book, block, _pack_diff(*a, *_diff), ops.raw_stream()))
+         softmax_scale, min(softcap, 1e38), 0 if ws is None else ws.data_ptr(), need)
+    if diff:
+        _launched(L.kvq_paged_diff_attn(book, block, _pack_diff(*a, *diff), ops.raw_stream()))
     else:
         _launched(L.kvq_paged_attn(book, block, _pack_attn(*a), ops.raw_stream()))
     return out
@@ -465,8 +471,8 @@ def paged_differential_attention(q, lambdas, q_start, rows, pages, layer, causal
         if not 0.0 <= norm_eps <= 3.4e38:
             raise RuntimeError("norm_eps must not be negative")
         at_weight = norm_weight.data_ptr()
-    return paged_attention.__wrapped__(q, q_start, rows, pages, layer, causal, window, prefix, first, softcap, alibi_slopes, 0.125 if softmax_scale is None else softmax_scale,
-                                       max_new, max_tokens, max_chunks, out, (lambdas.data_ptr(), at_weight, norm_eps))
+    return _attend(q, q_start, rows, pages, layer, causal, window, prefix, first, softcap, alibi_slopes, 0.125 if softmax_scale is None else softmax_scale, max_new, max_tokens,
+                   max_chunks, out, (lambdas.data_ptr(), at_weight, norm_eps if at_weight else 0.0))
 
 
 class PagedStep(NamedTuple):

@@ -1,6 +1,10 @@
 """Differential attention over pages without a GPU: what a call asks for beside its tensors."""
-import pytest
+import inspect
 
+import pytest
+import torch
+
+import kvmix_b200 as kv
 from kvmix_b200 import paged
 from test_paged_host import layer
 
@@ -24,3 +28,15 @@ def test_a_cut_is_still_made():
     L = paged._library()
     assert L.kvq_paged_diff_attn_workspace_bytes(layer(Hkv=8), 1, 2048, 32, 2048, 34816, 1) == 2 * 2048 * 64 * 520
     assert 0 < L.kvq_paged_diff_attn_workspace_bytes(layer(Hkv=8), 1, 2400, 32, 2400, 34816, 1) <= 160 * MB
+
+
+def test_plain_attention_takes_no_more_than_it_says():
+    """Addresses of the differential form are not to be had through the plain one."""
+    names = inspect.signature(kv.paged_attention).parameters
+    assert not [n for n in names if n.startswith("_")]
+    i = torch.zeros(1, dtype=torch.int32)
+    cache = kv.KVmixPagedCache([(4, 2)], 1, 128, 2, 256, 1, 2, 64, device="cpu")
+    with pytest.raises(TypeError):
+        kv.paged_attention(torch.zeros(1, 1, 128).half(), i, i, cache.book, cache.layers[0], True, None, None, None, None, None, None, None, None, None, None, (1, 2, 3.0))
+    with pytest.raises(TypeError):
+        kv.paged_attention(torch.zeros(1, 1, 128).half(), i, i, cache.book, cache.layers[0], _diff=(1, 2, 3.0))
