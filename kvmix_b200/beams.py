@@ -33,7 +33,8 @@ def beam_select(logits, scores, beams, n=None, ends=None):
 
     logits [requests * beams, vocabulary] fp16, bf16 or fp32, any row stride; scores fp32 [requests * beams], the beams' so far.  A continuation's score is
     scores[beam] + log_softmax(logits[beam])[token]; the ``n`` best of a request (None: twice the beams, or beams * (1 + number of ends) where that is more; at most 128, beams at
-    most 64) come in order, equal ones by (beam, token).  ends: int32 tensor of tokens that end a sequence; n must leave ``beams`` others.  Sums of exponentials are kept in
+    most 64) come in order, equal ones by (beam, token).  ends: int32 tensor of tokens that end a sequence; n must leave ``beams`` others, so beams * (1 + number of ends)
+    is at most 128 too: one end for 64 beams, 31 for four.  Sums of exponentials are kept in
     64 bits across threads, so that the order of two beams' continuations does not hang on them.
     A beam offers -infinity everywhere where its score is not finite (a beam that is not there: -infinity), its logits hold a NaN or +infinity, or all of
     them are masked (-infinity)."""
@@ -52,16 +53,24 @@ def beam_select(logits, scores, beams, n=None, ends=None):
         if ends.dtype is not torch.int32 or ends.dim() != 1 or ends.get_device() != dev or not ends.is_contiguous():
             raise RuntimeError(f"ends must be a contiguous int32 tensor on cuda:{dev}")
         n_ends, at_ends = ends.numel(), ends.data_ptr()
-    all_of_them, needed = beams * vocabulary, beams * (1 + n_ends)
-    n = min(max(2 * beams, needed), all_of_them) if n is None else int(n)
-    if not min(needed, all_of_them) <= n <= min(all_of_them, _lib.MOST_BEST):
-        raise RuntimeError(f"n must be {min(needed, all_of_them)} to {min(all_of_them, _lib.MOST_BEST)} for {beams} beams and {n_ends} ends")
+    n = _how_many(n, beams, n_ends, vocabulary)
     if logits.stride(1) != 1 and vocabulary > 1:
         logits = logits.contiguous()
     if dev != _current_device():
         with torch.cuda.device(dev):
             return _select(logits, scores, beams, n, n_ends, at_ends)
     return _select(logits, scores, beams, n, n_ends, at_ends)
+
+
+def _how_many(n, beams, n_ends, vocabulary):
+    all_of_them = beams * vocabulary
+    least, most = min(beams * (1 + n_ends), all_of_them), min(all_of_them, _lib.MOST_BEST)
+    if least > most:
+        raise RuntimeError(f"{beams} beams and {n_ends} ends take the {least} best continuations: beams * (1 + number of ends) is at most {most}")
+    n = min(max(2 * beams, least), most) if n is None else int(n)
+    if not least <= n <= most:
+        raise RuntimeError(f"n must be {least} to {most} for {beams} beams and {n_ends} ends")
+    return n
 
 
 @functools.lru_cache(maxsize=None)
