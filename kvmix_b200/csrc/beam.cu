@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(512) beam_join_kernel(const __grid_constant__ 
 static int beam_parts(const kvq_beam_args &a) {
     const int64_t rows = (int64_t)a.requests * a.beams;
     int64_t parts = (rows > 148 ? 4 * 148 : rows * a.vocabulary >= 6 << 20 && a.n <= 32 ? 2 * 148 : 148) / (rows > 0 ? rows : 1);
-    const int64_t most = (a.vocabulary + kScanThreads * kTurn - 1) / (kScanThreads * kTurn);
+    const int64_t most = ((int64_t)a.vocabulary + kScanThreads * kTurn - 1) / (kScanThreads * kTurn);
     if (parts > most) parts = most;
     if (parts > kMostParts) parts = kMostParts;
     if (parts > 1024 / a.n) parts = 1024 / a.n;

@@ -1,7 +1,8 @@
 """How many continuations a selection may be asked for, without a GPU."""
 import pytest
 
-from kvmix_b200 import beams
+from kvmix_b200 import beams, paged
+from test_beam_host import select
 
 
 @pytest.mark.parametrize("b,ends,V,want", [(1, 0, 100, 2), (4, 0, 100, 8), (4, 1, 100, 8), (4, 2, 100, 12), (64, 0, 100, 128), (64, 1, 100, 128), (4, 31, 1000, 128), (1, 127, 1000, 128),
@@ -22,3 +23,10 @@ def test_more_ends_than_can_be_told_apart(b, ends, V, n):
 def test_out_of_range(n, b, ends, V, low, high):
     with pytest.raises(RuntimeError, match=f"n must be {low} to {high} "):
         beams._how_many(n, b, ends, V)
+
+
+@pytest.mark.parametrize("V", [1 << 24, (1 << 31) - 4096, (1 << 31) - 4095, (1 << 31) - 1])
+def test_parts_of_the_widest_rows(V):
+    """One row is 32 parts however wide it is."""
+    n = 8
+    assert paged._library().kvq_beam_select_workspace_bytes(select(requests=1, beams=1, vocabulary=V, n=n)) == 32 * (8 * n + 16)
