@@ -483,6 +483,7 @@ class PagedStep(NamedTuple):
     max_new: int
     max_tokens: int
     max_chunks: int
+    positions: int = 0                # the new tokens' are all below it
 
 
 class KVmixPagedCache:
@@ -562,7 +563,7 @@ class KVmixPagedCache:
         for r, c in zip(rows, counts):
             self.lengths[r] += c
         return PagedStep(at, both[n:], starts[-1], max(counts, default=0), max((self.lengths[r] for r in rows), default=0),
-                         sum(c > 1 for c in counts))
+                         sum(c > 1 for c in counts), max((self.lengths[r] for r, c in zip(rows, counts) if c), default=0))
 
     def write(self, layer, k, v, step):
         if k.shape[0] != step.tokens or v.shape[0] != step.tokens:
@@ -588,8 +589,8 @@ class KVmixPagedCache:
         parts."""
         if k.shape[0] != step.tokens or v.shape[0] != step.tokens or (q is not None and q.shape[0] != step.tokens):
             raise RuntimeError("keys, values and queries for every new token of the step")
-        if options.get("positions") is None and cos.shape[0] < step.max_tokens:
-            raise RuntimeError(f"angles for {cos.shape[0]} positions, the step has tokens up to {step.max_tokens}")
+        if options.get("positions") is None and cos.shape[0] < step.positions:
+            raise RuntimeError(f"angles for {cos.shape[0]} positions, the step has new tokens up to {step.positions}")
         return page_append(k, v, cos, sin, step.q_start, step.rows, self.book, self.layers[layer], q=q, **options)
 
     def settle(self, rows=None):
