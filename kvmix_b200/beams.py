@@ -34,8 +34,9 @@ def beam_select(logits, scores, beams, n=None, ends=None):
     logits [requests * beams, vocabulary] fp16, bf16 or fp32, any row stride; scores fp32 [requests * beams], the beams' so far.  A continuation's score is
     scores[beam] + log_softmax(logits[beam])[token]; the ``n`` best of a request (None: twice the beams, or beams * (1 + number of ends) where that is more; at most 128, beams at
     most 64) come in order, equal ones by (beam, token).  ends: int32 tensor of tokens that end a sequence; n must leave ``beams`` others, so beams * (1 + number of ends)
-    is at most 128 too: one end for 64 beams, 31 for four.  Sums of exponentials are kept in
-    64 bits across threads, so that the order of two beams' continuations does not hang on them.
+    is at most 128 too: one end for 64 beams, 31 for four.  A thread's sum of exponentials is fp32 (terms
+    to 2^-22 of themselves, vocabulary / 256 of them at most and some hundred in large calls of few rows), from there they are 64-bit; rows alike have sums alike, to the last bit, but two
+    beams whose continuations lie within that of each other may come in either order.
     A beam offers -infinity everywhere where its score is not finite (a beam that is not there: -infinity), its logits hold a NaN or +infinity, or all of
     them are masked (-infinity)."""
     dev = logits.get_device()

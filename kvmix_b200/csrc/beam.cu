@@ -9,7 +9,8 @@
 // joins the parts of each beam, then the beams of each request (beam_join_kernel).
 // A candidate within a beam is one 64-bit key, the logit in an order of unsigned numbers above the complement of the token: keys are
 // all different, the largest is the best and ties go to the lowest token, in whatever order threads come.
-// Sums are fp32 within a thread (some hundred terms) and 64-bit from there: which of two beams goes on may hang on the last bits of their sums.
+// Sums are fp32 within a thread -- V / (256 parts) terms, each to 2^-22 of itself -- and 64-bit from there: which of two beams goes on may hang on the last bits of
+// their sums, and 64 bits add nothing to the error of the terms.
 #include "beam_reach.cuh"
 #include "quant_core.cuh"
 

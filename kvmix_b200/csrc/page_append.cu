@@ -9,7 +9,8 @@ namespace kvq {
 // A thread takes 16 channels of a (token, head) row -- eight and their eight partners, or 16 that are not rotated -- of one row after the other: queries, keys
 // and values of its token, 32 rows of a CTA at a time, or those of several tokens where a token has fewer (AppendShape), so that no index takes a
 // division.  The first rows are asked for before anything else; meanwhile a thread a token looks up where its keys go, a chain of four dependent loads.  Angles
-// are read anew for every row, from L1: kept in registers they cost a CTA of four an SM.  Bound: bytes in long calls (two prompts of 8k, 32 and 2 x 16 heads: 101 us,
+// are read anew for every row, from L1: kept in registers they cost a CTA of four an SM.  Rows that are not 16-byte aligned (a slice of a fused projection at
+// an odd offset) are read element by element and take twice as long (two prompts of 8k, cold: 209 us against 111); those instances of 2-byte types spill 112 to 136 bytes.  Bound: bytes in long calls (two prompts of 8k, 32 and 2 x 16 heads: 101 us,
 // 5.4 TB/s; 118 with divisions and rows in fours), that chain in short ones (64 tokens: 4.9 us).
 constexpr int kAppendThreads = 256, kAppendRows = kAppendThreads / 8;      // eight threads a row
 constexpr int kAppendTokens = 128;                                         // of a CTA

@@ -159,7 +159,9 @@ struct FewShared {
 };
 
 // DIFF: heads are two rows each (PagedArgs), R is even, CK is 1.  A channel belongs to one half of the keys, so the score columns of a k-step are those of the
-// rows whose half it is in, and a page's scores come half by half: a head's two rows take as many products with the keys as one row of 128 channels.
+// rows whose half it is in, and a page's scores come half by half: a head's two rows take as many products with the keys as one row of 128 channels.  Three CTAs an SM leave
+// 168 registers, of which instances over keys of 1, 2 and 4 bits spill 8 to 24 bytes, 4 over 3 bits.  p * scale is rounded to fp16 once: columns for pairs of hi and lo, as
+// the plain instances have them, would halve the rows of a CTA.
 template <int KB, int VB, int CK, bool DIFF>
 __global__ void __launch_bounds__(kFewWarps * 32, DIFF || KB == 3 || VB == 3 || CK == 2 ? 3 : 4)
     paged_few_kernel(const __grid_constant__ PagedArgs p, int R, int row_blocks, int stages, int stage_rows, int stage_bytes) {
